@@ -417,6 +417,36 @@ int DLGpuBatchNormalizationAndReluBackward(const DLArrayHandle input, const DLAr
                                            void ***activation_list, void **handle, int *memorytoSaving,
                                            void **stream);
 
+/* --------------------------------------- layer norm, gated feed-forward (no counterparts in the reference) */
+
+/* output = gamma (input - mean) / sqrt(variance + eps) + beta over the last axis of an input of any rank; gamma and
+ * beta hold one value for each of its columns.  `output` may be `input`.  Takes no scratch. */
+int DLGpuLayerNormalizationForward(const DLArrayHandle input, const DLArrayHandle gamma, const DLArrayHandle beta,
+                                   DLArrayHandle output, float eps, void **stream);
+/* Its gradients, those of dinput, dgamma and dbeta that are not NULL, from the forward pass's input: nothing is kept
+ * between the two.  dgamma or dbeta take scratch, and are refused on a stream that is being captured into a graph. */
+int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const DLArrayHandle gamma, const DLArrayHandle doutput,
+                                    DLArrayHandle dinput, DLArrayHandle dgamma, DLArrayHandle dbeta, float eps,
+                                    int *memorytoSaving, void **stream);
+
+/* g = input gate, u = input up, output = act(g) u, for input [M, K], gate and up [K, F], output [M, F]; pre [2, M, F]
+ * receives g and u, which the backward pass reads.  One of pre and output may be NULL.
+ * activation: sigmoid=0, relu=1, silu=2, gelu=3 (with erf).  Arrays of 2 GiB or more (a half of pre counts as one)
+ * are rejected.  The two backward calls and this one take scratch and are refused on a stream that is being captured
+ * into a graph.  Results must not overlap what they are computed from. */
+int DLGpuGatedFeedForward(const DLArrayHandle input, const DLArrayHandle gate, const DLArrayHandle up,
+                          DLArrayHandle pre, DLArrayHandle output, int activation, int *memorytoSaving, void **stream);
+/* With dg = doutput u act'(g), du = doutput act(g): dinput = dg gate^T + du up^T, dgate = input^T dg, dup = input^T du,
+ * those of them that are not NULL.  pre NULL: doutput is [2, M, F] and holds dg and du. */
+int DLGpuGatedFeedForwardBackward(const DLArrayHandle input, const DLArrayHandle gate, const DLArrayHandle up,
+                                  const DLArrayHandle pre, const DLArrayHandle doutput, DLArrayHandle dinput,
+                                  DLArrayHandle dgate, DLArrayHandle dup, int activation, int *memorytoSaving,
+                                  void **stream);
+/* The pointwise part alone: output = act(pre[0]) pre[1], and dpre = (dg, du).  dpre may be pre. */
+int DLGpuGatedActivation(const DLArrayHandle pre, DLArrayHandle output, int activation, void **stream);
+int DLGpuGatedActivationBackward(const DLArrayHandle pre, const DLArrayHandle doutput, DLArrayHandle dpre,
+                                 int activation, void **stream);
+
 /* ----------------------------------------------------- dropout, concatenation */
 
 /* Element-count descriptor that dropout takes in place of the reference's cuDNN
@@ -436,6 +466,14 @@ int DLGpuDropoutForward(const DLArrayHandle input, DLArrayHandle output, int dat
  * ref: c_runtime_api.h:445-449, gpu_op.cu:3647-3693 */
 int DLGpuDropoutBackward(const DLArrayHandle doutput, DLArrayHandle dinput, void **reserveSpace_p,
                          void ***cudnnlist, void **handle, void **stream);
+
+/* No counterpart in the reference: dropout whose mask is never stored.
+ * output[i] = (w_i >= floor(dropout * 2^32) ? input[i] / (1 - dropout) : 0) + residual[i], with w_i word i mod 4 of
+ * Philox4x32-10 at counter (i / 4, offset) and key `seed` (64 bits each; a seed below 2^31 at offset 0 has the mask of
+ * DLGpuDropoutForward).  `residual` may be NULL.  The gradient is the same call on doutput, without residual.
+ * `output` may be `input` or `residual` itself.  A dropped element is 0 whatever it held. */
+int DLGpuCounterDropout(const DLArrayHandle input, const DLArrayHandle residual, DLArrayHandle output, float dropout,
+                        uint64_t seed, uint64_t offset, void **stream);
 
 /* Concatenation of two tensors along axis 1 and the two slices that are its
  * gradients.  ref: c_runtime_api.h:226-228, gpu_op.cu:967-1084 */

@@ -14,6 +14,10 @@
 // mask is a pure function of (seed, element index, dropout), so any grid shape
 // reproduces it; cuDNN's own generator is not reproducible outside cuDNN.
 //
+// Counter dropout (no counterpart in the reference) has no mask at all: the backward pass draws the same words again.
+// Its counter is (i / 4, offset) and its key the seed, 64 bits each, so the masks of a seed below 2^31 at
+// offset 0 are those of the calls above.
+//
 // Concatenation along axis 1 replaces src/gpu_op.cu:967-1084.
 #include "gemm_core.h"
 #include "internal.h"
@@ -100,6 +104,53 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(const float *__restri
     reinterpret_cast<float4 *>(out + base)[1] = ob;
   } else {
     for (int j = 0; j < 8 && base + j < count; ++j) out[base + j] = ((bits >> j) & 1u) ? in[base + j] * scale : 0.f;
+  }
+}
+
+// out[i] = kept(i) ? in[i] * scale : 0, plus residual[i].  Blocks of four elements are dealt to lanes kBlocksPerLane
+// at a time, 64 blocks of a wave side by side.
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4u __attribute__((aligned(4)));
+constexpr int kBlocksPerLane = 4;
+template <bool RESIDUAL>
+__global__ __launch_bounds__(kThreads) void counter_dropout_kernel(const float *in, const float *residual, float *out,
+                                                                  int64_t count, uint64_t seed, uint64_t offset,
+                                                                  uint32_t threshold, float scale) {
+  const int64_t first = (int64_t)blockIdx.x * (kThreads * kBlocksPerLane) + threadIdx.x;
+  f32x4 v[kBlocksPerLane], r[kBlocksPerLane];
+#pragma unroll
+  for (int e = 0; e < kBlocksPerLane; ++e) {
+    const int64_t i = 4 * (first + e * kThreads);
+    if (i + 4 <= count) {
+      v[e] = *reinterpret_cast<const f32x4u *>(in + i);
+      if (RESIDUAL) r[e] = *reinterpret_cast<const f32x4u *>(residual + i);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[e][j] = i + j < count ? in[i + j] : 0.f;
+        r[e][j] = RESIDUAL && i + j < count ? residual[i + j] : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kBlocksPerLane; ++e) {
+    const int64_t block = first + e * kThreads, i = 4 * block;
+    const u32x4 w = philox4x32_10((uint32_t)block, (uint32_t)(block >> 32), (uint32_t)offset, (uint32_t)(offset >> 32),
+                                  (uint32_t)seed, (uint32_t)(seed >> 32));
+    const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+    f32x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[j] = word[j] >= threshold ? v[e][j] * scale : 0.f;
+      if (RESIDUAL) o[j] += r[e][j];
+    }
+    if (i + 4 <= count) {
+      *reinterpret_cast<f32x4u *>(out + i) = o;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < count) out[i + j] = o[j];
+    }
   }
 }
 
@@ -244,6 +295,29 @@ extern "C" int DLGpuDropoutBackward(const DLArrayHandle doutput, DLArrayHandle d
   free(*cudnnlist);
   *cudnnlist = nullptr;
   return finish(s, "DLGpuDropoutBackward");
+}
+
+extern "C" int DLGpuCounterDropout(const DLArrayHandle input, const DLArrayHandle residual, DLArrayHandle output,
+                                   float dropout, uint64_t seed, uint64_t offset, void **stream) {
+  TF_REQUIRE(on_gpu(input) && on_gpu(output) && (!residual || on_gpu(residual)), "arrays must live on the GPU");
+  TF_REQUIRE(same_shape(input, output) && (!residual || same_shape(input, residual)), "arrays must have one shape");
+  TF_REQUIRE(same_device({input, residual, output}), "arrays must live on one device");
+  for (const DLArray *read : {(const DLArray *)input, (const DLArray *)residual})
+    TF_REQUIRE(!overlaps(read, output) || read->data == output->data, "output must be an input or not overlap it");
+  TF_REQUIRE(dropout >= 0.f && dropout < 1.f, "dropout probability %g outside [0, 1)", (double)dropout);
+  announce_write(output);
+  hipStream_t s = stream_of(stream);
+  const int64_t count = numel(input), a_group = (int64_t)kThreads * kBlocksPerLane * 4;
+  const int64_t groups = (count + a_group - 1) / a_group;
+  TF_REQUIRE(groups <= 0x7fffffff, "too many elements");
+  if (count == 0) return 0;
+  // a float below 1 is at most 1 - 2^-24: the product is exact and below 2^32
+  const uint32_t threshold = (uint32_t)((double)dropout * 4294967296.0);
+  const float scale = 1.0f / (1.0f - dropout);
+  const float *x = (const float *)input->data, *r = residual ? (const float *)residual->data : nullptr;
+  hipLaunchKernelGGL(residual ? counter_dropout_kernel<true> : counter_dropout_kernel<false>, dim3((unsigned)groups),
+                     dim3(kThreads), 0, s, x, r, (float *)output->data, count, seed, offset, threshold, scale);
+  return finish(s, "DLGpuCounterDropout");
 }
 
 extern "C" int DLGpuConcatForward(const DLArrayHandle input1, const DLArrayHandle input2, DLArrayHandle output,

@@ -6,6 +6,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
+#include <initializer_list>
 
 #include "c_runtime_api.h"
 
@@ -33,6 +34,7 @@ void order_others_behind(hipStream_t s);    // what is launched from now on on a
 int host_waits_for_other_streams(hipStream_t s);  // the same before a launch on `s`, by waiting here
 bool other_streams_busy(hipStream_t s);     // whether there is any such thing
 bool idle(hipStream_t s);                   // nothing of what was enqueued on it is left to run
+bool being_captured(hipStream_t s);         // into a graph
 void feed_forget_stream(hipStream_t s);     // feed.hip: gives back what feeds on the stream keep (waits for it)
 bool feed_give_back(bool for_good);         // the device memory of all feeds; for good: they do without from then on
 bool sync_every_op();                    // TINYFLOW_SYNC_EVERY_OP=1
@@ -55,6 +57,20 @@ inline bool same_shape(const DLArray *a, const DLArray *b) {
   return true;
 }
 inline bool on_gpu(const DLArray *a) { return a && a->data && a->ctx.device_type == kGPU; }
+// Of the arrays that are not NULL: whether all are on one device, and whether two share a byte.
+inline bool same_device(std::initializer_list<const DLArray *> arrays) {
+  const DLArray *first = nullptr;
+  for (const DLArray *a : arrays) {
+    if (a && first && a->ctx.device_id != first->ctx.device_id) return false;
+    if (a && !first) first = a;
+  }
+  return true;
+}
+inline bool overlaps(const DLArray *a, const DLArray *b) {
+  if (!a || !b) return false;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a->data), pb = reinterpret_cast<uintptr_t>(b->data);
+  return pa < pb + (uintptr_t)numel(b) * sizeof(float) && pb < pa + (uintptr_t)numel(a) * sizeof(float);
+}
 
 inline int cdiv(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 

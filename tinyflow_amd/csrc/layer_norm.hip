@@ -1,0 +1,430 @@
+// Layer norm over the last axis, forward and backward (no counterpart in the reference, whose only norm is the batch
+// norm of bn.hip).
+//
+//   mu = mean(x), v = mean((x - mu)^2), s = 1 / sqrt(v + eps), xh = (x - mu) s
+//   y  = gamma xh + beta
+//   a  = gamma dy,  dx = s (a - mean(a) - xh mean(a xh)),  dgamma = sum over rows of dy xh,  dbeta = sum over rows of dy
+//
+// Nothing is kept between the two passes: the backward pass has the row of x in registers anyway and computes mu and s
+// again from there, which moves no byte, and neither pass depends on the other having run.
+//
+// Bound: HBM.  A row is read once into registers, by a wave or, from 1 024 / 2 048 columns on, by a workgroup, and both
+// statistics are taken from there, the squares after the mean is known (a sum of x^2 would cancel where the mean is
+// large).  Sums are divided by the column count, not multiplied by its reciprocal: a row of one value then has that value for
+// its mean.  All sums are fp32; their order depends on the shape alone.
+#include "internal.h"
+
+#include <algorithm>
+
+using namespace tf;
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4u __attribute__((aligned(4)));  // rows of any length start anywhere: 16-byte accesses on 4-byte alignment
+
+__device__ inline float wave_sum(float v) {
+#pragma unroll
+  for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+
+// Sum over the T lanes that share a row; `room` is T / 64 floats that nobody else uses until the next barrier but one.
+template <int T>
+__device__ inline float row_sum(float v, float *room) {
+  v = wave_sum(v);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.f;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) v += room[w];
+  }
+  return v;
+}
+
+// VPT vectors of a row in the registers of T lanes: vector e of lane l holds columns 4 (e T + l) and the three behind it;
+// columns past the row's end read as zero and are not written.
+template <int T, int VPT>
+struct Row {
+  f32x4 v[VPT];
+  __device__ inline void load(const float *__restrict__ row, int cols, int lane) {
+#pragma unroll
+    for (int e = 0; e < VPT; ++e) {
+      const int c = 4 * (e * T + lane);
+      v[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (c + 4 <= cols) {
+        v[e] = *reinterpret_cast<const f32x4u *>(row + c);
+      } else if (c < cols) {
+        v[e][0] = row[c];
+        if (c + 1 < cols) v[e][1] = row[c + 1];
+        if (c + 2 < cols) v[e][2] = row[c + 2];
+      }
+    }
+  }
+  __device__ inline void store(float *__restrict__ row, int cols, int lane) const {
+#pragma unroll
+    for (int e = 0; e < VPT; ++e) {
+      const int c = 4 * (e * T + lane);
+      if (c + 4 <= cols) {
+        *reinterpret_cast<f32x4u *>(row + c) = v[e];
+      } else if (c < cols) {
+        row[c] = v[e][0];
+        if (c + 1 < cols) row[c + 1] = v[e][1];
+        if (c + 2 < cols) row[c + 2] = v[e][2];
+      }
+    }
+  }
+  __device__ inline float sum() const {
+    f32x4 s = v[0];
+#pragma unroll
+    for (int e = 1; e < VPT; ++e) s += v[e];
+    return (s[0] + s[1]) + (s[2] + s[3]);
+  }
+  // v - m inside the row, zero past its end
+  __device__ inline void subtract(float m, int cols, int lane) {
+#pragma unroll
+    for (int e = 0; e < VPT; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[e][i] = 4 * (e * T + lane) + i < cols ? v[e][i] - m : 0.f;
+  }
+  __device__ inline float dot(const Row &o) const {
+    f32x4 s = v[0] * o.v[0];
+#pragma unroll
+    for (int e = 1; e < VPT; ++e) s += v[e] * o.v[e];
+    return (s[0] + s[1]) + (s[2] + s[3]);
+  }
+};
+
+__device__ inline float inverse_std(float square_sum, float n, float eps) {
+  return 1.f / sqrtf(square_sum / n + eps);
+}
+
+// T lanes a row, WG / T rows a workgroup.
+template <int T, int VPT>
+__global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
+                                                                  const float *__restrict__ beta, float *__restrict__ y,
+                                                                  int64_t rows, int cols, float n, float eps) {
+  constexpr int WG = T > 256 ? T : 256;
+  __shared__ float room[2][T / 64];
+  const int lane = threadIdx.x % T;
+  const int64_t r = (int64_t)blockIdx.x * (WG / T) + threadIdx.x / T;
+  if (r >= rows) return;  // whole waves, and no barrier where several rows share a workgroup
+  Row<T, VPT> row, g, b;
+  row.load(x + r * cols, cols, lane);
+  g.load(gamma, cols, lane);
+  b.load(beta, cols, lane);
+  row.subtract(row_sum<T>(row.sum(), room[0]) / n, cols, lane);
+  const float s = inverse_std(row_sum<T>(row.dot(row), room[1]), n, eps);
+#pragma unroll
+  for (int e = 0; e < VPT; ++e) row.v[e] = row.v[e] * s * g.v[e] + b.v[e];
+  row.store(y + r * cols, cols, lane);
+}
+
+// Rows that do not fit registers: three passes, the later two mostly out of the caches.
+constexpr int kLong = 1024;
+__global__ __launch_bounds__(kLong) void forward_long_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
+                                                            const float *__restrict__ beta, float *__restrict__ y,
+                                                            int cols, float n, float eps) {
+  __shared__ float room[2][kLong / 64];
+  const float *row = x + (int64_t)blockIdx.x * cols;
+  float s = 0.f;
+  for (int c = threadIdx.x; c < cols; c += kLong) s += row[c];
+  const float mean = row_sum<kLong>(s, room[0]) / n;
+  s = 0.f;
+  for (int c = threadIdx.x; c < cols; c += kLong) {
+    const float d = row[c] - mean;
+    s += d * d;
+  }
+  const float istd = inverse_std(row_sum<kLong>(s, room[1]), n, eps);
+  float *out = y + (int64_t)blockIdx.x * cols;
+  for (int c = threadIdx.x; c < cols; c += kLong) out[c] = (row[c] - mean) * istd * gamma[c] + beta[c];
+}
+
+// Rows blockIdx.x * (WG / T) + ..., then gridDim.x * (WG / T) further on, and so on: every lane keeps the sums of dy xh and
+// dy of its columns over the rows that it sees.  At the end the workgroup's rows are added through LDS, in their order, and
+// go to partial[blockIdx.x][2][cols].
+template <int T, int VPT, bool PARAMS>
+__global__ __launch_bounds__(T > 256 ? T : 256) void backward_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
+                                                                   const float *__restrict__ dy, float *__restrict__ dx,
+                                                                   float *__restrict__ partial, int64_t rows, int cols,
+                                                                   float n, float eps) {
+  constexpr int WG = T > 256 ? T : 256, ROWS = WG / T;
+  __shared__ float room[3][T / 64][2];
+  const int lane = threadIdx.x % T, sub = threadIdx.x / T;
+  Row<T, VPT> g, dgamma, dbeta;
+  if (dx) g.load(gamma, cols, lane);
+#pragma unroll
+  for (int e = 0; e < VPT; ++e) dgamma.v[e] = dbeta.v[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int64_t r = (int64_t)blockIdx.x * ROWS + sub; r < rows; r += (int64_t)gridDim.x * ROWS) {
+    Row<T, VPT> xh, d;
+    xh.load(x + r * cols, cols, lane);
+    d.load(dy + r * cols, cols, lane);
+    xh.subtract(row_sum<T>(xh.sum(), &room[0][0][0]) / n, cols, lane);
+    const float s = inverse_std(row_sum<T>(xh.dot(xh), &room[1][0][0]), n, eps);
+#pragma unroll
+    for (int e = 0; e < VPT; ++e) xh.v[e] *= s;
+    if (PARAMS) {
+#pragma unroll
+      for (int e = 0; e < VPT; ++e) {
+        dgamma.v[e] += d.v[e] * xh.v[e];
+        dbeta.v[e] += d.v[e];
+      }
+    }
+    if (dx) {
+#pragma unroll
+      for (int e = 0; e < VPT; ++e) d.v[e] *= g.v[e];
+      float a = wave_sum(d.sum()), b = wave_sum(d.dot(xh));
+      if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) {
+          room[2][threadIdx.x >> 6][0] = a;
+          room[2][threadIdx.x >> 6][1] = b;
+        }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) {
+          a += room[2][w][0];
+          b += room[2][w][1];
+        }
+      }
+      a /= n;
+      b /= n;
+#pragma unroll
+      for (int e = 0; e < VPT; ++e) d.v[e] = (d.v[e] - a - xh.v[e] * b) * s;
+      d.store(dx + r * cols, cols, lane);
+    }
+  }
+  if constexpr (PARAMS) {
+    if constexpr (ROWS > 1) {
+      __shared__ f32x4 sums[ROWS - 1][VPT][T];
+      for (int half = 0; half < 2; ++half) {
+        Row<T, VPT> &mine = half ? dbeta : dgamma;
+        if (half) __syncthreads();
+        if (sub > 0) {
+#pragma unroll
+          for (int e = 0; e < VPT; ++e) sums[sub - 1][e][lane] = mine.v[e];
+        }
+        __syncthreads();
+        if (sub == 0) {
+#pragma unroll
+          for (int w = 0; w < ROWS - 1; ++w)
+#pragma unroll
+            for (int e = 0; e < VPT; ++e) mine.v[e] += sums[w][e][lane];
+        }
+      }
+      if (sub > 0) return;
+    }
+    float *out = partial + (int64_t)blockIdx.x * 2 * cols;
+    dgamma.store(out, cols, lane);
+    dbeta.store(out + cols, cols, lane);
+  }
+}
+
+// Long rows: the statistics go to `stats`, for the sums over rows that follow.
+__global__ __launch_bounds__(kLong) void backward_long_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
+                                                             const float *__restrict__ dy, float *__restrict__ dx,
+                                                             float *__restrict__ stats, int cols, float n, float eps) {
+  __shared__ float room[4][kLong / 64];
+  const int64_t base = (int64_t)blockIdx.x * cols;
+  const float *row = x + base, *d = dy + base;
+  float s = 0.f;
+  for (int c = threadIdx.x; c < cols; c += kLong) s += row[c];
+  const float mean = row_sum<kLong>(s, room[0]) / n;
+  s = 0.f;
+  for (int c = threadIdx.x; c < cols; c += kLong) s += (row[c] - mean) * (row[c] - mean);
+  const float istd = inverse_std(row_sum<kLong>(s, room[1]), n, eps);
+  if (stats && threadIdx.x == 0) {
+    stats[2 * (int64_t)blockIdx.x] = mean;
+    stats[2 * (int64_t)blockIdx.x + 1] = istd;
+  }
+  if (!dx) return;
+  float a = 0.f, b = 0.f;
+  for (int c = threadIdx.x; c < cols; c += kLong) {
+    const float t = d[c] * gamma[c];
+    a += t;
+    b += t * ((row[c] - mean) * istd);
+  }
+  a = row_sum<kLong>(a, room[2]) / n;
+  b = row_sum<kLong>(b, room[3]) / n;
+  for (int c = threadIdx.x; c < cols; c += kLong)
+    dx[base + c] = (d[c] * gamma[c] - a - (row[c] - mean) * istd * b) * istd;
+}
+
+// 64 columns and a run of rows a workgroup; partial as above.
+__global__ __launch_bounds__(256) void column_sums_kernel(const float *__restrict__ x, const float *__restrict__ dy,
+                                                         const float *__restrict__ stats, float *__restrict__ partial,
+                                                         int64_t rows, int cols) {
+  __shared__ float sums[2][3][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+  float dgamma = 0.f, dbeta = 0.f;
+  if (c < cols)
+    for (int64_t r = (int64_t)blockIdx.y * 4 + wave; r < rows; r += (int64_t)gridDim.y * 4) {
+      const float d = dy[r * cols + c];
+      dgamma += d * ((x[r * cols + c] - stats[2 * r]) * stats[2 * r + 1]);
+      dbeta += d;
+    }
+  if (wave > 0) {
+    sums[0][wave - 1][lane] = dgamma;
+    sums[1][wave - 1][lane] = dbeta;
+  }
+  __syncthreads();
+  if (wave > 0 || c >= cols) return;
+  for (int w = 0; w < 3; ++w) {
+    dgamma += sums[0][w][lane];
+    dbeta += sums[1][w][lane];
+  }
+  float *out = partial + (int64_t)blockIdx.y * 2 * cols;
+  out[c] = dgamma;
+  out[cols + c] = dbeta;
+}
+
+// dgamma and dbeta from `pieces` partial sums: 16 lanes a column pair of lines of 64 columns, each every sixteenth piece, added up
+// in their order.  No pieces (no rows): zeros.
+__global__ __launch_bounds__(1024) void sum_pieces_kernel(const float *__restrict__ partial, float *__restrict__ dgamma,
+                                                         float *__restrict__ dbeta, int pieces, int cols) {
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 64 + lane, width = 2 * (int64_t)cols;
+  float s = 0.f;
+  if (c < width) {
+    int p = wave;
+    for (; p + 48 < pieces; p += 64) {
+      const float a = partial[p * width + c], b = partial[(p + 16) * width + c];
+      const float d = partial[(p + 32) * width + c], e = partial[(p + 48) * width + c];
+      s += (a + b) + (d + e);
+    }
+    for (; p < pieces; p += 16) s += partial[p * width + c];
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave > 0 || c >= width) return;
+  for (int w = 1; w < 16; ++w) s += sums[w][lane];
+  float *out = c < cols ? dgamma : dbeta;
+  if (out) out[c < cols ? c : c - cols] = s;
+}
+
+// x [rows, cols] as the last axis makes it, or an error
+int geometry(const char *what, const DLArray *x, const DLArray *gamma, int64_t &rows, int64_t &cols) {
+  if (!on_gpu(x) || !on_gpu(gamma)) {
+    fprintf(stderr, "[tinyflow_amd] %s: arrays must live on the GPU\n", what);
+    return -1;
+  }
+  if (x->ndim < 1 || gamma->ndim != 1 || gamma->shape[0] != x->shape[x->ndim - 1] || gamma->shape[0] > 0x3fffffff) {
+    fprintf(stderr, "[tinyflow_amd] %s: gamma must hold one value for each column of the last axis (fewer than 2^30)\n", what);
+    return -1;
+  }
+  cols = gamma->shape[0];
+  rows = cols ? numel(x) / cols : 0;
+  if (rows > 0x7fffffff) {
+    fprintf(stderr, "[tinyflow_amd] %s: 2^31 rows or more are not supported\n", what);
+    return -1;
+  }
+  return 0;
+}
+
+constexpr int kMaxForward = 16384, kMaxBackward = 16384;  // columns that registers hold
+
+}  // namespace
+
+extern "C" int DLGpuLayerNormalizationForward(const DLArrayHandle input, const DLArrayHandle gamma,
+                                              const DLArrayHandle beta, DLArrayHandle output, float eps, void **stream) {
+  int64_t rows, cols;
+  if (geometry(__func__, input, gamma, rows, cols) != 0) return -1;
+  TF_REQUIRE(on_gpu(beta) && on_gpu(output), "arrays must live on the GPU");
+  TF_REQUIRE(same_shape(beta, gamma), "beta must have gamma's shape");
+  TF_REQUIRE(same_shape(input, output), "output must have the input's shape");
+  TF_REQUIRE(same_device({input, gamma, beta, output}), "arrays must live on one device");
+  TF_REQUIRE(!overlaps(output, gamma) && !overlaps(output, beta), "output must not overlap gamma or beta");
+  TF_REQUIRE(input->data == output->data || !overlaps(input, output), "output must be the input or not overlap it");
+  TF_REQUIRE(eps >= 0.f, "eps must not be negative");
+  announce_write(output);
+  hipStream_t s = stream_of(stream);
+  if (rows == 0 || cols == 0) return 0;
+  const float *x = (const float *)input->data, *g = (const float *)gamma->data, *b = (const float *)beta->data;
+  float *y = (float *)output->data;
+  const float n = (float)cols;
+  auto go = [&](auto kernel, int wg, int rows_a_group) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + rows_a_group - 1) / rows_a_group)), dim3(wg), 0, s, x, g, b, y, rows,
+                       (int)cols, n, eps);
+  };
+  if (cols <= 256) go(forward_kernel<64, 1>, 256, 4);
+  else if (cols <= 512) go(forward_kernel<64, 2>, 256, 4);
+  else if (cols <= 1024) go(forward_kernel<64, 4>, 256, 4);
+  else if (cols <= 2048) go(forward_kernel<256, 2>, 256, 1);
+  else if (cols <= 4096) go(forward_kernel<256, 4>, 256, 1);
+  else if (cols <= 8192) go(forward_kernel<1024, 2>, 1024, 1);
+  else if (cols <= kMaxForward) go(forward_kernel<1024, 4>, 1024, 1);
+  else
+    hipLaunchKernelGGL(forward_long_kernel, dim3((unsigned)rows), dim3(kLong), 0, s, x, g, b, y, (int)cols, n, eps);
+  return finish(s, "DLGpuLayerNormalizationForward");
+}
+
+extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const DLArrayHandle gamma,
+                                               const DLArrayHandle doutput, DLArrayHandle dinput, DLArrayHandle dgamma,
+                                               DLArrayHandle dbeta, float eps, int *memorytoSaving, void **stream) {
+  int64_t rows, cols;
+  if (geometry(__func__, input, gamma, rows, cols) != 0) return -1;
+  TF_REQUIRE(on_gpu(doutput) && same_shape(input, doutput), "doutput must live on the GPU and have the input's shape");
+  TF_REQUIRE(dinput || dgamma || dbeta, "no gradient is asked for");
+  TF_REQUIRE(!dinput || (on_gpu(dinput) && same_shape(input, dinput)), "dinput must live on the GPU and have the input's shape");
+  TF_REQUIRE(!dgamma || (on_gpu(dgamma) && same_shape(gamma, dgamma)), "dgamma must live on the GPU and have gamma's shape");
+  TF_REQUIRE(!dbeta || (on_gpu(dbeta) && same_shape(gamma, dbeta)), "dbeta must live on the GPU and have gamma's shape");
+  TF_REQUIRE(same_device({input, gamma, doutput, dinput, dgamma, dbeta}), "arrays must live on one device");
+  for (const DLArray *read : {(const DLArray *)input, (const DLArray *)gamma, (const DLArray *)doutput})
+    for (const DLArray *written : {(const DLArray *)dinput, (const DLArray *)dgamma, (const DLArray *)dbeta})
+      TF_REQUIRE(!overlaps(read, written), "gradients must not overlap what they are computed from");
+  TF_REQUIRE(!overlaps(dinput, dgamma) && !overlaps(dinput, dbeta) && !overlaps(dgamma, dbeta), "gradients must not overlap");
+  TF_REQUIRE(eps >= 0.f, "eps must not be negative");
+  for (const DLArray *written : {(const DLArray *)dinput, (const DLArray *)dgamma, (const DLArray *)dbeta}) announce_write(written);
+  hipStream_t s = stream_of(stream);
+  if (cols == 0) return 0;
+  const bool params = dgamma || dbeta, in_registers = cols <= kMaxBackward;
+  TF_REQUIRE(!params || !being_captured(s), "the gradients of the weights take scratch, which a captured stream cannot give back");
+
+  // How many workgroups share the rows, each with a partial sum of the weights' gradients.
+  const int rows_a_group = in_registers && cols <= 1024 ? 4 : 1;
+  const int64_t groups = (rows + rows_a_group - 1) / rows_a_group;
+  int pieces = 0;
+  if (in_registers) pieces = (int)std::min<int64_t>(groups, params ? 2 * num_cus() : 0x7fffffff);
+  else if (rows) pieces = (int)std::min<int64_t>((rows + 3) / 4, std::max<int64_t>(1, 4 * num_cus() * 64 / cols));
+  float *partial = nullptr, *stats = nullptr;
+  if (params && rows) {
+    const size_t partial_bytes = (size_t)pieces * 2 * cols * 4, stats_bytes = in_registers ? 0 : (size_t)rows * 8;
+    partial = (float *)device_alloc(partial_bytes + stats_bytes, s);
+    if (!partial) {
+      if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(partial_bytes + stats_bytes));
+      return 0;
+    }
+    if (stats_bytes) stats = partial + (size_t)pieces * 2 * cols;
+  }
+  const float *x = (const float *)input->data, *g = (const float *)gamma->data, *dy = (const float *)doutput->data;
+  float *dx = dinput ? (float *)dinput->data : nullptr;
+  const float n = (float)cols;
+  if (rows) {
+    auto go = [&](auto with, auto without, int wg) {
+      hipLaunchKernelGGL(params ? with : without, dim3((unsigned)pieces), dim3(wg), 0, s, x, g, dy, dx, partial, rows,
+                         (int)cols, n, eps);
+    };
+    if (cols <= 256) go(backward_kernel<64, 1, true>, backward_kernel<64, 1, false>, 256);
+    else if (cols <= 512) go(backward_kernel<64, 2, true>, backward_kernel<64, 2, false>, 256);
+    else if (cols <= 1024) go(backward_kernel<64, 4, true>, backward_kernel<64, 4, false>, 256);
+    else if (cols <= 2048) go(backward_kernel<256, 2, true>, backward_kernel<256, 2, false>, 256);
+    else if (cols <= 4096) go(backward_kernel<256, 4, true>, backward_kernel<256, 4, false>, 256);
+    else if (cols <= 8192) go(backward_kernel<1024, 2, true>, backward_kernel<1024, 2, false>, 1024);
+    else if (in_registers) go(backward_kernel<1024, 4, true>, backward_kernel<1024, 4, false>, 1024);
+    else {
+      hipLaunchKernelGGL(backward_long_kernel, dim3((unsigned)rows), dim3(kLong), 0, s, x, g, dy, dx, stats, (int)cols, n, eps);
+      if (params)
+        hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 63) / 64), (unsigned)pieces), dim3(256), 0, s, x, dy,
+                           stats, partial, rows, (int)cols);
+    }
+  }
+  if (params)
+    hipLaunchKernelGGL(sum_pieces_kernel, dim3((unsigned)((2 * cols + 63) / 64)), dim3(1024), 0, s, partial,
+                       dgamma ? (float *)dgamma->data : nullptr, dbeta ? (float *)dbeta->data : nullptr, rows ? pieces : 0,
+                       (int)cols);
+  if (partial) device_free(partial, s);
+  return finish(s, "DLGpuLayerNormalizationBackward");
+}

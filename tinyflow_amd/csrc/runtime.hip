@@ -371,6 +371,8 @@ static bool capturing(hipStream_t s) {
   return status != hipStreamCaptureStatusNone;
 }
 
+bool being_captured(hipStream_t s) { return capturing(s); }
+
 // `s` behind all that is enqueued on `other`; false when that cannot be had.  With the lock held.
 static bool wait_for_stream(StreamRec &other, hipStream_t s) {
   if (other.stream == s || !other.runs_kernels || capturing(s) || capturing(other.stream) || idle(other.stream)) return true;

@@ -18,6 +18,7 @@ _PADDING = {"SAME": 1, "VALID": 0}              # reference gpu_op.py:443-448
 _POOLING = {"max": 0, "mean": 1}                # reference gpu_op.py:610-615
 _ACTIVATION = {"sigmoid": 0, "relu": 1, "tanh": 2, "softmax": 3}  # gpu_op.py:501-510
 _BATCHNORM = {"pre_activation": 0, "spatial": 1}                  # gpu_op.py:778-783
+_GATE = {"sigmoid": 0, "relu": 1, "silu": 2, "gelu": 3}           # no counterpart in the reference
 
 
 def _enum(table, key):
@@ -37,6 +38,11 @@ def _cell(depth):
 def _nd_args(*arrays):
     for a in arrays:
         assert isinstance(a, _nd.NDArray)
+
+
+def _handle(array):
+    """Of an array that may be None."""
+    return None if array is None else array.handle
 
 
 # ------------------------------------------------------------ streams / handles
@@ -444,6 +450,58 @@ def bn_and_relu_backward(input, bn_output, relu_output, doutput, drelu, dinput, 
     return wanted.value
 
 
+# ------------------------------- layer norm, gated feed-forward (no counterparts in the reference)
+
+def layer_norm_forward(input, gamma, beta, output, eps, cudaStream):
+    """output = gamma * (input - mean) / sqrt(variance + eps) + beta over the last axis"""
+    _nd_args(input, gamma, beta, output)
+    check_call(_LIB.DLGpuLayerNormalizationForward(input.handle, gamma.handle, beta.handle, output.handle,
+                                                   ctypes.c_float(eps), cudaStream))
+
+
+def layer_norm_backward(input, gamma, doutput, dinput, dgamma, dbeta, eps, cudaStream):
+    """Those of the three gradients that are not None, from the forward pass's input."""
+    _nd_args(input, gamma, doutput, *[a for a in (dinput, dgamma, dbeta) if a is not None])
+    wanted = ctypes.c_int(0)
+    check_call(_LIB.DLGpuLayerNormalizationBackward(input.handle, gamma.handle, doutput.handle, _handle(dinput),
+                                                    _handle(dgamma), _handle(dbeta), ctypes.c_float(eps),
+                                                    ctypes.byref(wanted), cudaStream))
+    return wanted.value
+
+
+def gated_feed_forward(input, gate, up, pre, output, activation, cudaStream):
+    """output = activation(input gate) * (input up); ``pre`` receives the two projections, stacked.  One of the two may be
+    None: a pass that is never differentiated needs no ``pre``."""
+    _nd_args(input, gate, up, *[a for a in (pre, output) if a is not None])
+    wanted = ctypes.c_int(0)
+    check_call(_LIB.DLGpuGatedFeedForward(input.handle, gate.handle, up.handle, _handle(pre), _handle(output),
+                                          _enum(_GATE, activation), ctypes.byref(wanted), cudaStream))
+    return wanted.value
+
+
+def gated_feed_forward_backward(input, gate, up, pre, doutput, dinput, dgate, dup, activation, cudaStream):
+    """Those of the three gradients that are not None.  ``pre`` None: ``doutput`` is the gradient of the stacked projections."""
+    _nd_args(input, gate, up, doutput, *[a for a in (pre, dinput, dgate, dup) if a is not None])
+    wanted = ctypes.c_int(0)
+    check_call(_LIB.DLGpuGatedFeedForwardBackward(input.handle, gate.handle, up.handle, _handle(pre), doutput.handle,
+                                                  _handle(dinput), _handle(dgate), _handle(dup),
+                                                  _enum(_GATE, activation), ctypes.byref(wanted), cudaStream))
+    return wanted.value
+
+
+def gated_activation(pre, output, activation, cudaStream):
+    """output = activation(pre[0]) * pre[1]"""
+    _nd_args(pre, output)
+    check_call(_LIB.DLGpuGatedActivation(pre.handle, output.handle, _enum(_GATE, activation), cudaStream))
+
+
+def gated_activation_backward(pre, doutput, dpre, activation, cudaStream):
+    """The gradient of ``gated_activation`` with respect to ``pre``."""
+    _nd_args(pre, doutput, dpre)
+    check_call(_LIB.DLGpuGatedActivationBackward(pre.handle, doutput.handle, dpre.handle, _enum(_GATE, activation),
+                                                 cudaStream))
+
+
 # ------------------------------------------------------------------- optimizers
 
 def sgd_update(output, g, learning_rate, cudaStream):
@@ -585,6 +643,16 @@ def dropout_backward(doutput, dinput, reserveSpace_p, cudnnlist, cudnnHandle, cu
     _nd_args(doutput, dinput)
     check_call(_LIB.DLGpuDropoutBackward(doutput.handle, dinput.handle, reserveSpace_p, cudnnlist,
                                          cudnnHandle, cudaStream))
+
+
+def counter_dropout(input, residual, output, dropout, seed, offset, cudaStream):
+    """output = dropout(input) + residual with a mask that is a function of (seed, offset, index) and never stored;
+    ``residual`` may be None.  The gradient is the same call on it, without residual (no counterpart in the reference)."""
+    _nd_args(input, output, *([] if residual is None else [residual]))
+    for word in (seed, offset):
+        assert 0 <= word < 2 ** 64, "seed and offset are 64-bit words"
+    check_call(_LIB.DLGpuCounterDropout(input.handle, _handle(residual), output.handle, ctypes.c_float(dropout),
+                                        ctypes.c_uint64(seed), ctypes.c_uint64(offset), cudaStream))
 
 
 def concat_forward(in_arr_a, in_arr_b, out_arr, cudaStream):
