@@ -2,6 +2,17 @@
 //
 //   g = x Wg, u = x Wu, h = act(g) u        x [M, K], Wg and Wu [K, F]
 //   dg = dh u act'(g), du = dh act(g);  dx = dg Wg^T + du Wu^T,  dWg = x^T dg,  dWu = x^T du
+//
+// Large products run on fp16 pairs (gemm_pair.h), in three launches a pass:
+//
+//   maxima   the largest magnitude of every row (and column) of the operands, by runs of them
+//   split    every operand into its two fp16 numbers, in the order in which the products fetch them.  The gradients dg and du are
+//            computed from g, u and dh on the way, in both launches, and never stored; they are split twice, by rows for dx and
+//            by columns for dWg and dWu, because every sum needs a scale of its own for each of its operands
+//   product  forward: the two weights' columns alternate in blocks of 32, so that a lane holds g and u of the same element and
+//            the activation and the product of the two are the epilogue.  dx is one product over dg and du one behind the other, dWg
+//            and dWu one launch of two halves.
+#include "gemm_pair.h"
 #include "internal.h"
 
 #include <algorithm>
@@ -95,6 +106,472 @@ __global__ __launch_bounds__(kThreads) void activation_backward_kernel(const flo
       du[j] = d * act;
     }
   }
+}
+
+// ---- operands of the large products ----------------------------------------------------------------------
+using namespace tf::gemm;
+
+// One or two matrices of one shape: weights, or the gradients of the projections, given or to be computed (dh).
+struct Source {
+  const float *p[2];
+  const float *dh;   // not NULL: p are g and u, and the matrices are their gradients
+  int rows, cols, activation;
+
+  __device__ inline void gradients(float g, float u, float d, float &dg, float &du) const {
+    float act, slope;
+    switch (activation) {
+      case kSigmoid: act_and_slope<kSigmoid>(g, act, slope); break;
+      case kRelu: act_and_slope<kRelu>(g, act, slope); break;
+      case kSilu: act_and_slope<kSilu>(g, act, slope); break;
+      default: act_and_slope<kGelu>(g, act, slope); break;
+    }
+    dg = d * u * slope;
+    du = d * act;
+  }
+  __device__ inline float at(int which, int r, int c) const {
+    if (r >= rows || c >= cols) return 0.f;
+    const size_t i = (size_t)r * cols + c;
+    if (!dh) return p[which][i];
+    float v[2];
+    gradients(p[0][i], p[1][i], dh[i], v[0], v[1]);
+    return v[which];
+  }
+  // four columns from c on of both matrices; zeros past the end
+  __device__ inline void four(int r, int c, f32x4 (&v)[2]) const {
+    v[0] = v[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (r >= rows || c >= cols) return;
+    const size_t i = (size_t)r * cols + c;
+    f32x4 d = v[0];
+    if (c + 4 <= cols) {
+      v[0] = *reinterpret_cast<const f32x4u *>(p[0] + i);
+      if (p[1]) v[1] = *reinterpret_cast<const f32x4u *>(p[1] + i);
+      if (dh) d = *reinterpret_cast<const f32x4u *>(dh + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (c + e < cols) {
+          v[0][e] = p[0][i + e];
+          if (p[1]) v[1][e] = p[1][i + e];
+          if (dh) d[e] = dh[i + e];
+        }
+    }
+    if (dh)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float dg, du;
+        gradients(v[0][e], v[1][e], d[e], dg, du);
+        v[0][e] = dg;
+        v[1][e] = du;
+      }
+  }
+};
+
+// What is made of a source.  By rows: both matrices behind each other along the reduction, `half_steps` steps each, a row's
+// exponent common to both.  By columns: matrix w's block of 32 columns b is block b * col_mul + w * col_add.
+// Maxima: [matrix][run of columns][row], [matrix][run of rows][column]; by rows the matrices' are one.
+struct Job {
+  Source src;
+  int matrices;
+  char *row_planes, *col_planes;  // NULL: not wanted
+  int *row_exps, *col_exps;
+  uint32_t *row_max, *col_max;
+  int half_steps, col_steps, col_mul, col_add;
+  bool col_wanted[2];
+  int first_max, first_split;     // the job's first workgroup of each launch
+};
+struct Jobs {
+  Job job[3];
+  int n;
+};
+
+constexpr int kMaxRows = 128, kMaxCols = 256;  // a workgroup's part of the maxima
+constexpr int kSplitTile = 64;                 // rows and columns of a workgroup's part of the split
+
+__device__ inline uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+// Bit patterns of magnitudes are in the order of the magnitudes, infinities and NaN above all.
+__global__ __launch_bounds__(kThreads) void maxima_kernel(const Jobs jobs) {
+  int n = jobs.n - 1;
+  while (n > 0 && (int)blockIdx.x < jobs.job[n].first_max) --n;
+  const Job &job = jobs.job[n];
+  const int rows = job.src.rows, cols = job.src.cols, runs_c = (cols + kMaxCols - 1) / kMaxCols;
+  const int run_c = ((int)blockIdx.x - job.first_max) % runs_c, run_r = ((int)blockIdx.x - job.first_max) / runs_c;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = run_c * kMaxCols + 4 * lane;
+  __shared__ uint32_t of_waves[2][4][kMaxCols];
+  uint32_t col[2][4] = {};
+#pragma unroll 4
+  for (int e = 0; e < kMaxRows / 4; ++e) {
+    const int r = run_r * kMaxRows + 4 * e + wave;
+    f32x4 v[2];
+    job.src.four(r, c, v);
+    uint32_t row = 0;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t m = magnitude(v[w][i]);
+        col[w][i] = max(col[w][i], m);
+        row = max(row, m);
+      }
+    if (job.row_planes) {
+#pragma unroll
+      for (int m = 32; m > 0; m >>= 1) row = max(row, (uint32_t)__shfl_xor((int)row, m, 64));
+      if (lane == 0 && r < rows) job.row_max[(size_t)run_c * rows + r] = row;
+    }
+  }
+  if (!job.col_planes) return;
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) of_waves[w][wave][4 * lane + i] = col[w][i];
+  __syncthreads();
+  const int runs_r = (rows + kMaxRows - 1) / kMaxRows, at = run_c * kMaxCols + (int)threadIdx.x;
+  if (at >= cols) return;
+  for (int w = 0; w < job.matrices; ++w)
+    job.col_max[((size_t)w * runs_r + run_r) * cols + at] =
+        max(max(of_waves[w][0][threadIdx.x], of_waves[w][1][threadIdx.x]), max(of_waves[w][2][threadIdx.x], of_waves[w][3][threadIdx.x]));
+}
+
+// The power of two that brings the largest magnitude into [2^14, 2^15)
+__device__ inline int exponent_of(uint32_t largest) {
+  if (largest >= 0x7f800000u) return pair::kNotFinite;
+  return largest == 0 ? 0 : 15 - __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, largest));
+}
+
+// Eight elements to the two halves of a lane's place in a fragment pair.
+__device__ inline void split_eight(const float (&x)[8], int exponent, char *at) {
+  pair::f16x8 h, l;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float v = __builtin_ldexpf(x[i], exponent);
+    h[i] = (_Float16)v;
+    l[i] = (_Float16)(v - (float)h[i]);
+  }
+  *reinterpret_cast<pair::f16x8 *>(at) = h;
+  *reinterpret_cast<pair::f16x8 *>(at + pair::kFragment) = l;
+}
+
+__global__ __launch_bounds__(kThreads) void split_kernel(const Jobs jobs) {
+  constexpr int T = kSplitTile, LD = T + 4;
+  int n = jobs.n - 1;
+  while (n > 0 && (int)blockIdx.x < jobs.job[n].first_split) --n;
+  const Job &job = jobs.job[n];
+  const int rows = job.src.rows, cols = job.src.cols, tiles_c = (cols + T - 1) / T;
+  const int r0 = ((int)blockIdx.x - job.first_split) / tiles_c * T, c0 = ((int)blockIdx.x - job.first_split) % tiles_c * T;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __align__(16) float tile[2][T][LD];
+  __shared__ int row_exp[T], col_exp[2][T];
+
+  // the tile, 16 lanes a row
+#pragma unroll
+  for (int e = 0; e < T / 16; ++e) {
+    const int r = e * 16 + tid / 16, c = tid % 16 * 4;
+    f32x4 v[2];
+    job.src.four(r0 + r, c0 + c, v);
+    *reinterpret_cast<f32x4 *>(&tile[0][r][c]) = v[0];
+    if (job.matrices > 1) *reinterpret_cast<f32x4 *>(&tile[1][r][c]) = v[1];
+  }
+  // the exponents, four lanes each; the tiles at the reduction's beginning write them down
+  const int of = tid / 4, part = tid % 4;
+  auto largest = [&](const uint32_t *from, int runs, int64_t stride) {
+    uint32_t m = 0;
+    for (int i = part; i < runs; i += 4) m = max(m, from[i * stride]);
+    m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
+    return max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
+  };
+  if (job.row_planes) {
+    const int r = r0 + of;
+    const int e = exponent_of(largest(job.row_max + min(r, rows - 1), (cols + kMaxCols - 1) / kMaxCols, rows));
+    if (part == 0) {
+      row_exp[of] = e == pair::kNotFinite ? 0 : e;
+      if (c0 == 0 && r < (rows + 31) / 32 * 32) job.row_exps[r] = r < rows ? e : 0;
+    }
+  }
+  if (job.col_planes) {
+    const int runs = (rows + kMaxRows - 1) / kMaxRows, c = c0 + of;
+    for (int w = 0; w < job.matrices; ++w) {
+      if (!job.col_wanted[w]) continue;
+      const int e = exponent_of(largest(job.col_max + (size_t)w * runs * cols + min(c, cols - 1), runs, cols));
+      if (part == 0) {
+        col_exp[w][of] = e == pair::kNotFinite ? 0 : e;
+        if (r0 == 0 && c < (cols + 31) / 32 * 32) job.col_exps[(c / 32 * job.col_mul + w * job.col_add) * 32 + c % 32] = c < cols ? e : 0;
+      }
+    }
+  }
+  __syncthreads();
+  const int along = lane & 31, eight = lane >> 5 << 3;  // a lane's row and its elements in a fragment
+  for (int w = 0; w < job.matrices; ++w)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int b = (wave + 4 * i) >> 2, step = wave & 3;
+      float x[8];
+      if (job.row_planes && r0 / 32 + b < (rows + 31) / 32 && c0 / 16 + step < job.half_steps) {
+        const float *from = &tile[w][b * 32 + along][step * 16 + eight];
+#pragma unroll
+        for (int k = 0; k < 8; k += 4) {
+          const f32x4 v = *reinterpret_cast<const f32x4 *>(from + k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[k + j] = v[j];
+        }
+        const size_t at = (size_t)(r0 / 32 + b) * (job.matrices * job.half_steps) + w * job.half_steps + c0 / 16 + step;
+        split_eight(x, row_exp[b * 32 + along], job.row_planes + at * pair::kStepBytes + lane * 16);
+      }
+      if (job.col_planes && job.col_wanted[w] && c0 / 32 + b < (cols + 31) / 32 && r0 / 16 + step < job.col_steps) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = tile[w][step * 16 + eight + k][b * 32 + along];
+        const size_t at = (size_t)((c0 / 32 + b) * job.col_mul + w * job.col_add) * job.col_steps + r0 / 16 + step;
+        split_eight(x, col_exp[w][b * 32 + along], job.col_planes + at * pair::kStepBytes + lane * 16);
+      }
+    }
+}
+
+// ---- the products' ends ------------------------------------------------------------------------------------
+// Stores past the last row fall behind the buffer, those past the last column are sent there.
+struct Rows {
+  __amdgpu_buffer_rsrc_t rsrc;
+  __device__ inline Rows(float *out, int m0, int rows, int cols)
+      : rsrc(make_rsrc(out ? out + (size_t)m0 * cols : nullptr, out ? (uint32_t)min(rows - m0, pair::BM) * (uint32_t)cols * 4u : 0u)) {}
+};
+
+// h = act(g) u from the two columns that a lane holds, and g and u themselves where pre is wanted
+template <int ACT>
+struct StoreGated {
+  float *g, *u, *h;  // NULL: not wanted
+  int rows, cols;
+  struct State {
+    Rows g, u, h;
+  };
+  __device__ inline State begin(int m0, int) const { return {Rows(g, m0, rows, cols), Rows(u, m0, rows, cols), Rows(h, m0, rows, cols)}; }
+  template <int TN>
+  __device__ inline void store(const State &s, int m, int block, int lcol, const float (&v)[TN]) const {
+#pragma unroll
+    for (int j = 0; j < TN; j += 2) {
+      const int f = (block + j) / 2 * 32 + lcol;
+      const uint32_t off = f < cols ? ((uint32_t)m * (uint32_t)cols + (uint32_t)f) * 4u : OOB;
+      if (g) {  // uniform
+        buf_store(s.g.rsrc, off, v[j]);
+        buf_store(s.u.rsrc, off, v[j + 1]);
+      }
+      if (h) buf_store(s.h.rsrc, off, act_of<ACT>(v[j]) * v[j + 1]);
+    }
+  }
+};
+struct StoreHalves {
+  float *out[2];
+  int rows, cols;
+  using State = Rows;
+  __device__ inline State begin(int m0, int half) const { return Rows(half ? out[1] : out[0], m0, rows, cols); }
+  template <int TN>
+  __device__ inline void store(const State &s, int m, int block, int lcol, const float (&v)[TN]) const {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int n = (block + j) * 32 + lcol;
+      buf_store(s.rsrc, n < cols ? ((uint32_t)m * (uint32_t)cols + (uint32_t)n) * 4u : OOB, v[j]);
+    }
+  }
+};
+
+// Operands as they were, for tiles with rows that are not finite
+struct OfRows {  // of one matrix
+  static constexpr bool kAlongRows = false;
+  Source src;
+  __device__ inline float operator()(int row, int k) const { return src.at(0, row, k); }
+};
+struct OfColumns {
+  static constexpr bool kAlongRows = true;
+  Source src;
+  __device__ inline float operator()(int row, int k) const { return src.at(0, k, row); }
+};
+struct OfRowsOfBoth {  // behind each other along the reduction
+  static constexpr bool kAlongRows = false;
+  Source src;
+  int half_k;
+  __device__ inline float operator()(int row, int k) const { return k < half_k ? src.at(0, row, k) : src.at(1, row, k - half_k); }
+  __device__ inline float operator()(int, int row, int k) const { return (*this)(row, k); }
+};
+struct OfColumnsInTurn {  // in blocks of 32
+  static constexpr bool kAlongRows = true;
+  Source src;
+  __device__ inline float operator()(int, int row, int k) const { return src.at(row / 32 % 2, k, row / 64 * 32 + row % 32); }
+};
+struct OfColumnsOfHalf {
+  static constexpr bool kAlongRows = true;
+  Source src;
+  __device__ inline float operator()(int half, int row, int k) const { return src.at(half, k, row); }
+};
+
+int steps_of(int k) { return cdiv(k, 32) * 2; }  // an even number
+
+// Scratch of a call, laid out before it is had.
+struct Layout {
+  size_t bytes = 0;
+  size_t take(size_t n) {
+    const size_t at = bytes;
+    bytes += (n + 255) / 256 * 256;
+    return at;
+  }
+};
+struct PackedAt {
+  size_t planes, exps;
+  int blocks, steps;
+  PackedAt() = default;
+  PackedAt(Layout &l, int blocks_, int steps_, int operands = 1)
+      : planes(l.take((size_t)operands * blocks_ * steps_ * pair::kStepBytes)), exps(l.take((size_t)operands * blocks_ * 32 * 4)),
+        blocks(blocks_), steps(steps_) {}
+  pair::Packed in(char *base) const { return {base + planes, (const int *)(base + exps), blocks, steps}; }
+};
+
+// Tiles and pieces of a product.  Pieces where the tiles leave CUs idle, of 16 steps at least: 2048 x 512 x 4096, 64 tiles,
+// in 1 / 2 / 3 / 4 / 6 pieces 62 / 42 / 36 / 35 / 40 us; 512 x 4096 x 2048, 128 tiles, 37 / 32 / 35; 777 x 3074 x 1000, 175 tiles, 24 / 29;
+// 4096 x 1024 x 8192, 256 tiles, 187 / 181.
+struct Product {
+  pair::Work work;
+  size_t scratch = 0;  // offset, pieces > 1
+  Product() = default;
+  Product(Layout &l, int m_blocks, int n_blocks, int halves, int steps) {
+    const int tile = pair::BM / 32;
+    work.tiles_m = cdiv(m_blocks, tile);
+    work.half_tiles = cdiv(n_blocks, tile);
+    work.first_half = 0;
+    work.tiles_n = work.half_tiles * halves;
+    const int tiles = work.tiles_m * work.tiles_n;
+    int pieces = std::max(1, std::min({4, num_cus() / tiles, steps / 16}));
+    work.steps_per_piece = cdiv(steps / 2, pieces) * 2;
+    work.pieces = cdiv(steps, work.steps_per_piece);
+    work.scratch = nullptr;
+    work.tickets = nullptr;
+    if (work.pieces > 1) scratch = l.take((size_t)tiles * work.pieces * pair::BM * pair::BN * 4);
+  }
+  template <class EP, class EA, class EB>
+  void launch(const pair::Packed &a, const pair::Packed &b, const EP &ep, const EA &ea, const EB &eb, char *base, unsigned *tickets,
+              hipStream_t s) {
+    if (work.pieces > 1) {
+      work.scratch = (float *)(base + scratch);
+      work.tickets = tickets;
+    }
+    hipLaunchKernelGGL((pair::gemm_kernel<EP, EA, EB>), dim3((unsigned)(work.tiles_m * work.tiles_n * work.pieces)), dim3(THREADS), 0, s,
+                       a, b, work, ep, ea, eb);
+  }
+};
+
+// The two launches in front of the products.
+struct Splitting {
+  Jobs jobs{};
+  int maxima_groups = 0, split_groups = 0;
+  size_t row_max[3], col_max[3];
+  void add(Layout &l, const Source &src, int matrices, bool by_rows, bool by_columns) {
+    Job &j = jobs.job[jobs.n];
+    j.src = src;
+    j.matrices = matrices;
+    const int runs_c = cdiv(src.cols, kMaxCols), runs_r = cdiv(src.rows, kMaxRows);
+    row_max[jobs.n] = by_rows ? l.take((size_t)runs_c * src.rows * 4) : 0;
+    col_max[jobs.n] = by_columns ? l.take((size_t)matrices * runs_r * src.cols * 4) : 0;
+    j.half_steps = steps_of(src.cols);
+    j.col_steps = steps_of(src.rows);
+    j.col_mul = 1;
+    j.col_add = cdiv(src.cols, 32);
+    j.col_wanted[0] = j.col_wanted[1] = true;
+    j.first_max = maxima_groups;
+    j.first_split = split_groups;
+    maxima_groups += runs_c * runs_r;
+    split_groups += cdiv(src.rows, kSplitTile) * cdiv(src.cols, kSplitTile);
+    ++jobs.n;
+  }
+  void rows_to(int n, const PackedAt &p, char *base) {
+    jobs.job[n].row_planes = base + p.planes;
+    jobs.job[n].row_exps = (int *)(base + p.exps);
+    jobs.job[n].row_max = (uint32_t *)(base + row_max[n]);
+  }
+  void columns_to(int n, const PackedAt &p, char *base) {
+    jobs.job[n].col_planes = base + p.planes;
+    jobs.job[n].col_exps = (int *)(base + p.exps);
+    jobs.job[n].col_max = (uint32_t *)(base + col_max[n]);
+  }
+  void launch(hipStream_t s) const {
+    hipLaunchKernelGGL(maxima_kernel, dim3((unsigned)maxima_groups), dim3(kThreads), 0, s, jobs);
+    hipLaunchKernelGGL(split_kernel, dim3((unsigned)split_groups), dim3(kThreads), 0, s, jobs);
+  }
+};
+
+bool on_pairs(int64_t M, int64_t K, int64_t F) {
+  return M >= 256 && K >= 128 && F >= 128 && K < 1 << 22 && F < 1 << 22;
+}
+
+// 0, -1, or the bytes of scratch that could not be had
+int64_t forward_on_pairs(int M, int K, int F, const float *x, const float *gate, const float *up, float *pre, float *h, int activation,
+                         hipStream_t s) {
+  Layout l;
+  Splitting split;
+  const Source xs{{x, nullptr}, nullptr, M, K, 0}, ws{{gate, up}, nullptr, K, F, 0};
+  split.add(l, xs, 1, true, false);
+  split.add(l, ws, 2, false, true);
+  const int f_blocks = cdiv(F, 32);
+  const PackedAt a(l, cdiv(M, 32), steps_of(K)), b(l, 2 * f_blocks, steps_of(K));
+  Product product(l, a.blocks, b.blocks, 1, a.steps);
+  unsigned *tickets = fold_tickets(s);
+  char *base = tickets ? (char *)device_alloc(l.bytes, s) : nullptr;
+  if (!base) return (int64_t)block_bytes(l.bytes);
+  split.rows_to(0, a, base);
+  split.columns_to(1, b, base);
+  split.jobs.job[1].col_mul = 2;
+  split.jobs.job[1].col_add = 1;
+  split.launch(s);
+  with_activation(activation, [&](auto act) {
+    product.launch(a.in(base), b.in(base), StoreGated<decltype(act)::value>{pre, pre ? pre + (size_t)M * F : nullptr, h, M, F},
+                   OfRows{xs}, OfColumnsInTurn{ws}, base, tickets, s);
+  });
+  device_free(base, s);
+  return 0;
+}
+
+int64_t backward_on_pairs(int M, int K, int F, const float *x, const float *gate, const float *up, const Source &d, float *dx,
+                          float *dgate, float *dup, hipStream_t s) {
+  Layout l;
+  Splitting split;
+  const Source xs{{x, nullptr}, nullptr, M, K, 0}, ws{{gate, up}, nullptr, K, F, 0};
+  const bool weights = dgate || dup;
+  PackedAt d_rows, w_rows, d_cols, x_cols;
+  Product to_x, to_w;
+  split.add(l, d, 2, dx != nullptr, weights);
+  if (dx) split.add(l, ws, 2, true, false);
+  if (weights) split.add(l, xs, 1, false, true);
+  const int f_blocks = cdiv(F, 32), k_blocks = cdiv(K, 32), m_blocks = cdiv(M, 32);
+  if (dx) {
+    d_rows = PackedAt(l, m_blocks, 2 * steps_of(F));
+    w_rows = PackedAt(l, k_blocks, 2 * steps_of(F));
+    to_x = Product(l, m_blocks, k_blocks, 1, d_rows.steps);
+  }
+  if (weights) {
+    d_cols = PackedAt(l, f_blocks, steps_of(M), 2);
+    x_cols = PackedAt(l, k_blocks, steps_of(M));
+    to_w = Product(l, k_blocks, f_blocks, 2, d_cols.steps);
+    if (!dgate || !dup) {  // tiles and pieces are those of both
+      to_w.work.tiles_n = to_w.work.half_tiles;
+      to_w.work.first_half = dgate ? 0 : 1;
+    }
+  }
+  unsigned *tickets = fold_tickets(s);
+  char *base = tickets ? (char *)device_alloc(l.bytes, s) : nullptr;
+  if (!base) return (int64_t)block_bytes(l.bytes);
+  if (dx) {
+    split.rows_to(0, d_rows, base);
+    split.rows_to(1, w_rows, base);
+  }
+  if (weights) {
+    split.columns_to(0, d_cols, base);
+    split.jobs.job[0].col_wanted[0] = dgate != nullptr;
+    split.jobs.job[0].col_wanted[1] = dup != nullptr;
+    split.columns_to(dx ? 2 : 1, x_cols, base);
+  }
+  split.launch(s);
+  if (dx)
+    to_x.launch(d_rows.in(base), w_rows.in(base), StoreHalves{{dx, nullptr}, M, K}, OfRowsOfBoth{d, steps_of(F) * pair::BK},
+                OfRowsOfBoth{ws, steps_of(F) * pair::BK}, base, tickets, s);
+  if (weights)
+    to_w.launch(x_cols.in(base), d_cols.in(base), StoreHalves{{dgate, dup}, K, F}, OfColumns{xs}, OfColumnsOfHalf{d}, base, tickets, s);
+  device_free(base, s);
+  return 0;
 }
 
 unsigned vectors_grid(int64_t count) { return (unsigned)((count + 4 * kThreads - 1) / (4 * kThreads)); }
@@ -192,6 +669,13 @@ extern "C" int DLGpuGatedFeedForward(const DLArrayHandle input, const DLArrayHan
   hipStream_t s = stream_of(stream);
   TF_REQUIRE(!being_captured(s), "the call takes scratch, which a captured stream cannot give back");
   if (M == 0 || F == 0) return 0;
+  if (on_pairs(M, K, F)) {
+    const int64_t wanted = forward_on_pairs((int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data,
+                                            (const float *)up->data, pre ? (float *)pre->data : nullptr,
+                                            output ? (float *)output->data : nullptr, activation, s);
+    if (wanted && memorytoSaving) *memorytoSaving = shortfall((size_t)wanted);
+    return wanted ? 0 : finish(s, "DLGpuGatedFeedForward");
+  }
   float *p = pre ? (float *)pre->data : (float *)device_alloc((size_t)M * F * 8, s);
   if (!p) {
     if (memorytoSaving) *memorytoSaving = shortfall(block_bytes((size_t)M * F * 8));
@@ -237,6 +721,15 @@ extern "C" int DLGpuGatedFeedForwardBackward(const DLArrayHandle input, const DL
   for (const DLArray *written : {(const DLArray *)dinput, (const DLArray *)dgate, (const DLArray *)dup}) announce_write(written);
   hipStream_t s = stream_of(stream);
   TF_REQUIRE(!being_captured(s), "the call takes scratch, which a captured stream cannot give back");
+  if (on_pairs(M, K, F)) {
+    const float *g = pre ? (const float *)pre->data : (const float *)doutput->data;
+    const Source d{{g, g + M * F}, pre ? (const float *)doutput->data : nullptr, (int)M, (int)F, activation};
+    const int64_t wanted = backward_on_pairs((int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data,
+                                             (const float *)up->data, d, dinput ? (float *)dinput->data : nullptr,
+                                             dgate ? (float *)dgate->data : nullptr, dup ? (float *)dup->data : nullptr, s);
+    if (wanted && memorytoSaving) *memorytoSaving = shortfall((size_t)wanted);
+    return wanted ? 0 : finish(s, "DLGpuGatedFeedForwardBackward");
+  }
   const size_t bytes = ((pre ? (size_t)M * F * 2 : 0) + (dinput ? (size_t)M * K : 0)) * 4;
   float *scratch = (float *)device_alloc(bytes, s);
   if (!scratch) {
