@@ -118,10 +118,15 @@ __global__ __launch_bounds__(THREADS, 2) void gemm_kernel(const Packed A, const 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int m_wave = wave % 2 * WM, n_wave = wave / 2 * WN;
   const int tiles = work.tiles_m * work.tiles_n;
+  // An XCD's tiles are neighbours in both directions, runs of eight tile rows of one tile column after the other: its L2 then
+  // fetches a quarter of A and half of B of 4096 x 1024 x 8192, not all of A and an eighth of B.
+  constexpr int RUN = 8;
   const int logical = xcd_contiguous((int)blockIdx.x, tiles * work.pieces);
   const int tile = logical % tiles, piece = logical / tiles;
-  const int half = work.first_half + tile / work.tiles_m / work.half_tiles;
-  const int mb = tile % work.tiles_m * (BM / 32), nb = tile / work.tiles_m % work.half_tiles * (BN / 32);  // first blocks of 32 rows
+  const int run = tile / (RUN * work.tiles_n), in_run = tile % (RUN * work.tiles_n), run_rows = min(RUN, work.tiles_m - run * RUN);
+  const int tile_n = in_run / run_rows;
+  const int half = work.first_half + tile_n / work.half_tiles;
+  const int mb = (run * RUN + in_run % run_rows) * (BM / 32), nb = tile_n % work.half_tiles * (BN / 32);  // first blocks of 32 rows
   const int b_first = half * B.blocks;  // of the half
   const int s_begin = piece * work.steps_per_piece, s_end = min(A.steps, s_begin + work.steps_per_piece);
 
