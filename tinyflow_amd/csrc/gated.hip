@@ -25,7 +25,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4u __attribute__((aligned(4)));
 constexpr int kThreads = 256;
 
-enum Activation { kSigmoid = 0, kRelu = 1, kSilu = 2, kGelu = 3 };
+enum Activation { kSigmoid = 0, kRelu = 1, kSilu = 2, kGelu = 3, kGiven = -1 };
 
 // Both from the hardware's exp2 and reciprocal, which are right to a step of the last place: what that leaves off is 2^-24 of
 // the exponent's size, relative, on a value that gets small as the exponent grows; next to 1 it does not show.  The activations and
@@ -133,16 +133,12 @@ using namespace tf::gemm;
 struct Source {
   const float *p[2];
   const float *dh;   // not NULL: p are g and u, and the matrices are their gradients
-  int rows, cols, activation;
+  int rows, cols, activation;  // kGiven without dh
 
-  __device__ inline void gradients(float g, float u, float d, float &dg, float &du) const {
+  template <int ACT>
+  static __device__ inline void gradients(float g, float u, float d, float &dg, float &du) {
     float act, slope;
-    switch (activation) {
-      case kSigmoid: act_and_slope<kSigmoid>(g, act, slope); break;
-      case kRelu: act_and_slope<kRelu>(g, act, slope); break;
-      case kSilu: act_and_slope<kSilu>(g, act, slope); break;
-      default: act_and_slope<kGelu>(g, act, slope); break;
-    }
+    act_and_slope<ACT>(g, act, slope);
     dg = d * u * slope;
     du = d * act;
   }
@@ -150,11 +146,18 @@ struct Source {
     if (r >= rows || c >= cols) return 0.f;
     const size_t i = (size_t)r * cols + c;
     if (!dh) return p[which][i];
+    const float g = p[0][i], u = p[1][i], d = dh[i];
     float v[2];
-    gradients(p[0][i], p[1][i], dh[i], v[0], v[1]);
+    switch (activation) {
+      case kSigmoid: gradients<kSigmoid>(g, u, d, v[0], v[1]); break;
+      case kRelu: gradients<kRelu>(g, u, d, v[0], v[1]); break;
+      case kSilu: gradients<kSilu>(g, u, d, v[0], v[1]); break;
+      default: gradients<kGelu>(g, u, d, v[0], v[1]); break;
+    }
     return v[which];
   }
-  // four columns from c on of both matrices; zeros past the end
+  // four columns from c on of both matrices; zeros past the end.  ACT as `activation` says, kGiven: the matrices as they are
+  template <int ACT>
   __device__ inline void four(int r, int c, f32x4 (&v)[2]) const {
     v[0] = v[1] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (r >= rows || c >= cols) return;
@@ -162,27 +165,40 @@ struct Source {
     f32x4 d = v[0];
     if (c + 4 <= cols) {
       v[0] = *reinterpret_cast<const f32x4u *>(p[0] + i);
-      if (p[1]) v[1] = *reinterpret_cast<const f32x4u *>(p[1] + i);
-      if (dh) d = *reinterpret_cast<const f32x4u *>(dh + i);
+      if (ACT != kGiven || p[1]) v[1] = *reinterpret_cast<const f32x4u *>(p[1] + i);
+      if (ACT != kGiven) d = *reinterpret_cast<const f32x4u *>(dh + i);
     } else {
 #pragma unroll
       for (int e = 0; e < 3; ++e)
         if (c + e < cols) {
           v[0][e] = p[0][i + e];
-          if (p[1]) v[1][e] = p[1][i + e];
-          if (dh) d[e] = dh[i + e];
+          if (ACT != kGiven || p[1]) v[1][e] = p[1][i + e];
+          if (ACT != kGiven) d[e] = dh[i + e];
         }
     }
-    if (dh)
+    if constexpr (ACT != kGiven) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float dg, du;
-        gradients(v[0][e], v[1][e], d[e], dg, du);
+        gradients<ACT>(v[0][e], v[1][e], d[e], dg, du);
         v[0][e] = dg;
         v[1][e] = du;
       }
+    }
   }
 };
+
+// Calls f with the source's activation as a compile-time constant: one branch a workgroup, not one an element.
+template <class F>
+__device__ __forceinline__ void by_activation(const Source &src, F &&f) {
+  switch (src.activation) {
+    case kGiven: f(std::integral_constant<int, kGiven>{}); break;
+    case kSigmoid: f(std::integral_constant<int, kSigmoid>{}); break;
+    case kRelu: f(std::integral_constant<int, kRelu>{}); break;
+    case kSilu: f(std::integral_constant<int, kSilu>{}); break;
+    default: f(std::integral_constant<int, kGelu>{}); break;
+  }
+}
 
 // What is made of a source.  By rows: both matrices behind each other along the reduction, `half_steps` steps each, a row's
 // exponent common to both.  By columns: matrix w's block of 32 columns b is block b * col_mul + w * col_add.
@@ -219,20 +235,22 @@ __global__ __launch_bounds__(kThreads) void maxima_kernel(const Jobs jobs) {
   const int c = run_c * kMaxCols + 4 * lane;
   __shared__ uint32_t of_groups[2][8][kMaxCols];
   uint32_t col[2][4] = {}, row[kMaxRows / 8];
+  by_activation(job.src, [&](auto act) {
 #pragma unroll
-  for (int e = 0; e < kMaxRows / 8; ++e) {
-    f32x4 v[2];
-    job.src.four(run_r * kMaxRows + 8 * e + group, c, v);
-    row[e] = 0;
+    for (int e = 0; e < kMaxRows / 8; ++e) {
+      f32x4 v[2];
+      job.src.four<decltype(act)::value>(run_r * kMaxRows + 8 * e + group, c, v);
+      row[e] = 0;
 #pragma unroll
-    for (int w = 0; w < 2; ++w)
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t m = magnitude(v[w][i]);
-        col[w][i] = max(col[w][i], m);
-        row[e] = max(row[e], m);
-      }
-  }
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t m = magnitude(v[w][i]);
+          col[w][i] = max(col[w][i], m);
+          row[e] = max(row[e], m);
+        }
+    }
+  });
   if (job.row_planes) {
 #pragma unroll
     for (int e = 0; e < kMaxRows / 8; ++e) {
@@ -287,14 +305,16 @@ __global__ __launch_bounds__(kThreads) void split_kernel(const Jobs jobs) {
   __shared__ int row_exp[T], col_exp[2][T];
 
   // the tile, 16 lanes a row
+  by_activation(job.src, [&](auto act) {
 #pragma unroll
-  for (int e = 0; e < T / 16; ++e) {
-    const int r = e * 16 + tid / 16, c = tid % 16 * 4;
-    f32x4 v[2];
-    job.src.four(r0 + r, c0 + c, v);
-    *reinterpret_cast<f32x4 *>(&tile[0][r][c]) = v[0];
-    if (job.matrices > 1) *reinterpret_cast<f32x4 *>(&tile[1][r][c]) = v[1];
-  }
+    for (int e = 0; e < T / 16; ++e) {
+      const int r = e * 16 + tid / 16, c = tid % 16 * 4;
+      f32x4 v[2];
+      job.src.four<decltype(act)::value>(r0 + r, c0 + c, v);
+      *reinterpret_cast<f32x4 *>(&tile[0][r][c]) = v[0];
+      if (job.matrices > 1) *reinterpret_cast<f32x4 *>(&tile[1][r][c]) = v[1];
+    }
+  });
   // the exponents, four lanes each; the tiles at the reduction's beginning write them down
   const int of = tid / 4, part = tid % 4;
   auto largest = [&](const uint32_t *from, int runs, int64_t stride) {
@@ -531,7 +551,7 @@ int64_t forward_on_pairs(int M, int K, int F, const float *x, const float *gate,
                          hipStream_t s) {
   Layout l;
   Splitting split;
-  const Source xs{{x, nullptr}, nullptr, M, K, 0}, ws{{gate, up}, nullptr, K, F, 0};
+  const Source xs{{x, nullptr}, nullptr, M, K, kGiven}, ws{{gate, up}, nullptr, K, F, kGiven};
   split.add(l, xs, 1, true, false);
   split.add(l, ws, 2, false, true);
   const int f_blocks = cdiv(F, 32);
@@ -557,7 +577,7 @@ int64_t backward_on_pairs(int M, int K, int F, const float *x, const float *gate
                           float *dgate, float *dup, hipStream_t s) {
   Layout l;
   Splitting split;
-  const Source xs{{x, nullptr}, nullptr, M, K, 0}, ws{{gate, up}, nullptr, K, F, 0};
+  const Source xs{{x, nullptr}, nullptr, M, K, kGiven}, ws{{gate, up}, nullptr, K, F, kGiven};
   const bool weights = dgate || dup;
   PackedAt d_rows, w_rows, d_cols, x_cols;
   Product to_x, to_w;
@@ -751,7 +771,7 @@ extern "C" int DLGpuGatedFeedForwardBackward(const DLArrayHandle input, const DL
   TF_REQUIRE(!being_captured(s), "the call takes scratch, which a captured stream cannot give back");
   if (on_pairs(M, K, F)) {
     const float *g = pre ? (const float *)pre->data : (const float *)doutput->data;
-    const Source d{{g, g + M * F}, pre ? (const float *)doutput->data : nullptr, (int)M, (int)F, activation};
+    const Source d{{g, g + M * F}, pre ? (const float *)doutput->data : nullptr, (int)M, (int)F, pre ? activation : kGiven};
     const int64_t wanted = backward_on_pairs((int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data,
                                              (const float *)up->data, d, dinput ? (float *)dinput->data : nullptr,
                                              dgate ? (float *)dgate->data : nullptr, dup ? (float *)dup->data : nullptr, s);
