@@ -421,32 +421,32 @@ struct StoreHalves {
 };
 
 // Operands as they were, for tiles with rows that are not finite
-struct OfRows {  // of one matrix
-  static constexpr bool kAlongRows = false;
-  Source src;
-  __device__ inline float operator()(int row, int k) const { return src.at(0, row, k); }
-};
-struct OfColumns {
-  static constexpr bool kAlongRows = true;
-  Source src;
-  __device__ inline float operator()(int row, int k) const { return src.at(0, k, row); }
-};
-struct OfRowsOfBoth {  // behind each other along the reduction
+struct OfRows {  // of a matrix, or of two behind each other along the reduction, half_k elements each
   static constexpr bool kAlongRows = false;
   Source src;
   int half_k;
   __device__ inline float operator()(int row, int k) const { return k < half_k ? src.at(0, row, k) : src.at(1, row, k - half_k); }
-  __device__ inline float operator()(int, int row, int k) const { return (*this)(row, k); }
 };
-struct OfColumnsInTurn {  // in blocks of 32
+struct OfColumnsInTurn {  // of two, in blocks of 32
   static constexpr bool kAlongRows = true;
   Source src;
   __device__ inline float operator()(int, int row, int k) const { return src.at(row / 32 % 2, k, row / 64 * 32 + row % 32); }
 };
-struct OfColumnsOfHalf {
-  static constexpr bool kAlongRows = true;
-  Source src;
-  __device__ inline float operator()(int half, int row, int k) const { return src.at(half, k, row); }
+struct OfEither {  // of a backward product: dx by rows, the weights' gradients by columns
+  static constexpr bool kAlongRows = false;
+  OfRows rows;
+  bool columns;
+  __device__ inline float operator()(int row, int k) const { return (*this)(0, row, k); }
+  __device__ inline float operator()(int half, int row, int k) const { return columns ? rows.src.at(half, k, row) : rows(row, k); }
+};
+template <int ACT>
+struct Forward {
+  static constexpr int kCount = 1;
+  pair::Product<StoreGated<ACT>, OfRows, OfColumnsInTurn> p[1];
+};
+struct Backward {
+  static constexpr int kCount = 2;
+  pair::Product<StoreHalves, OfEither, OfEither> p[2];  // without a workgroup where it is not wanted
 };
 
 int steps_of(int k) { return cdiv(k, 32) * 2; }  // an even number
@@ -470,38 +470,41 @@ struct PackedAt {
   pair::Packed in(char *base) const { return {base + planes, (const int *)(base + exps), blocks, steps}; }
 };
 
-// Tiles and pieces of a product.  Pieces where the tiles leave CUs idle, of 16 steps at least: 2048 x 512 x 4096, 64 tiles,
-// in 1 / 2 / 3 / 4 / 6 pieces 62 / 42 / 36 / 35 / 40 us; 512 x 4096 x 2048, 128 tiles, 37 / 32 / 35; 777 x 3074 x 1000, 175 tiles, 24 / 29;
-// 4096 x 1024 x 8192, 256 tiles, 187 / 181.
-struct Product {
-  pair::Work work;
-  size_t scratch = 0;  // offset, pieces > 1
-  Product() = default;
-  Product(Layout &l, int m_blocks, int n_blocks, int halves, int steps) {
-    const int tile = pair::BM / 32;
-    work.tiles_m = cdiv(m_blocks, tile);
-    work.half_tiles = cdiv(n_blocks, tile);
-    work.first_half = 0;
-    work.tiles_n = work.half_tiles * halves;
-    const int tiles = work.tiles_m * work.tiles_n;
-    int pieces = std::max(1, std::min({4, num_cus() / tiles, steps / 16}));
-    work.steps_per_piece = cdiv(steps / 2, pieces) * 2;
-    work.pieces = cdiv(steps, work.steps_per_piece);
-    work.scratch = nullptr;
-    work.tickets = nullptr;
-    if (work.pieces > 1) scratch = l.take((size_t)tiles * work.pieces * pair::BM * pair::BN * 4);
+// Tiles of a product.
+pair::Work tiles_of(int m_blocks, int n_blocks, int halves) {
+  const int tile = pair::BM / 32;
+  pair::Work w{};
+  w.tiles_m = cdiv(m_blocks, tile);
+  w.half_tiles = cdiv(n_blocks, tile);
+  w.tiles_n = w.half_tiles * halves;
+  return w;
+}
+// Pieces of the products of a launch, so that there is about a workgroup a CU and all have about as many steps, 16 at least: a
+// piece writes and reads its tile once more.  us in 1 / 2 / 3 / 4 / 6 pieces: 2048 x 512 x 4096, 64 tiles, 62 / 42 / 36 / 35 / 40;
+// 512 x 4096 x 2048, 128 tiles, 37 / 32 / 35; 777 x 3074 x 1000, 175 tiles, 24 / 29; 4096 x 1024 x 8192, 256 tiles, 187 / 181.
+constexpr int kMaxPieces = 4;
+int steps_a_group(std::initializer_list<std::pair<pair::Work, int>> products) {
+  int64_t steps = 0;
+  for (const auto &p : products) steps += (int64_t)p.first.tiles_m * p.first.tiles_n * p.second;
+  return (int)std::max<int64_t>(16, steps / num_cus());
+}
+// Its scratch's place, where there are several
+size_t cut(Layout &l, pair::Work &w, int steps, int steps_a_group) {
+  const int pieces = std::max(1, std::min(kMaxPieces, (steps + steps_a_group / 2) / steps_a_group));
+  w.steps_per_piece = cdiv(steps / 2, pieces) * 2;
+  w.pieces = cdiv(steps, w.steps_per_piece);
+  if ((int64_t)w.tiles_m * w.tiles_n > kFoldTicketSlots / 2) {
+    w.pieces = 1;
+    w.steps_per_piece = steps;
   }
-  template <class EP, class EA, class EB>
-  void launch(const pair::Packed &a, const pair::Packed &b, const EP &ep, const EA &ea, const EB &eb, char *base, unsigned *tickets,
-              hipStream_t s) {
-    if (work.pieces > 1) {
-      work.scratch = (float *)(base + scratch);
-      work.tickets = tickets;
-    }
-    hipLaunchKernelGGL((pair::gemm_kernel<EP, EA, EB>), dim3((unsigned)(work.tiles_m * work.tiles_n * work.pieces)), dim3(THREADS), 0, s,
-                       a, b, work, ep, ea, eb);
-  }
-};
+  return w.pieces > 1 ? l.take((size_t)w.tiles_m * w.tiles_n * w.pieces * pair::BM * pair::BN * 4) : 0;
+}
+// `tickets`: one for each of its tiles
+void give(pair::Work &w, char *base, size_t scratch, unsigned *tickets) {
+  if (w.pieces < 2) return;
+  w.scratch = (float *)(base + scratch);
+  w.tickets = tickets;
+}
 
 // The two launches in front of the products.
 struct Splitting {
@@ -556,7 +559,8 @@ int64_t forward_on_pairs(int M, int K, int F, const float *x, const float *gate,
   split.add(l, ws, 2, false, true);
   const int f_blocks = cdiv(F, 32);
   const PackedAt a(l, cdiv(M, 32), steps_of(K)), b(l, 2 * f_blocks, steps_of(K));
-  Product product(l, a.blocks, b.blocks, 1, a.steps);
+  pair::Work work = tiles_of(a.blocks, b.blocks, 1);
+  const size_t scratch = cut(l, work, a.steps, steps_a_group({{work, a.steps}}));
   unsigned *tickets = fold_tickets(s);
   char *base = tickets ? (char *)device_alloc(l.bytes, s) : nullptr;
   if (!base) return (int64_t)block_bytes(l.bytes);
@@ -565,9 +569,12 @@ int64_t forward_on_pairs(int M, int K, int F, const float *x, const float *gate,
   split.jobs.job[1].col_mul = 2;
   split.jobs.job[1].col_add = 1;
   split.launch(s);
+  give(work, base, scratch, tickets);
   with_activation(activation, [&](auto act) {
-    product.launch(a.in(base), b.in(base), StoreGated<decltype(act)::value>{pre, pre ? pre + (size_t)M * F : nullptr, h, M, F},
-                   OfRows{xs}, OfColumnsInTurn{ws}, base, tickets, s);
+    constexpr int ACT = decltype(act)::value;
+    const Forward<ACT> product{{{a.in(base), b.in(base), work, StoreGated<ACT>{pre, pre ? pre + (size_t)M * F : nullptr, h, M, F},
+                                 OfRows{xs, a.steps * pair::BK}, OfColumnsInTurn{ws}}}};
+    hipLaunchKernelGGL(pair::gemm_kernel<Forward<ACT>>, dim3((unsigned)product.p[0].groups()), dim3(THREADS), 0, s, product);
   });
   device_free(base, s);
   return 0;
@@ -580,7 +587,7 @@ int64_t backward_on_pairs(int M, int K, int F, const float *x, const float *gate
   const Source xs{{x, nullptr}, nullptr, M, K, kGiven}, ws{{gate, up}, nullptr, K, F, kGiven};
   const bool weights = dgate || dup;
   PackedAt d_rows, w_rows, d_cols, x_cols;
-  Product to_x, to_w;
+  pair::Work to_x{}, to_w{};
   split.add(l, d, 2, dx != nullptr, weights);
   if (dx) split.add(l, ws, 2, true, false);
   if (weights) split.add(l, xs, 1, false, true);
@@ -588,16 +595,20 @@ int64_t backward_on_pairs(int M, int K, int F, const float *x, const float *gate
   if (dx) {
     d_rows = PackedAt(l, m_blocks, 2 * steps_of(F));
     w_rows = PackedAt(l, k_blocks, 2 * steps_of(F));
-    to_x = Product(l, m_blocks, k_blocks, 1, d_rows.steps);
+    to_x = tiles_of(m_blocks, k_blocks, 1);
   }
   if (weights) {
     d_cols = PackedAt(l, f_blocks, steps_of(M), 2);
     x_cols = PackedAt(l, k_blocks, steps_of(M));
-    to_w = Product(l, k_blocks, f_blocks, 2, d_cols.steps);
-    if (!dgate || !dup) {  // tiles and pieces are those of both
-      to_w.work.tiles_n = to_w.work.half_tiles;
-      to_w.work.first_half = dgate ? 0 : 1;
-    }
+    to_w = tiles_of(k_blocks, f_blocks, 2);
+  }
+  // pieces as for all three gradients, so that each has the same bits alone
+  const int x_steps = 2 * steps_of(F), w_steps = steps_of(M);
+  const int a_group = steps_a_group({{tiles_of(m_blocks, k_blocks, 1), x_steps}, {tiles_of(k_blocks, f_blocks, 2), w_steps}});
+  const size_t x_scratch = dx ? cut(l, to_x, x_steps, a_group) : 0, w_scratch = weights ? cut(l, to_w, w_steps, a_group) : 0;
+  if (weights && (!dgate || !dup)) {
+    to_w.tiles_n = to_w.half_tiles;
+    to_w.first_half = dgate ? 0 : 1;
   }
   unsigned *tickets = fold_tickets(s);
   char *base = tickets ? (char *)device_alloc(l.bytes, s) : nullptr;
@@ -613,11 +624,16 @@ int64_t backward_on_pairs(int M, int K, int F, const float *x, const float *gate
     split.columns_to(dx ? 2 : 1, x_cols, base);
   }
   split.launch(s);
+  give(to_x, base, x_scratch, tickets);
+  give(to_w, base, w_scratch, tickets + kFoldTicketSlots / 2);
+  Backward products{};
   if (dx)
-    to_x.launch(d_rows.in(base), w_rows.in(base), StoreHalves{{dx, nullptr}, M, K}, OfRowsOfBoth{d, steps_of(F) * pair::BK},
-                OfRowsOfBoth{ws, steps_of(F) * pair::BK}, base, tickets, s);
+    products.p[0] = {d_rows.in(base), w_rows.in(base), to_x, StoreHalves{{dx, nullptr}, M, K},
+                     {{d, steps_of(F) * pair::BK}, false}, {{ws, steps_of(F) * pair::BK}, false}};
   if (weights)
-    to_w.launch(x_cols.in(base), d_cols.in(base), StoreHalves{{dgate, dup}, K, F}, OfColumns{xs}, OfColumnsOfHalf{d}, base, tickets, s);
+    products.p[1] = {x_cols.in(base), d_cols.in(base), to_w, StoreHalves{{dgate, dup}, K, F}, {{xs, 0}, true}, {{d, 0}, true}};
+  hipLaunchKernelGGL(pair::gemm_kernel<Backward>, dim3((unsigned)(products.p[0].groups() + products.p[1].groups())), dim3(THREADS),
+                     0, s, products);
   device_free(base, s);
   return 0;
 }

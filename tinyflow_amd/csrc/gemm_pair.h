@@ -106,9 +106,24 @@ __device__ __forceinline__ void exact_tile(f32x16 (&acc)[TM][TN], float *lds, co
 // 1024 x 8192 x 4096 167, 230 and 164, 4096 x 8192 x 1024 202, 199 and 227.  With one step under way instead of three 368 us.
 constexpr int BM = 128, BN = 128, SLOTS = 4;
 constexpr int BLOCKS = (BM + BN) / 32, SLOT = BLOCKS * kStepBytes, FETCHES = BLOCKS / 2;  // fetches: a wave's a step
+//
+// A launch may be two products: the workgroups of the second stand behind those of the first.
 template <class Epilogue, class ExactA, class ExactB>
-__global__ __launch_bounds__(THREADS, 2) void gemm_kernel(const Packed A, const Packed B, const Work work, const Epilogue ep,
-                                                        const ExactA exact_a, const ExactB exact_b) {
+struct Product {
+  Packed A, B;
+  Work work;
+  Epilogue ep;
+  ExactA exact_a;
+  ExactB exact_b;
+  __host__ __device__ int groups() const { return work.tiles_m * work.tiles_n * work.pieces; }
+};
+template <class Products>
+__global__ __launch_bounds__(THREADS, 2) void gemm_kernel(const Products products) {
+  const bool is_second = Products::kCount > 1 && (int)blockIdx.x >= products.p[0].groups();
+  const auto &product = products.p[is_second];
+  const Packed A = product.A, B = product.B;
+  const Work work = product.work;
+  const int group = (int)blockIdx.x - (is_second ? products.p[0].groups() : 0);
   constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 32, TN = WN / 32;
   static_assert(SLOTS * SLOT >= 16 * (BM + 4 + BN + 4) * 4, "the fp32 pass reuses the slots");
   __shared__ __align__(16) char lds[SLOTS * SLOT];
@@ -121,7 +136,7 @@ __global__ __launch_bounds__(THREADS, 2) void gemm_kernel(const Packed A, const 
   // An XCD's tiles are neighbours in both directions, runs of eight tile rows of one tile column after the other: its L2 then
   // fetches a quarter of A and half of B of 4096 x 1024 x 8192, not all of A and an eighth of B.
   constexpr int RUN = 8;
-  const int logical = xcd_contiguous((int)blockIdx.x, tiles * work.pieces);
+  const int logical = xcd_contiguous(group, tiles * work.pieces);
   const int tile = logical % tiles, piece = logical / tiles;
   const int run = tile / (RUN * work.tiles_n), in_run = tile % (RUN * work.tiles_n), run_rows = min(RUN, work.tiles_m - run * RUN);
   const int tile_n = in_run / run_rows;
@@ -230,7 +245,7 @@ __global__ __launch_bounds__(THREADS, 2) void gemm_kernel(const Packed A, const 
       for (int j = 0; j < TN; ++j) acc[i][j] += low[i][j];
   } else {
     arrived(none);
-    exact_tile<BM, BN>(acc, reinterpret_cast<float *>(lds), exact_a, exact_b, half, mb * 32, nb * 32, s_begin * BK, s_end * BK,
+    exact_tile<BM, BN>(acc, reinterpret_cast<float *>(lds), product.exact_a, product.exact_b, half, mb * 32, nb * 32, s_begin * BK, s_end * BK,
                        m_wave, n_wave, tid);
   }
 
@@ -281,7 +296,7 @@ __global__ __launch_bounds__(THREADS, 2) void gemm_kernel(const Packed A, const 
   }
 
   // Exponents: those of this lane's columns, and of four rows at a time
-  const typename Epilogue::State state = ep.begin(mb * 32, half);
+  const auto state = product.ep.begin(mb * 32, half);
   int eb[TN];
   const int lhalf = lane >> 5, lcol = lane & 31;
 #pragma unroll
@@ -298,7 +313,7 @@ __global__ __launch_bounds__(THREADS, 2) void gemm_kernel(const Packed A, const 
         float v[TN];
 #pragma unroll
         for (int j = 0; j < TN; ++j) v[j] = __builtin_ldexpf(acc[i][j][4 * q + e], eb[j] - ea[e]);
-        ep.template store<TN>(state, m_wave + 32 * i + row + e, nb + n_wave / 32, lcol, v);
+        product.ep.template store<TN>(state, m_wave + 32 * i + row + e, nb + n_wave / 32, lcol, v);
       }
     }
 }
