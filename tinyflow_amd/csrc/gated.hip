@@ -545,12 +545,25 @@ struct Splitting {
   }
 };
 
-bool on_pairs(int64_t M, int64_t K, int64_t F) {
-  return M >= 256 && K >= 128 && F >= 128 && K < 1 << 22 && F < 1 << 22;
+// Whether the forward pass runs on pairs, or on the fp32 instruction with nothing split (namespace few): us, fitted.  K x F, rows, few
+// / pairs: 1 024 x 4 096, 128 29 / 54, 256 43 / 53, 512 84 / 54; 2 048 x 8 192, 128 84 / 132, 256 151 / 131; 512 x 1 376, 256
+// 19 / 30; 256 x 1 024, 256 12 / 23.
+bool forward_on_pairs(int64_t M, int64_t K, int64_t F) {
+  if (K >= 1 << 22 || F >= 1 << 22) return false;  // a tile's rows would pass a buffer's end
+  const double m = (double)cdiv(M, 32) * 32, k = (double)cdiv(K, 32) * 32, f = (double)cdiv(F, 32) * 32;
+  const double few = 6.0 + 4.0 * m * k * f / 115e6;
+  const double pairs = 18.0 + (24.0 * k * f + 12.0 * m * k) / 4.8e6 + 4.0 * m * k * f / 380e6;
+  return pairs < few;
+}
+// The backward pass: from 128 rows on, or where the weights are small.  Else products of the matrix multiply, which split nothing,
+// around the pointwise pass.  products / pairs: 1 024 x 4 096, 32 rows 45 / 65, 128 75 / 74, 256 113 / 81; 2 048 x 8 192, 64
+// 115 / 212, 128 181 / 229, 256 318 / 245; 512 x 1 376, 8 35 / 35, 128 43 / 42; 128 x 512, 8 30 / 26, 256 43 / 31.
+bool backward_on_pairs(int64_t M, int64_t K, int64_t F) {
+  return M > 0 && K > 0 && F > 0 && K < 1 << 22 && F < 1 << 22 && (M >= 128 || K * F <= 1 << 20);
 }
 
 // 0, -1, or the bytes of scratch that could not be had
-int64_t forward_on_pairs(int M, int K, int F, const float *x, const float *gate, const float *up, float *pre, float *h, int activation,
+int64_t forward_by_pairs(int M, int K, int F, const float *x, const float *gate, const float *up, float *pre, float *h, int activation,
                          hipStream_t s) {
   Layout l;
   Splitting split;
@@ -580,7 +593,7 @@ int64_t forward_on_pairs(int M, int K, int F, const float *x, const float *gate,
   return 0;
 }
 
-int64_t backward_on_pairs(int M, int K, int F, const float *x, const float *gate, const float *up, const Source &d, float *dx,
+int64_t backward_by_pairs(int M, int K, int F, const float *x, const float *gate, const float *up, const Source &d, float *dx,
                           float *dgate, float *dup, hipStream_t s) {
   Layout l;
   Splitting split;
@@ -637,6 +650,266 @@ int64_t backward_on_pairs(int M, int K, int F, const float *x, const float *gate
   device_free(base, s);
   return 0;
 }
+
+// ---- few rows ---------------------------------------------------------------------------------------------------
+// Both projections, the activation and the product for up to 32 rows a workgroup, bound by reading the weights: nothing is staged.
+// A wave owns 128 columns of both weights and a run of the reduction; a load is 512 bytes of two of their rows, the four
+// columns of a lane are four fp32 matrix instructions' operands (columns 4 (lane mod 32) + j of the j-th), so that the lanes'
+// order costs nothing, and eight instructions use one value of x.  In a group of eight reduction elements lanes 0..31 hold
+// the first four and lanes 32..63 the others.  The four waves of a workgroup have four runs of the reduction, added
+// through LDS, and several workgroups more of them, added by the last one to finish (gemm_core.h: Fold), in their order.
+namespace few {
+constexpr int kRows = 32, kCols = 128, kWaves = 4;
+
+struct Args {
+  const float *x, *gate, *up;
+  float *g, *u, *h;  // NULL: not wanted
+  int M, K, F, strips, k_per_group, pieces;
+  float *scratch;    // [row group][strip][piece][g, u][rows][kCols]
+  unsigned *tickets;
+};
+
+template <int ACT>
+__global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Args a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, along = lane & 31;
+  const int strip = blockIdx.x % a.strips, piece = blockIdx.y, m0 = blockIdx.x / a.strips * kRows;
+  const int rows = min(kRows, a.M - m0), c0 = strip * kCols;
+  const int k_begin = piece * a.k_per_group + wave * (a.k_per_group / kWaves);
+  const int k_end = min(a.K, k_begin + a.k_per_group / kWaves);
+  __shared__ f32x4v part[2][kWaves - 1][2][4][64];  // [wave that adds][wave that has][g, u][row][lane]
+  __shared__ unsigned last;
+
+  const uint32_t bytes = (uint32_t)a.K * (uint32_t)a.F * 4u;
+  const __amdgpu_buffer_rsrc_t rsrc[2] = {make_rsrc(a.gate, bytes), make_rsrc(a.up, bytes)};
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, (uint32_t)a.M * (uint32_t)a.K * 4u);
+  // a lane's columns past the end may hold the next row's values: they are not stored
+  const uint32_t col_off = c0 + 4 * along < a.F ? (uint32_t)(c0 + 4 * along) * 4u : OOB;
+  const uint32_t row_off = along < rows ? (uint32_t)(m0 + along) * (uint32_t)a.K * 4u : OOB;
+
+  f32x16 acc[2][4];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[w][j][v] = 0.f;
+
+  // x: four reduction elements of one row; weights: four rows of four columns
+  f32x4v xv[2], wv[2][2][4];
+  auto load = [&](int at, int k0) {
+    const int k = k0 + 4 * half;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t off = k + s < k_end ? col_off + (uint32_t)(k + s) * (uint32_t)a.F * 4u : OOB;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) wv[at][w][s] = buf_load4(rsrc[w], off | (col_off & OOB));
+    }
+    const f32x4v v = buf_load4(xr, k < k_end ? (row_off + (uint32_t)k * 4u) | (row_off & OOB) : OOB);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) xv[at][s] = k + s < k_end ? v[s] : 0.f;
+  };
+  auto multiply = [&](int at) {
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[w][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[at][s], wv[at][w][s][j], acc[w][j], 0, 0, 0);
+  };
+  load(0, k_begin);
+  for (int k0 = k_begin; k0 < k_end; k0 += 16) {
+    load(1, k0 + 8);
+    multiply(0);
+    load(0, k0 + 16);
+    multiply(1);
+  }
+
+  // Wave q adds up rows 8 q + 4 half + 0..3, accumulators 4 q + 0..3, two waves' worth at a time.
+  f32x4v sum[2][4];  // [g, u][row], four columns
+#pragma unroll
+  for (int pair = 0; pair < 2; ++pair) {
+    if (16 * pair >= rows) break;  // uniform, as all that depends on rows and q below
+    if (pair) __syncthreads();
+#pragma unroll
+    for (int q = 2 * pair; q < 2 * pair + 2; ++q) {
+      if (8 * q >= rows) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (8 * q + i >= rows) continue;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const f32x4v o = {acc[w][0][4 * q + i], acc[w][1][4 * q + i], acc[w][2][4 * q + i], acc[w][3][4 * q + i]};
+          if (wave == q) sum[w][i] = o;
+          else part[q % 2][wave - (wave > q)][w][i][lane] = o;
+        }
+      }
+    }
+    __syncthreads();
+    if (wave / 2 == pair)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (8 * wave + i >= rows) continue;
+#pragma unroll
+        for (int o = 0; o < kWaves - 1; ++o)
+#pragma unroll
+          for (int w = 0; w < 2; ++w) sum[w][i] += part[wave % 2][o][w][i][lane];
+      }
+  }
+  const int live = min(4, rows - 8 * wave);  // rows of the half wave 0 that this wave has, at most 0: none
+  if (a.pieces > 1) {
+    constexpr int SC1 = 16;
+    constexpr uint32_t kPieceBytes = 2u * kRows * kCols * 4u;
+    const int slot = (int)blockIdx.x;
+    const __amdgpu_buffer_rsrc_t pieces = make_rsrc(a.scratch + (size_t)slot * a.pieces * (kPieceBytes / 4), (uint32_t)a.pieces * kPieceBytes);
+    auto offset = [&](int p, int w, int i) {
+      return (int)((uint32_t)p * kPieceBytes + (uint32_t)(((wave * 4 + i) * 2 + w) * 64 + lane) * 16u);
+    };
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i >= live) continue;
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(__attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned, sum[w][i]),
+                                               pieces, offset(piece, w, i), 0, SC1);
+    }
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(a.tickets + slot, 1u) == (unsigned)(a.pieces - 1);
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) a.tickets[slot] = 0u;
+    if (live <= 0) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[0][i] = sum[1][i] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    // rows that are not live were not written, and are not used
+#pragma unroll 4
+    for (int p = 0; p < a.pieces; ++p)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          sum[w][i] += __builtin_bit_cast(
+              f32x4v, __builtin_amdgcn_raw_buffer_load_b128(pieces, i < live ? offset(p, w, i) : (int)OOB, 0, SC1));
+  }
+  const int c = c0 + 4 * along;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int m = 8 * wave + 4 * half + i;
+    if (m >= rows) continue;
+    const size_t at = (size_t)(m0 + m) * a.F + c;
+    f32x4v h;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = act_of<ACT>(sum[0][i][j]) * sum[1][i][j];
+    auto put = [&](float *out, const f32x4v &value) {
+      if (!out) return;
+      if (c + 4 <= a.F) {
+        *reinterpret_cast<f32x4u *>(out + at) = value;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (c + j < a.F) out[at + j] = value[j];
+      }
+    };
+    put(a.g, sum[0][i]);
+    put(a.u, sum[1][i]);
+    put(a.h, h);
+  }
+}
+
+// Up to four rows: vector multiply-adds.  Sixteen waves share 32 columns, eight lanes a row of the weights with four columns each, so
+// that 4 096 columns already keep half of the CUs' loads going without a run of the reduction to be added across
+// workgroups, which costs as long as reading 20 MB.
+constexpr int kFewest = 4, kNarrow = 32, kWide = 1024;
+template <int ACT, int ROWS>
+__global__ __launch_bounds__(kWide) void fewest_kernel(const Args a) {
+  constexpr int WAVES = kWide / 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * kNarrow + 4 * (lane & 7);
+  __shared__ f32x4v part[WAVES][2][ROWS][8];
+  const uint32_t bytes = (uint32_t)a.K * (uint32_t)a.F * 4u;
+  const __amdgpu_buffer_rsrc_t rsrc[2] = {make_rsrc(a.gate, bytes), make_rsrc(a.up, bytes)};
+  const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, (uint32_t)a.M * (uint32_t)a.K * 4u);
+  f32x4v acc[2][ROWS];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) acc[w][m] = f32x4v{0.f, 0.f, 0.f, 0.f};
+  constexpr int DEPTH = ROWS > 2 ? 4 : 8;
+  for (int k0 = wave * 8 + (lane >> 3); k0 < a.K; k0 += DEPTH * 8 * WAVES) {
+    f32x4v wv[DEPTH][2];
+    float xv[DEPTH][ROWS];
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const int k = k0 + d * 8 * WAVES;
+      // columns past the end hold the next row's values, which are not stored
+      const uint32_t off = k < a.K && c < a.F ? ((uint32_t)k * (uint32_t)a.F + (uint32_t)c) * 4u : OOB;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) wv[d][w] = buf_load4(rsrc[w], off);
+#pragma unroll
+      for (int m = 0; m < ROWS; ++m) xv[d][m] = buf_load(xr, k < a.K ? ((uint32_t)m * (uint32_t)a.K + (uint32_t)k) * 4u : OOB);
+    }
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int m = 0; m < ROWS; ++m) acc[w][m] += xv[d][m] * wv[d][w];
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int m = 0; m < ROWS; ++m) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int o = 32; o >= 8; o >>= 1) acc[w][m][j] += __shfl_xor(acc[w][m][j], o, 64);
+      if (lane < 8) part[wave][w][m][lane] = acc[w][m];
+    }
+  __syncthreads();
+  const int m = threadIdx.x / kNarrow, n = blockIdx.x * kNarrow + (int)threadIdx.x % kNarrow;
+  if (m >= ROWS || m >= a.M || n >= a.F) return;
+  float sum[2] = {0.f, 0.f};
+#pragma unroll
+  for (int o = 0; o < WAVES; ++o)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) sum[w] += part[o][w][m][threadIdx.x % kNarrow / 4][threadIdx.x % 4];
+  const size_t at = (size_t)m * a.F + n;
+  if (a.g) {
+    a.g[at] = sum[0];
+    a.u[at] = sum[1];
+  }
+  if (a.h) a.h[at] = act_of<ACT>(sum[0]) * sum[1];
+}
+
+int64_t forward(int M, int K, int F, const float *x, const float *gate, const float *up, float *pre, float *h, int activation,
+                hipStream_t s) {
+  Args a{x, gate, up, pre, pre ? pre + (size_t)M * F : nullptr, h, M, K, F, cdiv(F, kCols), 0, 1, nullptr, nullptr};
+  if (M <= kFewest && K <= 2560) {
+    with_activation(activation, [&](auto act) {
+      hipLaunchKernelGGL((M > 2 ? fewest_kernel<decltype(act)::value, 4> : M > 1 ? fewest_kernel<decltype(act)::value, 2> : fewest_kernel<decltype(act)::value, 1>),
+                         dim3((unsigned)cdiv(F, kNarrow)), dim3(kWide), 0, s, a);
+    });
+    return 0;
+  }
+  const int64_t groups = (int64_t)a.strips * cdiv(M, kRows);
+  // about two workgroups a CU, a wave's run 32 reduction elements at least
+  int pieces = (int)std::max<int64_t>(1, std::min<int64_t>({2 * num_cus() / groups, K / (kWaves * 32), 32}));
+  a.k_per_group = cdiv(K, pieces * kWaves * 8) * kWaves * 8;
+  a.pieces = K ? cdiv(K, a.k_per_group) : 1;
+  if (a.pieces > 1) {
+    const size_t bytes = (size_t)groups * a.pieces * 2 * kRows * kCols * 4;
+    a.tickets = fold_tickets(s);
+    a.scratch = a.tickets ? (float *)device_alloc(bytes, s) : nullptr;
+    if (!a.scratch) return (int64_t)block_bytes(bytes);
+  }
+  with_activation(activation, [&](auto act) {
+    hipLaunchKernelGGL(forward_kernel<decltype(act)::value>, dim3((unsigned)groups, (unsigned)a.pieces), dim3(kThreads), 0, s, a);
+  });
+  if (a.scratch) device_free(a.scratch, s);
+  return 0;
+}
+}  // namespace few
 
 unsigned vectors_grid(int64_t count) { return (unsigned)((count + 4 * kThreads - 1) / (4 * kThreads)); }
 
@@ -733,28 +1006,11 @@ extern "C" int DLGpuGatedFeedForward(const DLArrayHandle input, const DLArrayHan
   hipStream_t s = stream_of(stream);
   TF_REQUIRE(!being_captured(s), "the call takes scratch, which a captured stream cannot give back");
   if (M == 0 || F == 0) return 0;
-  if (on_pairs(M, K, F)) {
-    const int64_t wanted = forward_on_pairs((int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data,
-                                            (const float *)up->data, pre ? (float *)pre->data : nullptr,
-                                            output ? (float *)output->data : nullptr, activation, s);
-    if (wanted && memorytoSaving) *memorytoSaving = shortfall((size_t)wanted);
-    return wanted ? 0 : finish(s, "DLGpuGatedFeedForward");
-  }
-  float *p = pre ? (float *)pre->data : (float *)device_alloc((size_t)M * F * 8, s);
-  if (!p) {
-    if (memorytoSaving) *memorytoSaving = shortfall(block_bytes((size_t)M * F * 8));
-    return 0;
-  }
-  View g(p, M, F, input->ctx), u(p + M * F, M, F, input->ctx);
-  int rc = DLGpuMatrixMultiply(input, false, gate, false, &g.array, nullptr, stream);
-  if (rc == 0) rc = DLGpuMatrixMultiply(input, false, up, false, &u.array, nullptr, stream);
-  if (rc == 0 && output)
-    with_activation(activation, [&](auto act) {
-      hipLaunchKernelGGL(activation_kernel<decltype(act)::value>, dim3(vectors_grid(M * F)), dim3(kThreads), 0, s, p, p + M * F,
-                         (float *)output->data, M * F);
-    });
-  if (!pre) device_free(p, s);
-  return rc != 0 ? rc : finish(s, "DLGpuGatedFeedForward");
+  const int64_t wanted = (forward_on_pairs(M, K, F) ? forward_by_pairs : few::forward)(
+      (int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data, (const float *)up->data,
+      pre ? (float *)pre->data : nullptr, output ? (float *)output->data : nullptr, activation, s);
+  if (wanted && memorytoSaving) *memorytoSaving = shortfall((size_t)wanted);
+  return wanted ? 0 : finish(s, "DLGpuGatedFeedForward");
 }
 
 extern "C" int DLGpuGatedFeedForwardBackward(const DLArrayHandle input, const DLArrayHandle gate, const DLArrayHandle up,
@@ -785,10 +1041,10 @@ extern "C" int DLGpuGatedFeedForwardBackward(const DLArrayHandle input, const DL
   for (const DLArray *written : {(const DLArray *)dinput, (const DLArray *)dgate, (const DLArray *)dup}) announce_write(written);
   hipStream_t s = stream_of(stream);
   TF_REQUIRE(!being_captured(s), "the call takes scratch, which a captured stream cannot give back");
-  if (on_pairs(M, K, F)) {
+  if (backward_on_pairs(M, K, F)) {
     const float *g = pre ? (const float *)pre->data : (const float *)doutput->data;
     const Source d{{g, g + M * F}, pre ? (const float *)doutput->data : nullptr, (int)M, (int)F, pre ? activation : kGiven};
-    const int64_t wanted = backward_on_pairs((int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data,
+    const int64_t wanted = backward_by_pairs((int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data,
                                              (const float *)up->data, d, dinput ? (float *)dinput->data : nullptr,
                                              dgate ? (float *)dgate->data : nullptr, dup ? (float *)dup->data : nullptr, s);
     if (wanted && memorytoSaving) *memorytoSaving = shortfall((size_t)wanted);
