@@ -112,7 +112,7 @@ __global__ __launch_bounds__(kThreads) void dropout_kernel(const float *__restri
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4u __attribute__((aligned(4)));
 constexpr int kBlocksPerLane = 4;
-template <bool RESIDUAL>
+template <bool RESIDUAL, bool PAST>
 __global__ __launch_bounds__(kThreads) void counter_dropout_kernel(const float *in, const float *residual, float *out,
                                                                   int64_t count, uint64_t seed, uint64_t offset,
                                                                   uint32_t threshold, float scale) {
@@ -145,7 +145,8 @@ __global__ __launch_bounds__(kThreads) void counter_dropout_kernel(const float *
       if (RESIDUAL) o[j] += r[e][j];
     }
     if (i + 4 <= count) {
-      *reinterpret_cast<f32x4u *>(out + i) = o;
+      if (PAST) __builtin_nontemporal_store(o, reinterpret_cast<f32x4u *>(out + i));
+      else *reinterpret_cast<f32x4u *>(out + i) = o;
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -315,8 +316,11 @@ extern "C" int DLGpuCounterDropout(const DLArrayHandle input, const DLArrayHandl
   const uint32_t threshold = (uint32_t)((double)dropout * 4294967296.0);
   const float scale = 1.0f / (1.0f - dropout);
   const float *x = (const float *)input->data, *r = residual ? (const float *)residual->data : nullptr;
-  hipLaunchKernelGGL(residual ? counter_dropout_kernel<true> : counter_dropout_kernel<false>, dim3((unsigned)groups),
-                     dim3(kThreads), 0, s, x, r, (float *)output->data, count, seed, offset, threshold, scale);
+  // half of what the L2s hold together, and more, goes past them: 67 MB 24.5 -> 20.5 us (6.5 TB/s)
+  const bool past = count * 4 >= (int64_t)16 << 20;
+  hipLaunchKernelGGL((residual ? past ? counter_dropout_kernel<true, true> : counter_dropout_kernel<true, false>
+                               : past ? counter_dropout_kernel<false, true> : counter_dropout_kernel<false, false>),
+                     dim3((unsigned)groups), dim3(kThreads), 0, s, x, r, (float *)output->data, count, seed, offset, threshold, scale);
   return finish(s, "DLGpuCounterDropout");
 }
 

@@ -375,7 +375,12 @@ __global__ __launch_bounds__(kThreads) void split_kernel(const Jobs jobs) {
 }
 
 // ---- the products' ends ------------------------------------------------------------------------------------
-// Stores past the last row fall behind the buffer, those past the last column are sent there.
+// Stores past the last row fall behind the buffer, those past the last column are sent there.  They go past the caches, which hold
+// the operands: 4 096 x 1 024 x 4 096 forward 227 -> 216 us, the sublayer that reads h next 277 -> 276.
+__device__ inline void store_past(__amdgpu_buffer_rsrc_t r, uint32_t byte_off, float v) {
+  constexpr int NT = 2;  // in the cache-policy operand
+  __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(int, v), r, (int)byte_off, 0, NT);
+}
 struct Rows {
   __amdgpu_buffer_rsrc_t rsrc;
   __device__ inline Rows(float *out, int m0, int rows, int cols)
@@ -398,10 +403,10 @@ struct StoreGated {
       const int f = (block + j) / 2 * 32 + lcol;
       const uint32_t off = f < cols ? ((uint32_t)m * (uint32_t)cols + (uint32_t)f) * 4u : OOB;
       if (g) {  // uniform
-        buf_store(s.g.rsrc, off, v[j]);
-        buf_store(s.u.rsrc, off, v[j + 1]);
+        store_past(s.g.rsrc, off, v[j]);
+        store_past(s.u.rsrc, off, v[j + 1]);
       }
-      if (h) buf_store(s.h.rsrc, off, act_of<ACT>(v[j]) * v[j + 1]);
+      if (h) store_past(s.h.rsrc, off, act_of<ACT>(v[j]) * v[j + 1]);
     }
   }
 };
@@ -415,7 +420,7 @@ struct StoreHalves {
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
       const int n = (block + j) * 32 + lcol;
-      buf_store(s.rsrc, n < cols ? ((uint32_t)m * (uint32_t)cols + (uint32_t)n) * 4u : OOB, v[j]);
+      store_past(s.rsrc, n < cols ? ((uint32_t)m * (uint32_t)cols + (uint32_t)n) * 4u : OOB, v[j]);
     }
   }
 };

@@ -8,18 +8,21 @@
 // Nothing is kept between the two passes: the backward pass has the row of x in registers anyway and computes mu and s
 // again from there, which moves no byte, and neither pass depends on the other having run.
 //
-// Bound: HBM.  A row is read once into registers, by a wave or, from 1 024 / 2 048 columns on, by a workgroup, and both
+// Bound: HBM.  A row is read once into registers, by a wave or by as many waves as it takes, and both
 // statistics are taken from there, the squares after the mean is known (a sum of x^2 would cancel where the mean is
 // large).  Sums are divided by the column count, not multiplied by its reciprocal: a row of one value then has that value for
 // its mean.  All sums are fp32; their order depends on the shape alone.
 #include "internal.h"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace tf;
 
 namespace {
 
+template <int V>
+using IC = std::integral_constant<int, V>;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4u __attribute__((aligned(4)));  // rows of any length start anywhere: 16-byte accesses on 4-byte alignment
 
@@ -29,12 +32,13 @@ __device__ inline float wave_sum(float v) {
   return v;
 }
 
-// Sum over the T lanes that share a row; `room` is T / 64 floats that nobody else uses until the next barrier but one.
+// Sum over the T lanes that share a row; `room` is T / 64 floats of that row's that nothing else uses until the next barrier but
+// one.  Rows of several waves pass a barrier: all rows of a workgroup get here together.
 template <int T>
 __device__ inline float row_sum(float v, float *room) {
   v = wave_sum(v);
   if constexpr (T > 64) {
-    if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) room[threadIdx.x % T / 64] = v;
     __syncthreads();
     v = 0.f;
 #pragma unroll
@@ -62,12 +66,14 @@ struct Row {
       }
     }
   }
+  template <bool PAST = false>
   __device__ inline void store(float *__restrict__ row, int cols, int lane) const {
 #pragma unroll
     for (int e = 0; e < VPT; ++e) {
       const int c = 4 * (e * T + lane);
       if (c + 4 <= cols) {
-        *reinterpret_cast<f32x4u *>(row + c) = v[e];
+        if (PAST) __builtin_nontemporal_store(v[e], reinterpret_cast<f32x4u *>(row + c));
+        else *reinterpret_cast<f32x4u *>(row + c) = v[e];
       } else if (c < cols) {
         row[c] = v[e][0];
         if (c + 1 < cols) row[c + 1] = v[e][1];
@@ -101,7 +107,7 @@ __device__ inline float inverse_std(float square_sum, float n, float eps) {
 }
 
 // T lanes a row, WG / T rows a workgroup.
-template <int T, int VPT>
+template <int T, int VPT, bool PAST>
 __global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
                                                                   const float *__restrict__ beta, float *__restrict__ y,
                                                                   int64_t rows, int cols, float n, float eps) {
@@ -118,7 +124,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float 
   const float s = inverse_std(row_sum<T>(row.dot(row), room[1]), n, eps);
 #pragma unroll
   for (int e = 0; e < VPT; ++e) row.v[e] = row.v[e] * s * g.v[e] + b.v[e];
-  row.store(y + r * cols, cols, lane);
+  row.template store<PAST>(y + r * cols, cols, lane);
 }
 
 // Rows that do not fit registers: three passes, the later two mostly out of the caches.
@@ -141,30 +147,41 @@ __global__ __launch_bounds__(kLong) void forward_long_kernel(const float *__rest
   for (int c = threadIdx.x; c < cols; c += kLong) out[c] = (row[c] - mean) * istd * gamma[c] + beta[c];
 }
 
-// Rows blockIdx.x * (WG / T) + ..., then gridDim.x * (WG / T) further on, and so on: every lane keeps the sums of dy xh and
-// dy of its columns over the rows that it sees.  At the end the workgroup's rows are added through LDS, in their order, and
-// go to partial[blockIdx.x][2][cols].
-template <int T, int VPT, bool PARAMS>
-__global__ __launch_bounds__(T > 256 ? T : 256) void backward_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
-                                                                   const float *__restrict__ dy, float *__restrict__ dx,
-                                                                   float *__restrict__ partial, int64_t rows, int cols,
-                                                                   float n, float eps) {
-  constexpr int WG = T > 256 ? T : 256, ROWS = WG / T;
-  __shared__ float room[3][T / 64][2];
-  const int lane = threadIdx.x % T, sub = threadIdx.x / T;
-  Row<T, VPT> g, dgamma, dbeta;
-  if (dx) g.load(gamma, cols, lane);
+// Rows blockIdx.x * (WG / T) + ..., then gridDim.x * (WG / T) further on, and so on, the next one on its way while one is worked
+// on: every lane keeps the sums of dy xh and dy of its columns over the rows that it sees.  At the end the workgroup's rows are
+// added through LDS, in their order, and go to partial[blockIdx.x][2][cols].
+template <int T, int VPT, int WG, bool PARAMS, bool PAST>
+__global__ __launch_bounds__(WG) void backward_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
+                                                    const float *__restrict__ dy, float *__restrict__ dx,
+                                                    float *__restrict__ partial, int64_t rows, int cols, float n, float eps) {
+  constexpr int ROWS = WG / T;
+  constexpr bool HOLD = T * VPT < 4096;  // gamma in registers; else from the caches, row by row
+  __shared__ float rooms[ROWS][3][T / 64][2];
+  const int lane = threadIdx.x % T, sub = threadIdx.x / T, wave = lane / 64;
+  auto &room = rooms[sub];
+  const int64_t step = (int64_t)gridDim.x * ROWS;
+  Row<T, VPT> g, dgamma, dbeta, xh, d;
+  if (dx && HOLD) g.load(gamma, cols, lane);
 #pragma unroll
   for (int e = 0; e < VPT; ++e) dgamma.v[e] = dbeta.v[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int64_t r = (int64_t)blockIdx.x * ROWS + sub; r < rows; r += (int64_t)gridDim.x * ROWS) {
-    Row<T, VPT> xh, d;
-    xh.load(x + r * cols, cols, lane);
-    d.load(dy + r * cols, cols, lane);
+  // a row behind the last one is worked on for the barriers' sake, on the last one's values, and left out of everything
+  auto load = [&](int64_t r, Row<T, VPT> &of_x, Row<T, VPT> &of_dy) {
+    r = r < rows ? r : rows - 1;
+    of_x.load(x + r * cols, cols, lane);
+    of_dy.load(dy + r * cols, cols, lane);
+  };
+  int64_t first = (int64_t)blockIdx.x * ROWS;
+  if (first < rows) load(first + sub, xh, d);
+  for (; first < rows; first += step) {
+    const int64_t r = first + sub;
+    const bool live = r < rows;  // of whole waves
+    Row<T, VPT> next_x, next_d;
+    if (first + step < rows) load(r + step, next_x, next_d);
     xh.subtract(row_sum<T>(xh.sum(), &room[0][0][0]) / n, cols, lane);
     const float s = inverse_std(row_sum<T>(xh.dot(xh), &room[1][0][0]), n, eps);
 #pragma unroll
     for (int e = 0; e < VPT; ++e) xh.v[e] *= s;
-    if (PARAMS) {
+    if (PARAMS && live) {
 #pragma unroll
       for (int e = 0; e < VPT; ++e) {
         dgamma.v[e] += d.v[e] * xh.v[e];
@@ -172,13 +189,14 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void backward_kernel(const float
       }
     }
     if (dx) {
+      if (!HOLD) g.load(gamma, cols, lane);
 #pragma unroll
       for (int e = 0; e < VPT; ++e) d.v[e] *= g.v[e];
       float a = wave_sum(d.sum()), b = wave_sum(d.dot(xh));
       if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) {
-          room[2][threadIdx.x >> 6][0] = a;
-          room[2][threadIdx.x >> 6][1] = b;
+          room[2][wave][0] = a;
+          room[2][wave][1] = b;
         }
         __syncthreads();
         a = b = 0.f;
@@ -192,8 +210,10 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void backward_kernel(const float
       b /= n;
 #pragma unroll
       for (int e = 0; e < VPT; ++e) d.v[e] = (d.v[e] - a - xh.v[e] * b) * s;
-      d.store(dx + r * cols, cols, lane);
+      if (live) d.template store<PAST>(dx + r * cols, cols, lane);
     }
+    xh = next_x;
+    d = next_d;
   }
   if constexpr (PARAMS) {
     if constexpr (ROWS > 1) {
@@ -324,6 +344,11 @@ int geometry(const char *what, const DLArray *x, const DLArray *gamma, int64_t &
   return 0;
 }
 
+// Results of half of what the L2s hold together and more go past them: forward of 8 192 x 2 048 29.2 -> 22.0 us, backward of
+// 5 003 x 1 537 22.9 -> 20.4, of 4 096 x 1 024 13.2 -> 11.8; of smaller ones the next reader finds a part, and the writer gains
+// nothing (forward of 1 024 x 2 048 4.6 and 4.4).
+bool past_caches(int64_t elements) { return elements * 4 >= (int64_t)16 << 20; }
+
 constexpr int kMaxForward = 16384, kMaxBackward = 16384;  // columns that registers hold
 
 }  // namespace
@@ -345,17 +370,18 @@ extern "C" int DLGpuLayerNormalizationForward(const DLArrayHandle input, const D
   const float *x = (const float *)input->data, *g = (const float *)gamma->data, *b = (const float *)beta->data;
   float *y = (float *)output->data;
   const float n = (float)cols;
-  auto go = [&](auto kernel, int wg, int rows_a_group) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + rows_a_group - 1) / rows_a_group)), dim3(wg), 0, s, x, g, b, y, rows,
-                       (int)cols, n, eps);
+  auto go = [&](auto t, auto vectors) {
+    constexpr int T = decltype(t)::value, VPT = decltype(vectors)::value, WG = T > 256 ? T : 256, ROWS = WG / T;
+    hipLaunchKernelGGL((past_caches(rows * cols) ? forward_kernel<T, VPT, true> : forward_kernel<T, VPT, false>),
+                       dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(WG), 0, s, x, g, b, y, rows, (int)cols, n, eps);
   };
-  if (cols <= 256) go(forward_kernel<64, 1>, 256, 4);
-  else if (cols <= 512) go(forward_kernel<64, 2>, 256, 4);
-  else if (cols <= 1024) go(forward_kernel<64, 4>, 256, 4);
-  else if (cols <= 2048) go(forward_kernel<256, 2>, 256, 1);
-  else if (cols <= 4096) go(forward_kernel<256, 4>, 256, 1);
-  else if (cols <= 8192) go(forward_kernel<1024, 2>, 1024, 1);
-  else if (cols <= kMaxForward) go(forward_kernel<1024, 4>, 1024, 1);
+  if (cols <= 256) go(IC<64>{}, IC<1>{});
+  else if (cols <= 512) go(IC<64>{}, IC<2>{});
+  else if (cols <= 1024) go(IC<256>{}, IC<1>{});
+  else if (cols <= 2048) go(IC<256>{}, IC<2>{});
+  else if (cols <= 4096) go(IC<256>{}, IC<4>{});
+  else if (cols <= 8192) go(IC<1024>{}, IC<2>{});
+  else if (cols <= kMaxForward) go(IC<1024>{}, IC<4>{});
   else
     hipLaunchKernelGGL(forward_long_kernel, dim3((unsigned)rows), dim3(kLong), 0, s, x, g, b, y, (int)cols, n, eps);
   return finish(s, "DLGpuLayerNormalizationForward");
@@ -383,11 +409,12 @@ extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const 
   const bool params = dgamma || dbeta, in_registers = cols <= kMaxBackward;
   TF_REQUIRE(!params || !being_captured(s), "the gradients of the weights take scratch, which a captured stream cannot give back");
 
-  // How many workgroups share the rows, each with a partial sum of the weights' gradients.
-  const int rows_a_group = in_registers && cols <= 1024 ? 4 : 1;
+  // How many workgroups share the rows, each with a partial sum of the weights' gradients: as many as are resident.  us at 256 / 512 /
+  // 768 / 1 024: 4 096 x 1 024 15.1 / 13.1 / - / 15.1, 5 003 x 1 537 35.8 / 24.4 / 22.7 / 28.1, 4 096 x 4 096 54 / 41 / - / 46.
+  const int rows_a_group = !in_registers ? 1 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1;
   const int64_t groups = (rows + rows_a_group - 1) / rows_a_group;
   int pieces = 0;
-  if (in_registers) pieces = (int)std::min<int64_t>(groups, params ? 2 * num_cus() : 0x7fffffff);
+  if (in_registers) pieces = (int)std::min<int64_t>(groups, params ? (cols <= 1024 ? 2 : cols <= 2048 ? 3 : cols <= 4096 ? 2 : 1) * num_cus() : 0x7fffffff);
   else if (rows) pieces = (int)std::min<int64_t>((rows + 3) / 4, std::max<int64_t>(1, 4 * num_cus() * 64 / cols));
   float *partial = nullptr, *stats = nullptr;
   if (params && rows) {
@@ -403,17 +430,20 @@ extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const 
   float *dx = dinput ? (float *)dinput->data : nullptr;
   const float n = (float)cols;
   if (rows) {
-    auto go = [&](auto with, auto without, int wg) {
-      hipLaunchKernelGGL(params ? with : without, dim3((unsigned)pieces), dim3(wg), 0, s, x, g, dy, dx, partial, rows,
-                         (int)cols, n, eps);
+    auto go = [&](auto t, auto vectors) {
+      constexpr int T = decltype(t)::value, VPT = decltype(vectors)::value, WG = T > 256 ? T : 256;
+      const bool past = past_caches(rows * cols);
+      hipLaunchKernelGGL((params ? past ? backward_kernel<T, VPT, WG, true, true> : backward_kernel<T, VPT, WG, true, false>
+                                 : past ? backward_kernel<T, VPT, WG, false, true> : backward_kernel<T, VPT, WG, false, false>),
+                         dim3((unsigned)pieces), dim3(WG), 0, s, x, g, dy, dx, partial, rows, (int)cols, n, eps);
     };
-    if (cols <= 256) go(backward_kernel<64, 1, true>, backward_kernel<64, 1, false>, 256);
-    else if (cols <= 512) go(backward_kernel<64, 2, true>, backward_kernel<64, 2, false>, 256);
-    else if (cols <= 1024) go(backward_kernel<64, 4, true>, backward_kernel<64, 4, false>, 256);
-    else if (cols <= 2048) go(backward_kernel<256, 2, true>, backward_kernel<256, 2, false>, 256);
-    else if (cols <= 4096) go(backward_kernel<256, 4, true>, backward_kernel<256, 4, false>, 256);
-    else if (cols <= 8192) go(backward_kernel<1024, 2, true>, backward_kernel<1024, 2, false>, 1024);
-    else if (in_registers) go(backward_kernel<1024, 4, true>, backward_kernel<1024, 4, false>, 1024);
+    if (cols <= 256) go(IC<64>{}, IC<1>{});
+    else if (cols <= 512) go(IC<64>{}, IC<2>{});
+    else if (cols <= 1024) go(IC<64>{}, IC<4>{});
+    else if (cols <= 2048) go(IC<128>{}, IC<4>{});
+    else if (cols <= 4096) go(IC<512>{}, IC<2>{});
+    else if (cols <= 8192) go(IC<1024>{}, IC<2>{});
+    else if (in_registers) go(IC<1024>{}, IC<4>{});
     else {
       hipLaunchKernelGGL(backward_long_kernel, dim3((unsigned)rows), dim3(kLong), 0, s, x, g, dy, dx, stats, (int)cols, n, eps);
       if (params)
