@@ -556,7 +556,8 @@ class SwapExecutor(object):
                         for t, ids in table.items()} for table in self.wire_schedule]
             self.swap_out_at, self.swap_in_at, self.release_at, self.recompute_at = by_node
             return
-        cheap = (ad.BNForwardOp, ad.ActivationForwardOp, ad.ReluOp)
+        cheap = (ad.BNForwardOp, ad.ActivationForwardOp, ad.ReluOp, ad.LayerNormForwardOp, ad.GatedActivationOp,
+                 ad.CounterDropoutOp)
         again = (lambda n: isinstance(n.op, cheap)) if (self.swap and self.recompute) else None
         timing = {}
         if self.host_link_bytes_per_second:
@@ -596,6 +597,10 @@ class SwapExecutor(object):
             flops = 2.0 * np.prod(y, dtype=np.float64) * w[1] * w[2] * w[3]
             if w[2] == 3 and w[3] == 3 and getattr(node, "u", 1) == 1 and getattr(node, "v", 1) == 1:
                 rate = 200e12
+        elif isinstance(node.op, (ad.GatedProjectionOp, ad.GatedBackwardOp)):
+            # both projections; dx, or one of the two weights' gradients
+            rows, (width, inner) = self.tensors[node.inputs[0]].shape[0], self.tensors[node.inputs[1]].shape
+            flops, rate = (2.0 if getattr(node, "type", 0) else 4.0) * rows * width * inner, 300e12
         elif isinstance(node.op, ad.MatMulOp):
             a = self.tensors[node.inputs[0]].shape
             flops = 2.0 * np.prod(self.tensors[node].shape, dtype=np.float64) * (a[0] if node.matmul_attr_trans_A
@@ -770,13 +775,13 @@ class SwapExecutor(object):
             return
         input_vals = [self._on_gpu(self.tensors[i], node.inputs) for i in node.inputs]
         out = self._alloc(t.shape, node.name + " (recompute)", node.inputs)
-        wanted = node.op.compute(node, input_vals, out, *handles)
+        wanted = node.op.compute_again(node, input_vals, out, *handles)
         for _ in range(3):
             if not wanted:
                 break
             # no room for the op's scratch (a convolution): make room and run it again
             self._alloc(((int(wanted) + 3) // 4,), node.name + " scratch", node.inputs).free_gpu()
-            wanted = node.op.compute(node, input_vals, out, *handles)
+            wanted = node.op.compute_again(node, input_vals, out, *handles)
         if wanted:
             raise MemoryError("%s: %d bytes of device scratch could not be allocated" % (node.name, wanted))
         t.gpu, t.state = out, GPU

@@ -110,13 +110,21 @@ class TrainExecutor(object):
         in_group = {n for members in groups.values() for n in members}
         joined = {n: r for n, r in joined.items() if n not in in_group}
         by_join = set(joined.values())
+        siblings = find_siblings(self.topo_order, set(feed_dict) | unread_zeros)
+        by_sibling = {n for members in siblings.values() for n in members[1:]}
         for node in self.topo_order:
             if node in groups:
                 for n in groups[node]:
                     self.node_to_arr_map[n] = self._alloc(self.node_to_shape_map[n])
                 plan.append((_group_compute(groups[node], self.node_to_shape_map, self.node_to_arr_map), node, None, None))
-            if node in by_join or node in in_group:
-                continue   # computed with its first operand, or with the first of its group
+            if node in by_join or node in in_group or node in by_sibling:
+                continue   # computed with its first operand, or with the first of its group or of its siblings
+            if node in siblings:
+                members = siblings[node]
+                outputs = [self._alloc(self.node_to_shape_map[n]) for n in members]
+                self.node_to_arr_map.update(zip(members, outputs))
+                plan.append((_sibling_compute(members), node, [self.node_to_arr_map[i] for i in node.inputs], outputs))
+                continue
             if node in joined:
                 reader = joined[node]
                 outputs = [self._alloc(self.node_to_shape_map[n]) for n in (node, reader)]
@@ -532,6 +540,44 @@ def find_groups(topo_order, shapes, unavailable, roles, joins):
             groups[first] = members
             taken |= set(members)
     return groups
+
+
+def find_siblings(topo_order, unavailable):
+    """Nodes that one call computes: the gradients of a layer norm or of a gated feed-forward product, which have the same
+    inputs, and a gated product with the projections that it is made of.  Returns first node -> all of them, in order; they
+    run at the first one's place, where its inputs are there and no parameter that they read has been updated, since updates stand behind
+    the last reader.  Every array holds what it would."""
+    siblings, first_of = {}, {}
+    for n in topo_order:
+        if n in unavailable:
+            continue
+        if isinstance(n.op, (ad.LayerNormBackwardOp, ad.GatedBackwardOp)):
+            key = (n.op, tuple(n.inputs), n.eps if isinstance(n.op, ad.LayerNormBackwardOp) else n.activation)
+        elif isinstance(n.op, ad.GatedProjectionOp):
+            key = n
+        elif isinstance(n.op, ad.GatedActivationOp) and n.inputs[0] in first_of:
+            key = n.inputs[0]
+        else:
+            continue
+        first = first_of.setdefault(key, n)
+        members = siblings.setdefault(first, [])
+        # a second node for the same value keeps its own call
+        if not any(type(m.op) is type(n.op) and getattr(m, "type", None) == getattr(n, "type", None) for m in members):
+            members.append(n)
+    return {first: members for first, members in siblings.items() if len(members) > 1}
+
+
+def _sibling_compute(members):
+    """Plan entry (same signature as ``Op.compute``) of such nodes: ``output_val`` are the arrays of all."""
+    if isinstance(members[0].op, ad.GatedProjectionOp):
+        def compute(node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream):
+            return gpu_op.gated_feed_forward(*input_vals, *output_val, members[1].activation, cudaStream)
+    else:
+        types = [n.type for n in members]
+
+        def compute(node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream):
+            return node.op.compute_several(dict(zip(types, output_val)), node, input_vals, cudaStream)
+    return compute
 
 
 def _group_compute(members, shapes, arrays):

@@ -82,6 +82,10 @@ class Op(object):
         scratch bytes that could not be allocated."""
         raise NotImplementedError
 
+    def compute_again(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream):
+        """The value that ``compute`` gave this step once more, where a planner had it released."""
+        return self.compute(node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream)
+
     def gradient(self, node, output_grad):
         """Nodes computing the gradient with respect to each input."""
         raise NotImplementedError
@@ -817,6 +821,203 @@ class FullyBNForwardOp(BNForwardOp):
         return (shape[0], 1, shape[1])
 
 
+# ------------------ layer norm, gated feed-forward, counter dropout (no counterparts in the reference)
+
+class LayerNormForwardOp(Op):
+    """gamma * (x - mean) / sqrt(variance + eps) + beta over the last axis.  Keeps nothing for the backward nodes."""
+
+    def __call__(self, node_A, gamma, beta, eps=1e-5):
+        node = Op.__call__(self)
+        node.inputs = [node_A, gamma, beta]
+        node.name = "LayerNormForward"
+        node.eps = eps
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        gpu_op.layer_norm_forward(*input_vals, output_val, node.eps, cudaStream)
+        return 0
+
+    def gradient(self, node, output_grad):
+        x, gamma, _ = node.inputs
+        return [layer_norm_backward_op(x, gamma, output_grad, type, node.eps) for type in range(3)]
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        x, gamma, beta = input_shapes
+        if tuple(gamma) != tuple(x[-1:]) or tuple(beta) != tuple(gamma):
+            raise ValueError("layer norm: gamma %s and beta %s for an input %s" % (gamma, beta, x))
+        return x
+
+
+class LayerNormBackwardOp(Op):
+    """inputs: x, gamma, dy; type 0: gradient w.r.t. x, 1: gamma, 2: beta"""
+
+    def __call__(self, node_A, gamma, node_C, type, eps):
+        node = Op.__call__(self)
+        node.inputs = [node_A, gamma, node_C]
+        node.name = "LayerNormBackward"
+        node.type = type
+        node.eps = eps
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        return self.compute_several({node.type: output_val}, node, input_vals, cudaStream)
+
+    @staticmethod
+    def compute_several(outputs, node, input_vals, cudaStream):
+        """Those of the three gradients that ``outputs`` has, by type, in one call."""
+        return gpu_op.layer_norm_backward(*input_vals, *[outputs.get(type) for type in range(3)], node.eps, cudaStream)
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[0] if node.type == 0 else input_shapes[1]
+
+
+class GatedProjectionOp(Op):
+    """Both projections of a gated feed-forward product, x gate and x up, stacked: (2, rows, columns)."""
+
+    def __call__(self, node_A, gate, up):
+        node = Op.__call__(self)
+        node.inputs = [node_A, gate, up]
+        node.name = "GatedProjection"
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        # without a product the activation does not matter
+        return gpu_op.gated_feed_forward(*input_vals, output_val, None, "relu", cudaStream)
+
+    def gradient(self, node, output_grad):
+        if isinstance(output_grad.op, GatedActivationBackwardOp) and output_grad.inputs[0] is node:
+            # the product's only reader: its gradient is computed on the way, and never stored
+            return [gated_backward_op(*node.inputs, node, output_grad.inputs[1], type, output_grad.activation)
+                    for type in range(3)]
+        return [gated_backward_op(*node.inputs, None, output_grad, type, None) for type in range(3)]
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        x, gate, up = input_shapes
+        if len(x) != 2 or len(gate) != 2 or tuple(gate) != tuple(up) or x[1] != gate[0]:
+            raise ValueError("gated feed-forward: weights %s and %s for an input %s" % (gate, up, x))
+        return (2, x[0], gate[1])
+
+
+class GatedActivationOp(Op):
+    """activation(pre[0]) * pre[1] of stacked projections."""
+
+    def __call__(self, node_A, activation):
+        node = Op.__call__(self)
+        node.inputs = [node_A]
+        node.name = "GatedActivation"
+        node.activation = activation
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        gpu_op.gated_activation(input_vals[0], output_val, node.activation, cudaStream)
+        return 0
+
+    def gradient(self, node, output_grad):
+        return [gated_activation_backward_op(node.inputs[0], output_grad, node.activation)]
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return tuple(input_shapes[0][1:])
+
+
+class GatedActivationBackwardOp(Op):
+    """inputs: pre, dy"""
+
+    def __call__(self, node_A, node_B, activation):
+        node = Op.__call__(self)
+        node.inputs = [node_A, node_B]
+        node.name = "GatedActivationBackward"
+        node.activation = activation
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        gpu_op.gated_activation_backward(input_vals[0], input_vals[1], output_val, node.activation, cudaStream)
+        return 0
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[0]
+
+
+class GatedBackwardOp(Op):
+    """inputs: x, gate, up, pre, dy with the product's gradient dy, or x, gate, up, dpre with the stacked projections'
+    (``pre`` and the activation None); type 0: gradient w.r.t. x, 1: gate, 2: up"""
+
+    def __call__(self, node_A, gate, up, pre, node_E, type, activation):
+        node = Op.__call__(self)
+        node.inputs = [node_A, gate, up] + ([] if pre is None else [pre]) + [node_E]
+        node.name = "GatedBackward"
+        node.type = type
+        node.activation = activation
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        return self.compute_several({node.type: output_val}, node, input_vals, cudaStream)
+
+    @staticmethod
+    def compute_several(outputs, node, input_vals, cudaStream):
+        """Those of the three gradients that ``outputs`` has, by type, in one call."""
+        x, gate, up = input_vals[:3]
+        pre = None if node.activation is None else input_vals[3]
+        return gpu_op.gated_feed_forward_backward(x, gate, up, pre, input_vals[-1],
+                                                  *[outputs.get(type) for type in range(3)],
+                                                  node.activation or "relu", cudaStream)
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[node.type]
+
+
+class CounterDropoutOp(Op):
+    """dropout(x), plus a residual if there is one, with a mask that is never stored: it is drawn from a counter, which
+    every evaluation advances, and a seed, by default from Python's ``random`` module; the backward node draws it again."""
+
+    def __call__(self, node_A, dropout, residual=None, seed=None):
+        node = Op.__call__(self)
+        node.inputs = [node_A] + ([] if residual is None else [residual])
+        node.name = "CounterDropout"
+        node.dropout = dropout
+        node.draw = [random.getrandbits(64) if seed is None else seed, -1]  # shared with the backward node
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        node.draw[1] = (node.draw[1] + 1) % 2 ** 64
+        return self.compute_again(node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream)
+
+    def compute_again(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream):
+        residual = input_vals[1] if len(input_vals) > 1 else None
+        gpu_op.counter_dropout(input_vals[0], residual, output_val, node.dropout, *node.draw, cudaStream)
+        return 0
+
+    def gradient(self, node, output_grad):
+        grads = [counter_dropout_backward_op(output_grad, node.dropout, node.draw), output_grad]
+        return grads[:len(node.inputs)]
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[0]
+
+
+class CounterDropoutBackwardOp(Op):
+    def __call__(self, node_A, dropout, draw):
+        node = Op.__call__(self)
+        node.inputs = [node_A]
+        node.name = "CounterDropoutBackward"
+        node.dropout = dropout
+        node.draw = draw
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        gpu_op.counter_dropout(input_vals[0], None, output_val, node.dropout, *node.draw, cudaStream)
+        return 0
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[0]
+
+
 # -------------------------------------------------------------------- optimizer
 
 class SgdOp(Op):
@@ -869,6 +1070,11 @@ def dense(X, W, b):
     """X W + broadcast(b)   (reference autodiff.py:2126-2129)"""
     xw = matmul_op(X, W)
     return xw + broadcastto_op(b, xw)
+
+
+def gated_feed_forward(X, gate, up, activation="silu"):
+    """activation(X gate) * (X up), "sigmoid", "relu", "silu" or "gelu" (no counterpart in the reference)"""
+    return gated_activation_op(gated_projection_op(X, gate, up), activation)
 
 
 def conv2withbias(input, filter, bias, dataformat, padding, strideh, stridew):
@@ -1046,6 +1252,14 @@ pooling_2d_backward_op = Pooling2DBackwardOp()
 bn_forward_op = BNForwardOp()
 bn_backward_op = BNBackwardOp()
 fullybn_forward_op = FullyBNForwardOp()
+layer_norm_forward_op = LayerNormForwardOp()
+layer_norm_backward_op = LayerNormBackwardOp()
+gated_projection_op = GatedProjectionOp()
+gated_activation_op = GatedActivationOp()
+gated_activation_backward_op = GatedActivationBackwardOp()
+gated_backward_op = GatedBackwardOp()
+counter_dropout_op = CounterDropoutOp()
+counter_dropout_backward_op = CounterDropoutBackwardOp()
 sgd_op = SgdOp()
 adam_op = AdamOp()
 dropout_forward_op = DropoutForwardOp()

@@ -567,7 +567,10 @@ bool backward_on_pairs(int64_t M, int64_t K, int64_t F) {
   return M > 0 && K > 0 && F > 0 && K < 1 << 22 && F < 1 << 22 && (M >= 128 || K * F <= 1 << 20);
 }
 
-// 0, -1, or the bytes of scratch that could not be had
+// Scratch goes back to the pool when a call returns; a graph would go on using it.
+constexpr int64_t kCaptured = -1;
+
+// These return 0, the bytes of scratch that could not be had, or kCaptured.
 int64_t forward_by_pairs(int M, int K, int F, const float *x, const float *gate, const float *up, float *pre, float *h, int activation,
                          hipStream_t s) {
   Layout l;
@@ -579,6 +582,7 @@ int64_t forward_by_pairs(int M, int K, int F, const float *x, const float *gate,
   const PackedAt a(l, cdiv(M, 32), steps_of(K)), b(l, 2 * f_blocks, steps_of(K));
   pair::Work work = tiles_of(a.blocks, b.blocks, 1);
   const size_t scratch = cut(l, work, a.steps, steps_a_group({{work, a.steps}}));
+  if (being_captured(s)) return kCaptured;
   unsigned *tickets = fold_tickets(s);
   char *base = tickets ? (char *)device_alloc(l.bytes, s) : nullptr;
   if (!base) return (int64_t)block_bytes(l.bytes);
@@ -904,6 +908,7 @@ int64_t forward(int M, int K, int F, const float *x, const float *gate, const fl
   a.pieces = K ? cdiv(K, a.k_per_group) : 1;
   if (a.pieces > 1) {
     const size_t bytes = (size_t)groups * a.pieces * 2 * kRows * kCols * 4;
+    if (being_captured(s)) return kCaptured;
     a.tickets = fold_tickets(s);
     a.scratch = a.tickets ? (float *)device_alloc(bytes, s) : nullptr;
     if (!a.scratch) return (int64_t)block_bytes(bytes);
@@ -1009,11 +1014,11 @@ extern "C" int DLGpuGatedFeedForward(const DLArrayHandle input, const DLArrayHan
   if (pre) announce_write(pre);
   if (output) announce_write(output);
   hipStream_t s = stream_of(stream);
-  TF_REQUIRE(!being_captured(s), "the call takes scratch, which a captured stream cannot give back");
   if (M == 0 || F == 0) return 0;
   const int64_t wanted = (forward_on_pairs(M, K, F) ? forward_by_pairs : few::forward)(
       (int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data, (const float *)up->data,
       pre ? (float *)pre->data : nullptr, output ? (float *)output->data : nullptr, activation, s);
+  TF_REQUIRE(wanted != kCaptured, "the call takes scratch, which a captured stream cannot give back");
   if (wanted && memorytoSaving) *memorytoSaving = shortfall((size_t)wanted);
   return wanted ? 0 : finish(s, "DLGpuGatedFeedForward");
 }
