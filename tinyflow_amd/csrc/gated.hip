@@ -662,21 +662,39 @@ int64_t backward_by_pairs(int M, int K, int F, const float *x, const float *gate
 
 // ---- few rows ---------------------------------------------------------------------------------------------------
 // Both projections, the activation and the product for up to 32 rows a workgroup, bound by reading the weights: nothing is staged.
-// A wave owns 128 columns of both weights and a run of the reduction; a load is 512 bytes of two of their rows, the four
-// columns of a lane are four fp32 matrix instructions' operands (columns 4 (lane mod 32) + j of the j-th), so that the lanes'
-// order costs nothing, and eight instructions use one value of x.  In a group of eight reduction elements lanes 0..31 hold
-// the first four and lanes 32..63 the others.  The four waves of a workgroup have four runs of the reduction, added
-// through LDS, and several workgroups more of them, added by the last one to finish (gemm_core.h: Fold), in their order.
+// A wave owns 32 C columns of both weights and a run of the reduction; the C columns of a lane's load are the operands of C
+// fp32 matrix instructions (columns C (lane mod 32) + j of the j-th), so that the lanes' order costs nothing, and 2 C
+// instructions use one value of x.  In a group of eight reduction elements lanes 0..31 hold the first four and lanes 32..63 the
+// others; DEPTH groups are under way.  The waves of a workgroup have runs of their own, added through LDS, and several workgroups
+// more of them, added by the last one to finish (gemm_core.h: Fold), in their order.
+//
+// 24 rows of 1 000 x 2 731 14.6 us, of 1 024 x 4 096 14.9 (2.3 TB/s), of 2 048 x 8 192 37 (3.6 TB/s); with four columns a lane and two groups
+// under way 17.9, 17.5 and 36, with eight waves 17.6, 15.3 and 35.
 namespace few {
-constexpr int kRows = 32, kCols = 128, kWaves = 4;
+constexpr int kRows = 32, C = 2, kCols = 32 * C, kWaves = 4, kDepth = 4;
+typedef float Columns __attribute__((ext_vector_type(C)));
+typedef Columns ColumnsU __attribute__((aligned(4)));
 
 struct Args {
   const float *x, *gate, *up;
   float *g, *u, *h;  // NULL: not wanted
   int M, K, F, strips, k_per_group, pieces;
-  float *scratch;    // [row group][strip][piece][g, u][rows][kCols]
+  float *scratch;    // [row group][strip][piece][accumulator][g, u][lane][C]
   unsigned *tickets;
 };
+
+template <int N, int POLICY>
+__device__ inline auto load_columns(__amdgpu_buffer_rsrc_t r, uint32_t byte_off) {
+  typedef float V __attribute__((ext_vector_type(N)));
+  if constexpr (N == 4) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, (int)byte_off, 0, POLICY));
+  else return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(r, (int)byte_off, 0, POLICY));
+}
+template <int POLICY, class V>
+__device__ inline void store_columns(__amdgpu_buffer_rsrc_t r, uint32_t byte_off, const V &v) {
+  if constexpr (sizeof(V) == 16)
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(__attribute__((__vector_size__(16))) unsigned, v), r, (int)byte_off, 0, POLICY);
+  else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(__attribute__((__vector_size__(8))) unsigned, v), r, (int)byte_off, 0, POLICY);
+}
 
 template <int ACT>
 __global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Args a) {
@@ -686,138 +704,137 @@ __global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Args a) {
   const int rows = min(kRows, a.M - m0), c0 = strip * kCols;
   const int k_begin = piece * a.k_per_group + wave * (a.k_per_group / kWaves);
   const int k_end = min(a.K, k_begin + a.k_per_group / kWaves);
-  __shared__ f32x4v part[2][kWaves - 1][2][4][64];  // [wave that adds][wave that has][g, u][row][lane]
+  // Wave q adds up accumulators OWN q .. OWN q + OWN - 1, ROUND waves at a time; accumulator v holds rows 8 (v / 4) + 4 half + v mod 4.
+  constexpr int OWN = 16 / kWaves, ROUND = kWaves / 2;
+  __shared__ Columns part[ROUND][kWaves - 1][OWN][2][64];  // [wave that adds][wave that has][accumulator][g, u][lane]
   __shared__ unsigned last;
 
   const uint32_t bytes = (uint32_t)a.K * (uint32_t)a.F * 4u;
   const __amdgpu_buffer_rsrc_t rsrc[2] = {make_rsrc(a.gate, bytes), make_rsrc(a.up, bytes)};
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, (uint32_t)a.M * (uint32_t)a.K * 4u);
   // a lane's columns past the end may hold the next row's values: they are not stored
-  const uint32_t col_off = c0 + 4 * along < a.F ? (uint32_t)(c0 + 4 * along) * 4u : OOB;
+  const int c = c0 + C * along;
+  const uint32_t col_off = c < a.F ? (uint32_t)c * 4u : OOB;
   const uint32_t row_off = along < rows ? (uint32_t)(m0 + along) * (uint32_t)a.K * 4u : OOB;
 
-  f32x16 acc[2][4];
+  f32x16 acc[2][C];
 #pragma unroll
   for (int w = 0; w < 2; ++w)
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < C; ++j)
 #pragma unroll
       for (int v = 0; v < 16; ++v) acc[w][j][v] = 0.f;
 
-  // x: four reduction elements of one row; weights: four rows of four columns
-  f32x4v xv[2], wv[2][2][4];
+  // x: four reduction elements of one row; weights: four rows of C columns
+  f32x4v xv[kDepth];
+  Columns wv[kDepth][2][4];
   auto load = [&](int at, int k0) {
     const int k = k0 + 4 * half;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const uint32_t off = k + s < k_end ? col_off + (uint32_t)(k + s) * (uint32_t)a.F * 4u : OOB;
+      const uint32_t off = k + s < k_end ? (col_off + (uint32_t)(k + s) * (uint32_t)a.F * 4u) | (col_off & OOB) : OOB;
 #pragma unroll
-      for (int w = 0; w < 2; ++w) wv[at][w][s] = buf_load4(rsrc[w], off | (col_off & OOB));
+      for (int w = 0; w < 2; ++w) wv[at][w][s] = load_columns<C, 0>(rsrc[w], off);
     }
     const f32x4v v = buf_load4(xr, k < k_end ? (row_off + (uint32_t)k * 4u) | (row_off & OOB) : OOB);
 #pragma unroll
     for (int s = 0; s < 4; ++s) xv[at][s] = k + s < k_end ? v[s] : 0.f;
   };
-  auto multiply = [&](int at) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+  for (int d = 0; d < kDepth; ++d) load(d, k_begin + 8 * d);
+  for (int k0 = k_begin; k0 < k_end; k0 += 8 * kDepth)
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
+    for (int d = 0; d < kDepth; ++d) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[w][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[at][s], wv[at][w][s][j], acc[w][j], 0, 0, 0);
-  };
-  load(0, k_begin);
-  for (int k0 = k_begin; k0 < k_end; k0 += 16) {
-    load(1, k0 + 8);
-    multiply(0);
-    load(0, k0 + 16);
-    multiply(1);
-  }
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+#pragma unroll
+          for (int j = 0; j < C; ++j)
+            acc[w][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[d][s], wv[d][w][s][j], acc[w][j], 0, 0, 0);
+      load(d, k0 + 8 * (d + kDepth));
+    }
 
-  // Wave q adds up rows 8 q + 4 half + 0..3, accumulators 4 q + 0..3, two waves' worth at a time.
-  f32x4v sum[2][4];  // [g, u][row], four columns
+  auto first_row = [](int v) { return 8 * (v / 4) + v % 4; };
+  Columns sum[2][OWN];
 #pragma unroll
-  for (int pair = 0; pair < 2; ++pair) {
-    if (16 * pair >= rows) break;  // uniform, as all that depends on rows and q below
-    if (pair) __syncthreads();
+  for (int round = 0; round < kWaves / ROUND; ++round) {
+    if (first_row(round * ROUND * OWN) >= rows) break;  // uniform, as all that depends on rows below
+    if (round) __syncthreads();
 #pragma unroll
-    for (int q = 2 * pair; q < 2 * pair + 2; ++q) {
-      if (8 * q >= rows) continue;
+    for (int q = round * ROUND; q < (round + 1) * ROUND; ++q)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (8 * q + i >= rows) continue;
+      for (int i = 0; i < OWN; ++i) {
+        if (first_row(q * OWN + i) >= rows) continue;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          const f32x4v o = {acc[w][0][4 * q + i], acc[w][1][4 * q + i], acc[w][2][4 * q + i], acc[w][3][4 * q + i]};
+          Columns o;
+#pragma unroll
+          for (int j = 0; j < C; ++j) o[j] = acc[w][j][q * OWN + i];
           if (wave == q) sum[w][i] = o;
-          else part[q % 2][wave - (wave > q)][w][i][lane] = o;
+          else part[q % ROUND][wave - (wave > q)][i][w][lane] = o;
         }
       }
-    }
     __syncthreads();
-    if (wave / 2 == pair)
+    if (wave / ROUND == round)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (8 * wave + i >= rows) continue;
+      for (int i = 0; i < OWN; ++i) {
+        if (first_row(wave * OWN + i) >= rows) continue;
 #pragma unroll
         for (int o = 0; o < kWaves - 1; ++o)
 #pragma unroll
-          for (int w = 0; w < 2; ++w) sum[w][i] += part[wave % 2][o][w][i][lane];
+          for (int w = 0; w < 2; ++w) sum[w][i] += part[wave % ROUND][o][i][w][lane];
       }
   }
-  const int live = min(4, rows - 8 * wave);  // rows of the half wave 0 that this wave has, at most 0: none
   if (a.pieces > 1) {
     constexpr int SC1 = 16;
     constexpr uint32_t kPieceBytes = 2u * kRows * kCols * 4u;
-    const int slot = (int)blockIdx.x;
-    const __amdgpu_buffer_rsrc_t pieces = make_rsrc(a.scratch + (size_t)slot * a.pieces * (kPieceBytes / 4), (uint32_t)a.pieces * kPieceBytes);
+    const __amdgpu_buffer_rsrc_t pieces =
+        make_rsrc(a.scratch + (size_t)blockIdx.x * a.pieces * (kPieceBytes / 4), (uint32_t)a.pieces * kPieceBytes);
     auto offset = [&](int p, int w, int i) {
-      return (int)((uint32_t)p * kPieceBytes + (uint32_t)(((wave * 4 + i) * 2 + w) * 64 + lane) * 16u);
+      return (int)((uint32_t)p * kPieceBytes + (uint32_t)(((wave * OWN + i) * 2 + w) * 64 + lane) * (4u * C));
     };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i >= live) continue;
+    for (int i = 0; i < OWN; ++i) {
+      if (first_row(wave * OWN + i) >= rows) continue;
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(__attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned, sum[w][i]),
-                                               pieces, offset(piece, w, i), 0, SC1);
+      for (int w = 0; w < 2; ++w) {
+        store_columns<SC1>(pieces, (uint32_t)offset(piece, w, i), sum[w][i]);
+      }
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.tickets + slot, 1u) == (unsigned)(a.pieces - 1);
+    if (threadIdx.x == 0) last = atomicAdd(a.tickets + blockIdx.x, 1u) == (unsigned)(a.pieces - 1);
     __syncthreads();
     if (!last) return;
-    if (threadIdx.x == 0) a.tickets[slot] = 0u;
-    if (live <= 0) return;
+    if (threadIdx.x == 0) a.tickets[blockIdx.x] = 0u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum[0][i] = sum[1][i] = f32x4v{0.f, 0.f, 0.f, 0.f};
-    // rows that are not live were not written, and are not used
+    for (int i = 0; i < OWN; ++i) sum[0][i] = sum[1][i] = Columns{};
+    // accumulators without a row were not written, and are not used
 #pragma unroll 4
     for (int p = 0; p < a.pieces; ++p)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < OWN; ++i)
 #pragma unroll
-        for (int w = 0; w < 2; ++w)
-          sum[w][i] += __builtin_bit_cast(
-              f32x4v, __builtin_amdgcn_raw_buffer_load_b128(pieces, i < live ? offset(p, w, i) : (int)OOB, 0, SC1));
+        for (int w = 0; w < 2; ++w) {
+          sum[w][i] += load_columns<C, SC1>(pieces, first_row(wave * OWN + i) < rows ? (uint32_t)offset(p, w, i) : OOB);
+        }
   }
-  const int c = c0 + 4 * along;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = 8 * wave + 4 * half + i;
+  for (int i = 0; i < OWN; ++i) {
+    const int m = first_row(wave * OWN + i) + 4 * half;
     if (m >= rows) continue;
     const size_t at = (size_t)(m0 + m) * a.F + c;
-    f32x4v h;
+    Columns h;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = act_of<ACT>(sum[0][i][j]) * sum[1][i][j];
-    auto put = [&](float *out, const f32x4v &value) {
+    for (int j = 0; j < C; ++j) h[j] = act_of<ACT>(sum[0][i][j]) * sum[1][i][j];
+    auto put = [&](float *out, const Columns &value) {
       if (!out) return;
-      if (c + 4 <= a.F) {
-        *reinterpret_cast<f32x4u *>(out + at) = value;
+      if (c + C <= a.F) {
+        *reinterpret_cast<ColumnsU *>(out + at) = value;
       } else {
 #pragma unroll
-        for (int j = 0; j < 3; ++j)
+        for (int j = 0; j < C - 1; ++j)
           if (c + j < a.F) out[at + j] = value[j];
       }
     };
@@ -829,7 +846,8 @@ __global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Args a) {
 
 // Up to four rows: vector multiply-adds.  Sixteen waves share 32 columns, eight lanes a row of the weights with four columns each, so
 // that 4 096 columns already keep half of the CUs' loads going without a run of the reduction to be added across
-// workgroups, which costs as long as reading 20 MB.
+// workgroups, which costs as long as reading 20 MB.  One row of 1 024 x 4 096 7.9 us (4.3 TB/s), of 2 048 x 8 192 28 (4.8); with runs
+// across workgroups 12.6 and 32, but of 4 096 x 11 008 90 and 78, where half a CU's share is a workgroup too many.
 constexpr int kFewest = 4, kNarrow = 32, kWide = 1024;
 template <int ACT, int ROWS>
 __global__ __launch_bounds__(kWide) void fewest_kernel(const Args a) {
@@ -902,8 +920,8 @@ int64_t forward(int M, int K, int F, const float *x, const float *gate, const fl
     return 0;
   }
   const int64_t groups = (int64_t)a.strips * cdiv(M, kRows);
-  // about two workgroups a CU, a wave's run 32 reduction elements at least
-  int pieces = (int)std::max<int64_t>(1, std::min<int64_t>({2 * num_cus() / groups, K / (kWaves * 32), 32}));
+  // about a workgroup a CU, a wave's run 32 reduction elements at least
+  int pieces = (int)std::max<int64_t>(1, std::min<int64_t>({num_cus() / groups, K / (kWaves * 32), 32}));
   a.k_per_group = cdiv(K, pieces * kWaves * 8) * kWaves * 8;
   a.pieces = K ? cdiv(K, a.k_per_group) : 1;
   if (a.pieces > 1) {
