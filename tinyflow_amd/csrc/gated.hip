@@ -551,13 +551,14 @@ struct Splitting {
 };
 
 // Whether the forward pass runs on pairs, or on the fp32 instruction with nothing split (namespace few): us, fitted.  K x F, rows, few
-// / pairs: 1 024 x 4 096, 128 29 / 54, 256 43 / 53, 512 84 / 54; 2 048 x 8 192, 128 84 / 132, 256 151 / 131; 512 x 1 376, 256
-// 19 / 30; 256 x 1 024, 256 12 / 23.
+// / pairs: 1 024 x 4 096, 128 26 / 52, 256 42 / 51, 320 62 / 50, 512 81 / 53; 2 048 x 8 192, 128 86 / 128, 192 126 / 129, 256 162 /
+// 139; 4 096 x 11 008, 128 272 / 346, 192 414 / 394; 1 000 x 2 731, 320 50 / 53, 512 71 / 48; 512 x 1 376, 512 24 / 32, 1 024 38 / 32;
+// 256 x 1 024, 1 024 17 / 24.
 bool forward_on_pairs(int64_t M, int64_t K, int64_t F) {
   if (K >= 1 << 22 || F >= 1 << 22) return false;  // a tile's rows would pass a buffer's end
   const double m = (double)cdiv(M, 32) * 32, k = (double)cdiv(K, 32) * 32, f = (double)cdiv(F, 32) * 32;
-  const double few = 6.0 + 4.0 * m * k * f / 115e6;
-  const double pairs = 18.0 + (24.0 * k * f + 12.0 * m * k) / 4.8e6 + 4.0 * m * k * f / 380e6;
+  const double few = 8.0 + 4.0 * m * k * f / 100e6;
+  const double pairs = 22.0 + (24.0 * k * f + 12.0 * m * k) / 4.8e6 + 4.0 * m * k * f / 380e6;
   return pairs < few;
 }
 // The backward pass: from 128 rows on, or where the weights are small.  Else products of the matrix multiply, which split nothing,
@@ -668,8 +669,8 @@ int64_t backward_by_pairs(int M, int K, int F, const float *x, const float *gate
 // others; DEPTH groups are under way.  The waves of a workgroup have runs of their own, added through LDS, and several workgroups
 // more of them, added by the last one to finish (gemm_core.h: Fold), in their order.
 //
-// 24 rows of 1 000 x 2 731 14.6 us, of 1 024 x 4 096 14.9 (2.3 TB/s), of 2 048 x 8 192 37 (3.6 TB/s); with four columns a lane and two groups
-// under way 17.9, 17.5 and 36, with eight waves 17.6, 15.3 and 35.
+// 24 rows, us: 1 000 x 2 731 14.6, 1 024 x 4 096 14.5 (2.3 TB/s), 2 048 x 8 192 37 (3.7), 4 096 x 11 008 102 (3.6); with four columns a
+// lane and two groups under way 18.0, 17.9, 37, 79; with eight waves 18.1, 15.0, 35, 95.
 namespace few {
 constexpr int kRows = 32, C = 2, kCols = 32 * C, kWaves = 4, kDepth = 4;
 typedef float Columns __attribute__((ext_vector_type(C)));
@@ -846,8 +847,9 @@ __global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Args a) {
 
 // Up to four rows: vector multiply-adds.  Sixteen waves share 32 columns, eight lanes a row of the weights with four columns each, so
 // that 4 096 columns already keep half of the CUs' loads going without a run of the reduction to be added across
-// workgroups, which costs as long as reading 20 MB.  One row of 1 024 x 4 096 7.9 us (4.3 TB/s), of 2 048 x 8 192 28 (4.8); with runs
-// across workgroups 12.6 and 32, but of 4 096 x 11 008 90 and 78, where half a CU's share is a workgroup too many.
+// workgroups, which costs as long as reading 20 MB.  A longer reduction is better cut.  This / cut, us, one row: 1 024 x 4 096 8.5 /
+// 12.6 (7.8 measured alone: 4.3 TB/s), 2 048 x 8 192 27.9 / 33.9, 2 560 x 512 12.7 / 13.1, 4 096 x 512 19.1 / 17.7, 8 192 x 2 048 66 / 34;
+// four rows: 1 000 x 2 731 12.9 / 13.6, 2 560 x 512 17.3 / 13.7.
 constexpr int kFewest = 4, kNarrow = 32, kWide = 1024;
 template <int ACT, int ROWS>
 __global__ __launch_bounds__(kWide) void fewest_kernel(const Args a) {
@@ -920,7 +922,8 @@ int64_t forward(int M, int K, int F, const float *x, const float *gate, const fl
     return 0;
   }
   const int64_t groups = (int64_t)a.strips * cdiv(M, kRows);
-  // about a workgroup a CU, a wave's run 32 reduction elements at least
+  // about a workgroup a CU, a wave's run 32 reduction elements at least; two a CU: 24 rows of 1 024 x 4 096 14.8 / 16.3 us,
+  // 2 048 x 8 192 38.0 / 35.7, 2 048 x 16 384 56.6 / 60.1
   int pieces = (int)std::max<int64_t>(1, std::min<int64_t>({num_cus() / groups, K / (kWaves * 32), 32}));
   a.k_per_group = cdiv(K, pieces * kWaves * 8) * kWaves * 8;
   a.pieces = K ? cdiv(K, a.k_per_group) : 1;
