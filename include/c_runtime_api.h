@@ -420,7 +420,7 @@ int DLGpuBatchNormalizationAndReluBackward(const DLArrayHandle input, const DLAr
 /* --------------------------------------- layer norm, gated feed-forward (no counterparts in the reference) */
 
 /* output = gamma (input - mean) / sqrt(variance + eps) + beta over the last axis of an input of any rank; gamma and
- * beta hold one value for each of its columns.  `output` may be `input`.  Takes no scratch. */
+ * beta hold one value for each of its columns, 2^26 at most.  `output` may be `input`.  Takes no scratch. */
 int DLGpuLayerNormalizationForward(const DLArrayHandle input, const DLArrayHandle gamma, const DLArrayHandle beta,
                                    DLArrayHandle output, float eps, void **stream);
 /* Its gradients, those of dinput, dgamma and dbeta that are not NULL, from the forward pass's input: nothing is kept
@@ -432,7 +432,7 @@ int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const DLArrayHand
 /* g = input gate, u = input up, output = act(g) u, for input [M, K], gate and up [K, F], output [M, F]; pre [2, M, F]
  * receives g and u, which the backward pass reads.  One of pre and output may be NULL.
  * activation: sigmoid=0, relu=1, silu=2, gelu=3 (with erf).  Arrays of 2 GiB or more (a half of pre counts as one)
- * are rejected.  Results must not overlap what they are computed from.  Scratch: none for up to four rows of up to 2 560
+ * and more than 2^26 rows or columns are rejected.  Results must not overlap what they are computed from.  Scratch: none for up to four rows of up to 2 560
  * columns; a call that takes some is refused on a stream that is being captured into a graph, as is the backward call. */
 int DLGpuGatedFeedForward(const DLArrayHandle input, const DLArrayHandle gate, const DLArrayHandle up,
                           DLArrayHandle pre, DLArrayHandle output, int activation, int *memorytoSaving, void **stream);
@@ -442,7 +442,8 @@ int DLGpuGatedFeedForwardBackward(const DLArrayHandle input, const DLArrayHandle
                                   const DLArrayHandle pre, const DLArrayHandle doutput, DLArrayHandle dinput,
                                   DLArrayHandle dgate, DLArrayHandle dup, int activation, int *memorytoSaving,
                                   void **stream);
-/* The pointwise part alone: output = act(pre[0]) pre[1], and dpre = (dg, du).  dpre may be pre. */
+/* The pointwise part alone: output = act(pre[0]) pre[1], and dpre = (dg, du), for fewer than 2^33 elements of output.
+ * dpre may be pre. */
 int DLGpuGatedActivation(const DLArrayHandle pre, DLArrayHandle output, int activation, void **stream);
 int DLGpuGatedActivationBackward(const DLArrayHandle pre, const DLArrayHandle doutput, DLArrayHandle dpre,
                                  int activation, void **stream);

@@ -190,3 +190,17 @@ def test_counter_dropout_refuses():
     _refused(f, x, _Fake((4, 6), dev_id=1), y, 0.5, 1, 1)
     for seed, offset in ((-1, 0), (2 ** 64, 0), (0, -1), (0, 2 ** 64)):
         _refused(f, x, None, y, 0.5, seed, offset)
+
+
+def test_more_than_a_launch_can_count_refuses():
+    gamma, x = _Fake(((1 << 26) + 1,)), _Fake((1, (1 << 26) + 1))
+    _refused(gpu_op.layer_norm_forward, x, gamma, gamma, x, 1e-5)
+    x, h, w = _Fake(((1 << 26) + 1, 1)), _Fake(((1 << 26) + 1, 1)), _Fake((1, 1))
+    _refused(gpu_op.gated_feed_forward, x, w, w, None, h, "silu")
+    x, h, w = _Fake((1, 1)), _Fake((1, (1 << 26) + 1)), _Fake((1, (1 << 26) + 1))
+    _refused(gpu_op.gated_feed_forward, x, w, w, None, h, "silu")
+    pre, h = _Fake((2, 1 << 33)), _Fake((1 << 33,))
+    _refused(gpu_op.gated_activation, pre, h, "silu")
+    _refused(gpu_op.gated_activation_backward, pre, h, pre, "silu")
+    x = _Fake((1 << 36,))
+    _refused(gpu_op.counter_dropout, x, None, x, 0.5, 1, 1)

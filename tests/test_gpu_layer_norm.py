@@ -171,3 +171,23 @@ def test_another_stream_behind_the_first(rt):
         for got, (value, tol) in zip(out, wanted):
             ref.assert_within(got.asnumpy(), value, tol, "on its stream")
     gpu_op.destroy_cudaStream(other)
+
+
+def test_more_waves_than_a_grid_dimension_counts(rt):
+    """2^26 rows and a wave each pass 2^32 lanes in one dimension: the rows at both ends, and each side of where it wraps."""
+    from tinyflow_amd import gpu_op, ndarray
+    rows = (1 << 26) + 5
+    x = np.empty((rows, 2), np.float32)
+    x[:, 0] = np.arange(rows, dtype=np.float32) % 1021 + 1
+    x[:, 1] = -x[:, 0]
+    ax, ag, ab = _device(rt, x, np.float32([1, 2]), np.float32([0.5, -0.25]))
+    y = ndarray.empty(x.shape, ctx=rt.ctx)
+    gpu_op.array_set(y, 7.25, rt.stream)   # what is not written shows
+    gpu_op.layer_norm_forward(ax, ag, ab, y, 0.0, rt.stream)
+    # every row is (v, -v): its mean is 0 and its deviation v, a division and a root off by half a step each, the product by another
+    np.testing.assert_allclose(y.asnumpy(), np.broadcast_to(np.float32([1.5, -2.25]), x.shape), rtol=0, atol=2 * 4 * 2.0 ** -24)
+    gpu_op.layer_norm_backward(ax, ag, ax, y, None, None, 1e30, rt.stream)
+    # an eps of 1e30 makes s = 1e-15 and xh next to nothing: dx = s (a - mean(a)), a = (v, -2 v), so s (1.5 v, -1.5 v)
+    s = 1 / np.sqrt(1e30)
+    want = (np.float64(1.5 * s) * x).astype(np.float32)
+    np.testing.assert_allclose(y.asnumpy(), want, rtol=8 * 2.0 ** -24, atol=0)

@@ -310,7 +310,7 @@ extern "C" int DLGpuCounterDropout(const DLArrayHandle input, const DLArrayHandl
   hipStream_t s = stream_of(stream);
   const int64_t count = numel(input), a_group = (int64_t)kThreads * kBlocksPerLane * 4;
   const int64_t groups = (count + a_group - 1) / a_group;
-  TF_REQUIRE(groups <= 0x7fffffff, "too many elements");
+  TF_REQUIRE(groups * kThreads < (int64_t)1 << 32, "2^36 elements or more are not supported");
   if (count == 0) return 0;
   // a float below 1 is at most 1 - 2^-24: the product is exact and below 2^32
   const uint32_t threshold = (uint32_t)((double)dropout * 4294967296.0);

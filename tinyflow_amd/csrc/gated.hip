@@ -971,6 +971,7 @@ int geometry(const char *what, const DLArray *x, const DLArray *gate, const DLAr
   const int64_t most = ((int64_t)1 << 29) - 1;
   if (M > most || K > most || F > most || M * K > most || K * F > most || M * F > most)
     return fail("arrays of 2 GiB or more are not supported");
+  if (M > 1 << 26 || F > 1 << 26) return fail("more than 2^26 rows or columns are not supported");
   return 0;
 }
 
@@ -983,7 +984,7 @@ extern "C" int DLGpuGatedActivation(const DLArrayHandle pre, DLArrayHandle outpu
   TF_REQUIRE(same_device({pre, output}), "arrays must live on one device");
   TF_REQUIRE(!overlaps(pre, output), "output must not overlap pre");
   const int64_t n = numel(output);
-  TF_REQUIRE(n < (int64_t)1 << 40, "too many elements");
+  TF_REQUIRE(n < (int64_t)1 << 33, "2^33 elements or more are not supported");
   announce_write(output);
   hipStream_t s = stream_of(stream);
   if (n == 0) return 0;
@@ -1004,7 +1005,7 @@ extern "C" int DLGpuGatedActivationBackward(const DLArrayHandle pre, const DLArr
   TF_REQUIRE(!overlaps(dpre, doutput) && (pre->data == dpre->data || !overlaps(pre, dpre)),
              "dpre must be pre or overlap neither pre nor doutput");
   const int64_t n = numel(doutput);
-  TF_REQUIRE(n < (int64_t)1 << 40, "too many elements");
+  TF_REQUIRE(n < (int64_t)1 << 33, "2^33 elements or more are not supported");
   announce_write(dpre);
   hipStream_t s = stream_of(stream);
   if (n == 0) return 0;

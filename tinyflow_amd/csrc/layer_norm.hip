@@ -106,6 +106,10 @@ __device__ inline float inverse_std(float square_sum, float n, float eps) {
   return 1.f / sqrtf(square_sum / n + eps);
 }
 
+// Workgroups as a grid none of whose dimensions, times the workgroup, passes 2^32.
+dim3 grid_of(int64_t groups) { return dim3((unsigned)std::min<int64_t>(groups, 1 << 20), (unsigned)((groups + (1 << 20) - 1) >> 20)); }
+__device__ inline int64_t group_index() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // T lanes a row, WG / T rows a workgroup.
 template <int T, int VPT, bool PAST>
 __global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
@@ -114,7 +118,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float 
   constexpr int WG = T > 256 ? T : 256;
   __shared__ float room[2][T / 64];
   const int lane = threadIdx.x % T;
-  const int64_t r = (int64_t)blockIdx.x * (WG / T) + threadIdx.x / T;
+  const int64_t r = group_index() * (WG / T) + threadIdx.x / T;
   if (r >= rows) return;  // whole waves, and no barrier where several rows share a workgroup
   Row<T, VPT> row, g, b;
   row.load(x + r * cols, cols, lane);
@@ -131,9 +135,10 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float 
 constexpr int kLong = 1024;
 __global__ __launch_bounds__(kLong) void forward_long_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
                                                             const float *__restrict__ beta, float *__restrict__ y,
-                                                            int cols, float n, float eps) {
+                                                            int64_t rows, int cols, float n, float eps) {
   __shared__ float room[2][kLong / 64];
-  const float *row = x + (int64_t)blockIdx.x * cols;
+  if (group_index() >= rows) return;
+  const float *row = x + group_index() * cols;
   float s = 0.f;
   for (int c = threadIdx.x; c < cols; c += kLong) s += row[c];
   const float mean = row_sum<kLong>(s, room[0]) / n;
@@ -143,7 +148,7 @@ __global__ __launch_bounds__(kLong) void forward_long_kernel(const float *__rest
     s += d * d;
   }
   const float istd = inverse_std(row_sum<kLong>(s, room[1]), n, eps);
-  float *out = y + (int64_t)blockIdx.x * cols;
+  float *out = y + group_index() * cols;
   for (int c = threadIdx.x; c < cols; c += kLong) out[c] = (row[c] - mean) * istd * gamma[c] + beta[c];
 }
 
@@ -331,8 +336,8 @@ int geometry(const char *what, const DLArray *x, const DLArray *gamma, int64_t &
     fprintf(stderr, "[tinyflow_amd] %s: arrays must live on the GPU\n", what);
     return -1;
   }
-  if (x->ndim < 1 || gamma->ndim != 1 || gamma->shape[0] != x->shape[x->ndim - 1] || gamma->shape[0] > 0x3fffffff) {
-    fprintf(stderr, "[tinyflow_amd] %s: gamma must hold one value for each column of the last axis (fewer than 2^30)\n", what);
+  if (x->ndim < 1 || gamma->ndim != 1 || gamma->shape[0] != x->shape[x->ndim - 1] || gamma->shape[0] > 1 << 26) {
+    fprintf(stderr, "[tinyflow_amd] %s: gamma must hold one value for each column of the last axis (2^26 at most)\n", what);
     return -1;
   }
   cols = gamma->shape[0];
@@ -373,7 +378,7 @@ extern "C" int DLGpuLayerNormalizationForward(const DLArrayHandle input, const D
   auto go = [&](auto t, auto vectors) {
     constexpr int T = decltype(t)::value, VPT = decltype(vectors)::value, WG = T > 256 ? T : 256, ROWS = WG / T;
     hipLaunchKernelGGL((past_caches(rows * cols) ? forward_kernel<T, VPT, true> : forward_kernel<T, VPT, false>),
-                       dim3((unsigned)((rows + ROWS - 1) / ROWS)), dim3(WG), 0, s, x, g, b, y, rows, (int)cols, n, eps);
+                       grid_of((rows + ROWS - 1) / ROWS), dim3(WG), 0, s, x, g, b, y, rows, (int)cols, n, eps);
   };
   if (cols <= 256) go(IC<64>{}, IC<1>{});
   else if (cols <= 512) go(IC<64>{}, IC<2>{});
@@ -383,7 +388,7 @@ extern "C" int DLGpuLayerNormalizationForward(const DLArrayHandle input, const D
   else if (cols <= 8192) go(IC<1024>{}, IC<2>{});
   else if (cols <= kMaxForward) go(IC<1024>{}, IC<4>{});
   else
-    hipLaunchKernelGGL(forward_long_kernel, dim3((unsigned)rows), dim3(kLong), 0, s, x, g, b, y, (int)cols, n, eps);
+    hipLaunchKernelGGL(forward_long_kernel, grid_of(rows), dim3(kLong), 0, s, x, g, b, y, rows, (int)cols, n, eps);
   return finish(s, "DLGpuLayerNormalizationForward");
 }
 
@@ -414,7 +419,7 @@ extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const 
   const int rows_a_group = !in_registers ? 1 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1;
   const int64_t groups = (rows + rows_a_group - 1) / rows_a_group;
   int pieces = 0;
-  if (in_registers) pieces = (int)std::min<int64_t>(groups, params ? (cols <= 1024 ? 2 : cols <= 2048 ? 3 : cols <= 4096 ? 2 : 1) * num_cus() : 0x7fffffff);
+  if (in_registers) pieces = (int)std::min<int64_t>(groups, params ? (cols <= 1024 ? 2 : cols <= 2048 ? 3 : cols <= 4096 ? 2 : 1) * num_cus() : 1 << 20);
   else if (rows) pieces = (int)std::min<int64_t>((rows + 3) / 4, std::max<int64_t>(1, 4 * num_cus() * 64 / cols));
   float *partial = nullptr, *stats = nullptr;
   if (params && rows) {
@@ -445,6 +450,7 @@ extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const 
     else if (cols <= 8192) go(IC<1024>{}, IC<2>{});
     else if (in_registers) go(IC<1024>{}, IC<4>{});
     else {
+      // three arrays of 2^22 such rows are more than the memory
       hipLaunchKernelGGL(backward_long_kernel, dim3((unsigned)rows), dim3(kLong), 0, s, x, g, dy, dx, stats, (int)cols, n, eps);
       if (params)
         hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 63) / 64), (unsigned)pieces), dim3(256), 0, s, x, dy,
