@@ -127,10 +127,10 @@ def gated_backward(x, gate, up, dpre, d_dpre):
     return [product(both, weights.T, d_a=d_both), product(xt, dpre[0], d_b=d_dpre[0]), product(xt, dpre[1], d_b=d_dpre[1])]
 
 
-def philox(count, seed, offset):
-    """The generator's words, one an element."""
+def philox(count, seed, offset, first=0):
+    """The generator's words, one an element, from element ``first`` on, a multiple of four."""
     low = np.uint64(0xFFFFFFFF)
-    block = np.arange((count + 3) // 4, dtype=np.uint64)
+    block = np.arange(first // 4, first // 4 + (count + 3) // 4, dtype=np.uint64)
     c = [block & low, block >> np.uint64(32), np.full_like(block, offset & 0xFFFFFFFF), np.full_like(block, offset >> 32)]
     k = [seed & 0xFFFFFFFF, seed >> 32]
     for _ in range(10):
@@ -140,8 +140,8 @@ def philox(count, seed, offset):
     return np.stack(c, 1).ravel()[:count]
 
 
-def kept(count, dropout, seed, offset):
-    return philox(count, seed, offset) >= np.uint64(math.floor(float(np.float32(dropout)) * 2 ** 32))
+def kept(count, dropout, seed, offset, first=0):
+    return philox(count, seed, offset, first) >= np.uint64(math.floor(float(np.float32(dropout)) * 2 ** 32))
 
 
 def assert_within(got, ref, tol, what):

@@ -268,3 +268,75 @@ def test_no_room_for_scratch(rt):
     assert gpu_op.gated_feed_forward_backward(*arrays, *out, "silu", rt.stream) == 0
     for got, value in zip(out, grads):
         np.testing.assert_array_equal(got.asnumpy(), value)
+
+
+# ---------------------------------------------------------------- sizes of the forward pass on pairs, and long maxima
+
+# the last three: 64 runs and more of the maxima's rows, of the weights' rows, of both
+LARGE = [(1027, 1030, 700), (513, 1000, 1543), (2050, 300, 1100), (4040, 130, 1200), (700, 4100, 400), (4100, 4130, 100)]
+
+
+@pytest.mark.parametrize("m,k,f", LARGE)
+def test_large_forward(rt, m, k, f):
+    activation = ACTIVATIONS[(m + k + f) % 4]
+    x, gate, up, _ = _data(m, k, f, stable_seed((m, k, f)))
+    (pre_ref, pre_tol), (h_ref, h_tol) = ref.gated(x, gate, up, activation)
+    pre, h = _forward(rt, x, gate, up, activation)
+    ref.assert_within(pre, pre_ref, pre_tol, "pre")
+    ref.assert_within(h, h_ref, h_tol, "h")
+    for want in ("pre", "h"):
+        alone, = _forward(rt, x, gate, up, activation, (want,))
+        np.testing.assert_array_equal(alone, pre if want == "pre" else h)
+
+
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+def test_large_forward_of_every_activation(rt, activation):
+    x, gate, up, _ = _data(1100, 1030, 700, 6)
+    gate *= 3   # into the activations' bends
+    (pre_ref, pre_tol), (h_ref, h_tol) = ref.gated(x, gate, up, activation)
+    pre, h = _forward(rt, x, gate, up, activation)
+    ref.assert_within(pre, pre_ref, pre_tol, "pre")
+    ref.assert_within(h, h_ref, h_tol, "h")
+
+
+def test_large_forward_with_values_that_are_not_finite(rt):
+    m, k, f = 1027, 1030, 700
+    x, gate, up, _ = _data(m, k, f, 19)
+    (pre_ref, pre_tol), (h_ref, h_tol) = ref.gated(x, gate, up, "silu")
+    rows = np.ones(m, bool)
+    for row, value in ((0, np.nan), (130, np.inf), (m - 1, -np.inf)):
+        x[row, k // 3] = value
+        rows[row] = False
+    cols = np.ones(f, bool)
+    cols[[5, f - 1]] = False
+    bad = gate.copy()
+    bad[k - 1, 5], bad[0, f - 1] = -np.inf, np.nan
+    pre, h = _forward(rt, x, bad, up, "silu")
+    ref.assert_within(pre[0][np.ix_(rows, cols)], pre_ref[0][np.ix_(rows, cols)], pre_tol[0][np.ix_(rows, cols)], "g")
+    ref.assert_within(pre[1][rows], pre_ref[1][rows], pre_tol[1][rows], "u")
+    ref.assert_within(h[np.ix_(rows, cols)], h_ref[np.ix_(rows, cols)], h_tol[np.ix_(rows, cols)], "h")
+    assert np.isnan(pre[0][:, f - 1]).all() and np.isinf(pre[0][rows, 5]).all() and not np.isfinite(pre[:, ~rows]).any()
+    np.testing.assert_array_equal(pre[1, 130], np.sign(up[k // 3]) * np.float32(np.inf))
+
+
+@pytest.mark.parametrize("m,k,f", [(4100, 40, 70), (130, 33, 8200), (129, 4100, 60)])
+def test_backward_with_long_maxima(rt, m, k, f):
+    x, gate, up, dh = _data(m, k, f, stable_seed((m, k, f, 1)))
+    dh[m // 2] = 0
+    dh[m - 1, f - 1] = np.float32(3e4)   # in the last run of both
+    pre = np.stack([x @ gate, x @ up])
+    dpre, d_dpre = ref.pointwise_gradient(pre, dh, "silu")
+    got = _backward(rt, x, gate, up, pre, dh, "silu")
+    wanted = ref.gated_backward(x, gate, up, dpre, d_dpre)
+    for what, a, (value, tol) in zip(("dx", "dgate", "dup"), got, wanted):
+        ref.assert_within(a, value, tol, what)
+    for which in range(3):
+        want = [i == which for i in range(3)]
+        alone, = _backward(rt, x, gate, up, pre, dh, "silu", want)
+        np.testing.assert_array_equal(alone, got[which])
+    dh[m - 1, f - 1] = np.inf
+    dx, dgate, dup = _backward(rt, x, gate, up, pre, dh, "silu")
+    assert not np.isfinite(dx[m - 1]).any() and not np.isfinite(dgate[:, f - 1]).any() and not np.isfinite(dup[:, f - 1]).any()
+    ref.assert_within(dx[:m - 1], wanted[0][0][:m - 1], wanted[0][1][:m - 1], "dx")
+    ref.assert_within(dgate[:, :f - 1], wanted[1][0][:, :f - 1], wanted[1][1][:, :f - 1], "dgate")
+    ref.assert_within(dup[:, :f - 1], wanted[2][0][:, :f - 1], wanted[2][1][:, :f - 1], "dup")

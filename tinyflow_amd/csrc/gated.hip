@@ -3,7 +3,7 @@
 //   g = x Wg, u = x Wu, h = act(g) u        x [M, K], Wg and Wu [K, F]
 //   dg = dh u act'(g), du = dh act(g);  dx = dg Wg^T + du Wu^T,  dWg = x^T dg,  dWu = x^T du
 //
-// Large products run on fp16 pairs (gemm_pair.h), in three launches a pass:
+// Large products run on fp16 pairs (gemm_pair.h), in three launches a pass (four for long maxima):
 //
 //   maxima   the largest magnitude of every row (and column) of the operands, by runs of them
 //   split    every operand into its two fp16 numbers, in the order in which the products fetch them.  The gradients dg and du are
@@ -211,11 +211,12 @@ struct Job {
   uint32_t *row_max, *col_max;
   int half_steps, col_steps, col_mul, col_add;
   bool col_wanted[2];
-  int first_max, first_split;     // the job's first workgroup of each launch
+  int first_max, first_exps, first_split;  // the job's first workgroup of each launch
 };
 struct Jobs {
   Job job[3];
   int n;
+  bool exps_apart;  // the exponents have a launch of their own
 };
 
 constexpr int kMaxRows = 64, kMaxCols = 128;   // a workgroup's part of the maxima
@@ -280,6 +281,48 @@ __device__ inline int exponent_of(uint32_t largest) {
   return largest == 0 ? 0 : 15 - __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, largest));
 }
 
+__device__ inline int finite(int exponent) { return exponent == pair::kNotFinite ? 0 : exponent; }
+// the place of a column's exponent
+__device__ inline int col_at(const Job &job, int w, int c) { return (c / 32 * job.col_mul + w * job.col_add) * 32 + c % 32; }
+
+// The runs' maxima to exponents, those of 64 rows or columns a workgroup.  A launch of its own where there are kRunsApart runs and
+// more, which every tile of the split would go through otherwise.  With it / without, us: backward of 1 024 x 4 096, 2 048 rows
+// (32 runs) 284 / 284, 4 096 530 / 547, 16 384 1 884 / 2 113, 65 536 7 547 / 11 618; of 1 000 x 1 537, 777 rows 72 / 70, 4 096 212 /
+// 214; forward of 512 x 1 376, 4 096 rows 60 / 56.
+constexpr int kRunsApart = 64;
+constexpr int kExpsThreads = 1024;
+__global__ __launch_bounds__(kExpsThreads) void exponents_kernel(const Jobs jobs) {
+  int n = jobs.n - 1;
+  while (n > 0 && (int)blockIdx.x < jobs.job[n].first_exps) --n;
+  const Job &job = jobs.job[n];
+  const int rows = job.src.rows, cols = job.src.cols, of_rows = job.row_planes ? (rows + 63) / 64 : 0, of_cols = (cols + 63) / 64;
+  const int group = (int)blockIdx.x - job.first_exps, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool by_rows = group < of_rows;
+  const int w = by_rows ? 0 : (group - of_rows) / of_cols, at = (by_rows ? group : (group - of_rows) % of_cols) * 64 + lane;
+  if (!by_rows && !job.col_wanted[w]) return;
+  const int count = by_rows ? rows : cols;
+  const int runs = by_rows ? (cols + kMaxCols - 1) / kMaxCols : (rows + kMaxRows - 1) / kMaxRows;
+  const uint32_t *from = (by_rows ? job.row_max : job.col_max + (size_t)w * runs * cols) + min(at, count - 1);
+  constexpr int WAVES = kExpsThreads / 64, LOADS = 4;
+  uint32_t m = 0;
+  for (int i = wave; i < runs; i += LOADS * WAVES) {
+    uint32_t v[LOADS];  // a repeated value does not matter
+#pragma unroll
+    for (int e = 0; e < LOADS; ++e) v[e] = from[(size_t)min(i + e * WAVES, runs - 1) * count];
+#pragma unroll
+    for (int e = 0; e < LOADS; ++e) m = max(m, v[e]);
+  }
+  __shared__ uint32_t of_waves[WAVES][64];
+  of_waves[wave][lane] = m;
+  __syncthreads();
+  if (wave > 0 || at >= (count + 31) / 32 * 32) return;
+#pragma unroll
+  for (int o = 1; o < WAVES; ++o) m = max(m, of_waves[o][lane]);
+  const int exponent = at < count ? exponent_of(m) : 0;
+  if (by_rows) job.row_exps[at] = exponent;
+  else job.col_exps[col_at(job, w, at)] = exponent;
+}
+
 // Eight elements to the two halves of a lane's place in a fragment pair.
 __device__ inline void split_eight(const float (&x)[8], int exponent, char *at) {
   pair::f16x8 h, l;
@@ -315,35 +358,43 @@ __global__ __launch_bounds__(kThreads) void split_kernel(const Jobs jobs) {
       if (job.matrices > 1) *reinterpret_cast<f32x4 *>(&tile[1][r][c]) = v[1];
     }
   });
-  // the exponents, four lanes each; the tiles at the reduction's beginning write them down
-  const int of = tid / 4, part = tid % 4;
-  auto largest = [&](const uint32_t *from, int runs, int64_t stride) {
-    uint32_t m = 0;
-    for (int i = part; i < runs; i += 16) {
-      uint32_t v[4];  // a repeated value does not matter
+  if (jobs.exps_apart) {
+    if (tid < T) {
+      if (job.row_planes) row_exp[tid] = finite(job.row_exps[min(r0 + tid, rows - 1)]);
+      if (job.col_planes)
+        for (int w = 0; w < job.matrices; ++w)
+          if (job.col_wanted[w]) col_exp[w][tid] = finite(job.col_exps[col_at(job, w, min(c0 + tid, cols - 1))]);
+    }
+  } else {  // four lanes each; the tiles at the reduction's beginning write them down
+    const int of = tid / 4, part = tid % 4;
+    auto largest = [&](const uint32_t *from, int runs, int64_t stride) {
+      uint32_t m = 0;
+      for (int i = part; i < runs; i += 16) {
+        uint32_t v[4];  // a repeated value does not matter
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = from[min(i + 4 * e, runs - 1) * stride];
-      m = max(m, max(max(v[0], v[1]), max(v[2], v[3])));
-    }
-    m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
-    return max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
-  };
-  if (job.row_planes) {
-    const int r = r0 + of;
-    const int e = exponent_of(largest(job.row_max + min(r, rows - 1), (cols + kMaxCols - 1) / kMaxCols, rows));
-    if (part == 0) {
-      row_exp[of] = e == pair::kNotFinite ? 0 : e;
-      if (c0 == 0 && r < (rows + 31) / 32 * 32) job.row_exps[r] = r < rows ? e : 0;
-    }
-  }
-  if (job.col_planes) {
-    const int runs = (rows + kMaxRows - 1) / kMaxRows, c = c0 + of;
-    for (int w = 0; w < job.matrices; ++w) {
-      if (!job.col_wanted[w]) continue;
-      const int e = exponent_of(largest(job.col_max + (size_t)w * runs * cols + min(c, cols - 1), runs, cols));
+        for (int e = 0; e < 4; ++e) v[e] = from[min(i + 4 * e, runs - 1) * stride];
+        m = max(m, max(max(v[0], v[1]), max(v[2], v[3])));
+      }
+      m = max(m, (uint32_t)__shfl_xor((int)m, 1, 64));
+      return max(m, (uint32_t)__shfl_xor((int)m, 2, 64));
+    };
+    if (job.row_planes) {
+      const int r = r0 + of;
+      const int e = exponent_of(largest(job.row_max + min(r, rows - 1), (cols + kMaxCols - 1) / kMaxCols, rows));
       if (part == 0) {
-        col_exp[w][of] = e == pair::kNotFinite ? 0 : e;
-        if (r0 == 0 && c < (cols + 31) / 32 * 32) job.col_exps[(c / 32 * job.col_mul + w * job.col_add) * 32 + c % 32] = c < cols ? e : 0;
+        row_exp[of] = finite(e);
+        if (c0 == 0 && r < (rows + 31) / 32 * 32) job.row_exps[r] = r < rows ? e : 0;
+      }
+    }
+    if (job.col_planes) {
+      const int runs = (rows + kMaxRows - 1) / kMaxRows, c = c0 + of;
+      for (int w = 0; w < job.matrices; ++w) {
+        if (!job.col_wanted[w]) continue;
+        const int e = exponent_of(largest(job.col_max + (size_t)w * runs * cols + min(c, cols - 1), runs, cols));
+        if (part == 0) {
+          col_exp[w][of] = finite(e);
+          if (r0 == 0 && c < (cols + 31) / 32 * 32) job.col_exps[col_at(job, w, c)] = c < cols ? e : 0;
+        }
       }
     }
   }
@@ -514,7 +565,7 @@ void give(pair::Work &w, char *base, size_t scratch, unsigned *tickets) {
 // The two launches in front of the products.
 struct Splitting {
   Jobs jobs{};
-  int maxima_groups = 0, split_groups = 0;
+  int maxima_groups = 0, exps_groups = 0, split_groups = 0;
   size_t row_max[3], col_max[3];
   void add(Layout &l, const Source &src, int matrices, bool by_rows, bool by_columns) {
     Job &j = jobs.job[jobs.n];
@@ -529,8 +580,11 @@ struct Splitting {
     j.col_add = cdiv(src.cols, 32);
     j.col_wanted[0] = j.col_wanted[1] = true;
     j.first_max = maxima_groups;
+    j.first_exps = exps_groups;
     j.first_split = split_groups;
     maxima_groups += runs_c * runs_r;
+    exps_groups += (by_rows ? cdiv(src.rows, 64) : 0) + (by_columns ? matrices * cdiv(src.cols, 64) : 0);
+    jobs.exps_apart |= (by_rows && runs_c >= kRunsApart) || (by_columns && runs_r >= kRunsApart);
     split_groups += cdiv(src.rows, kSplitTile) * cdiv(src.cols, kSplitTile);
     ++jobs.n;
   }
@@ -546,6 +600,8 @@ struct Splitting {
   }
   void launch(hipStream_t s) const {
     hipLaunchKernelGGL(maxima_kernel, dim3((unsigned)maxima_groups), dim3(kThreads), 0, s, jobs);
+    if (jobs.exps_apart)
+      hipLaunchKernelGGL(exponents_kernel, dim3((unsigned)exps_groups), dim3(kExpsThreads), 0, s, jobs);
     hipLaunchKernelGGL(split_kernel, dim3((unsigned)split_groups), dim3(kThreads), 0, s, jobs);
   }
 };
