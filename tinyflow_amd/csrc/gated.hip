@@ -16,6 +16,7 @@
 #include "internal.h"
 
 #include <algorithm>
+#include <cmath>
 
 using namespace tf;
 
@@ -535,25 +536,57 @@ pair::Work tiles_of(int m_blocks, int n_blocks, int halves) {
   w.tiles_n = w.half_tiles * halves;
   return w;
 }
-// Pieces of the products of a launch, so that there is about a workgroup a CU and all have about as many steps, 16 at least: a
-// piece writes and reads its tile once more.  us in 1 / 2 / 3 / 4 / 6 pieces: 2048 x 512 x 4096, 64 tiles, 62 / 42 / 36 / 35 / 40;
-// 512 x 4096 x 2048, 128 tiles, 37 / 32 / 35; 777 x 3074 x 1000, 175 tiles, 24 / 29; 4096 x 1024 x 8192, 256 tiles, 187 / 181.
-constexpr int kMaxPieces = 4;
-int steps_a_group(std::initializer_list<std::pair<pair::Work, int>> products) {
-  int64_t steps = 0;
-  for (const auto &p : products) steps += (int64_t)p.first.tiles_m * p.first.tiles_n * p.second;
-  return (int)std::max<int64_t>(16, steps / num_cus());
+// Pieces of a launch's one or two products, those that take the least time by a model: a step takes a workgroup that has its CU for itself 0.4 us
+// and two that share one 0.65, a launch of more than two workgroups a CU ends with a part of them idle, and every piece writes its
+// tile, all of which one workgroup reads, 6 us for a CU's piece times the pieces.  Over 110 sizes of both passes what it picks takes 0.6 per cent longer than the
+// fastest that there is; pieces of as many steps as a CU has in all, four at most, 3.0.  us in 1 x 1 / picked: backward of
+// 1 024 x 4 096, 777 rows 187 / 133, 4 096 rows 528 / 501; of 2 048 x 8 192, 777 rows 511 / 429; forward of 4 096 x 1 024, 512 rows
+// 94 / 66.
+constexpr int kMaxPieces = 8, kLeastSteps = 12;
+struct Extent {
+  int tiles, steps, pieces;  // no tiles: not there
+  int steps_a_piece() const { return cdiv(steps / 2, pieces) * 2; }
+};
+double cost(const Extent (&e)[2]) {
+  const double alone = 0.4, shared = 0.326, cus = num_cus();
+  double groups = 0, work = 0, longest = 0, shortest = 1e30, folds = 0, last = 0;
+  for (const Extent &x : e) {
+    if (x.tiles == 0) continue;
+    const double n = (double)x.tiles * x.pieces;
+    last = x.steps_a_piece();
+    groups += n;
+    work += n * last;
+    longest = std::max(longest, last);
+    shortest = std::min(shortest, last);
+    if (x.pieces > 1) folds += 6.0 * n * x.pieces / cus + 2.0;
+  }
+  if (groups <= cus) return longest * alone + folds;
+  double time = std::max(work / cus * shared, longest * alone);
+  const double idle = std::fmod(groups, 2 * cus) / (2 * cus);
+  if (groups <= 2 * cus) time = std::max(time, 2 * shared * shortest + alone * (longest - shortest));
+  else if (idle > 0) time = std::max(time, work / cus * shared + last * shared * (1 - idle));
+  return time + folds;
+}
+void choose_pieces(Extent (&e)[2]) {
+  Extent trial[2] = {e[0], e[1]};
+  auto most = [](const Extent &x) {  // a ticket a tile
+    return x.tiles == 0 || x.tiles > kFoldTicketSlots / 2 ? 1 : std::max(1, std::min(kMaxPieces, x.steps / kLeastSteps));
+  };
+  double least = 1e30;
+  for (trial[0].pieces = 1; trial[0].pieces <= most(e[0]); ++trial[0].pieces)
+    for (trial[1].pieces = 1; trial[1].pieces <= most(e[1]); ++trial[1].pieces) {
+      const double c = cost(trial);
+      if (c >= least) continue;
+      least = c;
+      e[0] = trial[0];
+      e[1] = trial[1];
+    }
 }
 // Its scratch's place, where there are several
-size_t cut(Layout &l, pair::Work &w, int steps, int steps_a_group) {
-  const int pieces = std::max(1, std::min(kMaxPieces, (steps + steps_a_group / 2) / steps_a_group));
-  w.steps_per_piece = cdiv(steps / 2, pieces) * 2;
-  w.pieces = cdiv(steps, w.steps_per_piece);
-  if ((int64_t)w.tiles_m * w.tiles_n > kFoldTicketSlots / 2) {
-    w.pieces = 1;
-    w.steps_per_piece = steps;
-  }
-  return w.pieces > 1 ? l.take((size_t)w.tiles_m * w.tiles_n * w.pieces * pair::BM * pair::BN * 4) : 0;
+size_t cut(Layout &l, pair::Work &w, const Extent &e) {
+  w.steps_per_piece = e.steps_a_piece();
+  w.pieces = cdiv(e.steps, w.steps_per_piece);
+  return w.pieces > 1 ? l.take((size_t)e.tiles * w.pieces * pair::BM * pair::BN * 4) : 0;
 }
 // `tickets`: one for each of its tiles
 void give(pair::Work &w, char *base, size_t scratch, unsigned *tickets) {
@@ -638,7 +671,9 @@ int64_t forward_by_pairs(int M, int K, int F, const float *x, const float *gate,
   const int f_blocks = cdiv(F, 32);
   const PackedAt a(l, cdiv(M, 32), steps_of(K)), b(l, 2 * f_blocks, steps_of(K));
   pair::Work work = tiles_of(a.blocks, b.blocks, 1);
-  const size_t scratch = cut(l, work, a.steps, steps_a_group({{work, a.steps}}));
+  Extent pieces[2] = {{work.tiles_m * work.tiles_n, a.steps, 1}, {0, 0, 1}};
+  choose_pieces(pieces);
+  const size_t scratch = cut(l, work, pieces[0]);
   if (being_captured(s)) return kCaptured;
   unsigned *tickets = fold_tickets(s);
   char *base = tickets ? (char *)device_alloc(l.bytes, s) : nullptr;
@@ -682,9 +717,10 @@ int64_t backward_by_pairs(int M, int K, int F, const float *x, const float *gate
     to_w = tiles_of(k_blocks, f_blocks, 2);
   }
   // pieces as for all three gradients, so that each has the same bits alone
-  const int x_steps = 2 * steps_of(F), w_steps = steps_of(M);
-  const int a_group = steps_a_group({{tiles_of(m_blocks, k_blocks, 1), x_steps}, {tiles_of(k_blocks, f_blocks, 2), w_steps}});
-  const size_t x_scratch = dx ? cut(l, to_x, x_steps, a_group) : 0, w_scratch = weights ? cut(l, to_w, w_steps, a_group) : 0;
+  const pair::Work all_x = tiles_of(m_blocks, k_blocks, 1), all_w = tiles_of(k_blocks, f_blocks, 2);
+  Extent pieces[2] = {{all_x.tiles_m * all_x.tiles_n, 2 * steps_of(F), 1}, {all_w.tiles_m * all_w.tiles_n, steps_of(M), 1}};
+  choose_pieces(pieces);
+  const size_t x_scratch = dx ? cut(l, to_x, pieces[0]) : 0, w_scratch = weights ? cut(l, to_w, pieces[1]) : 0;
   if (weights && (!dgate || !dup)) {
     to_w.tiles_n = to_w.half_tiles;
     to_w.first_half = dgate ? 0 : 1;
