@@ -14,6 +14,7 @@
 //            and dWu one launch of two halves.
 #include "gemm_pair.h"
 #include "internal.h"
+#include "lanes.h"
 
 #include <algorithm>
 #include <cmath>
@@ -256,8 +257,7 @@ __global__ __launch_bounds__(kThreads) void maxima_kernel(const Jobs jobs) {
   if (job.row_planes) {
 #pragma unroll
     for (int e = 0; e < kMaxRows / 8; ++e) {
-#pragma unroll
-      for (int m = 16; m > 0; m >>= 1) row[e] = max(row[e], (uint32_t)__shfl_xor((int)row[e], m, 32));
+      row[e] = lanes::largest<32>(row[e]);
       const int r = run_r * kMaxRows + 8 * e + group;
       if (lane == 0 && r < rows) job.row_max[(size_t)run_c * rows + r] = row[e];
     }
@@ -982,9 +982,7 @@ __global__ __launch_bounds__(kWide) void fewest_kernel(const Args a) {
 #pragma unroll
     for (int m = 0; m < ROWS; ++m) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int o = 32; o >= 8; o >>= 1) acc[w][m][j] += __shfl_xor(acc[w][m][j], o, 64);
+      for (int j = 0; j < 4; ++j) acc[w][m][j] = lanes::sum<8>(acc[w][m][j]);
       if (lane < 8) part[wave][w][m][lane] = acc[w][m];
     }
   __syncthreads();

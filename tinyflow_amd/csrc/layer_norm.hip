@@ -13,6 +13,7 @@
 // large).  Sums are divided by the column count, not multiplied by its reciprocal: a row of one value then has that value for
 // its mean.  All sums are fp32; their order depends on the shape alone.
 #include "internal.h"
+#include "lanes.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -26,17 +27,11 @@ using IC = std::integral_constant<int, V>;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f32x4 f32x4u __attribute__((aligned(4)));  // rows of any length start anywhere: 16-byte accesses on 4-byte alignment
 
-__device__ inline float wave_sum(float v) {
-#pragma unroll
-  for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
-  return v;
-}
-
 // Sum over the T lanes that share a row; `room` is T / 64 floats of that row's that nothing else uses until the next barrier but
 // one.  Rows of several waves pass a barrier: all rows of a workgroup get here together.
 template <int T>
 __device__ inline float row_sum(float v, float *room) {
-  v = wave_sum(v);
+  v = lanes::sum(v);
   if constexpr (T > 64) {
     if ((threadIdx.x & 63) == 0) room[threadIdx.x % T / 64] = v;
     __syncthreads();
@@ -197,7 +192,7 @@ __global__ __launch_bounds__(WG) void backward_kernel(const float *__restrict__ 
       if (!HOLD) g.load(gamma, cols, lane);
 #pragma unroll
       for (int e = 0; e < VPT; ++e) d.v[e] *= g.v[e];
-      float a = wave_sum(d.sum()), b = wave_sum(d.dot(xh));
+      float a = lanes::sum(d.sum()), b = lanes::sum(d.dot(xh));
       if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) {
           room[2][wave][0] = a;
