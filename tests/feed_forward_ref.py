@@ -51,7 +51,7 @@ class Norm(object):
         inner = np.abs(a) + np.abs(m1) + np.abs(self.xh * m2)
         dx_tol = self.s * (d_m1 + np.abs(self.xh) * d_m2 + self.d_xh * np.abs(m2) + U * (self.n + 8) * inner)
         rows = len(dy)
-        chain = 64 + rows / 16   # rows of one workgroup, its four rows, every sixteenth piece, sixteen of those
+        chain = 64 + rows / 16   # rows of one workgroup, its four rows, every 32nd piece, 32 of those
         dgamma, dbeta = (dy * self.xh).sum(0), dy.sum(0)
         dgamma_tol = (U * chain * np.abs(dy * self.xh) + np.abs(dy) * self.d_xh).sum(0)
         dbeta_tol = (U * chain * np.abs(dy)).sum(0)

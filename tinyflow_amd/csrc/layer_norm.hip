@@ -300,27 +300,30 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const float *__restric
   out[cols + c] = dbeta;
 }
 
-// dgamma and dbeta from `pieces` partial sums: 16 lanes a column pair of lines of 64 columns, each every sixteenth piece, added up
-// in their order.  No pieces (no rows): zeros.
+// dgamma and dbeta from `pieces` partial sums: kSumCols columns of both, one behind the other, a workgroup, and every kSlices-th
+// piece a lane, added up in their order.  No pieces (no rows): zeros.  4 096 x 1 024 and 5 003 x 1 537, whole backward pass, with 64 /
+// 32 / 16 / 8 columns: 15.7 / 14.5 / 14.7 / 16.1 and 25.4 / 23.8 / 25.1 / 28.0 us.
+constexpr int kSumCols = 32, kSlices = 1024 / kSumCols;
 __global__ __launch_bounds__(1024) void sum_pieces_kernel(const float *__restrict__ partial, float *__restrict__ dgamma,
                                                          float *__restrict__ dbeta, int pieces, int cols) {
-  __shared__ float sums[16][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane, width = 2 * (int64_t)cols;
+  __shared__ float sums[kSlices][kSumCols];
+  const int along = threadIdx.x % kSumCols, slice = threadIdx.x / kSumCols;
+  const int64_t c = (int64_t)blockIdx.x * kSumCols + along, width = 2 * (int64_t)cols;
   float s = 0.f;
   if (c < width) {
-    int p = wave;
-    for (; p + 48 < pieces; p += 64) {
-      const float a = partial[p * width + c], b = partial[(p + 16) * width + c];
-      const float d = partial[(p + 32) * width + c], e = partial[(p + 48) * width + c];
-      s += (a + b) + (d + e);
+    int p = slice;
+    for (; p + 3 * kSlices < pieces; p += 4 * kSlices) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = partial[(p + e * kSlices) * width + c];
+      s += (v[0] + v[1]) + (v[2] + v[3]);
     }
-    for (; p < pieces; p += 16) s += partial[p * width + c];
+    for (; p < pieces; p += kSlices) s += partial[p * width + c];
   }
-  sums[wave][lane] = s;
+  sums[slice][along] = s;
   __syncthreads();
-  if (wave > 0 || c >= width) return;
-  for (int w = 1; w < 16; ++w) s += sums[w][lane];
+  if (threadIdx.x >= kSumCols || c >= width) return;
+  for (int w = 1; w < kSlices; ++w) s += sums[w][along];
   float *out = c < cols ? dgamma : dbeta;
   if (out) out[c < cols ? c : c - cols] = s;
 }
@@ -453,7 +456,7 @@ extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const 
     }
   }
   if (params)
-    hipLaunchKernelGGL(sum_pieces_kernel, dim3((unsigned)((2 * cols + 63) / 64)), dim3(1024), 0, s, partial,
+    hipLaunchKernelGGL(sum_pieces_kernel, dim3((unsigned)((2 * cols + kSumCols - 1) / kSumCols)), dim3(1024), 0, s, partial,
                        dgamma ? (float *)dgamma->data : nullptr, dbeta ? (float *)dbeta->data : nullptr, rows ? pieces : 0,
                        (int)cols);
   if (partial) device_free(partial, s);
