@@ -319,6 +319,56 @@ def test_large_forward_with_values_that_are_not_finite(rt):
     np.testing.assert_array_equal(pre[1, 130], np.sign(up[k // 3]) * np.float32(np.inf))
 
 
+# workgroups of 64 rows, each with one lane group, one row or one column in its last tile
+WIDE = [(70, 40, 8300), (65, 16, 8193), (200, 131, 2501), (640, 33, 1000), (129, 1, 4100), (191, 700, 2999)]
+
+
+@pytest.mark.parametrize("m,k,f", WIDE)
+def test_workgroups_of_64_rows(rt, m, k, f):
+    activation = ACTIVATIONS[(m + k + f) % 4]
+    x, gate, up, _ = _data(m, k, f, stable_seed((m, k, f)))
+    (pre_ref, pre_tol), (h_ref, h_tol) = ref.gated(x, gate, up, activation)
+    pre, h = _forward(rt, x, gate, up, activation)
+    ref.assert_within(pre, pre_ref, pre_tol, "pre")
+    ref.assert_within(h, h_ref, h_tol, "h")
+    for want in ("pre", "h"):
+        alone, = _forward(rt, x, gate, up, activation, (want,))
+        np.testing.assert_array_equal(alone, pre if want == "pre" else h)
+
+
+@pytest.mark.parametrize("m,k,f", [(9, 0, 6), (40, 0, 70), (200, 0, 2501)])
+def test_no_reduction(rt, m, k, f):
+    pre, h = _forward(rt, np.ones((m, k), np.float32), *(np.ones((k, f), np.float32) for _ in range(2)), "sigmoid")
+    assert not pre.any() and not h.any()
+
+
+@pytest.mark.parametrize("m,k,f", [(6, 203, 70), (24, 1000, 300), (40, 3000, 70), (200, 131, 2501)])
+@pytest.mark.parametrize("value", [np.inf, np.nan, 3e38])
+def test_values_that_cannot_be_sliced(rt, m, k, f, value):
+    """Infinities, NaN and values next to the largest in x and in both weights, at the ends of waves' and workgroups' runs of the
+    reduction: each stays in the rows and columns that it is of, with its sign."""
+    x, gate, up, _ = _data(m, k, f, stable_seed((m, k, f)))
+    x, gate, up = (np.clip(v, -1, 1) for v in (x, gate, up))   # products with the largest stay in the range
+    along = sorted({0, 7, 8, 15, 16, k // 4, k // 2 - 1, k // 2, k - 1})
+    for i, at in enumerate(along):
+        gate[at, (5 * i) % f] = value * (-1) ** i
+        up[at, (7 * i + 3) % f] = -value * (-1) ** i
+    (pre_ref, pre_tol), _ = ref.gated(x, np.where(np.abs(gate) <= 1, gate, 0), np.where(np.abs(up) <= 1, up, 0), "relu")
+    pre, = _forward(rt, x, gate, up, "relu", ("pre",))
+    for half, w in enumerate((gate, up)):
+        plain = (np.abs(w) <= 1).all(0)
+        ref.assert_within(pre[half][:, plain], pre_ref[half][:, plain], pre_tol[half][:, plain], "columns without")
+        with np.errstate(all="ignore"):
+            wanted = x.astype(np.float64) @ w.astype(np.float64)
+        for c in np.flatnonzero(~plain):
+            if np.isfinite(value):
+                tol = ref.product(x, w[:, c:c + 1])[1]
+                ref.assert_within(pre[half][:, c:c + 1], wanted[:, c:c + 1], tol, "columns with")
+            else:
+                np.testing.assert_array_equal(pre[half][:, c], wanted[:, c].astype(np.float32) if np.isinf(value) else
+                                              np.full(m, np.nan, np.float32))
+
+
 @pytest.mark.parametrize("m,k,f", [(4100, 40, 70), (130, 33, 8200), (129, 4100, 60)])
 def test_backward_with_long_maxima(rt, m, k, f):
     x, gate, up, dh = _data(m, k, f, stable_seed((m, k, f, 1)))

@@ -13,6 +13,7 @@
 //            the activation and the product of the two are the epilogue.  dx is one product over dg and du one behind the other, dWg
 //            and dWu one launch of two halves.
 #include "gemm_pair.h"
+#include "gemm_split.h"
 #include "internal.h"
 #include "lanes.h"
 
@@ -639,15 +640,24 @@ struct Splitting {
   }
 };
 
-// Whether the forward pass runs on pairs, or on the fp32 instruction with nothing split (namespace few): us, fitted.  K x F, rows, few
-// / pairs: 1 024 x 4 096, 128 26 / 52, 256 42 / 51, 320 62 / 50, 512 81 / 53; 2 048 x 8 192, 128 86 / 128, 192 126 / 129, 256 162 /
-// 139; 4 096 x 11 008, 128 272 / 346, 192 414 / 394; 1 000 x 2 731, 320 50 / 53, 512 71 / 48; 512 x 1 376, 512 24 / 32, 1 024 38 / 32;
-// 256 x 1 024, 1 024 17 / 24.
+// Rows of a workgroup where few are: 64 once that fills half of the CUs.  32 / 64, us: 192 rows of 1 000 x 2 731 (129 workgroups of 64) 38.6 /
+// 30.7, 64 of 4 096 x 11 008 (172) 156 / 110, 256 of 1 024 x 4 096 (256) 36.1 / 34.2; 128 of 1 024 x 4 096 (128) 21.3 / 25.1, 64 of
+// 1 000 x 2 731 (43) 18.0 / 21.0.
+namespace few {
+constexpr int C = 2, kCols = 32 * C;  // columns of a lane, of a workgroup
+int rows_of(int64_t M, int64_t F) { return (int64_t)cdiv(F, kCols) * cdiv(M, 64) > num_cus() / 2 ? 64 : 32; }
+}  // namespace few
+
+// Whether the forward pass runs on pairs, or in registers with nothing stored split (namespace few): us, fitted.  K x F, rows, few
+// / pairs: 1 024 x 4 096, 128 22 / 43, 256 34 / 46, 320 61 / 49, 512 68 / 53; 2 048 x 8 192, 128 63 / 132, 192 114 / 133, 256 123 /
+// 135, 320 168 / 159; 4 096 x 11 008, 192 301 / 363, 320 445 / 433, 512 680 / 453; 1 000 x 2 731, 320 35 / 46, 384 64 / 45; 512 x
+// 1 376, 512 21 / 29, 768 41 / 31; 256 x 1 024, 1 024 17 / 24.
 bool forward_on_pairs(int64_t M, int64_t K, int64_t F) {
   if (K >= 1 << 22 || F >= 1 << 22) return false;  // a tile's rows would pass a buffer's end
+  const int rows = few::rows_of(M, F);
+  const double few = 12.0 + 4.0 * cdiv(M, rows) * rows * (double)K * cdiv(F, few::kCols) * few::kCols / 110e6;
   const double m = (double)cdiv(M, 32) * 32, k = (double)cdiv(K, 32) * 32, f = (double)cdiv(F, 32) * 32;
-  const double few = 8.0 + 4.0 * m * k * f / 100e6;
-  const double pairs = 22.0 + (24.0 * k * f + 12.0 * m * k) / 4.8e6 + 4.0 * m * k * f / 380e6;
+  const double pairs = 20.0 + (24.0 * k * f + 12.0 * m * k) / 4.8e6 + 4.0 * m * k * f / 380e6;
   return pairs < few;
 }
 // The backward pass: from 128 rows on, or where the weights are small.  Else products of the matrix multiply, which split nothing,
@@ -754,17 +764,20 @@ int64_t backward_by_pairs(int M, int K, int F, const float *x, const float *gate
 }
 
 // ---- few rows ---------------------------------------------------------------------------------------------------
-// Both projections, the activation and the product for up to 32 rows a workgroup, bound by reading the weights: nothing is staged.
-// A wave owns 32 C columns of both weights and a run of the reduction; the C columns of a lane's load are the operands of C
-// fp32 matrix instructions (columns C (lane mod 32) + j of the j-th), so that the lanes' order costs nothing, and 2 C
-// instructions use one value of x.  In a group of eight reduction elements lanes 0..31 hold the first four and lanes 32..63 the
-// others; DEPTH groups are under way.  The waves of a workgroup have runs of their own, added through LDS, and several workgroups
-// more of them, added by the last one to finish (gemm_core.h: Fold), in their order.
+// Both projections, the activation and the product for 32 or 64 rows a workgroup: nothing is staged.  A wave owns 32 C columns of both
+// weights and a run of the reduction; the C columns of a lane's load belong to C matrix instructions (columns C (lane mod 32) + j of
+// the j-th), so that the lanes' order costs nothing.  In a group of sixteen reduction elements lanes 0..31 hold the first eight and
+// lanes 32..63 the others, which is the operand of one bf16 instruction: the values are split in registers into three slices each
+// (gemm_split.h), six products of a weight's slices serve each 32 rows.  DEPTH groups are under way.  The waves of a workgroup have
+// runs of their own, added through LDS, and several workgroups more of them, added by the last one to finish (gemm_core.h: Fold), in
+// their order.  A run whose sums are not finite is computed again with the fp32 instruction.
 //
-// 24 rows, us: 1 000 x 2 731 14.6, 1 024 x 4 096 14.5 (2.3 TB/s), 2 048 x 8 192 37 (3.7), 4 096 x 11 008 102 (3.6); with four columns a
-// lane and two groups under way 18.0, 17.9, 37, 79; with eight waves 18.1, 15.0, 35, 95.
+// Bound by the weights' bytes for few rows, by the splitting (five and a half vector instructions a value) for more: with the fp32
+// instruction / so, us, rows of K x F: 24 of 1 000 x 2 731 14.5 / 13.1, of 2 048 x 8 192 36.5 / 31.5 (4.3 TB/s), of 4 096 x 11 008 102 / 85;
+// 128 of 1 024 x 4 096 26.2 / 21.3, of 2 048 x 8 192 86 / 63 (138 TFLOP/s); 256 of 1 000 x 2 731 47 / 32.  The loads' order matters as
+// much: where the compiler waits for both groups at once, 5 to 15 per cent.  Three groups under way need the registers of the second sums.
 namespace few {
-constexpr int kRows = 32, C = 2, kCols = 32 * C, kWaves = 4, kDepth = 4;
+constexpr int kWaves = 4, kDepth = 2, kGroup = 16;
 typedef float Columns __attribute__((ext_vector_type(C)));
 typedef Columns ColumnsU __attribute__((aligned(4)));
 
@@ -777,10 +790,10 @@ struct Args {
 };
 
 template <int N, int POLICY>
-__device__ inline auto load_columns(__amdgpu_buffer_rsrc_t r, uint32_t byte_off) {
+__device__ inline auto load_columns(__amdgpu_buffer_rsrc_t r, uint32_t byte_off, int uniform_off = 0) {
   typedef float V __attribute__((ext_vector_type(N)));
-  if constexpr (N == 4) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, (int)byte_off, 0, POLICY));
-  else return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(r, (int)byte_off, 0, POLICY));
+  if constexpr (N == 4) return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b128(r, (int)byte_off, uniform_off, POLICY));
+  else return __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(r, (int)byte_off, uniform_off, POLICY));
 }
 template <int POLICY, class V>
 __device__ inline void store_columns(__amdgpu_buffer_rsrc_t r, uint32_t byte_off, const V &v) {
@@ -789,16 +802,38 @@ __device__ inline void store_columns(__amdgpu_buffer_rsrc_t r, uint32_t byte_off
   else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(__attribute__((__vector_size__(8))) unsigned, v), r, (int)byte_off, 0, POLICY);
 }
 
-template <int ACT>
-__global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Args a) {
+// The three slices of eight reduction elements, as an operand.
+struct Slices {
+  split::bf16x8 of[3];
+  template <class Get>
+  __device__ inline explicit Slices(Get &&get) {
+    uint32_t words[3][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t pair_of[3];
+      split::split_pair(get(2 * i), get(2 * i + 1), pair_of);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) words[q][i] = pair_of[q];
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q)
+      of[q] = __builtin_bit_cast(split::bf16x8, split::u32x4v{words[q][0], words[q][1], words[q][2], words[q][3]});
+  }
+};
+
+// BLOCKS blocks of 32 rows
+template <int ACT, int BLOCKS>
+__global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(const Args a) {
+  constexpr int kRows = 32 * BLOCKS;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, along = lane & 31;
   const int strip = blockIdx.x % a.strips, piece = blockIdx.y, m0 = blockIdx.x / a.strips * kRows;
   const int rows = min(kRows, a.M - m0), c0 = strip * kCols;
   const int k_begin = piece * a.k_per_group + wave * (a.k_per_group / kWaves);
   const int k_end = min(a.K, k_begin + a.k_per_group / kWaves);
-  // Wave q adds up accumulators OWN q .. OWN q + OWN - 1, ROUND waves at a time; accumulator v holds rows 8 (v / 4) + 4 half + v mod 4.
-  constexpr int OWN = 16 / kWaves, ROUND = kWaves / 2;
+  // Wave q adds up accumulators OWN q .. OWN q + OWN - 1, ROUND waves at a time; accumulator v of a block holds rows 8 (v / 4) + 4 half
+  // + v mod 4.
+  constexpr int OWN = 16 * BLOCKS / kWaves, ROUND = kWaves / 2;
   __shared__ Columns part[ROUND][kWaves - 1][OWN][2][64];  // [wave that adds][wave that has][accumulator][g, u][lane]
   __shared__ unsigned last;
 
@@ -808,47 +843,127 @@ __global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Args a) {
   // a lane's columns past the end may hold the next row's values: they are not stored
   const int c = c0 + C * along;
   const uint32_t col_off = c < a.F ? (uint32_t)c * 4u : OOB;
-  const uint32_t row_off = along < rows ? (uint32_t)(m0 + along) * (uint32_t)a.K * 4u : OOB;
+  uint32_t row_off[BLOCKS];
+#pragma unroll
+  for (int i = 0; i < BLOCKS; ++i)
+    row_off[i] = 32 * i + along < rows ? (uint32_t)(m0 + 32 * i + along) * (uint32_t)a.K * 4u : OOB;
 
-  f32x16 acc[2][C];
+  f32x16 acc[2][C][BLOCKS], low[2][C][BLOCKS];  // products of the two highest slices, and of others
+  auto clear = [&](f32x16 (&sums)[2][C][BLOCKS]) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int j = 0; j < C; ++j)
+#pragma unroll
+        for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) sums[w][j][i][v] = 0.f;
+  };
+  clear(acc);
+  clear(low);
+
+  // COUNT reduction elements of a lane, those of the upper half of the wave COUNT further on: of x, of one row a block; of the weights,
+  // of C columns.  Behind the run's end they hold what there is: x counts as zero there, from `valid` of a lane's on, once it is used.  The
+  // uniform part of an address is a scalar, inside the buffer.
+  const uint32_t row_bytes = (uint32_t)a.F * 4u;
+  const int k_last = max(a.K - 1, 0);
+  auto load_x = [&](int k0, auto &to) {
+    constexpr int COUNT = sizeof(to[0]) / sizeof(float);
+    const int from = min(k0, k_last) * 4;
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+      for (int s = 0; s < COUNT; s += 4) {
+        const f32x4v v = __builtin_bit_cast(
+            f32x4v, __builtin_amdgcn_raw_buffer_load_b128(xr, (int)(row_off[i] + (uint32_t)(COUNT * half + s) * 4u), from, 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[i][s + e] = v[e];
+      }
+  };
+  auto load_weights = [&](int k0, auto &to) {
+    constexpr int COUNT = sizeof(to[0]) / sizeof(Columns);
+    const uint32_t lane_off = col_off + (uint32_t)(COUNT * half) * row_bytes;
+#pragma unroll
+    for (int s = 0; s < COUNT; ++s) {
+      const int from = (int)((uint32_t)min(k0 + s, k_last) * row_bytes);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) to[w][s] = load_columns<C, 0>(rsrc[w], lane_off, from);
+    }
+  };
+  float xv[kDepth][BLOCKS][8];
+  Columns wv[kDepth][2][8];
+  auto load = [&](int at, int k0) {
+    load_x(k0, xv[at]);
+    load_weights(k0, wv[at]);
+  };
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) {
+    load(d, k_begin + kGroup * d);
+    __builtin_amdgcn_sched_barrier(0);  // in the order of the loop: the wait for one group leaves the others under way
+  }
+  for (int k0 = k_begin; k0 < k_end; k0 += kGroup * kDepth)
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const int valid = k_end - (k0 + kGroup * d) - 8 * half;
+      split::bf16x8 xs[BLOCKS][3];
+#pragma unroll
+      for (int i = 0; i < BLOCKS; ++i) {
+        const Slices slices([&](int k) { return k < valid ? xv[d][i][k] : 0.f; });
+#pragma unroll
+        for (int q = 0; q < 3; ++q) xs[i][q] = slices.of[q];
+      }
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int j = 0; j < C; ++j) {
+          const Slices weights([&](int k) { return wv[d][w][k][j]; });
+#pragma unroll
+          for (int p = 0; p < 6; ++p) {
+            constexpr int of_x[6] = {0, 0, 1, 0, 1, 2}, of_w[6] = {0, 1, 0, 2, 1, 0};
+#pragma unroll
+            for (int i = 0; i < BLOCKS; ++i) {
+              f32x16 &sum = p == 0 ? acc[w][j][i] : low[w][j][i];
+              sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xs[i][of_x[p]], weights.of[of_w[p]], sum, 0, 0, 0);
+            }
+          }
+        }
+      load(d, k0 + kGroup * (d + kDepth));
+      __builtin_amdgcn_sched_barrier(0);  // nothing of the next group, whose loads may still be under way, in front of this one
+    }
+  float finite = 0.f;
 #pragma unroll
   for (int w = 0; w < 2; ++w)
 #pragma unroll
     for (int j = 0; j < C; ++j)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) acc[w][j][v] = 0.f;
-
-  // x: four reduction elements of one row; weights: four rows of C columns
-  f32x4v xv[kDepth];
-  Columns wv[kDepth][2][4];
-  auto load = [&](int at, int k0) {
-    const int k = k0 + 4 * half;
+      for (int i = 0; i < BLOCKS; ++i)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const uint32_t off = k + s < k_end ? (col_off + (uint32_t)(k + s) * (uint32_t)a.F * 4u) | (col_off & OOB) : OOB;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) wv[at][w][s] = load_columns<C, 0>(rsrc[w], off);
-    }
-    const f32x4v v = buf_load4(xr, k < k_end ? (row_off + (uint32_t)k * 4u) | (row_off & OOB) : OOB);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) xv[at][s] = k + s < k_end ? v[s] : 0.f;
-  };
-#pragma unroll
-  for (int d = 0; d < kDepth; ++d) load(d, k_begin + 8 * d);
-  for (int k0 = k_begin; k0 < k_end; k0 += 8 * kDepth)
-#pragma unroll
-    for (int d = 0; d < kDepth; ++d) {
+        for (int v = 0; v < 16; ++v) {
+          acc[w][j][i][v] = (acc[w][j][i][v] + low[w][j][i][v]) * split::kUnscale;
+          finite = __builtin_fmaf(acc[w][j][i][v], 0.f, finite);  // NaN of an infinity or a NaN
+        }
+  if (__any(finite != finite)) {
+    clear(acc);
+#pragma unroll 1
+    for (int k0 = k_begin; k0 < k_end; k0 += 8) {
+      float x4[BLOCKS][4];
+      Columns w4[2][4];
+      load_weights(k0, w4);
+      load_x(k0, x4);
+      const int valid = k_end - k0 - 4 * half;
 #pragma unroll
       for (int s = 0; s < 4; ++s)
 #pragma unroll
         for (int w = 0; w < 2; ++w)
 #pragma unroll
           for (int j = 0; j < C; ++j)
-            acc[w][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(xv[d][s], wv[d][w][s][j], acc[w][j], 0, 0, 0);
-      load(d, k0 + 8 * (d + kDepth));
+#pragma unroll
+            for (int i = 0; i < BLOCKS; ++i)
+              acc[w][j][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(s < valid ? x4[i][s] : 0.f, s < valid ? w4[w][s][j] : 0.f, acc[w][j][i], 0, 0, 0);
     }
+  }
 
-  auto first_row = [](int v) { return 8 * (v / 4) + v % 4; };
+  auto first_row = [](int v) { return 32 * (v / 16) + 8 * (v % 16 / 4) + v % 4; };
   Columns sum[2][OWN];
 #pragma unroll
   for (int round = 0; round < kWaves / ROUND; ++round) {
@@ -863,7 +978,7 @@ __global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Args a) {
         for (int w = 0; w < 2; ++w) {
           Columns o;
 #pragma unroll
-          for (int j = 0; j < C; ++j) o[j] = acc[w][j][q * OWN + i];
+          for (int j = 0; j < C; ++j) o[j] = acc[w][j][(q * OWN + i) / 16][(q * OWN + i) % 16];
           if (wave == q) sum[w][i] = o;
           else part[q % ROUND][wave - (wave > q)][i][w][lane] = o;
         }
@@ -1011,21 +1126,22 @@ int64_t forward(int M, int K, int F, const float *x, const float *gate, const fl
     });
     return 0;
   }
-  const int64_t groups = (int64_t)a.strips * cdiv(M, kRows);
-  // about a workgroup a CU, a wave's run 32 reduction elements at least; two a CU: 24 rows of 1 024 x 4 096 14.8 / 16.3 us,
-  // 2 048 x 8 192 38.0 / 35.7, 2 048 x 16 384 56.6 / 60.1
+  const int rows = rows_of(M, F);
+  const int64_t groups = (int64_t)a.strips * cdiv(M, rows);
+  // about a workgroup a CU, a wave's run 32 reduction elements at least
   int pieces = (int)std::max<int64_t>(1, std::min<int64_t>({num_cus() / groups, K / (kWaves * 32), 32}));
-  a.k_per_group = cdiv(K, pieces * kWaves * 8) * kWaves * 8;
+  a.k_per_group = cdiv(K, pieces * kWaves * kGroup) * kWaves * kGroup;
   a.pieces = K ? cdiv(K, a.k_per_group) : 1;
   if (a.pieces > 1) {
-    const size_t bytes = (size_t)groups * a.pieces * 2 * kRows * kCols * 4;
+    const size_t bytes = (size_t)groups * a.pieces * 2 * rows * kCols * 4;
     if (being_captured(s)) return kCaptured;
     a.tickets = fold_tickets(s);
     a.scratch = a.tickets ? (float *)device_alloc(bytes, s) : nullptr;
     if (!a.scratch) return (int64_t)block_bytes(bytes);
   }
   with_activation(activation, [&](auto act) {
-    hipLaunchKernelGGL(forward_kernel<decltype(act)::value>, dim3((unsigned)groups, (unsigned)a.pieces), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((rows > 32 ? forward_kernel<decltype(act)::value, 2> : forward_kernel<decltype(act)::value, 1>),
+                       dim3((unsigned)groups, (unsigned)a.pieces), dim3(kThreads), 0, s, a);
   });
   if (a.scratch) device_free(a.scratch, s);
   return 0;
