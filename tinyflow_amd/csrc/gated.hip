@@ -773,7 +773,7 @@ int64_t backward_by_pairs(int M, int K, int F, const float *x, const float *gate
 // their order.  A run whose sums are not finite is computed again with the fp32 instruction.
 //
 // Bound by the weights' bytes for few rows, by the splitting (five and a half vector instructions a value) for more: with the fp32
-// instruction / so, us, rows of K x F: 24 of 1 000 x 2 731 14.5 / 13.1, of 2 048 x 8 192 36.5 / 31.5 (4.3 TB/s), of 4 096 x 11 008 102 / 85;
+// instruction / so, us, rows of K x F: 24 of 1 000 x 2 731 14.5 / 12.5, of 2 048 x 8 192 36.5 / 31.5 (4.3 TB/s), of 4 096 x 11 008 102 / 85;
 // 128 of 1 024 x 4 096 26.2 / 21.3, of 2 048 x 8 192 86 / 63 (138 TFLOP/s); 256 of 1 000 x 2 731 47 / 32.  The loads' order matters as
 // much: where the compiler waits for both groups at once, 5 to 15 per cent.  Three groups under way need the registers of the second sums.
 namespace few {
@@ -785,7 +785,7 @@ struct Args {
   const float *x, *gate, *up;
   float *g, *u, *h;  // NULL: not wanted
   int M, K, F, strips, k_per_group, pieces;
-  float *scratch;    // [row group][strip][piece][accumulator][g, u][lane][C]
+  float *scratch;    // [strip][row group][piece][accumulator][g, u][lane][C]
   unsigned *tickets;
 };
 
@@ -801,6 +801,11 @@ __device__ inline void store_columns(__amdgpu_buffer_rsrc_t r, uint32_t byte_off
     __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(__attribute__((__vector_size__(16))) unsigned, v), r, (int)byte_off, 0, POLICY);
   else __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(__attribute__((__vector_size__(8))) unsigned, v), r, (int)byte_off, 0, POLICY);
 }
+
+// Whether neighbouring strips share an XCD: where they share lines, because the weights' rows start inside one.  Spread / so, us: one row of
+// 1 000 x 2 731 8.6 / 7.8, 64 rows 18.0 / 15.9, 128 rows 23.6 / 21.1; of 1 024 x 4 096 8.3 / 8.6, 16.3 / 16.4, 21.8 / 22.2, one row of
+// 2 048 x 8 192 27.4 / 29.6.
+__device__ inline bool by_neighbours(int F) { return F % 32 != 0; }
 
 // The three slices of eight reduction elements, as an operand.
 struct Slices {
@@ -827,7 +832,11 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
   constexpr int kRows = 32 * BLOCKS;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int half = lane >> 5, along = lane & 31;
-  const int strip = blockIdx.x % a.strips, piece = blockIdx.y, m0 = blockIdx.x / a.strips * kRows;
+  const int groups = gridDim.x, id = blockIdx.y * groups + blockIdx.x;
+  const int logical = by_neighbours(a.F) ? xcd_contiguous(id, groups * gridDim.y) : id;
+  const int piece = logical / groups, group = logical % groups, row_groups = groups / a.strips;
+  const int strip = by_neighbours(a.F) ? group / row_groups : group % a.strips;
+  const int m0 = (by_neighbours(a.F) ? group % row_groups : group / a.strips) * kRows;
   const int rows = min(kRows, a.M - m0), c0 = strip * kCols;
   const int k_begin = piece * a.k_per_group + wave * (a.k_per_group / kWaves);
   const int k_end = min(a.K, k_begin + a.k_per_group / kWaves);
@@ -837,7 +846,7 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
   __shared__ Columns part[ROUND][kWaves - 1][OWN][2][64];  // [wave that adds][wave that has][accumulator][g, u][lane]
   __shared__ unsigned last;
 
-  const uint32_t bytes = (uint32_t)a.K * (uint32_t)a.F * 4u;
+  const uint32_t bytes = (uint32_t)k_end * (uint32_t)a.F * 4u;  // nothing behind the run is fetched
   const __amdgpu_buffer_rsrc_t rsrc[2] = {make_rsrc(a.gate, bytes), make_rsrc(a.up, bytes)};
   const __amdgpu_buffer_rsrc_t xr = make_rsrc(a.x, (uint32_t)a.M * (uint32_t)a.K * 4u);
   // a lane's columns past the end may hold the next row's values: they are not stored
@@ -863,10 +872,10 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
   clear(low);
 
   // COUNT reduction elements of a lane, those of the upper half of the wave COUNT further on: of x, of one row a block; of the weights,
-  // of C columns.  Behind the run's end they hold what there is: x counts as zero there, from `valid` of a lane's on, once it is used.  The
-  // uniform part of an address is a scalar, inside the buffer.
+  // of C columns.  Behind the run's end they hold what there is, of the weights zeros and the last row again: x counts as zero there, from
+  // `valid` of a lane's on, once it is used.  The uniform part of an address is a scalar, inside the buffer.
   const uint32_t row_bytes = (uint32_t)a.F * 4u;
-  const int k_last = max(a.K - 1, 0);
+  const int k_last = max(k_end - 1, 0);
   auto load_x = [&](int k0, auto &to) {
     constexpr int COUNT = sizeof(to[0]) / sizeof(float);
     const int from = min(k0, k_last) * 4;
@@ -998,7 +1007,7 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
     constexpr int SC1 = 16;
     constexpr uint32_t kPieceBytes = 2u * kRows * kCols * 4u;
     const __amdgpu_buffer_rsrc_t pieces =
-        make_rsrc(a.scratch + (size_t)blockIdx.x * a.pieces * (kPieceBytes / 4), (uint32_t)a.pieces * kPieceBytes);
+        make_rsrc(a.scratch + (size_t)group * a.pieces * (kPieceBytes / 4), (uint32_t)a.pieces * kPieceBytes);
     auto offset = [&](int p, int w, int i) {
       return (int)((uint32_t)p * kPieceBytes + (uint32_t)(((wave * OWN + i) * 2 + w) * 64 + lane) * (4u * C));
     };
@@ -1012,10 +1021,10 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
     }
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (threadIdx.x == 0) last = atomicAdd(a.tickets + blockIdx.x, 1u) == (unsigned)(a.pieces - 1);
+    if (threadIdx.x == 0) last = atomicAdd(a.tickets + group, 1u) == (unsigned)(a.pieces - 1);
     __syncthreads();
     if (!last) return;
-    if (threadIdx.x == 0) a.tickets[blockIdx.x] = 0u;
+    if (threadIdx.x == 0) a.tickets[group] = 0u;
 #pragma unroll
     for (int i = 0; i < OWN; ++i) sum[0][i] = sum[1][i] = Columns{};
     // accumulators without a row were not written, and are not used
@@ -1061,7 +1070,8 @@ constexpr int kFewest = 4, kNarrow = 32, kWide = 1024;
 template <int ACT, int ROWS>
 __global__ __launch_bounds__(kWide) void fewest_kernel(const Args a) {
   constexpr int WAVES = kWide / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = blockIdx.x * kNarrow + 4 * (lane & 7);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = (by_neighbours(a.F) ? xcd_contiguous(blockIdx.x, gridDim.x) : (int)blockIdx.x) * kNarrow;
+  const int c = c0 + 4 * (lane & 7);
   __shared__ f32x4v part[WAVES][2][ROWS][8];
   const uint32_t bytes = (uint32_t)a.K * (uint32_t)a.F * 4u;
   const __amdgpu_buffer_rsrc_t rsrc[2] = {make_rsrc(a.gate, bytes), make_rsrc(a.up, bytes)};
@@ -1101,7 +1111,7 @@ __global__ __launch_bounds__(kWide) void fewest_kernel(const Args a) {
       if (lane < 8) part[wave][w][m][lane] = acc[w][m];
     }
   __syncthreads();
-  const int m = threadIdx.x / kNarrow, n = blockIdx.x * kNarrow + (int)threadIdx.x % kNarrow;
+  const int m = threadIdx.x / kNarrow, n = c0 + (int)threadIdx.x % kNarrow;
   if (m >= ROWS || m >= a.M || n >= a.F) return;
   float sum[2] = {0.f, 0.f};
 #pragma unroll
