@@ -369,7 +369,11 @@ def test_values_that_cannot_be_sliced(rt, m, k, f, value):
                                               np.full(m, np.nan, np.float32))
 
 
-@pytest.mark.parametrize("m,k,f", [(4100, 40, 70), (130, 33, 8200), (129, 4100, 60)])
+# (700 .. 4100, 200): on pairs, the last ones with 64 runs of maxima and more along rows, along columns, of the weights; (4100, 40)
+# .. (129, 4100, 60): in one launch, in pieces; (20, 300, 3000) .. (100, 700, 1500): a tile a wave
+@pytest.mark.parametrize("m,k,f", [(700, 520, 1000), (1027, 1030, 700), (513, 1000, 1543), (4100, 200, 520), (130, 330, 8200),
+                                   (129, 4100, 600), (4100, 40, 70), (130, 33, 8200), (129, 4100, 60), (20, 300, 3000),
+                                   (64, 65, 33), (100, 700, 1500)])
 def test_backward_with_long_maxima(rt, m, k, f):
     x, gate, up, dh = _data(m, k, f, stable_seed((m, k, f, 1)))
     dh[m // 2] = 0
@@ -390,3 +394,36 @@ def test_backward_with_long_maxima(rt, m, k, f):
     ref.assert_within(dx[:m - 1], wanted[0][0][:m - 1], wanted[0][1][:m - 1], "dx")
     ref.assert_within(dgate[:, :f - 1], wanted[1][0][:, :f - 1], wanted[1][1][:, :f - 1], "dgate")
     ref.assert_within(dup[:, :f - 1], wanted[2][0][:, :f - 1], wanted[2][1][:, :f - 1], "dup")
+
+
+@pytest.mark.parametrize("m,k,f", [(5, 70, 203), (40, 131, 1000), (300, 70, 97), (100, 700, 1500), (700, 520, 1000)])
+@pytest.mark.parametrize("value", [np.inf, np.nan])
+def test_gradients_of_values_that_are_not_finite(rt, m, k, f, value):
+    """In dh, in x and in a weight, at the ends of runs: each stays in the sums that it is a term of."""
+    x, gate, up, dh = _data(m, k, f, stable_seed((m, k, f)))
+    pre = np.stack([x @ gate, x @ up])
+    dpre, d_dpre = ref.pointwise_gradient(pre, dh, "silu")
+    wanted = ref.gated_backward(x, gate, up, dpre, d_dpre)
+    x, gate, dh = x.copy(), gate.copy(), dh.copy()
+    rows, cols = sorted({0, m // 2, m - 1}), sorted({0, 7, 8, f // 2, f - 1})
+    for i, c in enumerate(cols):
+        dh[rows[i % len(rows)], c] = value * (-1) ** i
+    gate[k - 1, f // 3], gate[k // 2, 0] = value, -value
+    dx, dgate, dup = _backward(rt, x, gate, up, pre, dh, "silu")
+    good_rows, good_cols = np.setdiff1d(np.arange(m), rows), np.setdiff1d(np.arange(f), cols)
+    good_k = np.setdiff1d(np.arange(k), [k - 1, k // 2])
+    assert not np.isfinite(dx[rows]).any()
+    assert not np.isfinite(dgate[:, cols]).any() and not np.isfinite(dup[:, cols]).any()
+    at = np.ix_(good_rows, good_k)
+    ref.assert_within(dx[at], wanted[0][0][at], wanted[0][1][at], "dx")
+    assert not np.isfinite(dx[:, [k - 1, k // 2]]).any()
+    for what, got, (v, tol) in (("dgate", dgate, wanted[1]), ("dup", dup, wanted[2])):
+        ref.assert_within(got[:, good_cols], v[:, good_cols], tol[:, good_cols], what)
+
+
+@pytest.mark.parametrize("m,k,f", [(0, 70, 40), (200, 0, 40), (200, 70, 0), (0, 700, 1500), (3, 0, 5), (3, 5, 0)])
+def test_backward_of_empty_extents(rt, m, k, f):
+    x, gate, up, dh = (np.ones(s, np.float32) for s in ((m, k), (k, f), (k, f), (m, f)))
+    for pre in (np.zeros((2, m, f), np.float32), None):
+        for g in _backward(rt, x, gate, up, pre, dh if pre is not None else np.zeros((2, m, f), np.float32), "sigmoid"):
+            assert not g.any()

@@ -161,8 +161,8 @@ def test_gated_feed_forward_next_to_2_gib(rt, room, m, k, f):
     t["h"].zero_()
     t["h"][picked("h")] = torch.from_numpy(dh).cuda()
     torch.cuda.synchronize()
-    if (k + 128) * f * 4 >= 1 << 32 or m == 1 << 26:
-        return   # a product that the matrix multiply refuses; scratch of 40 GB, which the pool would keep
+    if m == 1 << 26:
+        return   # scratch of 40 GB, which the pool would keep
     assert gpu_op.gated_feed_forward_backward(a["x"], a["gate"], a["up"], a["pre"], a["h"], a["dx"], a["dgate"], a["dup"], "silu",
                                               rt.stream) == 0
     torch.cuda.synchronize()

@@ -660,11 +660,15 @@ bool forward_on_pairs(int64_t M, int64_t K, int64_t F) {
   const double pairs = 20.0 + (24.0 * k * f + 12.0 * m * k) / 4.8e6 + 4.0 * m * k * f / 380e6;
   return pairs < few;
 }
-// The backward pass: from 128 rows on, or where the weights are small.  Else products of the matrix multiply, which split nothing,
-// around the pointwise pass.  products / pairs: 1 024 x 4 096, 32 rows 45 / 65, 128 75 / 74, 256 113 / 81; 2 048 x 8 192, 64
-// 115 / 212, 128 181 / 229, 256 318 / 245; 512 x 1 376, 8 35 / 35, 128 43 / 42; 128 x 512, 8 30 / 26, 256 43 / 31.
+// The backward pass likewise.  K x F, rows, few / pairs: 128 x 512, 1 024 20 / 35; 256 x 1 024, 1 024 36 / 40; 512 x 1 376, 64 17 / 38, 384 38 /
+// 41, 512 48 / 41; 1 000 x 1 537 (rows that start inside a line), 64 23 / 41, 128 37 / 43, 192 52 / 46; 1 024 x 4 096, 24 28 / 54, 128 55 /
+// 65, 192 76 / 71, 512 171 / 96; 2 048 x 8 192, 24 78 / 152, 64 120 / 168, 96 167 / 182, 128 198 / 187.
 bool backward_on_pairs(int64_t M, int64_t K, int64_t F) {
-  return M > 0 && K > 0 && F > 0 && K < 1 << 22 && F < 1 << 22 && (M >= 128 || K * F <= 1 << 20);
+  if (M == 0 || K == 0 || F == 0 || K >= 1 << 22 || F >= 1 << 22) return false;
+  const double m = (double)cdiv(M, 32) * 32, k = (double)cdiv(K, 64) * 64, f = (double)cdiv(F, 32) * 32;
+  const double few = 11.0 + 1.3e-6 * k * f + (F % 32 ? 110e-9 : 88e-9) * m * k * f;
+  const double pairs = 30.0 + 6.5e-6 * k * f + 0.59e-6 * m * (k + 3 * f) + 18.8e-9 * m * k * f;
+  return pairs < few;
 }
 
 // Scratch goes back to the pool when a call returns; a graph would go on using it.
@@ -1156,6 +1160,367 @@ int64_t forward(int M, int K, int F, const float *x, const float *gate, const fl
   if (a.scratch) device_free(a.scratch, s);
   return 0;
 }
+// ---- the backward pass of little work, in one launch with nothing stored split ------------------------------------------
+// Workgroups of dx (32 rows x 64 columns, along the inner axis, dg by gate and du by up in turn) and, behind them, of both weights'
+// gradients (64 rows x 32 columns of each, along the rows).  dg and du are computed from g, u and dh wherever they are an operand.  Everything
+// else is as in forward_kernel: a wave has a run of the reduction, its operands come from memory to registers and are split there, waves are
+// added through LDS and workgroups by the last one.
+struct BackwardArgs {
+  const float *x, *gate, *up, *g, *u, *dh;  // no dh: g and u are dg and du
+  float *dx, *dgate, *dup;                  // NULL: not wanted
+  int M, K, F;
+  struct Part {
+    int tiles, cols, pieces, run;  // tiles in all and side by side; reduction elements of a workgroup, a multiple of kWaves * kGroup
+    float *scratch;                // [tile][piece][accumulator of a lane][wave][lane]
+    unsigned *tickets;
+  } to_x, to_w;
+  bool alone;  // every wave has a tile of the weights' gradients for itself, a workgroup four side by side
+};
+
+template <int ACT>
+__device__ inline void projections_gradients(float g, float u, float d, float &dg, float &du) {
+  if constexpr (ACT == kGiven) {
+    dg = g;
+    du = u;
+  } else {
+    Source::gradients<ACT>(g, u, d, dg, du);
+  }
+}
+
+// Operands of a tile of dx: a, rows of dg and du, 32 of them; b, rows of the weights, 64 of them.
+template <int ACT>
+struct AlongInner {
+  static constexpr int SUBS = 2, BLOCKS = 1;
+  template <int COUNT>
+  struct Raw {
+    f32x4v d[3][COUNT / 4], w[2][2][COUNT / 4];
+  };
+  __amdgpu_buffer_rsrc_t d_rsrc[3], w_rsrc[2];
+  uint32_t d_off, w_off[2];
+  int half, k_end;
+  __device__ inline AlongInner(const BackwardArgs &a, int m0, int c0, int k_end_, int lane) : half(lane >> 5), k_end(k_end_) {
+    const uint32_t d_bytes = (uint32_t)a.M * (uint32_t)a.F * 4u, w_bytes = (uint32_t)a.K * (uint32_t)a.F * 4u;
+    d_rsrc[0] = make_rsrc(a.g, d_bytes);
+    d_rsrc[1] = make_rsrc(a.u, d_bytes);
+    d_rsrc[2] = make_rsrc(ACT == kGiven ? nullptr : a.dh, ACT == kGiven ? 0u : d_bytes);
+    w_rsrc[0] = make_rsrc(a.gate, w_bytes);
+    w_rsrc[1] = make_rsrc(a.up, w_bytes);
+    const int m = m0 + (lane & 31);
+    d_off = m < a.M ? (uint32_t)m * (uint32_t)a.F * 4u : OOB;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int k = c0 + 32 * j + (lane & 31);
+      w_off[j] = k < a.K ? (uint32_t)k * (uint32_t)a.F * 4u : OOB;
+    }
+  }
+  template <int COUNT>
+  __device__ inline void load(int k0, Raw<COUNT> &raw) const {
+    // behind the run's end what is there already, which counts as zero
+    const int from = (k0 < k_end ? k0 : max(k_end - 2 * COUNT, 0)) * 4;
+    auto four = [&](__amdgpu_buffer_rsrc_t r, uint32_t off) {
+      return __builtin_bit_cast(f32x4v, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, from, 0));
+    };
+#pragma unroll
+    for (int s = 0; s < COUNT / 4; ++s) {
+      const uint32_t at = (uint32_t)(COUNT * half + 4 * s) * 4u;
+#pragma unroll
+      for (int w = 0; w < (ACT == kGiven ? 2 : 3); ++w) raw.d[w][s] = four(d_rsrc[w], d_off + at);
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) raw.w[w][j][s] = four(w_rsrc[w], w_off[j] + at);
+    }
+  }
+  // EXACT: what counts as zero is zero in both, for the weights may hold an infinity there
+  template <bool EXACT, int COUNT>
+  __device__ inline void operands(int k0, const Raw<COUNT> &raw, float (&a)[SUBS][BLOCKS][COUNT], float (&b)[SUBS][2][COUNT]) const {
+    const int valid = k_end - k0 - COUNT * half;
+#pragma unroll
+    for (int s = 0; s < COUNT; ++s) {
+      float dg, du;
+      projections_gradients<ACT>(raw.d[0][s / 4][s % 4], raw.d[1][s / 4][s % 4], ACT == kGiven ? 0.f : raw.d[2][s / 4][s % 4], dg, du);
+      a[0][0][s] = s < valid ? dg : 0.f;
+      a[1][0][s] = s < valid ? du : 0.f;
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) b[w][j][s] = !EXACT || s < valid ? raw.w[w][j][s / 4][s % 4] : 0.f;
+    }
+  }
+};
+
+// Operands of a tile of the weights' gradients: a, 64 columns of x, two neighbours a lane; b, 32 columns of dg and of du.
+template <int ACT>
+struct AlongRows {
+  static constexpr int SUBS = 1, BLOCKS = 2;
+  template <int COUNT>
+  struct Raw {
+    split::f32x2v x[COUNT];
+    float d[3][COUNT];
+  };
+  __amdgpu_buffer_rsrc_t x_rsrc, d_rsrc[3];
+  uint32_t x_off, d_off, x_row, d_row;
+  int half, k_end;
+  __device__ inline AlongRows(const BackwardArgs &a, int k0, int f0, int k_end_, int lane) : half(lane >> 5), k_end(k_end_) {
+    x_row = (uint32_t)a.K * 4u;
+    d_row = (uint32_t)a.F * 4u;
+    x_rsrc = make_rsrc(a.x, (uint32_t)k_end * x_row);  // behind the run's end: zeros
+    d_rsrc[0] = make_rsrc(a.g, (uint32_t)k_end * d_row);
+    d_rsrc[1] = make_rsrc(a.u, (uint32_t)k_end * d_row);
+    d_rsrc[2] = make_rsrc(ACT == kGiven ? nullptr : a.dh, ACT == kGiven ? 0u : (uint32_t)k_end * d_row);
+    const int k = k0 + 2 * (lane & 31), f = f0 + (lane & 31);
+    x_off = k < a.K ? (uint32_t)k * 4u : OOB;
+    d_off = f < a.F ? (uint32_t)f * 4u : OOB;
+  }
+  template <int COUNT>
+  __device__ inline void load(int k0, Raw<COUNT> &raw) const {
+#pragma unroll
+    for (int s = 0; s < COUNT; ++s) {
+      const uint32_t row = (uint32_t)min(k0 + COUNT * half + s, k_end);
+      raw.x[s] = __builtin_bit_cast(split::f32x2v, __builtin_amdgcn_raw_buffer_load_b64(x_rsrc, (int)(x_off + row * x_row), 0, 0));
+#pragma unroll
+      for (int w = 0; w < (ACT == kGiven ? 2 : 3); ++w) raw.d[w][s] = buf_load(d_rsrc[w], d_off + row * d_row);
+    }
+  }
+  template <bool EXACT, int COUNT>
+  __device__ inline void operands(int, const Raw<COUNT> &raw, float (&a)[SUBS][BLOCKS][COUNT], float (&b)[SUBS][2][COUNT]) const {
+#pragma unroll
+    for (int s = 0; s < COUNT; ++s) {
+      a[0][0][s] = raw.x[s][0];
+      a[0][1][s] = raw.x[s][1];
+      projections_gradients<ACT>(raw.d[0][s], raw.d[1][s], ACT == kGiven ? 0.f : raw.d[2][s], b[0][0][s], b[0][1][s]);
+    }
+  }
+};
+
+// A tile's sums over one wave's run.
+template <class From>
+__device__ __forceinline__ void run_of_wave(const From &from, int k_begin, int k_end, f32x16 (&acc)[From::BLOCKS][2]) {
+  constexpr int BLOCKS = From::BLOCKS, SUBS = From::SUBS;
+  f32x16 low[BLOCKS][2];
+  auto clear = [](f32x16 (&sums)[BLOCKS][2]) {
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) sums[i][j][v] = 0.f;
+  };
+  clear(acc);
+  clear(low);
+  typename From::template Raw<8> raw[kDepth];
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) {
+    from.load(k_begin + kGroup * d, raw[d]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  for (int k0 = k_begin; k0 < k_end; k0 += kGroup * kDepth)
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      float a[SUBS][BLOCKS][8], b[SUBS][2][8];
+      from.template operands<false>(k0 + kGroup * d, raw[d], a, b);
+#pragma unroll
+      for (int sub = 0; sub < SUBS; ++sub) {
+        split::bf16x8 as[BLOCKS][3];
+#pragma unroll
+        for (int i = 0; i < BLOCKS; ++i) {
+          const Slices slices([&](int k) { return a[sub][i][k]; });
+#pragma unroll
+          for (int q = 0; q < 3; ++q) as[i][q] = slices.of[q];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const Slices bs([&](int k) { return b[sub][j][k]; });
+#pragma unroll
+          for (int p = 0; p < 6; ++p) {
+            constexpr int of_a[6] = {0, 0, 1, 0, 1, 2}, of_b[6] = {0, 1, 0, 2, 1, 0};
+#pragma unroll
+            for (int i = 0; i < BLOCKS; ++i) {
+              f32x16 &sum = p == 0 ? acc[i][j] : low[i][j];
+              sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as[i][of_a[p]], bs.of[of_b[p]], sum, 0, 0, 0);
+            }
+          }
+        }
+      }
+      from.load(k0 + kGroup * (d + kDepth), raw[d]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  float finite = 0.f;
+#pragma unroll
+  for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        acc[i][j][v] = (acc[i][j][v] + low[i][j][v]) * split::kUnscale;
+        finite = __builtin_fmaf(acc[i][j][v], 0.f, finite);
+      }
+  if (!__any(finite != finite)) return;
+  clear(acc);
+#pragma unroll 1
+  for (int k0 = k_begin; k0 < k_end; k0 += 8) {
+    typename From::template Raw<4> few_raw;
+    float a[SUBS][BLOCKS][4], b[SUBS][2][4];
+    from.load(k0, few_raw);
+    from.template operands<true>(k0, few_raw, a, b);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+        for (int i = 0; i < BLOCKS; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[sub][i][s], b[sub][j][s], acc[i][j], 0, 0, 0);
+  }
+}
+
+// The waves' sums added, and the pieces'; wave q then holds accumulators 4 q .. 4 q + 3 of every block, rows 8 q + 4 half + e.  False in
+// workgroups that have nothing left to do.
+template <int N>
+__device__ __forceinline__ bool join(const f32x16 (&acc)[N / 2][2], float *part, unsigned &last, const BackwardArgs::Part &p, int tile,
+                                     int piece, int wave, int lane, float (&own)[N][4]) {
+#pragma unroll
+  for (int q = 0; q < kWaves; ++q)
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = acc[b / 2][b % 2][4 * q + e];
+        if (wave == q) own[b][e] = v;
+        else part[((q * (kWaves - 1) + wave - (wave > q)) * 4 * N + b * 4 + e) * 64 + lane] = v;
+      }
+  __syncthreads();
+#pragma unroll
+  for (int o = 0; o < kWaves - 1; ++o)
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) own[b][e] += part[((wave * (kWaves - 1) + o) * 4 * N + b * 4 + e) * 64 + lane];
+  if (p.pieces == 1) return true;
+  constexpr int SC1 = 16;
+  constexpr uint32_t kPieceBytes = 4u * N * kThreads * 4u;
+  const __amdgpu_buffer_rsrc_t pieces = make_rsrc(p.scratch + (size_t)tile * p.pieces * (kPieceBytes / 4), (uint32_t)p.pieces * kPieceBytes);
+  auto offset = [&](int of, int b) { return (uint32_t)of * kPieceBytes + (uint32_t)((b * kWaves + wave) * 64 + lane) * 16u; };
+#pragma unroll
+  for (int b = 0; b < N; ++b) {
+    const f32x4v v = {own[b][0], own[b][1], own[b][2], own[b][3]};
+    store_columns<SC1>(pieces, offset(piece, b), v);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(p.tickets + tile, 1u) == (unsigned)(p.pieces - 1);
+  __syncthreads();
+  if (!last) return false;
+  if (threadIdx.x == 0) p.tickets[tile] = 0u;
+  f32x4v sum[N] = {};
+#pragma unroll 4
+  for (int of = 0; of < p.pieces; ++of)
+#pragma unroll
+    for (int b = 0; b < N; ++b) sum[b] += load_columns<4, SC1>(pieces, offset(of, b));
+#pragma unroll
+  for (int b = 0; b < N; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) own[b][e] = sum[b][e];
+  return true;
+}
+
+template <int ACT>
+__global__ __launch_bounds__(kThreads, 2) void backward_kernel(const BackwardArgs a) {
+  __shared__ float part[kWaves * (kWaves - 1) * 4 * 4 * 64];
+  __shared__ unsigned last;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int half = lane >> 5, along = lane & 31;
+  const int x_groups = a.to_x.tiles * a.to_x.pieces;
+  if ((int)blockIdx.x < x_groups) {
+    const int tile = blockIdx.x % a.to_x.tiles, piece = blockIdx.x / a.to_x.tiles;
+    const int m0 = tile / a.to_x.cols * 32, c0 = tile % a.to_x.cols * 64;
+    const int k_begin = piece * a.to_x.run + wave * (a.to_x.run / kWaves), k_end = min(a.F, k_begin + a.to_x.run / kWaves);
+    f32x16 acc[1][2];
+    run_of_wave(AlongInner<ACT>(a, m0, c0, k_end, lane), k_begin, k_end, acc);
+    float own[2][4];
+    if (!join<2>(acc, part, last, a.to_x, tile, piece, wave, lane, own)) return;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int m = m0 + 8 * wave + 4 * half + e, k = c0 + 32 * b + along;
+        if (m < a.M && k < a.K) a.dx[(size_t)m * a.K + k] = own[b][e];
+      }
+    return;
+  }
+  const int group = (int)blockIdx.x - x_groups;
+  const int tile = a.alone ? group * kWaves + wave : group % a.to_w.tiles, piece = a.alone ? 0 : group / a.to_w.tiles;
+  const int c0 = tile / a.to_w.cols * 64, f0 = tile % a.to_w.cols * 32;
+  const int of_wave = a.alone ? a.to_w.run : a.to_w.run / kWaves;
+  const int k_begin = a.alone ? 0 : piece * a.to_w.run + wave * of_wave, k_end = min(a.M, k_begin + of_wave);
+  f32x16 acc[2][2];
+  run_of_wave(AlongRows<ACT>(a, c0, f0, k_end, lane), k_begin, k_end, acc);
+  auto put = [&](int b, int row, float v) {
+    float *out = b % 2 ? a.dup : a.dgate;
+    const int k = c0 + 2 * row + b / 2, f = f0 + along;
+    if (out && k < a.K && f < a.F) out[(size_t)k * a.F + f] = v;
+  };
+  if (a.alone) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) put(b, 8 * (v / 4) + 4 * half + v % 4, acc[b / 2][b % 2][v]);
+    return;
+  }
+  float own[4][4];
+  if (!join<4>(acc, part, last, a.to_w, tile, piece, wave, lane, own)) return;
+#pragma unroll
+  for (int b = 0; b < 4; ++b)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) put(b, 8 * wave + 4 * half + e, own[b][e]);
+}
+
+int64_t backward(int M, int K, int F, const float *x, const float *gate, const float *up, const Source &d, float *dx, float *dgate,
+                 float *dup, hipStream_t s) {
+  BackwardArgs a{x, gate, up, d.p[0], d.p[1], d.dh, dx, dgate, dup, M, K, F, {}, {}, false};
+  // pieces as for all three gradients, so that each has the same bits alone
+  auto part = [](int rows, int cols, int steps) {
+    BackwardArgs::Part p{rows * cols, cols, 1, 0, nullptr, nullptr};
+    const int pieces = std::max(1, std::min({num_cus() / std::max(p.tiles, 1), steps / (kWaves * 2 * kGroup), 32}));
+    p.run = std::max(1, cdiv(steps, pieces * kWaves * kGroup)) * kWaves * kGroup;
+    p.pieces = std::max(1, cdiv(steps, p.run));
+    return p;
+  };
+  a.to_x = part(cdiv(M, 32), cdiv(K, 64), F);
+  a.to_w = part(cdiv(K, 64), cdiv(F, 32), M);
+  // A tile a wave where four waves would have a group each at most, or workgroups abound.  So / a tile a workgroup, us: 64 rows of
+  // 512 x 1 376 (344 tiles) 16.8 / 19.1, 128 rows 24.4 / 22.8; 128 rows of 1 000 x 1 537 (784) 37 / 40; 24 rows of 1 024 x 4 096 (2 048) 28 / 49.
+  a.alone = M <= kWaves * kGroup || a.to_w.tiles >= 2 * num_cus();
+  if (a.alone) {
+    a.to_w.run = M;
+    a.to_w.pieces = 1;
+  }
+  if (!dx) a.to_x.tiles = 0;
+  if (!dgate && !dup) a.to_w.tiles = 0;
+  Layout l;
+  const size_t x_at = a.to_x.pieces > 1 ? l.take((size_t)a.to_x.tiles * a.to_x.pieces * 32 * 64 * 4) : 0;
+  const size_t w_at = a.to_w.pieces > 1 ? l.take((size_t)a.to_w.tiles * a.to_w.pieces * 64 * 64 * 4) : 0;
+  char *base = nullptr;
+  if (l.bytes) {
+    unsigned *tickets = fold_tickets(s);
+    base = tickets ? (char *)device_alloc(l.bytes, s) : nullptr;
+    if (!base) return (int64_t)block_bytes(l.bytes);
+    a.to_x.scratch = (float *)(base + x_at);
+    a.to_w.scratch = (float *)(base + w_at);
+    a.to_x.tickets = tickets;
+    a.to_w.tickets = tickets + kFoldTicketSlots / 2;
+  }
+  const unsigned groups = (unsigned)(a.to_x.tiles * a.to_x.pieces + (a.alone ? cdiv(a.to_w.tiles, kWaves) : a.to_w.tiles * a.to_w.pieces));
+  if (groups == 0) return 0;
+  auto go = [&](auto act) {
+    hipLaunchKernelGGL(backward_kernel<decltype(act)::value>, dim3(groups), dim3(kThreads), 0, s, a);
+  };
+  if (d.dh) with_activation(d.activation, go);
+  else go(std::integral_constant<int, kGiven>{});
+  if (base) device_free(base, s);
+  return 0;
+}
 }  // namespace few
 
 unsigned vectors_grid(int64_t count) { return (unsigned)((count + 4 * kThreads - 1) / (4 * kThreads)); }
@@ -1164,12 +1529,6 @@ bool is_pair(const DLArray *pre, const DLArray *one) {
   return pre->ndim == one->ndim + 1 && pre->shape[0] == 2 &&
          std::equal(one->shape, one->shape + one->ndim, pre->shape + 1);
 }
-
-struct View {
-  int64_t shape[2];
-  DLArray array;
-  View(float *data, int64_t rows, int64_t cols, DLContext ctx) : shape{rows, cols}, array{data, ctx, 2, shape} {}
-};
 
 int geometry(const char *what, const DLArray *x, const DLArray *gate, const DLArray *up, int activation, int64_t &M,
              int64_t &K, int64_t &F) {
@@ -1289,38 +1648,11 @@ extern "C" int DLGpuGatedFeedForwardBackward(const DLArrayHandle input, const DL
   for (const DLArray *written : {(const DLArray *)dinput, (const DLArray *)dgate, (const DLArray *)dup}) announce_write(written);
   hipStream_t s = stream_of(stream);
   TF_REQUIRE(!being_captured(s), "the call takes scratch, which a captured stream cannot give back");
-  if (backward_on_pairs(M, K, F)) {
-    const float *g = pre ? (const float *)pre->data : (const float *)doutput->data;
-    const Source d{{g, g + M * F}, pre ? (const float *)doutput->data : nullptr, (int)M, (int)F, pre ? activation : kGiven};
-    const int64_t wanted = backward_by_pairs((int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data,
-                                             (const float *)up->data, d, dinput ? (float *)dinput->data : nullptr,
-                                             dgate ? (float *)dgate->data : nullptr, dup ? (float *)dup->data : nullptr, s);
-    if (wanted && memorytoSaving) *memorytoSaving = shortfall((size_t)wanted);
-    return wanted ? 0 : finish(s, "DLGpuGatedFeedForwardBackward");
-  }
-  const size_t bytes = ((pre ? (size_t)M * F * 2 : 0) + (dinput ? (size_t)M * K : 0)) * 4;
-  float *scratch = (float *)device_alloc(bytes, s);
-  if (!scratch) {
-    if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(bytes));
-    return 0;
-  }
-  float *d = pre ? scratch : (float *)doutput->data;
-  if (pre && M * F > 0)
-    with_activation(activation, [&](auto act) {
-      const float *g = (const float *)pre->data;
-      hipLaunchKernelGGL(activation_backward_kernel<decltype(act)::value>, dim3(vectors_grid(M * F)), dim3(kThreads), 0, s, g,
-                         g + M * F, (const float *)doutput->data, d, d + M * F, M * F);
-    });
-  View dg(d, M, F, input->ctx), du(d + M * F, M, F, input->ctx);
-  View other(scratch + (pre ? M * F * 2 : 0), M, K, input->ctx);
-  int rc = 0;
-  if (dinput) {
-    rc = DLGpuMatrixMultiply(&dg.array, false, gate, true, dinput, nullptr, stream);
-    if (rc == 0) rc = DLGpuMatrixMultiply(&du.array, false, up, true, &other.array, nullptr, stream);
-    if (rc == 0) rc = DLGpuMatrixElementwiseAdd(dinput, &other.array, dinput, stream);
-  }
-  if (rc == 0 && dgate) rc = DLGpuMatrixMultiply(input, true, &dg.array, false, dgate, nullptr, stream);
-  if (rc == 0 && dup) rc = DLGpuMatrixMultiply(input, true, &du.array, false, dup, nullptr, stream);
-  device_free(scratch, s);
-  return rc != 0 ? rc : finish(s, "DLGpuGatedFeedForwardBackward");
+  const float *g = pre ? (const float *)pre->data : (const float *)doutput->data;
+  const Source d{{g, g + M * F}, pre ? (const float *)doutput->data : nullptr, (int)M, (int)F, pre ? activation : kGiven};
+  const int64_t wanted = (backward_on_pairs(M, K, F) ? backward_by_pairs : few::backward)(
+      (int)M, (int)K, (int)F, (const float *)input->data, (const float *)gate->data, (const float *)up->data, d,
+      dinput ? (float *)dinput->data : nullptr, dgate ? (float *)dgate->data : nullptr, dup ? (float *)dup->data : nullptr, s);
+  if (wanted && memorytoSaving) *memorytoSaving = shortfall((size_t)wanted);
+  return wanted ? 0 : finish(s, "DLGpuGatedFeedForwardBackward");
 }
