@@ -320,7 +320,8 @@ def test_large_forward_with_values_that_are_not_finite(rt):
 
 
 # workgroups of 64 rows, each with one lane group, one row or one column in its last tile
-WIDE = [(70, 40, 8300), (65, 16, 8193), (200, 131, 2501), (640, 33, 1000), (129, 1, 4100), (191, 700, 2999)]
+WIDE = [(70, 40, 8300), (65, 16, 8193), (200, 131, 2501), (640, 33, 1000), (129, 1, 4100), (191, 700, 2999), (927, 34, 2382),
+        (600, 256, 2500), (2000, 130, 1030)]   # the last ones: a strip a wave
 
 
 @pytest.mark.parametrize("m,k,f", WIDE)
@@ -342,7 +343,7 @@ def test_no_reduction(rt, m, k, f):
     assert not pre.any() and not h.any()
 
 
-@pytest.mark.parametrize("m,k,f", [(6, 203, 70), (24, 1000, 300), (40, 3000, 70), (200, 131, 2501)])
+@pytest.mark.parametrize("m,k,f", [(6, 203, 70), (24, 1000, 300), (40, 3000, 70), (200, 131, 2501), (600, 70, 2500)])
 @pytest.mark.parametrize("value", [np.inf, np.nan, 3e38])
 def test_values_that_cannot_be_sliced(rt, m, k, f, value):
     """Infinities, NaN and values next to the largest in x and in both weights, at the ends of waves' and workgroups' runs of the

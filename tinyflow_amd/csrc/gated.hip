@@ -661,12 +661,12 @@ bool forward_on_pairs(int64_t M, int64_t K, int64_t F) {
   return pairs < few;
 }
 // The backward pass likewise.  K x F, rows, few / pairs: 128 x 512, 1 024 20 / 35; 256 x 1 024, 1 024 36 / 40; 512 x 1 376, 64 17 / 38, 384 38 /
-// 41, 512 48 / 41; 1 000 x 1 537 (rows that start inside a line), 64 23 / 41, 128 37 / 43, 192 52 / 46; 1 024 x 4 096, 24 28 / 54, 128 55 /
+// 41, 512 48 / 41; 1 000 x 1 537 (rows that start inside a line), 64 23 / 41, 128 37 / 43, 192 52 / 46; 2 083 x 6 733, 57 178 / 147; 1 024 x 4 096, 24 28 / 54, 128 55 /
 // 65, 192 76 / 71, 512 171 / 96; 2 048 x 8 192, 24 78 / 152, 64 120 / 168, 96 167 / 182, 128 198 / 187.
 bool backward_on_pairs(int64_t M, int64_t K, int64_t F) {
   if (M == 0 || K == 0 || F == 0 || K >= 1 << 22 || F >= 1 << 22) return false;
   const double m = (double)cdiv(M, 32) * 32, k = (double)cdiv(K, 64) * 64, f = (double)cdiv(F, 32) * 32;
-  const double few = 11.0 + 1.3e-6 * k * f + (F % 32 ? 110e-9 : 88e-9) * m * k * f;
+  const double few = 11.0 + 1.3e-6 * k * f + (F % 32 ? 150e-9 : 88e-9) * m * k * f;
   const double pairs = 30.0 + 6.5e-6 * k * f + 0.59e-6 * m * (k + 3 * f) + 18.8e-9 * m * k * f;
   return pairs < few;
 }
@@ -789,6 +789,7 @@ struct Args {
   const float *x, *gate, *up;
   float *g, *u, *h;  // NULL: not wanted
   int M, K, F, strips, k_per_group, pieces;
+  bool alone;        // every wave has a strip for itself, a workgroup four side by side
   float *scratch;    // [strip][row group][piece][accumulator][g, u][lane][C]
   unsigned *tickets;
 };
@@ -838,12 +839,13 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
   const int half = lane >> 5, along = lane & 31;
   const int groups = gridDim.x, id = blockIdx.y * groups + blockIdx.x;
   const int logical = by_neighbours(a.F) ? xcd_contiguous(id, groups * gridDim.y) : id;
-  const int piece = logical / groups, group = logical % groups, row_groups = groups / a.strips;
-  const int strip = by_neighbours(a.F) ? group / row_groups : group % a.strips;
-  const int m0 = (by_neighbours(a.F) ? group % row_groups : group / a.strips) * kRows;
+  const int across = a.alone ? (a.strips + kWaves - 1) / kWaves : a.strips;
+  const int piece = logical / groups, group = logical % groups, row_groups = groups / across;
+  const int strip = (by_neighbours(a.F) ? group / row_groups : group % across) * (a.alone ? kWaves : 1) + (a.alone ? wave : 0);
+  const int m0 = (by_neighbours(a.F) ? group % row_groups : group / across) * kRows;
   const int rows = min(kRows, a.M - m0), c0 = strip * kCols;
-  const int k_begin = piece * a.k_per_group + wave * (a.k_per_group / kWaves);
-  const int k_end = min(a.K, k_begin + a.k_per_group / kWaves);
+  const int of_wave = a.alone ? a.k_per_group : a.k_per_group / kWaves;
+  const int k_begin = a.alone ? 0 : piece * a.k_per_group + wave * of_wave, k_end = min(a.K, k_begin + of_wave);
   // Wave q adds up accumulators OWN q .. OWN q + OWN - 1, ROUND waves at a time; accumulator v of a block holds rows 8 (v / 4) + 4 half
   // + v mod 4.
   constexpr int OWN = 16 * BLOCKS / kWaves, ROUND = kWaves / 2;
@@ -976,7 +978,40 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
     }
   }
 
+  auto finish = [&](int m, const Columns &g, const Columns &u) {
+    if (m >= rows) return;
+    const size_t at = (size_t)(m0 + m) * a.F + c;
+    Columns h;
+#pragma unroll
+    for (int j = 0; j < C; ++j) h[j] = act_of<ACT>(g[j]) * u[j];
+    auto put = [&](float *out, const Columns &value) {
+      if (!out) return;
+      if (c + C <= a.F) {
+        *reinterpret_cast<ColumnsU *>(out + at) = value;
+      } else {
+#pragma unroll
+        for (int j = 0; j < C - 1; ++j)
+          if (c + j < a.F) out[at + j] = value[j];
+      }
+    };
+    put(a.g, g);
+    put(a.u, u);
+    put(a.h, h);
+  };
   auto first_row = [](int v) { return 32 * (v / 16) + 8 * (v % 16 / 4) + v % 4; };
+  if (a.alone) {
+#pragma unroll
+    for (int v = 0; v < 16 * BLOCKS; ++v) {
+      if (first_row(v) >= rows) continue;
+      Columns of[2];
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int j = 0; j < C; ++j) of[w][j] = acc[w][j][v / 16][v % 16];
+      finish(first_row(v) + 4 * half, of[0], of[1]);
+    }
+    return;
+  }
   Columns sum[2][OWN];
 #pragma unroll
   for (int round = 0; round < kWaves / ROUND; ++round) {
@@ -1042,27 +1077,7 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
         }
   }
 #pragma unroll
-  for (int i = 0; i < OWN; ++i) {
-    const int m = first_row(wave * OWN + i) + 4 * half;
-    if (m >= rows) continue;
-    const size_t at = (size_t)(m0 + m) * a.F + c;
-    Columns h;
-#pragma unroll
-    for (int j = 0; j < C; ++j) h[j] = act_of<ACT>(sum[0][i][j]) * sum[1][i][j];
-    auto put = [&](float *out, const Columns &value) {
-      if (!out) return;
-      if (c + C <= a.F) {
-        *reinterpret_cast<ColumnsU *>(out + at) = value;
-      } else {
-#pragma unroll
-        for (int j = 0; j < C - 1; ++j)
-          if (c + j < a.F) out[at + j] = value[j];
-      }
-    };
-    put(a.g, sum[0][i]);
-    put(a.u, sum[1][i]);
-    put(a.h, h);
-  }
+  for (int i = 0; i < OWN; ++i) finish(first_row(wave * OWN + i) + 4 * half, sum[0][i], sum[1][i]);
 }
 
 // Up to four rows: vector multiply-adds.  Sixteen waves share 32 columns, eight lanes a row of the weights with four columns each, so
@@ -1132,7 +1147,7 @@ __global__ __launch_bounds__(kWide) void fewest_kernel(const Args a) {
 
 int64_t forward(int M, int K, int F, const float *x, const float *gate, const float *up, float *pre, float *h, int activation,
                 hipStream_t s) {
-  Args a{x, gate, up, pre, pre ? pre + (size_t)M * F : nullptr, h, M, K, F, cdiv(F, kCols), 0, 1, nullptr, nullptr};
+  Args a{x, gate, up, pre, pre ? pre + (size_t)M * F : nullptr, h, M, K, F, cdiv(F, kCols), 0, 1, false, nullptr, nullptr};
   if (M <= kFewest && K <= 2560) {
     with_activation(activation, [&](auto act) {
       hipLaunchKernelGGL((M > 2 ? fewest_kernel<decltype(act)::value, 4> : M > 1 ? fewest_kernel<decltype(act)::value, 2> : fewest_kernel<decltype(act)::value, 1>),
@@ -1141,11 +1156,19 @@ int64_t forward(int M, int K, int F, const float *x, const float *gate, const fl
     return 0;
   }
   const int rows = rows_of(M, F);
-  const int64_t groups = (int64_t)a.strips * cdiv(M, rows);
+  // A strip a wave where the reduction is short and workgroups abound.  So / a strip a workgroup, us: 512 rows of 34 x 2 382 (304
+  // workgroups) 17 / 27, 927 rows (570) 18 / 40; of 96 x 2 000, 512 rows (256) 20 / 16, 927 (480) 21 / 29; 512 of 200 x 4 000 (504) 31 / 36; 927
+  // of 128 x 1 024 (240) 22 / 16.
+  a.alone = K <= 256 && (int64_t)a.strips * cdiv(M, rows) > num_cus();
+  const int64_t groups = (int64_t)(a.alone ? cdiv(a.strips, kWaves) : a.strips) * cdiv(M, rows);
   // about a workgroup a CU, a wave's run 32 reduction elements at least
   int pieces = (int)std::max<int64_t>(1, std::min<int64_t>({num_cus() / groups, K / (kWaves * 32), 32}));
   a.k_per_group = cdiv(K, pieces * kWaves * kGroup) * kWaves * kGroup;
   a.pieces = K ? cdiv(K, a.k_per_group) : 1;
+  if (a.alone) {
+    a.pieces = 1;
+    a.k_per_group = std::max(K, 1);
+  }
   if (a.pieces > 1) {
     const size_t bytes = (size_t)groups * a.pieces * 2 * rows * kCols * 4;
     if (being_captured(s)) return kCaptured;
