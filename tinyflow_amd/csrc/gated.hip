@@ -11,7 +11,9 @@
 //            by columns for dWg and dWu, because every sum needs a scale of its own for each of its operands
 //   product  forward: the two weights' columns alternate in blocks of 32, so that a lane holds g and u of the same element and
 //            the activation and the product of the two are the epilogue.  dx is one product over dg and du one behind the other, dWg
-//            and dWu one launch of two halves.
+//            and dWu one of two halves, all in one launch.
+//
+// Little work is done in one launch from operands that stay in registers (namespace few).
 #include "gemm_pair.h"
 #include "gemm_split.h"
 #include "internal.h"
@@ -767,7 +769,7 @@ int64_t backward_by_pairs(int M, int K, int F, const float *x, const float *gate
   return 0;
 }
 
-// ---- few rows ---------------------------------------------------------------------------------------------------
+// ---- little work: nothing stored split ---------------------------------------------------------------------------
 // Both projections, the activation and the product for 32 or 64 rows a workgroup: nothing is staged.  A wave owns 32 C columns of both
 // weights and a run of the reduction; the C columns of a lane's load belong to C matrix instructions (columns C (lane mod 32) + j of
 // the j-th), so that the lanes' order costs nothing.  In a group of sixteen reduction elements lanes 0..31 hold the first eight and
