@@ -260,3 +260,49 @@ def test_calls_without_scratch_in_a_captured_graph(rt):
         for g, arr in zip(got, (n, h, y, dx)):
             np.testing.assert_array_equal(g, arr.asnumpy())
     gpu_op.destroy_cudaStream(stream)
+
+
+# ------------------------------------------------------------------------ calls at once
+
+def test_two_threads_with_a_stream_each(rt):
+    """Scratch, tickets and the pool under calls that two threads make at the same time: the same bits as one after the other."""
+    import threading
+    from tinyflow_amd import gpu_op, ndarray
+    shapes = [(24, 300, 520), (700, 520, 1000)]   # folded in one launch; on pairs, with planes and pieces
+    work = []
+    for t, (rows, width, inner) in enumerate(shapes):
+        v = _values(rows, width, inner, 40 + t)
+        a = {k: ndarray.array(x, ctx=rt.ctx) for k, x in v.items()}
+        outs = [ndarray.empty(s, ctx=rt.ctx) for s in ((rows, width), (2, rows, inner), (rows, inner), (rows, width), (width, inner),
+                                                       (width, inner), (rows, width), (width,), (width,))]
+        work.append((a, outs, gpu_op.create_cudaStream()))
+
+    def calls(a, outs, stream):
+        n, pre, h, dx, dgate, dup, dn, dgamma, dbeta = outs
+        gpu_op.layer_norm_forward(a["x"], a["gamma"], a["beta"], n, EPS, stream)
+        assert gpu_op.gated_feed_forward(n, a["gate"], a["up"], pre, h, "silu", stream) == 0
+        assert gpu_op.gated_feed_forward_backward(n, a["gate"], a["up"], pre, h, dx, dgate, dup, "silu", stream) == 0
+        assert gpu_op.layer_norm_backward(a["x"], a["gamma"], dx, dn, dgamma, dbeta, EPS, stream) == 0
+
+    wanted = []
+    for w in work:
+        calls(*w)
+        wanted.append([o.asnumpy() for o in w[1]])
+    failures = []
+
+    def run(w):
+        try:
+            for _ in range(30):
+                calls(*w)
+        except Exception as e:   # the test's thread reports it
+            failures.append(e)
+    threads = [threading.Thread(target=run, args=(w,)) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    for w, values in zip(work, wanted):
+        for o, value in zip(w[1], values):
+            np.testing.assert_array_equal(o.asnumpy(), value)
+        gpu_op.destroy_cudaStream(w[2])

@@ -44,7 +44,7 @@ def test_counter_dropout(rt, room):
     count, some = (1 << 34) + 1026, 4096   # the counter of an element passes 32 bits at 2^34
     t = room(count)
     x = np.random.RandomState(3).normal(0, 1, some).astype(np.float32)
-    places = [0, (1 << 31) - 2048, (1 << 32) - 2048, (1 << 34) - 3072]
+    places = [0, (1 << 31) - 2048, (1 << 32) - 2048, (1 << 34) - 2048]
     for at in places:
         n = min(some, count - at)
         t[at:at + n] = torch.from_numpy(x[:n])
