@@ -10,8 +10,10 @@
 //
 // Bound: HBM.  A row is read once into registers, by a wave or by as many waves as it takes, and both
 // statistics are taken from there, the squares after the mean is known (a sum of x^2 would cancel where the mean is
-// large).  Sums are divided by the column count, not multiplied by its reciprocal: a row of one value then has that value for
-// its mean.  All sums are fp32; their order depends on the shape alone.
+// large).  The mean of fp32 sums is off by a few steps of its own last place, which next to a small spread is a large part of it (a row
+// of 777.7 in 5 000 columns: y off by 0.02).  So the deviations d = x - m from that first mean m are summed along with their
+// squares: with e = mean(d), mu = m + e and v = mean(d^2) - e^2, where next to nothing cancels, and xh = (d - e) s.  What is left is off by
+// steps of the deviations' last place.  All sums are fp32; their order depends on the shape alone.
 #include "internal.h"
 #include "lanes.h"
 
@@ -40,6 +42,26 @@ __device__ inline float row_sum(float v, float *room) {
     for (int w = 0; w < T / 64; ++w) v += room[w];
   }
   return v;
+}
+
+// Two sums at once.
+template <int T>
+__device__ inline void row_sums(float &a, float &b, float (*room)[2]) {
+  a = lanes::sum(a);
+  b = lanes::sum(b);
+  if constexpr (T > 64) {
+    if ((threadIdx.x & 63) == 0) {
+      room[threadIdx.x % T / 64][0] = a;
+      room[threadIdx.x % T / 64][1] = b;
+    }
+    __syncthreads();
+    a = b = 0.f;
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) {
+      a += room[w][0];
+      b += room[w][1];
+    }
+  }
 }
 
 // VPT vectors of a row in the registers of T lanes: vector e of lane l holds columns 4 (e T + l) and the three behind it;
@@ -97,9 +119,15 @@ struct Row {
   }
 };
 
-__device__ inline float inverse_std(float square_sum, float n, float eps) {
-  return 1.f / sqrtf(square_sum / n + eps);
-}
+// From the sums of a row's deviations d from its first mean and of their squares: xh = d s - es.
+struct Spread {
+  float s, es;
+  __device__ inline Spread(float sum, float square_sum, float n, float eps) {
+    const float e = sum / n, v = square_sum / n - e * e;
+    s = 1.f / sqrtf((v < 0.f ? 0.f : v) + eps);  // a NaN stays one
+    es = e * s;
+  }
+};
 
 // Workgroups as a grid none of whose dimensions, times the workgroup, passes 2^32.
 dim3 grid_of(int64_t groups) { return dim3((unsigned)std::min<int64_t>(groups, 1 << 20), (unsigned)((groups + (1 << 20) - 1) >> 20)); }
@@ -111,7 +139,7 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float 
                                                                   const float *__restrict__ beta, float *__restrict__ y,
                                                                   int64_t rows, int cols, float n, float eps) {
   constexpr int WG = T > 256 ? T : 256;
-  __shared__ float room[2][T / 64];
+  __shared__ float room[T / 64], rooms[T / 64][2];
   const int lane = threadIdx.x % T;
   const int64_t r = group_index() * (WG / T) + threadIdx.x / T;
   if (r >= rows) return;  // whole waves, and no barrier where several rows share a workgroup
@@ -119,32 +147,58 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float 
   row.load(x + r * cols, cols, lane);
   g.load(gamma, cols, lane);
   b.load(beta, cols, lane);
-  row.subtract(row_sum<T>(row.sum(), room[0]) / n, cols, lane);
-  const float s = inverse_std(row_sum<T>(row.dot(row), room[1]), n, eps);
+  row.subtract(row_sum<T>(row.sum(), room) / n, cols, lane);
+  float sum = row.sum(), squares = row.dot(row);
+  row_sums<T>(sum, squares, rooms);
+  const Spread of(sum, squares, n, eps);
 #pragma unroll
-  for (int e = 0; e < VPT; ++e) row.v[e] = row.v[e] * s * g.v[e] + b.v[e];
+  for (int e = 0; e < VPT; ++e) row.v[e] = (row.v[e] * of.s - of.es) * g.v[e] + b.v[e];
   row.template store<PAST>(y + r * cols, cols, lane);
 }
 
 // Rows that do not fit registers: three passes, the later two mostly out of the caches.
 constexpr int kLong = 1024;
+
+// f(column, sums) over a lane's columns of a row, in runs of kRun with sums of their own: of 2^26 columns no sum has more than 512 members.
+// One after the other the 65 536 of a lane leave the mean of a row of 777.7 at 777.25.
+constexpr int kRun = 256;
+template <class F>
+__device__ inline void sum_columns(int cols, float (&sums)[2], F &&f) {
+  sums[0] = sums[1] = 0.f;
+  for (int c0 = threadIdx.x; c0 < cols; c0 += kRun * kLong) {
+    float run[2] = {0.f, 0.f};
+    const int end = min(cols, c0 + kRun * kLong);
+    for (int c = c0; c < end; c += kLong) f(c, run);
+    sums[0] += run[0];
+    sums[1] += run[1];
+  }
+}
+
+// A long row's first mean and its spread about it.
+__device__ inline Spread long_spread(const float *row, int cols, float n, float eps, float (*rooms)[kLong / 64][2], float &mean) {
+  float sums[2];
+  sum_columns(cols, sums, [&](int c, float (&run)[2]) { run[0] += row[c]; });
+  row_sums<kLong>(sums[0], sums[1], rooms[0]);
+  const float m = mean = sums[0] / n;
+  sum_columns(cols, sums, [&](int c, float (&run)[2]) {
+    const float d = row[c] - m;
+    run[0] += d;
+    run[1] += d * d;
+  });
+  row_sums<kLong>(sums[0], sums[1], rooms[1]);
+  return Spread(sums[0], sums[1], n, eps);
+}
+
 __global__ __launch_bounds__(kLong) void forward_long_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
                                                             const float *__restrict__ beta, float *__restrict__ y,
                                                             int64_t rows, int cols, float n, float eps) {
-  __shared__ float room[2][kLong / 64];
+  __shared__ float rooms[2][kLong / 64][2];
   if (group_index() >= rows) return;
   const float *row = x + group_index() * cols;
-  float s = 0.f;
-  for (int c = threadIdx.x; c < cols; c += kLong) s += row[c];
-  const float mean = row_sum<kLong>(s, room[0]) / n;
-  s = 0.f;
-  for (int c = threadIdx.x; c < cols; c += kLong) {
-    const float d = row[c] - mean;
-    s += d * d;
-  }
-  const float istd = inverse_std(row_sum<kLong>(s, room[1]), n, eps);
+  float mean;
+  const Spread of = long_spread(row, cols, n, eps, rooms, mean);
   float *out = y + group_index() * cols;
-  for (int c = threadIdx.x; c < cols; c += kLong) out[c] = (row[c] - mean) * istd * gamma[c] + beta[c];
+  for (int c = threadIdx.x; c < cols; c += kLong) out[c] = ((row[c] - mean) * of.s - of.es) * gamma[c] + beta[c];
 }
 
 // Columns of a partial sum in memory: whole lines of kSumCols, so that a workgroup that adds them reads no neighbour's: 5 003 x 1 537 23.8 ->
@@ -153,7 +207,8 @@ constexpr int kSumCols = 32;
 __host__ __device__ inline int64_t padded(int64_t cols) { return (cols + kSumCols - 1) / kSumCols * kSumCols; }
 
 // Rows blockIdx.x * (WG / T) + ..., then gridDim.x * (WG / T) further on, and so on, the next one on its way while one is worked
-// on: every lane keeps the sums of dy xh and dy of its columns over the rows that it sees.  At the end the workgroup's rows are
+// on where PARAMS: without, workgroups have a row of each of their WG / T, and the registers are too few for a second one in the longest rows
+// (us with it / without: 1 000 x 16 000 45 / 37.6, 2 000 x 8 000 44 / 31.6, 4 096 x 1 024 7.2 / 6.3).  With PARAMS every lane keeps the sums of dy xh and dy of its columns over the rows that it sees.  At the end the workgroup's rows are
 // added through LDS, in their order, and go to partial[blockIdx.x][2][padded(cols)].
 template <int T, int VPT, int WG, bool PARAMS, bool PAST>
 __global__ __launch_bounds__(WG) void backward_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
@@ -162,7 +217,7 @@ __global__ __launch_bounds__(WG) void backward_kernel(const float *__restrict__ 
   constexpr int ROWS = WG / T;
   constexpr bool HOLD = T * VPT < 4096;  // gamma in registers; else from the caches, row by row
   __shared__ float rooms[ROWS][3][T / 64][2];
-  const int lane = threadIdx.x % T, sub = threadIdx.x / T, wave = lane / 64;
+  const int lane = threadIdx.x % T, sub = threadIdx.x / T;
   auto &room = rooms[sub];
   const int64_t step = (int64_t)gridDim.x * ROWS;
   Row<T, VPT> g, dgamma, dbeta, xh, d;
@@ -176,16 +231,19 @@ __global__ __launch_bounds__(WG) void backward_kernel(const float *__restrict__ 
     of_dy.load(dy + r * cols, cols, lane);
   };
   int64_t first = (int64_t)blockIdx.x * ROWS;
-  if (first < rows) load(first + sub, xh, d);
+  if (PARAMS && first < rows) load(first + sub, xh, d);
   for (; first < rows; first += step) {
     const int64_t r = first + sub;
     const bool live = r < rows;  // of whole waves
     Row<T, VPT> next_x, next_d;
-    if (first + step < rows) load(r + step, next_x, next_d);
+    if (!PARAMS) load(r, xh, d);
+    else if (first + step < rows) load(r + step, next_x, next_d);
     xh.subtract(row_sum<T>(xh.sum(), &room[0][0][0]) / n, cols, lane);
-    const float s = inverse_std(row_sum<T>(xh.dot(xh), &room[1][0][0]), n, eps);
+    float sum = xh.sum(), squares = xh.dot(xh);
+    row_sums<T>(sum, squares, room[1]);
+    const Spread of(sum, squares, n, eps);
 #pragma unroll
-    for (int e = 0; e < VPT; ++e) xh.v[e] *= s;
+    for (int e = 0; e < VPT; ++e) xh.v[e] = xh.v[e] * of.s - of.es;  // past the end not zero, where dy is
     if (PARAMS && live) {
 #pragma unroll
       for (int e = 0; e < VPT; ++e) {
@@ -197,28 +255,18 @@ __global__ __launch_bounds__(WG) void backward_kernel(const float *__restrict__ 
       if (!HOLD) g.load(gamma, cols, lane);
 #pragma unroll
       for (int e = 0; e < VPT; ++e) d.v[e] *= g.v[e];
-      float a = lanes::sum(d.sum()), b = lanes::sum(d.dot(xh));
-      if constexpr (T > 64) {
-        if ((threadIdx.x & 63) == 0) {
-          room[2][wave][0] = a;
-          room[2][wave][1] = b;
-        }
-        __syncthreads();
-        a = b = 0.f;
-#pragma unroll
-        for (int w = 0; w < T / 64; ++w) {
-          a += room[2][w][0];
-          b += room[2][w][1];
-        }
-      }
+      float a = d.sum(), b = d.dot(xh);
+      row_sums<T>(a, b, room[2]);
       a /= n;
       b /= n;
 #pragma unroll
-      for (int e = 0; e < VPT; ++e) d.v[e] = (d.v[e] - a - xh.v[e] * b) * s;
+      for (int e = 0; e < VPT; ++e) d.v[e] = (d.v[e] - a - xh.v[e] * b) * of.s;
       if (live) d.template store<PAST>(dx + r * cols, cols, lane);
     }
-    xh = next_x;
-    d = next_d;
+    if (PARAMS) {
+      xh = next_x;
+      d = next_d;
+    }
   }
   if constexpr (PARAMS) {
     if constexpr (ROWS > 1) {
@@ -246,34 +294,32 @@ __global__ __launch_bounds__(WG) void backward_kernel(const float *__restrict__ 
   }
 }
 
-// Long rows: the statistics go to `stats`, for the sums over rows that follow.
+// Long rows: mean, s and es go to `stats`, for the sums over rows that follow.
 __global__ __launch_bounds__(kLong) void backward_long_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
                                                              const float *__restrict__ dy, float *__restrict__ dx,
                                                              float *__restrict__ stats, int cols, float n, float eps) {
-  __shared__ float room[4][kLong / 64];
+  __shared__ float rooms[3][kLong / 64][2];
   const int64_t base = (int64_t)blockIdx.x * cols;
   const float *row = x + base, *d = dy + base;
-  float s = 0.f;
-  for (int c = threadIdx.x; c < cols; c += kLong) s += row[c];
-  const float mean = row_sum<kLong>(s, room[0]) / n;
-  s = 0.f;
-  for (int c = threadIdx.x; c < cols; c += kLong) s += (row[c] - mean) * (row[c] - mean);
-  const float istd = inverse_std(row_sum<kLong>(s, room[1]), n, eps);
+  float mean;
+  const Spread of = long_spread(row, cols, n, eps, rooms, mean);
   if (stats && threadIdx.x == 0) {
-    stats[2 * (int64_t)blockIdx.x] = mean;
-    stats[2 * (int64_t)blockIdx.x + 1] = istd;
+    float *to = stats + 3 * (int64_t)blockIdx.x;
+    to[0] = mean;
+    to[1] = of.s;
+    to[2] = of.es;
   }
   if (!dx) return;
-  float a = 0.f, b = 0.f;
-  for (int c = threadIdx.x; c < cols; c += kLong) {
+  float sums[2];
+  sum_columns(cols, sums, [&](int c, float (&run)[2]) {
     const float t = d[c] * gamma[c];
-    a += t;
-    b += t * ((row[c] - mean) * istd);
-  }
-  a = row_sum<kLong>(a, room[2]) / n;
-  b = row_sum<kLong>(b, room[3]) / n;
+    run[0] += t;
+    run[1] += t * ((row[c] - mean) * of.s - of.es);
+  });
+  row_sums<kLong>(sums[0], sums[1], rooms[2]);
+  const float a = sums[0] / n, b = sums[1] / n;
   for (int c = threadIdx.x; c < cols; c += kLong)
-    dx[base + c] = (d[c] * gamma[c] - a - (row[c] - mean) * istd * b) * istd;
+    dx[base + c] = (d[c] * gamma[c] - a - ((row[c] - mean) * of.s - of.es) * b) * of.s;
 }
 
 // 64 columns and a run of rows a workgroup; partial as above.
@@ -287,7 +333,7 @@ __global__ __launch_bounds__(256) void column_sums_kernel(const float *__restric
   if (c < cols)
     for (int64_t r = (int64_t)blockIdx.y * 4 + wave; r < rows; r += (int64_t)gridDim.y * 4) {
       const float d = dy[r * cols + c];
-      dgamma += d * ((x[r * cols + c] - stats[2 * r]) * stats[2 * r + 1]);
+      dgamma += d * ((x[r * cols + c] - stats[3 * r]) * stats[3 * r + 1] - stats[3 * r + 2]);
       dbeta += d;
     }
   if (wave > 0) {
@@ -425,7 +471,7 @@ extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const 
   else if (rows) pieces = (int)std::min<int64_t>((rows + 3) / 4, std::max<int64_t>(1, 4 * num_cus() * 64 / cols));
   float *partial = nullptr, *stats = nullptr;
   if (params && rows) {
-    const size_t partial_bytes = (size_t)pieces * 2 * padded(cols) * 4, stats_bytes = in_registers ? 0 : (size_t)rows * 8;
+    const size_t partial_bytes = (size_t)pieces * 2 * padded(cols) * 4, stats_bytes = in_registers ? 0 : (size_t)rows * 12;
     partial = (float *)device_alloc(partial_bytes + stats_bytes, s);
     if (!partial) {
       if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(partial_bytes + stats_bytes));
