@@ -208,8 +208,9 @@ __host__ __device__ inline int64_t padded(int64_t cols) { return (cols + kSumCol
 
 // Rows blockIdx.x * (WG / T) + ..., then gridDim.x * (WG / T) further on, and so on, the next one on its way while one is worked
 // on where PARAMS: without, workgroups have a row of each of their WG / T, and the registers are too few for a second one in the longest rows
-// (us with it / without: 1 000 x 16 000 45 / 37.6, 2 000 x 8 000 44 / 31.6, 4 096 x 1 024 7.2 / 6.3).  With PARAMS every lane keeps the sums of dy xh and dy of its columns over the rows that it sees.  At the end the workgroup's rows are
-// added through LDS, in their order, and go to partial[blockIdx.x][2][padded(cols)].
+// (us with it / without: 1 000 x 16 000 45 / 37.6, 2 000 x 8 000 44 / 31.6, 4 096 x 1 024 7.2 / 6.3).  With PARAMS every lane
+// keeps the sums of dy xh and dy of its columns over the rows that it sees.  At the end the workgroup's rows are added through LDS, in
+// their order, and go to partial[blockIdx.x][2][padded(cols)].
 template <int T, int VPT, int WG, bool PARAMS, bool PAST>
 __global__ __launch_bounds__(WG) void backward_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
                                                     const float *__restrict__ dy, float *__restrict__ dx,
@@ -297,14 +298,16 @@ __global__ __launch_bounds__(WG) void backward_kernel(const float *__restrict__ 
 // Long rows: mean, s and es go to `stats`, for the sums over rows that follow.
 __global__ __launch_bounds__(kLong) void backward_long_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
                                                              const float *__restrict__ dy, float *__restrict__ dx,
-                                                             float *__restrict__ stats, int cols, float n, float eps) {
+                                                             float *__restrict__ stats, int64_t rows, int cols, float n,
+                                                             float eps) {
   __shared__ float rooms[3][kLong / 64][2];
-  const int64_t base = (int64_t)blockIdx.x * cols;
+  if (group_index() >= rows) return;
+  const int64_t base = group_index() * cols;
   const float *row = x + base, *d = dy + base;
   float mean;
   const Spread of = long_spread(row, cols, n, eps, rooms, mean);
   if (stats && threadIdx.x == 0) {
-    float *to = stats + 3 * (int64_t)blockIdx.x;
+    float *to = stats + 3 * group_index();
     to[0] = mean;
     to[1] = of.s;
     to[2] = of.es;
@@ -498,8 +501,7 @@ extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const 
     else if (cols <= 8192) go(IC<1024>{}, IC<2>{});
     else if (in_registers) go(IC<1024>{}, IC<4>{});
     else {
-      // three arrays of 2^22 such rows are more than the memory
-      hipLaunchKernelGGL(backward_long_kernel, dim3((unsigned)rows), dim3(kLong), 0, s, x, g, dy, dx, stats, (int)cols, n, eps);
+      hipLaunchKernelGGL(backward_long_kernel, grid_of(rows), dim3(kLong), 0, s, x, g, dy, dx, stats, rows, (int)cols, n, eps);
       if (params)
         hipLaunchKernelGGL(column_sums_kernel, dim3((unsigned)((cols + 63) / 64), (unsigned)pieces), dim3(256), 0, s, x, dy,
                            stats, partial, rows, (int)cols);
