@@ -133,10 +133,10 @@ struct Spread {
 dim3 grid_of(int64_t groups) { return dim3((unsigned)std::min<int64_t>(groups, 1 << 20), (unsigned)((groups + (1 << 20) - 1) >> 20)); }
 __device__ inline int64_t group_index() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
 
-// T lanes a row, WG / T rows a workgroup.
+// T lanes a row, WG / T rows a workgroup.  y may be x, here and below.
 template <int T, int VPT, bool PAST>
-__global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
-                                                                  const float *__restrict__ beta, float *__restrict__ y,
+__global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float *x, const float *__restrict__ gamma,
+                                                                  const float *__restrict__ beta, float *y,
                                                                   int64_t rows, int cols, float n, float eps) {
   constexpr int WG = T > 256 ? T : 256;
   __shared__ float room[T / 64], rooms[T / 64][2];
@@ -189,8 +189,8 @@ __device__ inline Spread long_spread(const float *row, int cols, float n, float 
   return Spread(sums[0], sums[1], n, eps);
 }
 
-__global__ __launch_bounds__(kLong) void forward_long_kernel(const float *__restrict__ x, const float *__restrict__ gamma,
-                                                            const float *__restrict__ beta, float *__restrict__ y,
+__global__ __launch_bounds__(kLong) void forward_long_kernel(const float *x, const float *__restrict__ gamma,
+                                                            const float *__restrict__ beta, float *y,
                                                             int64_t rows, int cols, float n, float eps) {
   __shared__ float rooms[2][kLong / 64][2];
   if (group_index() >= rows) return;
