@@ -465,8 +465,12 @@ extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const 
   const bool params = dgamma || dbeta, in_registers = cols <= kMaxBackward;
   TF_REQUIRE(!params || !being_captured(s), "the gradients of the weights take scratch, which a captured stream cannot give back");
 
-  // How many workgroups share the rows, each with a partial sum of the weights' gradients: as many as are resident.  us at 256 / 512 /
-  // 768 / 1 024: 4 096 x 1 024 15.1 / 13.1 / - / 15.1, 5 003 x 1 537 35.8 / 24.4 / 22.7 / 28.1, 4 096 x 4 096 54 / 41 / - / 46.
+  // How many workgroups share the rows, each with a partial sum of the weights' gradients: two or three a CU, also of short rows, of which
+  // eight are resident but have as many more partial sums to write and to add.  us at 1 / 2 / 3 / 4 / 8 a CU: 8 192 x 100 12.2 / 10.6 /
+  // 10.7 / 11.4 / 13.5, x 512 15.4 / 14.3 / 13.7 / 15.3 / 19.4, x 1 024 24.8 / 21.7 / 21.6 / 24.8 / 29.2, x 2 048 47 / 37.2 / 37.4 / 39.6 /
+  // 43.8, x 4 096 90 / 71 / 81 / 79 / 93; 50 000 x 256 46 / 31.5 / 30.9 / 31.0 / 33.8, x 1 024 112 / 115 / 118 / 120 / 121, x 2 048 290 / 225 /
+  // 237 / 242 / 238, x 4 096 533 / 450 / 497 / 453 / 470; 2 048 rows of up to 1 024 the same within 5 %.  Of more than 4 096 columns a
+  // workgroup has 1 024 lanes, of which a CU holds one.
   const int rows_a_group = !in_registers ? 1 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1;
   const int64_t groups = (rows + rows_a_group - 1) / rows_a_group;
   int pieces = 0;
