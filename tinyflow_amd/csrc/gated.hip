@@ -334,7 +334,7 @@ __device__ inline void split_eight(const float (&x)[8], int exponent, char *at) 
   for (int i = 0; i < 8; ++i) {
     const float v = __builtin_ldexpf(x[i], exponent);
     h[i] = (_Float16)v;
-    l[i] = (_Float16)(v - (float)h[i]);
+    l[i] = (_Float16)((v - (float)h[i]) * pair::kLowScale);
   }
   *reinterpret_cast<pair::f16x8 *>(at) = h;
   *reinterpret_cast<pair::f16x8 *>(at + pair::kFragment) = l;
@@ -598,7 +598,7 @@ void give(pair::Work &w, char *base, size_t scratch, unsigned *tickets) {
   w.tickets = tickets;
 }
 
-// The two launches in front of the products.
+// The two launches in front of the products, three for long maxima.
 struct Splitting {
   Jobs jobs{};
   int maxima_groups = 0, exps_groups = 0, split_groups = 0;

@@ -3,13 +3,14 @@
 //   D[m, n] = sum_k A(m, k) B(n, k)
 //
 // Every row of A and of B (all that enters one sum) is multiplied by the power of two that brings its largest value into
-// [2^14, 2^15), and each element is then the sum of two fp16 numbers, x = h + l: h its nearest one, l the nearest of what is
-// left.  h keeps 11 significant bits and l eleven of the remaining thirteen and a sign, so at most 2^-23 of x is left off, as
-// long as l is a normal number: for everything down to 2^-17 of its row's largest value.  Below that the error stays at 2^-40 of that
-// value, where an fp32 product of rows of unlike magnitudes would go on being exact; what a sum of such products carries is
-// that against the largest terms.  Of the four products of two elements h h', h l' and l h' are computed, each exact in the
-// multiplier, and added up in fp32; l l' is at most 2^-23 of the product.  Three instructions take the place of the
-// six of three bf16 slices (gemm_split.h), with operands of four bytes an element, as many as fp32 has.
+// [2^14, 2^15), and each element is then made of two fp16 numbers, x = h + 2^-11 l: h its nearest one, l the nearest of 2^11 times what
+// is left.  h keeps 11 significant bits, and l eleven of the remaining thirteen and a sign, so at most 2^-23 of x is left off, as
+// long as neither leaves the normal numbers: for everything down to 2^-27 of its row's largest value.  Below that the error stays at
+// 2^-36, which is 2^-50 of that value at most, where an fp32 product of rows of unlike magnitudes would go on being exact.  (Without the factor
+// 2^11, l of everything below 2^-16 is subnormal, and the error stays at 2^-39: a reduction element 2^30 times the others and zero on the
+// other side took all but nine of their bits.)  Of the four products of two elements h h', h l' and l h' are computed, each exact in the
+// multiplier, and added up in fp32; |2^-11 l| is at most 2^-11 of x, so what the fourth would add is at most 2^-22 of the product.  Three
+// instructions take the place of the six of three bf16 slices (gemm_split.h), with operands of four bytes an element, as many as fp32 has.
 //
 // Rows that hold an infinity or a NaN cannot be split.  They carry kNotFinite for their exponent, and a tile that meets one
 // computes itself with the fp32 instruction from the operands as they were.
@@ -32,8 +33,10 @@ constexpr int kFragment = 1024;              // bytes: 32 rows x 16 reduction el
 constexpr int kStepBytes = 2 * kFragment;    // of 32 rows: h, then l
 constexpr int kNotFinite = INT32_MIN / 4;    // an exponent no finite row has
 
+constexpr float kLowScale = 0x1p11f, kLowUnscale = 0x1p-11f;  // of l, of the sums of products with one
+
 // A split operand: [block of 32 rows][step][h, l], the reduction padded with zeros to an even number of steps and the
-// rows to whole blocks; value = (h + l) * 2^-exps[row].
+// rows to whole blocks; value = (h + l kLowUnscale) * 2^-exps[row].
 struct Packed {
   const char *planes;
   const int *exps;
@@ -242,7 +245,7 @@ __global__ __launch_bounds__(THREADS, 2) void gemm_kernel(const Products product
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] += low[i][j];
+      for (int j = 0; j < TN; ++j) acc[i][j] += low[i][j] * kLowUnscale;
   } else {
     arrived(none);
     exact_tile<BM, BN>(acc, reinterpret_cast<float *>(lds), product.exact_a, product.exact_b, half, mb * 32, nb * 32, s_begin * BK, s_end * BK,
