@@ -650,12 +650,19 @@ constexpr int C = 2, kCols = 32 * C;  // columns of a lane, of a workgroup
 int rows_of(int64_t M, int64_t F) { return (int64_t)cdiv(F, kCols) * cdiv(M, 64) > num_cus() / 2 ? 64 : 32; }
 }  // namespace few
 
+// Whether the environment asks for the fp32 instruction, as it may of every other contraction: TINYFLOW_SPLIT=0.  Then all products are
+// those of namespace few, whose runs go the way of runs that cannot be sliced.
+bool on_fp32() {
+  const char *e = getenv("TINYFLOW_SPLIT");
+  return e && *e && atoi(e) == 0;
+}
+
 // Whether the forward pass runs on pairs, or in registers with nothing stored split (namespace few): us, fitted.  K x F, rows, few
 // / pairs: 1 024 x 4 096, 128 22 / 43, 256 34 / 46, 320 61 / 49, 512 68 / 53; 2 048 x 8 192, 128 63 / 132, 192 114 / 133, 256 123 /
 // 135, 320 168 / 159; 4 096 x 11 008, 192 301 / 363, 320 445 / 433, 512 680 / 453; 1 000 x 2 731, 320 35 / 46, 384 64 / 45; 512 x
 // 1 376, 512 21 / 29, 768 41 / 31; 256 x 1 024, 1 024 17 / 24.
 bool forward_on_pairs(int64_t M, int64_t K, int64_t F) {
-  if (K >= 1 << 22 || F >= 1 << 22) return false;  // a tile's rows would pass a buffer's end
+  if (K >= 1 << 22 || F >= 1 << 22 || on_fp32()) return false;  // a tile's rows would pass a buffer's end
   const int rows = few::rows_of(M, F);
   const double few = 12.0 + 4.0 * cdiv(M, rows) * rows * (double)K * cdiv(F, few::kCols) * few::kCols / 110e6;
   const double m = (double)cdiv(M, 32) * 32, k = (double)cdiv(K, 32) * 32, f = (double)cdiv(F, 32) * 32;
@@ -666,7 +673,7 @@ bool forward_on_pairs(int64_t M, int64_t K, int64_t F) {
 // 41, 512 48 / 41; 1 000 x 1 537 (rows that start inside a line), 64 23 / 41, 128 37 / 43, 192 52 / 46; 2 083 x 6 733, 57 178 / 147; 1 024 x 4 096, 24 28 / 54, 128 55 /
 // 65, 192 76 / 71, 512 171 / 96; 2 048 x 8 192, 24 78 / 152, 64 120 / 168, 96 167 / 182, 128 198 / 187.
 bool backward_on_pairs(int64_t M, int64_t K, int64_t F) {
-  if (M == 0 || K == 0 || F == 0 || K >= 1 << 22 || F >= 1 << 22) return false;
+  if (M == 0 || K == 0 || F == 0 || K >= 1 << 22 || F >= 1 << 22 || on_fp32()) return false;
   const double m = (double)cdiv(M, 32) * 32, k = (double)cdiv(K, 64) * 64, f = (double)cdiv(F, 32) * 32;
   const double few = 11.0 + 1.3e-6 * k * f + (F % 32 ? 150e-9 : 88e-9) * m * k * f;
   const double pairs = 30.0 + 6.5e-6 * k * f + 0.59e-6 * m * (k + 3 * f) + 18.8e-9 * m * k * f;
@@ -792,6 +799,8 @@ struct Args {
   float *g, *u, *h;  // NULL: not wanted
   int M, K, F, strips, k_per_group, pieces;
   bool alone;        // every wave has a strip for itself, a workgroup four side by side
+  bool exact;        // with the fp32 instruction from the start,
+  int skipped;       // the loop on slices left out: K then, else 0.  Two words: one would live through the loop, in a register that it needs
   float *scratch;    // [strip][row group][piece][accumulator][g, u][lane][C]
   unsigned *tickets;
 };
@@ -918,7 +927,7 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
     load(d, k_begin + kGroup * d);
     __builtin_amdgcn_sched_barrier(0);  // in the order of the loop: the wait for one group leaves the others under way
   }
-  for (int k0 = k_begin; k0 < k_end; k0 += kGroup * kDepth)
+  for (int k0 = k_begin + a.skipped; k0 < k_end; k0 += kGroup * kDepth)
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       const int valid = k_end - (k0 + kGroup * d) - 8 * half;
@@ -959,7 +968,7 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
           acc[w][j][i][v] = (acc[w][j][i][v] + low[w][j][i][v]) * split::kUnscale;
           finite = __builtin_fmaf(acc[w][j][i][v], 0.f, finite);  // NaN of an infinity or a NaN
         }
-  if (__any(finite != finite)) {
+  if (a.exact || __any(finite != finite)) {
     clear(acc);
 #pragma unroll 1
     for (int k0 = k_begin; k0 < k_end; k0 += 8) {
@@ -1149,7 +1158,7 @@ __global__ __launch_bounds__(kWide) void fewest_kernel(const Args a) {
 
 int64_t forward(int M, int K, int F, const float *x, const float *gate, const float *up, float *pre, float *h, int activation,
                 hipStream_t s) {
-  Args a{x, gate, up, pre, pre ? pre + (size_t)M * F : nullptr, h, M, K, F, cdiv(F, kCols), 0, 1, false, nullptr, nullptr};
+  Args a{x, gate, up, pre, pre ? pre + (size_t)M * F : nullptr, h, M, K, F, cdiv(F, kCols), 0, 1, false, on_fp32(), on_fp32() ? K : 0, nullptr, nullptr};
   if (M <= kFewest && K <= 2560) {
     with_activation(activation, [&](auto act) {
       hipLaunchKernelGGL((M > 2 ? fewest_kernel<decltype(act)::value, 4> : M > 1 ? fewest_kernel<decltype(act)::value, 2> : fewest_kernel<decltype(act)::value, 1>),
@@ -1200,6 +1209,8 @@ struct BackwardArgs {
     unsigned *tickets;
   } to_x, to_w;
   bool alone;  // every wave has a tile of the weights' gradients for itself, a workgroup four side by side
+  bool exact;   // as above,
+  int skipped;  // past any run's end
 };
 
 template <int ACT>
@@ -1320,7 +1331,7 @@ struct AlongRows {
 
 // A tile's sums over one wave's run.
 template <class From>
-__device__ __forceinline__ void run_of_wave(const From &from, int k_begin, int k_end, f32x16 (&acc)[From::BLOCKS][2]) {
+__device__ __forceinline__ void run_of_wave(const From &from, const BackwardArgs &args, int k_begin, int k_end, f32x16 (&acc)[From::BLOCKS][2]) {
   constexpr int BLOCKS = From::BLOCKS, SUBS = From::SUBS;
   f32x16 low[BLOCKS][2];
   auto clear = [](f32x16 (&sums)[BLOCKS][2]) {
@@ -1339,7 +1350,7 @@ __device__ __forceinline__ void run_of_wave(const From &from, int k_begin, int k
     from.load(k_begin + kGroup * d, raw[d]);
     __builtin_amdgcn_sched_barrier(0);
   }
-  for (int k0 = k_begin; k0 < k_end; k0 += kGroup * kDepth)
+  for (int k0 = k_begin + args.skipped; k0 < k_end; k0 += kGroup * kDepth)
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
       float a[SUBS][BLOCKS][8], b[SUBS][2][8];
@@ -1380,7 +1391,7 @@ __device__ __forceinline__ void run_of_wave(const From &from, int k_begin, int k
         acc[i][j][v] = (acc[i][j][v] + low[i][j][v]) * split::kUnscale;
         finite = __builtin_fmaf(acc[i][j][v], 0.f, finite);
       }
-  if (!__any(finite != finite)) return;
+  if (!args.exact && !__any(finite != finite)) return;
   clear(acc);
 #pragma unroll 1
   for (int k0 = k_begin; k0 < k_end; k0 += 8) {
@@ -1462,7 +1473,7 @@ __global__ __launch_bounds__(kThreads, 2) void backward_kernel(const BackwardArg
     const int m0 = tile / a.to_x.cols * 32, c0 = tile % a.to_x.cols * 64;
     const int k_begin = piece * a.to_x.run + wave * (a.to_x.run / kWaves), k_end = min(a.F, k_begin + a.to_x.run / kWaves);
     f32x16 acc[1][2];
-    run_of_wave(AlongInner<ACT>(a, m0, c0, k_end, lane), k_begin, k_end, acc);
+    run_of_wave(AlongInner<ACT>(a, m0, c0, k_end, lane), a, k_begin, k_end, acc);
     float own[2][4];
     if (!join<2>(acc, part, last, a.to_x, tile, piece, wave, lane, own)) return;
 #pragma unroll
@@ -1480,7 +1491,7 @@ __global__ __launch_bounds__(kThreads, 2) void backward_kernel(const BackwardArg
   const int of_wave = a.alone ? a.to_w.run : a.to_w.run / kWaves;
   const int k_begin = a.alone ? 0 : piece * a.to_w.run + wave * of_wave, k_end = min(a.M, k_begin + of_wave);
   f32x16 acc[2][2];
-  run_of_wave(AlongRows<ACT>(a, c0, f0, k_end, lane), k_begin, k_end, acc);
+  run_of_wave(AlongRows<ACT>(a, c0, f0, k_end, lane), a, k_begin, k_end, acc);
   auto put = [&](int b, int row, float v) {
     float *out = b % 2 ? a.dup : a.dgate;
     const int k = c0 + 2 * row + b / 2, f = f0 + along;
@@ -1503,7 +1514,7 @@ __global__ __launch_bounds__(kThreads, 2) void backward_kernel(const BackwardArg
 
 int64_t backward(int M, int K, int F, const float *x, const float *gate, const float *up, const Source &d, float *dx, float *dgate,
                  float *dup, hipStream_t s) {
-  BackwardArgs a{x, gate, up, d.p[0], d.p[1], d.dh, dx, dgate, dup, M, K, F, {}, {}, false};
+  BackwardArgs a{x, gate, up, d.p[0], d.p[1], d.dh, dx, dgate, dup, M, K, F, {}, {}, false, on_fp32(), on_fp32() ? 1 << 29 : 0};
   // pieces as for all three gradients, so that each has the same bits alone
   auto part = [](int rows, int cols, int steps) {
     BackwardArgs::Part p{rows * cols, cols, 1, 0, nullptr, nullptr};
