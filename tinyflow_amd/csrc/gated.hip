@@ -671,12 +671,17 @@ bool forward_on_pairs(int64_t M, int64_t K, int64_t F) {
 }
 // The backward pass likewise.  K x F, rows, few / pairs: 128 x 512, 1 024 20 / 35; 256 x 1 024, 1 024 36 / 40; 512 x 1 376, 64 17 / 38, 384 38 /
 // 41, 512 48 / 41; 1 000 x 1 537 (rows that start inside a line), 64 23 / 41, 128 37 / 43, 192 52 / 46; 2 083 x 6 733, 57 178 / 147; 1 024 x 4 096, 24 28 / 54, 128 55 /
-// 65, 192 76 / 71, 512 171 / 96; 2 048 x 8 192, 24 78 / 152, 64 120 / 168, 96 167 / 182, 128 198 / 187.
+// 65, 192 76 / 71, 512 171 / 96; 2 048 x 8 192, 24 78 / 152, 64 120 / 168, 96 167 / 182, 128 198 / 187.  Long reductions into few tiles:
+// 1 x 7, 524 288 389 / 1 264; 16 x 16, 1 048 576 758 / 2 543; 64 x 64, 16 384 33 / 64, 65 536 91 / 184; 128 x 256, 65 536 240 / 382; 256 x 512,
+// 16 384 210 / 146, 65 536 851 / 565; 128 x 512, 8 192 61 / 67; 128 x 65 536, 512 492 / 722; 512 x 16 384, 512 401 / 241.  That also keeps
+// pairs from narrow extents, which their blocks of 32 hold several times over (2^26 rows of 1 x 7: 43 GB beside arrays of 6).
 bool backward_on_pairs(int64_t M, int64_t K, int64_t F) {
   if (M == 0 || K == 0 || F == 0 || K >= 1 << 22 || F >= 1 << 22 || on_fp32()) return false;
   const double m = (double)cdiv(M, 32) * 32, k = (double)cdiv(K, 64) * 64, f = (double)cdiv(F, 32) * 32;
   const double few = 11.0 + 1.3e-6 * k * f + (F % 32 ? 150e-9 : 88e-9) * m * k * f;
-  const double pairs = 30.0 + 6.5e-6 * k * f + 0.59e-6 * m * (k + 3 * f) + 18.8e-9 * m * k * f;
+  // a piece of the longest reduction, one step behind the other: few tiles leave CUs idle
+  const double alone = 0.34 * std::max(steps_of((int)M), 2 * steps_of((int)F)) / kMaxPieces;
+  const double pairs = 30.0 + 6.5e-6 * k * f + 0.59e-6 * m * (k + 3 * f) + std::max(18.8e-9 * m * k * f, alone);
   return pairs < few;
 }
 
