@@ -431,9 +431,12 @@ int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const DLArrayHand
 
 /* g = input gate, u = input up, output = act(g) u, for input [M, K], gate and up [K, F], output [M, F]; pre [2, M, F]
  * receives g and u, which the backward pass reads.  One of pre and output may be NULL.
- * activation: sigmoid=0, relu=1, silu=2, gelu=3 (with erf).  Arrays of 2 GiB or more (a half of pre counts as one)
- * and more than 2^26 rows or columns are rejected.  Results must not overlap what they are computed from.  Scratch: none for up to four rows of up to 2 560
- * columns; a call that takes some is refused on a stream that is being captured into a graph, as is the backward call. */
+ * activation: sigmoid=0, relu=1, silu=2, gelu=3 (with erf), from the hardware's exponential and reciprocal: of x < 0
+ * sigmoid and SiLU are off by up to 2^-21 + |x| 2^-23 of themselves (0 from -87 on), GELU of any x by up to |x| 2^-21, of x < 0 by
+ * up to 4e-5 of itself where that is less (0 from -13 on).  TINYFLOW_SPLIT=0 in the environment keeps the products on the fp32
+ * instruction.  Arrays of 2 GiB or more (a half of pre counts as one) and more than 2^26 rows or columns are rejected.  Results must
+ * not overlap what they are computed from.  Scratch: none for up to four rows of up to 2 560 columns; a call that takes some is
+ * refused on a stream that is being captured into a graph, as is the backward call. */
 int DLGpuGatedFeedForward(const DLArrayHandle input, const DLArrayHandle gate, const DLArrayHandle up,
                           DLArrayHandle pre, DLArrayHandle output, int activation, int *memorytoSaving, void **stream);
 /* With dg = doutput u act'(g), du = doutput act(g): dinput = dg gate^T + du up^T, dgate = input^T dg, dup = input^T du,

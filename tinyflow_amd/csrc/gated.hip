@@ -34,12 +34,14 @@ enum Activation { kSigmoid = 0, kRelu = 1, kSilu = 2, kGelu = 3, kGiven = -1 };
 
 // Both from the hardware's exp2 and reciprocal, which are right to a step of the last place: what that leaves off is 2^-24 of
 // the exponent's size, relative, on a value that gets small as the exponent grows; next to 1 it does not show.  The activations and
-// their slopes are computed for every element of two passes, where expf and erff cost more than the loads.
+// their slopes are computed for every element of two passes, where expf and erff cost more than the loads.  Relative errors of sigmoid
+// and SiLU: 2.4e-7 at -1, 1e-6 at -20, 4e-6 at -86, below which the reciprocal is subnormal and becomes zero.
 __device__ inline float sigmoid(float g) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.44269504088896341f * g));
 }
 // Normal distribution function, and `bell` = exp(-g^2 / 2): the tail is t p(t) bell / 2 with t = 1 / (1 + |g| / sqrt 8) and p of six
-// degrees, fitted to it so that the function is off by 7e-8 at most (evaluated in fp32 by 1.8e-7).
+// degrees, fitted to it so that the function is off by 7e-8 at most (evaluated in fp32 by 1.8e-7); relative to itself by 2e-6 down to -2,
+// 5e-6 to -4, 3e-5 below.
 __device__ inline float normal(float g, float &bell) {
   bell = __builtin_amdgcn_exp2f(-0.721347520444481704f * g * g);
   const float t = __builtin_amdgcn_rcpf(1.f + 0.353553390593273762f * __builtin_fabsf(g));
@@ -89,7 +91,8 @@ void with_activation(int activation, F &&f) {
   }
 }
 
-// Bound by HBM: 12 and 20 bytes an element.
+// Bound by HBM: 12 and 20 bytes an element.  4 096 x 4 096 28.6 us (7.0 TB/s, a part out of the last-level cache) and 59.0 (5.7), 64 x 4 096
+// 3.6 and 3.8, a launch.
 template <int ACT>
 __global__ __launch_bounds__(kThreads) void activation_kernel(const float *g, const float *u, float *h, int64_t count) {
   const int64_t i = 4 * ((int64_t)blockIdx.x * kThreads + threadIdx.x);
@@ -1098,9 +1101,11 @@ __global__ __launch_bounds__(kThreads, BLOCKS == 1 ? 2 : 1) void forward_kernel(
 
 // Up to four rows: vector multiply-adds.  Sixteen waves share 32 columns, eight lanes a row of the weights with four columns each, so
 // that 4 096 columns already keep half of the CUs' loads going without a run of the reduction to be added across
-// workgroups, which costs as long as reading 20 MB.  A longer reduction is better cut.  This / cut, us, one row: 1 024 x 4 096 8.5 /
-// 12.6 (7.8 measured alone: 4.3 TB/s), 2 048 x 8 192 27.9 / 33.9, 2 560 x 512 12.7 / 13.1, 4 096 x 512 19.1 / 17.7, 8 192 x 2 048 66 / 34;
-// four rows: 1 000 x 2 731 12.9 / 13.6, 2 560 x 512 17.3 / 13.7.
+// workgroups, which costs as long as reading 20 MB.  A longer reduction is better cut, from where on depends on where the weights
+// come from.  This / cut, us, weights out of the last-level cache (the same ones again) and out of memory (700 MB of them in turn): one row of
+// 1 024 x 4 096 5.7 / 10.6 and 11.0 / 12.3, 2 560 x 512 8.1 / 14.6 and 21.5 / 15.2, 4 096 x 512 10.2 / 19.4 and 32.8 / 20.1, 4 096 x 4 096
+// 25.7 / 24.3 and 36.7 / 30.4; four rows of 1 000 x 2 731 9.2 / 11.1 and 13.7 / 12.2, 2 560 x 512 10.1 / 15.5 and 25.1 / 15.9.  The limit, one
+// for one to four rows, is that of the cache, and part of the interface: up to it a call takes no scratch and can be captured.
 constexpr int kFewest = 4, kNarrow = 32, kWide = 1024;
 template <int ACT, int ROWS>
 __global__ __launch_bounds__(kWide) void fewest_kernel(const Args a) {

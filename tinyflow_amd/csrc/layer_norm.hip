@@ -156,7 +156,9 @@ __global__ __launch_bounds__(T > 256 ? T : 256) void forward_kernel(const float 
   row.template store<PAST>(y + r * cols, cols, lane);
 }
 
-// Rows that do not fit registers: three passes, the later two mostly out of the caches.
+// Rows that do not fit registers: three passes, the later two mostly out of the caches, of four bytes a lane and load.  What bounds them is
+// a workgroup's latency, pass behind pass: 300 x 40 003 43 us (2.2 TB/s of what is needed), dx 63, all gradients 95; 1 000 x 17 000 42 and
+// 101, where 1 000 x 16 000 in registers takes 64 backward.  No model has rows of that length; the forms are there for the interface's range.
 constexpr int kLong = 1024;
 
 // f(column, sums) over a lane's columns of a row, in runs of kRun with sums of their own: of 2^26 columns no sum has more than 512 members.
