@@ -364,7 +364,8 @@ __global__ __launch_bounds__(1024) void sum_pieces_kernel(const float *__restric
                                                          float *__restrict__ dbeta, int pieces, int cols) {
   __shared__ float sums[kSlices][kSumCols];
   const int along = threadIdx.x % kSumCols, slice = threadIdx.x / kSumCols;
-  const int64_t c = (int64_t)blockIdx.x * kSumCols + along, width = 2 * padded(cols);  // c < width
+  const int64_t c = group_index() * kSumCols + along, width = 2 * padded(cols);
+  if (c >= width) return;  // the whole workgroup
   float s = 0.f;
   int p = slice;
   for (; p + 3 * kSlices < pieces; p += 4 * kSlices) {
@@ -514,7 +515,7 @@ extern "C" int DLGpuLayerNormalizationBackward(const DLArrayHandle input, const 
     }
   }
   if (params)
-    hipLaunchKernelGGL(sum_pieces_kernel, dim3((unsigned)(2 * padded(cols) / kSumCols)), dim3(1024), 0, s, partial,
+    hipLaunchKernelGGL(sum_pieces_kernel, grid_of(2 * padded(cols) / kSumCols), dim3(1024), 0, s, partial,
                        dgamma ? (float *)dgamma->data : nullptr, dbeta ? (float *)dbeta->data : nullptr, rows ? pieces : 0,
                        (int)cols);
   if (partial) device_free(partial, s);
