@@ -112,10 +112,9 @@ def test_a_captured_graph(rt):
             ref.assert_within(pre, pre_ref, pre_tol, "pre")
             ref.assert_within(h, h_ref, h_tol, "h")
         calls()
-        for (pre, h), (a, (m, k, f)) in zip(got, kept):
-            if m <= 2 or m > 4:   # three and four rows of a long reduction take scratch when they may
-                np.testing.assert_array_equal(pre, a[3].asnumpy())
-                np.testing.assert_array_equal(h, a[4].asnumpy())
+        for (pre, h), (a, _) in zip(got, kept):
+            np.testing.assert_array_equal(pre, a[3].asnumpy())
+            np.testing.assert_array_equal(h, a[4].asnumpy())
     for a in refused:
         assert (a[4].asnumpy() == np.float32(7.25)).all()
     gpu_op.destroy_cudaStream(stream)
