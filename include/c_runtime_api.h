@@ -451,6 +451,56 @@ int DLGpuGatedActivation(const DLArrayHandle pre, DLArrayHandle output, int acti
 int DLGpuGatedActivationBackward(const DLArrayHandle pre, const DLArrayHandle doutput, DLArrayHandle dpre,
                                  int activation, void **stream);
 
+/* ------------------------ norm, rotation and placement of heads, attention (no counterparts in the reference) */
+
+/* An array of heads: [.., heads * D] of any rank but four, or [.., .., heads, D].  A row is what the axes in front of them count. */
+typedef struct {
+  DLArrayHandle input;
+  DLArrayHandle gamma;   /* NULL: no norm */
+  DLArrayHandle output;
+  int heads, rotate, place;
+} DLHeadPart;
+/* One to four arrays of heads of D columns (1024 at most) and the same rows, in one launch:
+ *   y = x / sqrt(mean(x^2) + eps) * gamma over a head's columns, with gamma [D]; without it y = x;
+ *   with `rotate` the first 2 n of them, for n frequencies, are turned in pairs: (a, b) -> amplitude (a cos t - b sin t,
+ *   a sin t + b cos t), t = position * frequency, a product and a remainder in 64 bits.  Pairs are columns i and i + n, or 2 i and
+ *   2 i + 1 with `interleaved`.  `positions` hold a value for each row, or for the rows of a sequence that the rows repeat;
+ *   output has the input's shape and may be the input.  With `place` it is a cache [sequences, capacity rows, ..]: row t of sequence b,
+ *   with `slots` [sequences, rows of one], goes to its row slots[b, t]; a row whose slot is not a whole number below the capacity (2^24 at most) is
+ *   left out, and rows of the cache that no slot names stay as they were.  Of two rows of a call with the same slot columns of either may be kept.
+ * positions and frequencies may be NULL where no part rotates, slots where no part is placed.  Takes no scratch. */
+int DLGpuHeadRotary(const DLHeadPart *parts, int n_parts, const DLArrayHandle positions, const DLArrayHandle frequencies,
+                    float amplitude, int interleaved, float eps, const DLArrayHandle slots, void **stream);
+typedef struct {
+  DLArrayHandle input;     /* the forward pass's; not read without gamma */
+  DLArrayHandle gamma, doutput;
+  DLArrayHandle dinput, dgamma;  /* either may be NULL; dinput may be doutput */
+  int heads, rotate;
+} DLHeadGradientPart;
+/* Its gradients, from the forward pass's inputs: nothing is kept between the two.  A dgamma takes scratch, and is refused on a stream that is
+ * being captured into a graph. */
+int DLGpuHeadRotaryBackward(const DLHeadGradientPart *parts, int n_parts, const DLArrayHandle positions, const DLArrayHandle frequencies,
+                            float amplitude, int interleaved, float eps, int *memorytoSaving, void **stream);
+
+/* Attention of `heads` query heads over `key_heads` key and value heads, a divisor: query head h reads key head h / (heads / key_heads).
+ * query [batch * queries, heads * D] and key, value [batch * keys, key_heads * D] as head arrays, D up to 256, up to 2^24 queries and keys:
+ *   s_ij = cap tanh(scale q_i k_j / cap) - slopes[h] |i + keys - queries - j|, with cap 0 s = scale q k, without slopes no second term
+ *   output_i = sum_j exp(s_ij - statistics_i) v_j, statistics_i = log sum_j exp(s_ij), over the keys j that query i sees.
+ * These are spans[i] = (first, last): first <= j < last, spans [batch, queries, 2] or [queries, 2]; without spans all.  With `causal` of
+ * them those with j <= i + keys - queries.  A query that sees none has the output 0 and the statistic -inf.  What a query does not see counts for nothing, whatever
+ * it holds.  statistics [batch, heads, queries] are what the backward pass reads; one of output and statistics may be NULL.
+ * Results must not overlap what they are computed from.  A call that takes scratch is refused on a stream that is being captured
+ * into a graph: TINYFLOW_SPLIT=0 in the environment keeps the products on the fp32 instruction, where only few queries over many keys take some. */
+int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle value, const DLArrayHandle spans,
+                          const DLArrayHandle slopes, DLArrayHandle output, DLArrayHandle statistics, int batch, int heads,
+                          int key_heads, float scale, float cap, int causal, int *memorytoSaving, void **stream);
+/* Its gradients, those of dquery, dkey and dvalue that are not NULL, from the forward pass's inputs and both its results.  Refused on a stream
+ * that is being captured into a graph.  The slopes have no gradient. */
+int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle value, const DLArrayHandle spans,
+                           const DLArrayHandle slopes, const DLArrayHandle output, const DLArrayHandle statistics,
+                           const DLArrayHandle doutput, DLArrayHandle dquery, DLArrayHandle dkey, DLArrayHandle dvalue, int batch,
+                           int heads, int key_heads, float scale, float cap, int causal, int *memorytoSaving, void **stream);
+
 /* ----------------------------------------------------- dropout, concatenation */
 
 /* Element-count descriptor that dropout takes in place of the reference's cuDNN

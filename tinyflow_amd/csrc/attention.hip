@@ -1,0 +1,995 @@
+// Attention, forward and backward (no counterpart in the reference).  attention.h has the formulas and what rows are.
+//
+// Forms of the forward pass, and which one runs (choose_forward):
+//   few_kernel     up to 32 rows of a key head: every wave streams its own keys from memory to registers, nothing is staged; bound by HBM
+//   rows_kernel    128 rows a workgroup, the fp32 matrix instruction
+// Both can be cut along the keys: pieces write their unnormalised sums with their maximum, join_kernel adds them up in their order.
+// Backward: prepare_kernel (delta, what each row sees), dq_kernel (128 rows a workgroup, walks the keys), dkv_kernel (128 keys a workgroup, walks the
+// rows; cut along the rows where keys are few, sum_kernel adds the pieces).  Both compute the scores again; no sum goes
+// through atomics, so the bits do not depend on the order in which workgroups run.
+#include "attention.h"
+#include "internal.h"
+
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+using namespace tf;
+using namespace tf::attention;
+
+namespace {
+
+constexpr int kThreads = 256, kRows = 128, kKeys = 32;  // of a workgroup; rows in the forward pass, keys in dkv_kernel; steps of the other axis
+constexpr float kNone = -INFINITY;
+
+template <int V>
+using IC = std::integral_constant<int, V>;
+
+__device__ inline float other_half(float v) { return __shfl_xor(v, 32); }
+
+// ------------------------------------------------------------------------------ tiles of the fp32 instruction
+//
+// v_mfma_f32_32x32x2: a lane supplies A[lane % 32][half] and B[half][lane % 32], half = lane / 32, and holds D[8 (v / 4) + 4 half + v % 4][lane % 32].
+// A score tile is computed with what the lane keeps on the columns: rows in the forward pass and dq, keys in dkv.  Its 16 values are then, as they
+// are, the B operands of the products that follow: step v takes row 8 (v / 4) + 4 half + v % 4 of the tile on the other side.
+
+constexpr int key_of(int v, int half) { return 8 * (v / 4) + 4 * half + v % 4; }
+
+// 32 rows of DP columns in LDS, columns past `dim` and rows past `count` zero.  Four floats more than a row keep the reads apart.
+template <int DP>
+struct Tile {
+  static constexpr int LD = DP + 4;
+  float v[32][LD];
+
+  // rows of `at(r)`; CLEAN: what is not finite becomes 0, and its row's bit is set in `found`
+  template <class At>
+  __device__ inline void stage(const At &at, int count, int dim, bool clean, uint32_t *found) {
+    constexpr int A_ROW = DP / 4;
+#pragma unroll 4
+    for (int e = threadIdx.x; e < 32 * A_ROW; e += kThreads) {
+      const int r = e / A_ROW, c = e % A_ROW * 4;
+      f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      if (r < count && c < dim) x = load4(at(r) + c, dim - c);
+      if (clean) {
+        bool all = true;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool ok = finite(x[i]);
+          all &= ok;
+          if (!ok) x[i] = 0.f;
+        }
+        if (!all) atomicOr(found, 1u << r);
+      }
+      *reinterpret_cast<f32x4 *>(&v[r][c]) = x;
+    }
+  }
+};
+
+// The B operand of a product over columns: of the lane's row or key, columns 8 g + 4 half + e.
+template <int DP>
+struct Operand {
+  f32x4 v[DP / 8];
+  __device__ inline void load(const float *row, int dim, bool live) {
+    const int half = threadIdx.x % 64 / 32;
+#pragma unroll
+    for (int g = 0; g < DP / 8; ++g) {
+      const int c = 8 * g + 4 * half;
+      v[g] = live && c < dim ? load4(row + c, dim - c) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  __device__ inline float dot(const Operand &o) const {  // over all columns
+    f32x4 s = v[0] * o.v[0];
+#pragma unroll
+    for (int g = 1; g < DP / 8; ++g) s += v[g] * o.v[g];
+    const float t = (s[0] + s[1]) + (s[2] + s[3]);
+    return t + other_half(t);
+  }
+};
+
+template <int DP>
+__device__ inline f32x16 scores(const Tile<DP> &a, const Operand<DP> &b) {
+  const int half = threadIdx.x % 64 / 32, row = threadIdx.x % 32;
+  f32x16 s;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) s[v] = 0.f;
+#pragma unroll
+  for (int g = 0; g < DP / 8; ++g) {
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(&a.v[row][8 * g + 4 * half]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], b.v[g][e], s, 0, 0, 0);
+  }
+  return s;
+}
+
+// What staging took out of the tile, in the products again: those of rows `found`, from the operands as they were.
+template <int DP, class At>
+__device__ inline void repair(f32x16 &s, uint32_t found, const At &at, int dim, const Operand<DP> &b) {
+  const int half = threadIdx.x % 64 / 32;
+#pragma unroll 1
+  for (; found; found &= found - 1) {
+    const int r = __builtin_ctz(found), from = r / 4 % 2, e = r / 8 * 4 + r % 4;
+    Operand<DP> a;
+    a.load(at(r), dim, true);
+    const float x = a.dot(b);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = i == e && from == half ? x : s[i];
+  }
+}
+
+// sum[block][v] += of column 32 block + key_of(v, half), over the tile's rows with the lane's weights
+template <int DP>
+struct Sum {
+  f32x16 v[DP / 32];
+  __device__ inline void zero() {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[d][e] = 0.f;
+  }
+  __device__ inline void add(const Tile<DP> &a, const float (&w)[16]) {
+    const int half = threadIdx.x % 64 / 32, col = threadIdx.x % 32;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        v[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[key_of(e, half)][32 * d + col], w[e], v[d], 0, 0, 0);
+  }
+  // What staging took out of the tile, back with the weights that are not 0: rows `found`, read again at `at(row)`.
+  template <class At>
+  __device__ inline void add_back(uint32_t found, const At &at, int dim, const float (&w)[16]) {
+    const int half = threadIdx.x % 64 / 32;
+#pragma unroll 1
+    for (; found; found &= found - 1) {
+      const int r = __builtin_ctz(found), from = r / 4 % 2, e = r / 8 * 4 + r % 4;
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x = i == e ? w[i] : x;
+      const float weight = __shfl(x, threadIdx.x % 32 + 32 * from);
+      const float *row = at(r);
+#pragma unroll
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int c = 32 * d + key_of(i, half);
+          if (c < dim && !finite(row[c]) && weight != 0.f) v[d][i] += weight * row[c];
+        }
+    }
+  }
+  __device__ inline void scale(float by) {
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) v[d] *= by;
+  }
+  __device__ inline void store(float *row, int dim, float by) const {
+    const int half = threadIdx.x % 64 / 32;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int c = 32 * d + 8 * q + 4 * half;
+        if (c < dim) store4(row + c, dim - c, f32x4{v[d][4 * q] * by, v[d][4 * q + 1] * by, v[d][4 * q + 2] * by, v[d][4 * q + 3] * by});
+      }
+  }
+};
+
+// The least and the greatest of what a wave's 32 columns, or a workgroup's 128, see, empty ones aside; inner: what all of them see.
+struct Hull {
+  int lo, hi, inner_lo, inner_hi;
+  __device__ inline void of(int lo_, int hi_, bool live) {
+    const bool some = live && lo_ < hi_;
+    lo = some ? lo_ : INT32_MAX;
+    hi = some ? hi_ : 0;
+    inner_lo = some ? lo_ : INT32_MAX;
+    inner_hi = some ? hi_ : 0;
+#pragma unroll
+    for (int step = 1; step < 32; step *= 2) {
+      lo = min(lo, __shfl_xor(lo, step));
+      hi = max(hi, __shfl_xor(hi, step));
+      inner_lo = max(inner_lo, __shfl_xor(inner_lo, step));
+      inner_hi = min(inner_hi, __shfl_xor(inner_hi, step));
+    }
+  }
+  // over the four waves, through `room`
+  __device__ inline Hull all(int (*room)[4]) const {
+    const int wave = threadIdx.x / 64;
+    if (threadIdx.x % 64 == 0) room[wave][0] = lo, room[wave][1] = hi, room[wave][2] = inner_lo, room[wave][3] = inner_hi;
+    __syncthreads();
+    Hull h = *this;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      h.lo = min(h.lo, room[w][0]);
+      h.hi = max(h.hi, room[w][1]);
+      h.inner_lo = max(h.inner_lo, room[w][2]);
+      h.inner_hi = min(h.inner_hi, room[w][3]);
+    }
+    h.lo = __builtin_amdgcn_readfirstlane(h.lo);
+    h.hi = __builtin_amdgcn_readfirstlane(h.hi);
+    return h;
+  }
+  __device__ inline bool meets(int from, int to) const { return lo < to && hi > from; }
+  __device__ inline bool covers(int from, int to) const { return inner_lo <= from && inner_hi >= to; }
+};
+
+// Pieces of rows: [piece][row of all][dim] unnormalised sums and [piece][row of all] (maximum, sum); a row of all is (b, key head, row).
+struct Pieces {
+  float *sums;
+  float2 *marks;
+  int count;
+  int64_t rows;  // of all
+};
+
+// Writes a row's result or its piece.
+__device__ inline float row_end(const Call &c, const Pieces &to, float *out, float *stat, int b, int g, int r, int piece, float top, float total,
+                                bool writes_mark, float *&row) {
+  if (to.count > 1) {
+    const int64_t at = piece * to.rows + ((int64_t)b * c.key_heads + g) * c.rows + r;
+    if (writes_mark) to.marks[at] = make_float2(top, total);
+    row = to.sums + at * c.dim;
+    return 1.f;
+  }
+  if (stat && writes_mark) stat[c.stat_at(b, g, r)] = total == 0.f ? kNone : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  row = out ? out + c.query_at(b, g, r) : nullptr;
+  return total == 0.f ? 0.f : 1.f / total;
+}
+
+// ------------------------------------------------------------------------------ forward, 128 rows a workgroup
+
+template <int DP>
+__global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out, float *stat, const Pieces pieces, int tiles) {
+  __shared__ __align__(16) Tile<DP> kt, vt;
+  __shared__ int room[4][4];
+  __shared__ uint32_t found;
+  const int bg = (int)blockIdx.x % (c.batch * c.key_heads), rest = (int)blockIdx.x / (c.batch * c.key_heads);
+  const int b = bg / c.key_heads, g = bg % c.key_heads, tile = tiles - 1 - rest % tiles, piece = rest / tiles;
+  const int lane = threadIdx.x % 64, half = lane / 32;
+  const int r = tile * kRows + threadIdx.x / 64 * 32 + lane % 32;
+  const bool live = r < c.rows;
+  const int i = (live ? r : c.rows - 1) / c.group, ahead = i + c.tk - c.tq;
+  int lo, hi;
+  c.seen(b, i, lo, hi);
+  const float slope = c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
+  Operand<DP> q;
+  q.load(c.q + c.query_at(b, g, live ? r : 0), c.dim, live);
+  Hull mine;
+  mine.of(lo, hi, live);
+  const Hull all = mine.all(room);
+  // this piece's steps of the keys that any of the rows sees
+  const int first = all.lo < all.hi ? all.lo / kKeys : 0, steps = all.lo < all.hi ? (all.hi + kKeys - 1) / kKeys - first : 0;
+  const int begin = first + (int)((int64_t)steps * piece / pieces.count), end = first + (int)((int64_t)steps * (piece + 1) / pieces.count);
+  const Score score(c);
+  Sum<DP> o;
+  o.zero();
+  float top = kNone, total = 0.f;
+#pragma unroll 1
+  for (int step = begin; step < end; ++step) {
+    const int j0 = step * kKeys, count = min(kKeys, c.tk - j0);
+    const bool clean = !all.covers(j0, j0 + kKeys);
+    __syncthreads();
+    if (threadIdx.x == 0) found = 0u;
+    if (clean) __syncthreads();
+    kt.stage([&](int n) { return c.k + c.key_at(b, g, j0 + n); }, count, c.dim, false, nullptr);
+    vt.stage([&](int n) { return c.v + c.key_at(b, g, j0 + n); }, count, c.dim, clean, &found);
+    __syncthreads();
+    if (!mine.meets(j0, j0 + kKeys)) continue;
+    const f32x16 s = scores(kt, q);
+    float p[16], most = kNone;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int j = j0 + key_of(v, half);
+      p[v] = score(s[v]) - slope * fabsf((float)(ahead - j));
+      if (!mine.covers(j0, j0 + kKeys)) p[v] = j >= lo && j < hi ? p[v] : kNone;
+      most = fmaxf(most, p[v]);
+    }
+    most = fmaxf(most, other_half(most));
+    const float next = fmaxf(top, most), from = next == kNone ? 0.f : next;
+    const float fade = __builtin_amdgcn_exp2f(top - from);
+    top = next;
+    float sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      p[v] = __builtin_amdgcn_exp2f(p[v] - from);
+      sum += p[v];
+    }
+    total = total * fade + (sum + other_half(sum));
+    if (__any(fade != 1.f)) o.scale(fade);
+    o.add(vt, p);
+    if (clean && found) o.add_back(found, [&](int n) { return c.v + c.key_at(b, g, j0 + n); }, c.dim, p);
+  }
+  if (!live) return;
+  float *row;
+  const float by = row_end(c, pieces, out, stat, b, g, r, piece, top, total, half == 0, row);
+  if (row) o.store(row, c.dim, by);
+}
+
+// ------------------------------------------------------------------------------ forward, few rows
+
+// v_mfma_f32_16x16x4: a lane supplies A[lane % 16][lane / 16] and B[lane / 16][lane % 16] and holds D[4 (lane / 16) + v][lane % 16].  Scores: keys by
+// rows, columns 16 g + 4 (lane / 16) + e of both.  The values' product takes key 4 (lane / 16) + v at step v, as the scores lie,
+// and sums column 64 d + 4 (row of D) + e into sum[d][e]: both operands are 16-byte loads from where they lie in memory, 16 lanes side by side.
+constexpr int kFewKeys = 16;  // of a wave's step
+
+template <int DP, int NC>
+__global__ __launch_bounds__(kThreads) void few_kernel(const Call c, float *out, float *stat, const Pieces pieces, int keys_a_piece) {
+  constexpr int GD = DP / 16, VD = DP / 64;
+  const int bg = (int)blockIdx.x % (c.batch * c.key_heads), piece = (int)blockIdx.x / (c.batch * c.key_heads);
+  const int b = bg / c.key_heads, g = bg % c.key_heads;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, quarter = lane / 16, col = lane % 16;
+  int lo[NC], hi[NC], ahead[NC], all_lo = INT32_MAX, all_hi = 0, inner_lo = 0, inner_hi = INT32_MAX;
+  float slope[NC];
+  f32x4 q[NC][GD];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const int r = 16 * n + col;
+    const bool live = r < c.rows;
+    const int i = (live ? r : 0) / c.group;
+    c.seen(b, i, lo[n], hi[n]);
+    if (!live) hi[n] = 0;
+    ahead[n] = i + c.tk - c.tq;
+    slope[n] = c.slopes && live ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
+    const float *row = c.q + c.query_at(b, g, live ? r : 0);
+#pragma unroll
+    for (int e = 0; e < GD; ++e) {
+      const int d = 16 * e + 4 * quarter;
+      q[n][e] = live && d < c.dim ? load4(row + d, c.dim - d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (lo[n] < hi[n]) {
+      all_lo = min(all_lo, lo[n]);
+      all_hi = max(all_hi, hi[n]);
+    }
+    if (live) {  // columns that are no rows may hold anything
+      inner_lo = max(inner_lo, lo[n]);
+      inner_hi = min(inner_hi, hi[n]);
+    }
+  }
+#pragma unroll
+  for (int step = 1; step < 16; step *= 2) {
+    all_lo = min(all_lo, __shfl_xor(all_lo, step));
+    all_hi = max(all_hi, __shfl_xor(all_hi, step));
+    inner_lo = max(inner_lo, __shfl_xor(inner_lo, step));
+    inner_hi = min(inner_hi, __shfl_xor(inner_hi, step));
+  }
+  if (all_lo >= all_hi) all_lo = all_hi = 0;  // nothing is seen
+  const int begin = max(__builtin_amdgcn_readfirstlane(all_lo) / kFewKeys * kFewKeys, piece * keys_a_piece);
+  const int end = min(__builtin_amdgcn_readfirstlane(all_hi), (piece + 1) * keys_a_piece);  // a piece is a multiple of 64 keys
+  inner_lo = __builtin_amdgcn_readfirstlane(inner_lo);
+  inner_hi = __builtin_amdgcn_readfirstlane(inner_hi);
+
+  const Score score(c);
+  f32x4 o[NC][VD][4];
+  float top[NC], total[NC];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    top[n] = kNone;
+    total[n] = 0.f;
+#pragma unroll
+    for (int d = 0; d < VD; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][d][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int64_t key_step = (int64_t)c.key_heads * c.dim;
+  const float *k0 = c.k + c.key_at(b, g, 0), *v0 = c.v + c.key_at(b, g, 0);
+  f32x4 k[GD], vals[4][VD];
+  auto load_keys = [&](int j0) {  // keys behind the last are the last again
+    const float *row = k0 + (int64_t)min(j0 + col, end - 1) * key_step;
+#pragma unroll
+    for (int e = 0; e < GD; ++e) {
+      const int d = 16 * e + 4 * quarter;
+      k[e] = d < c.dim ? load4(row + d, c.dim - d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  auto load_values = [&](int j0) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const float *row = v0 + (int64_t)min(j0 + 4 * quarter + v, end - 1) * key_step;
+#pragma unroll
+      for (int d = 0; d < VD; ++d) {
+        const int at = 64 * d + 4 * col;
+        vals[v][d] = at < c.dim ? load4(row + at, c.dim - at) : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+  };
+  int j0 = begin + kFewKeys * wave;
+  if (j0 < end) load_keys(j0), load_values(j0);
+#pragma unroll 1
+  for (; j0 < end; j0 += 4 * kFewKeys) {
+    const bool whole = inner_lo <= j0 && inner_hi >= j0 + kFewKeys && end >= j0 + kFewKeys;
+    float p[NC][4];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < GD; ++e)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e][x], q[n][e][x], s, 0, 0, 0);
+      float most = kNone;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int j = j0 + 4 * quarter + v;
+        p[n][v] = score(s[v]) - slope[n] * fabsf((float)(ahead[n] - j));
+        if (!whole) p[n][v] = j >= lo[n] && j < hi[n] && j < end ? p[n][v] : kNone;
+        most = fmaxf(most, p[n][v]);
+      }
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, other_half(most));
+      const float next = fmaxf(top[n], most), from = next == kNone ? 0.f : next;
+      const float fade = __builtin_amdgcn_exp2f(top[n] - from);
+      top[n] = next;
+      float sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        p[n][v] = __builtin_amdgcn_exp2f(p[n][v] - from);
+        sum += p[n][v];
+      }
+      total[n] = total[n] * fade + sum;  // of this lane's keys
+      if (__any(fade != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < VD; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][d][e] *= fade;
+      }
+    }
+    const int next = j0 + 4 * kFewKeys;
+    if (next < end) load_keys(next);
+    if (!whole) {
+      // values that are not finite: only to the rows that see them
+      bool ok = true;
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int d = 0; d < VD; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ok &= finite(vals[v][d][e]);
+      if (__any(!ok)) {
+#pragma unroll 1
+        for (int t = 0; t < kFewKeys; ++t) {
+          const float *row = v0 + (int64_t)min(j0 + t, end - 1) * key_step;
+#pragma unroll
+          for (int n = 0; n < NC; ++n) {
+            float w = 0.f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) w = t % 4 == v ? p[n][v] : w;
+            w = __shfl(w, col + t / 4 * 16);
+#pragma unroll
+            for (int d = 0; d < VD; ++d)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                  const int at = 64 * d + 16 * quarter + 4 * v + e;
+                  if (at < c.dim && w != 0.f && !finite(row[at])) o[n][d][e][v] += w * row[at];
+                }
+          }
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+#pragma unroll
+          for (int d = 0; d < VD; ++d)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vals[v][d][e] = finite(vals[v][d][e]) ? vals[v][d][e] : 0.f;
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int d = 0; d < VD; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][d][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vals[v][d][e], p[n][v], o[n][d][e], 0, 0, 0);
+    if (next < end) load_values(next);
+  }
+
+  // the four waves' sums, through LDS in their order
+  __shared__ float marks[4][16][2];
+  __shared__ f32x4 parts[3][VD * 4][64];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    total[n] += __shfl_xor(total[n], 16);
+    total[n] += other_half(total[n]);
+    if (n) __syncthreads();
+    if (quarter == 0) {
+      marks[wave][col][0] = top[n];
+      marks[wave][col][1] = total[n];
+    }
+    __syncthreads();
+    float most = kNone, whole = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) most = fmaxf(most, marks[w][col][0]);
+    const float from = most == kNone ? 0.f : most;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) whole += marks[w][col][1] * __builtin_amdgcn_exp2f(marks[w][col][0] - from);
+    const float fade = __builtin_amdgcn_exp2f(top[n] - from);
+#pragma unroll
+    for (int d = 0; d < VD; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[n][d][e] *= fade;
+        if (wave > 0) parts[wave - 1][d * 4 + e][lane] = o[n][d][e];
+      }
+    __syncthreads();
+    const int r = 16 * n + col;
+    if (wave == 0 && r < c.rows) {
+      float *row;
+      const float by = row_end(c, pieces, out, stat, b, g, r, piece, most, whole, quarter == 0, row);
+#pragma unroll
+      for (int d = 0; d < VD; ++d) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int w = 0; w < 3; ++w) o[n][d][e] += parts[w][d * 4 + e][lane];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int at = 64 * d + 16 * quarter + 4 * v;
+          if (row && at < c.dim) store4(row + at, c.dim - at, f32x4{o[n][d][0][v] * by, o[n][d][1][v] * by, o[n][d][2][v] * by, o[n][d][3][v] * by});
+        }
+      }
+    }
+  }
+}
+
+// Rows of all from their pieces, in the pieces' order: a row to W waves, each with a run of the pieces.
+template <int W>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void join_kernel(const Call c, const Pieces pieces, float *out, float *stat) {
+  constexpr int ROWS = W > 4 ? 1 : 4 / W;
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, sub = wave % W;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + wave / W;
+  if (W <= 1 && row >= pieces.rows) return;
+  const int64_t at = row < pieces.rows ? row : pieces.rows - 1;
+  float top = kNone;
+  for (int p = lane; p < pieces.count; p += 64) top = fmaxf(top, pieces.marks[p * pieces.rows + at].x);
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) top = fmaxf(top, __shfl_xor(top, step));
+  const float from = top == kNone ? 0.f : top;
+  float total = 0.f;
+  for (int p = lane; p < pieces.count; p += 64) {
+    const float2 mark = pieces.marks[p * pieces.rows + at];
+    total += mark.y * __builtin_amdgcn_exp2f(mark.x - from);
+  }
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) total += __shfl_xor(total, step);
+  const int each = (pieces.count + W - 1) / W, begin = min(pieces.count, sub * each), end = min(pieces.count, begin + each);
+  constexpr int MOST = 4;  // columns of a lane
+  float sum[MOST] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = begin; p < end; ++p) {
+    const float2 mark = pieces.marks[p * pieces.rows + at];
+    if (mark.y == 0.f) continue;  // nothing seen: nothing stored that counts
+    const float by = __builtin_amdgcn_exp2f(mark.x - from);
+    const float *from_row = pieces.sums + (p * pieces.rows + at) * c.dim;
+#pragma unroll
+    for (int e = 0; e < MOST; ++e)
+      if (lane + 64 * e < c.dim) sum[e] += from_row[lane + 64 * e] * by;
+  }
+  if constexpr (W > 1) {
+    __shared__ float parts[ROWS][W][MOST][64];
+#pragma unroll
+    for (int e = 0; e < MOST; ++e) parts[wave / W][sub][e][lane] = sum[e];
+    __syncthreads();
+    if (sub > 0 || row >= pieces.rows) return;
+#pragma unroll
+    for (int e = 0; e < MOST; ++e)
+      for (int w = 1; w < W; ++w) sum[e] += parts[wave / W][w][e][lane];
+  }
+  const int r = (int)(row % c.rows), g = (int)(row / c.rows % c.key_heads), b = (int)(row / c.rows / c.key_heads);
+  if (stat && lane == 0) stat[c.stat_at(b, g, r)] = total == 0.f ? kNone : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  if (!out) return;
+  const float by = total == 0.f ? 0.f : 1.f / total;
+  float *to = out + c.query_at(b, g, r);
+#pragma unroll
+  for (int e = 0; e < MOST; ++e)
+    if (lane + 64 * e < c.dim) to[lane + 64 * e] = sum[e] * by;
+}
+
+// ------------------------------------------------------------------------------ backward
+
+// What the backward kernels read of a row: its statistic times log2 e, delta, and the keys that it sees.
+struct Row {
+  float stat, delta;
+  int lo, hi;
+};
+
+// A wave a row of all.
+__global__ __launch_bounds__(kThreads) void prepare_kernel(const Call c, const float *__restrict__ o, const float *__restrict__ stat,
+                                                           const float *__restrict__ dout, Row *__restrict__ rows, int64_t count) {
+  const int64_t at = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  if (at >= count) return;
+  const int r = (int)(at % c.rows), g = (int)(at / c.rows % c.key_heads), b = (int)(at / c.rows / c.key_heads), lane = threadIdx.x % 64;
+  const int64_t from = c.query_at(b, g, r);
+  float delta = 0.f;
+  for (int d = lane; d < c.dim; d += 64) delta += o[from + d] * dout[from + d];
+#pragma unroll
+  for (int step = 1; step < 64; step *= 2) delta += __shfl_xor(delta, step);
+  if (lane > 0) return;
+  Row row;
+  c.seen(b, r / c.group, row.lo, row.hi);
+  row.stat = stat[c.stat_at(b, g, r)] * kLog2e;
+  row.delta = delta;
+  if (row.lo >= row.hi || row.stat == kNone) row.lo = row.hi = 0;
+  rows[at] = row;
+}
+
+// p and ds / scale from the products of queries and keys, and of gradients and values.
+__device__ inline void gradient(const Score &score, float product, float dp, float bias, float stat, float delta, bool seen, float &p, float &ds) {
+  float t = product * score.factor, slope = 1.f;
+  if (score.capped) {
+    t = tanh_of(t);
+    slope = 1.f - t * t;
+    t *= score.top;
+  }
+  p = seen ? __builtin_amdgcn_exp2f(t - bias - stat) : 0.f;
+  ds = seen ? p * (dp - delta) * slope : 0.f;
+}
+
+template <int DP>
+__global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float *dout, const Row *rows, float *dq, int tiles) {
+  __shared__ __align__(16) Tile<DP> kt, vt;
+  __shared__ int room[4][4];
+  __shared__ uint32_t found;
+  const int bg = (int)blockIdx.x % (c.batch * c.key_heads), tile = tiles - 1 - (int)blockIdx.x / (c.batch * c.key_heads);
+  const int b = bg / c.key_heads, g = bg % c.key_heads;
+  const int lane = threadIdx.x % 64, half = lane / 32;
+  const int r = tile * kRows + threadIdx.x / 64 * 32 + lane % 32;
+  const bool live = r < c.rows;
+  const Row row = rows[(int64_t)bg * c.rows + (live ? r : 0)];
+  const int ahead = (live ? r : 0) / c.group + c.tk - c.tq;
+  const float slope = c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
+  const int64_t at = c.query_at(b, g, live ? r : 0);
+  Operand<DP> q, d;
+  q.load(c.q + at, c.dim, live);
+  d.load(dout + at, c.dim, live);
+  Hull mine;
+  mine.of(row.lo, row.hi, live);
+  const Hull all = mine.all(room);
+  const Score score(c);
+  Sum<DP> sum;
+  sum.zero();
+  const int begin = all.lo < all.hi ? all.lo / kKeys : 0, end = all.lo < all.hi ? (all.hi + kKeys - 1) / kKeys : 0;
+#pragma unroll 1
+  for (int step = begin; step < end; ++step) {
+    const int j0 = step * kKeys, count = min(kKeys, c.tk - j0);
+    const bool clean = !all.covers(j0, j0 + kKeys);
+    __syncthreads();
+    if (threadIdx.x == 0) found = 0u;
+    if (clean) __syncthreads();
+    kt.stage([&](int n) { return c.k + c.key_at(b, g, j0 + n); }, count, c.dim, clean, &found);
+    vt.stage([&](int n) { return c.v + c.key_at(b, g, j0 + n); }, count, c.dim, false, nullptr);
+    __syncthreads();
+    if (!mine.meets(j0, j0 + kKeys)) continue;
+    f32x16 s = scores(kt, q);
+    if (clean && found) repair(s, found, [&](int n) { return c.k + c.key_at(b, g, j0 + n); }, c.dim, q);
+    const f32x16 dp = scores(vt, d);
+    float ds[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int j = j0 + key_of(v, half);
+      float p;
+      gradient(score, s[v], dp[v], slope * fabsf((float)(ahead - j)), row.stat, row.delta, j >= row.lo && j < row.hi, p, ds[v]);
+    }
+    sum.add(kt, ds);
+    if (clean && found) sum.add_back(found, [&](int n) { return c.k + c.key_at(b, g, j0 + n); }, c.dim, ds);
+  }
+  if (live) sum.store(dq + at, c.dim, c.scale);
+}
+
+// 128 keys a workgroup, 32 a wave, which walks the rows of piece blockIdx.x / (tiles * heads).  Results go to dk and dv, or piece by piece to
+// [piece][2][b, key, key head][dim].
+template <int DP, bool DK, bool DV>
+__global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float *dout, const Row *rows, float *dk, float *dv, float *parts,
+                                                       int tiles, int pieces) {
+  __shared__ __align__(16) Tile<DP> qt, dt;
+  __shared__ Row info[32];
+  __shared__ float slopes[32];
+  __shared__ int meet[3];  // least and greatest key that a row of the step sees, whether any sees less than all of the tile
+  __shared__ uint32_t found_q, found_d;
+  const int bg = (int)blockIdx.x % (c.batch * c.key_heads), rest = (int)blockIdx.x / (c.batch * c.key_heads);
+  const int b = bg / c.key_heads, g = bg % c.key_heads, tile = rest % tiles, piece = rest / tiles;
+  const int lane = threadIdx.x % 64, half = lane / 32;
+  const int tile_lo = tile * kRows, tile_hi = min(c.tk, tile_lo + kRows);
+  const int j = tile_lo + threadIdx.x / 64 * 32 + lane % 32;
+  const bool live = j < c.tk;
+  const int64_t at = c.key_at(b, g, live ? j : 0);
+  Operand<DP> k, v;
+  k.load(c.k + at, c.dim, live);
+  if (DK) v.load(c.v + at, c.dim, live);
+  const Score score(c);
+  Sum<DP> dks, dvs;
+  if (DK) dks.zero();
+  if (DV) dvs.zero();
+  const int steps = (c.rows + 31) / 32;
+  const int begin = (int)((int64_t)steps * piece / pieces), end = (int)((int64_t)steps * (piece + 1) / pieces);
+  const Row *of = rows + (int64_t)bg * c.rows;
+#pragma unroll 1
+  for (int step = begin; step < end; ++step) {
+    const int r0 = step * 32, count = min(32, c.rows - r0);
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      const int r = r0 + threadIdx.x;
+      const bool is = threadIdx.x < (unsigned)count;
+      Row row = {0.f, 0.f, 0, 0};
+      if (is) row = of[r];
+      if (threadIdx.x < 32) {
+        info[threadIdx.x] = row;
+        slopes[threadIdx.x] = c.slopes && is ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
+      }
+      const bool sees = is && row.lo < tile_hi && row.hi > tile_lo;
+      const bool any = __any(sees), part = __any(threadIdx.x < 32 && !(is && row.lo <= tile_lo && row.hi >= tile_lo + kRows));
+      if (threadIdx.x == 0) {
+        meet[0] = any;
+        meet[1] = part;
+        found_q = found_d = 0u;
+      }
+    }
+    __syncthreads();
+    if (!meet[0]) continue;
+    const bool clean = meet[1] != 0;
+    auto q_at = [&](int n) { return c.q + c.query_at(b, g, r0 + n); };
+    auto d_at = [&](int n) { return dout + c.query_at(b, g, r0 + n); };
+    qt.stage(q_at, count, c.dim, clean && DK, &found_q);
+    dt.stage(d_at, count, c.dim, clean && DV, &found_d);
+    __syncthreads();
+    f32x16 s = scores(qt, k), dp = s;
+    if (DK) dp = scores(dt, v);
+    if (clean && DK && found_q) repair(s, found_q, q_at, c.dim, k);
+    if (clean && DK && DV && found_d) repair(dp, found_d, d_at, c.dim, v);
+    float p[16], ds[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int n = key_of(e, half);
+      const Row row = info[n];
+      const float bias = slopes[n] * fabsf((float)((r0 + n) / c.group + c.tk - c.tq - j));
+      gradient(score, s[e], dp[e], bias, row.stat, row.delta, live && j >= row.lo && j < row.hi, p[e], ds[e]);
+    }
+    if (DV) {
+      dvs.add(dt, p);
+      if (clean && found_d) dvs.add_back(found_d, d_at, c.dim, p);
+    }
+    if (DK) {
+      dks.add(qt, ds);
+      if (clean && found_q) dks.add_back(found_q, q_at, c.dim, ds);
+    }
+  }
+  if (!live) return;
+  const int64_t all = (int64_t)c.batch * c.tk * c.key_heads * c.dim;
+  if (DK) dks.store((pieces > 1 ? parts + (int64_t)piece * 2 * all : dk) + at, c.dim, c.scale);
+  if (DV) dvs.store((pieces > 1 ? parts + ((int64_t)piece * 2 + 1) * all : dv) + at, c.dim, 1.f);
+}
+
+// dk and dv from their pieces, in order; half blockIdx.y.
+__global__ __launch_bounds__(kThreads) void sum_kernel(const float *__restrict__ parts, float *__restrict__ dk, float *__restrict__ dv, int64_t all, int pieces) {
+  float *to = blockIdx.y ? dv : dk;
+  if (!to) return;
+  for (int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4; e < all; e += (int64_t)gridDim.x * kThreads * 4) {
+    const int n = (int)(all - e < 4 ? all - e : 4);
+    f32x4 s = load4(parts + blockIdx.y * all + e, n);
+    for (int p = 1; p < pieces; ++p) s += load4(parts + (2 * p + blockIdx.y) * all + e, n);
+    store4(to + e, n, s);
+  }
+}
+
+// ------------------------------------------------------------------------------ host
+
+constexpr int64_t kMaxTokens = 1 << 24;  // positions that a float of a span holds exactly
+constexpr int64_t kMaxGroups = 1 << 24;  // workgroups of a launch: 2^32 lanes
+
+// The head array `a` as [rows, heads, dim]; false where it is none.
+bool head_array(const DLArray *a, int heads, int64_t &rows, int64_t &dim) {
+  if (a->ndim < 1 || heads < 1) return false;
+  const int64_t last = a->shape[a->ndim - 1];
+  if (a->ndim == 4) {
+    if (a->shape[2] != heads) return false;
+    dim = last;
+    rows = a->shape[0] * a->shape[1];
+  } else {
+    if (last % heads != 0) return false;
+    dim = last / heads;
+    rows = 1;
+    for (int i = 0; i + 1 < a->ndim; ++i) rows *= a->shape[i];
+  }
+  return dim > 0;
+}
+
+int describe(const char *what, Call &c, const DLArray *query, const DLArray *key, const DLArray *value, const DLArray *spans,
+             const DLArray *slopes, int batch, int heads, int key_heads, float scale, float cap, int causal) {
+  auto refuse = [&](const char *why) {
+    fprintf(stderr, "[tinyflow_amd] %s: %s\n", what, why);
+    return -1;
+  };
+  if (!on_gpu(query) || !on_gpu(key) || !on_gpu(value)) return refuse("arrays must live on the GPU");
+  if (batch < 0 || heads < 1 || key_heads < 1 || heads % key_heads != 0) return refuse("heads must be a multiple of key_heads");
+  int64_t q_rows, k_rows, dim, key_dim;
+  if (!head_array(query, heads, q_rows, dim) || !head_array(key, key_heads, k_rows, key_dim) || dim != key_dim)
+    return refuse("queries and keys must have the same columns a head");
+  if (dim > 256) return refuse("heads of more than 256 columns are not supported");
+  if (!same_shape(key, value)) return refuse("keys and values must have one shape");
+  if (batch == 0 ? q_rows || k_rows : q_rows % batch || k_rows % batch) return refuse("rows must be a multiple of batch");
+  const int64_t tq = batch ? q_rows / batch : 0, tk = batch ? k_rows / batch : 0;
+  if (tq > kMaxTokens || tk > kMaxTokens) return refuse("more than 2^24 queries or keys of a sequence are not supported");
+  if (tq * (heads / key_heads) > INT32_MAX / 2) return refuse("too many queries of a key head");
+  if (!(scale > 0.f) || !finite(scale)) return refuse("scale must be positive");
+  if (!(cap >= 0.f) || !finite(cap)) return refuse("cap must be positive, or 0 for none");
+  if (spans) {
+    if (!on_gpu(spans) || spans->ndim < 2 || spans->shape[spans->ndim - 1] != 2) return refuse("spans must be [batch, queries, 2] or [queries, 2] and live on the GPU");
+    const int64_t n = numel(spans);
+    if (n != 2 * tq && n != 2 * tq * batch) return refuse("spans must hold a pair for each query");
+    c.spans = (const float *)spans->data;
+    c.span_stride = n == 2 * tq * batch ? 2 * tq : 0;
+  }
+  if (slopes) {
+    if (!on_gpu(slopes) || numel(slopes) != heads) return refuse("slopes must hold a value for each head and live on the GPU");
+    c.slopes = (const float *)slopes->data;
+  }
+  if (!same_device({query, key, value, spans, slopes})) return refuse("arrays must live on one device");
+  c.q = (const float *)query->data;
+  c.k = (const float *)key->data;
+  c.v = (const float *)value->data;
+  c.batch = batch;
+  c.tq = (int)tq;
+  c.tk = (int)tk;
+  c.heads = heads;
+  c.key_heads = key_heads;
+  c.group = heads / key_heads;
+  c.dim = (int)dim;
+  c.rows = (int)tq * c.group;
+  c.scale = scale;
+  c.cap = cap;
+  c.causal = causal != 0;
+  return 0;
+}
+
+template <class F>
+void with_columns(int dim, const F &f) {
+  if (dim <= 32) f(IC<32>{});
+  else if (dim <= 64) f(IC<64>{});
+  else if (dim <= 128) f(IC<128>{});
+  else f(IC<256>{});
+}
+
+// Pieces of rows_kernel along the keys: as many as it takes for two workgroups a CU, of 256 keys at least.
+int row_pieces(const Call &c, int64_t groups) {
+  if (groups == 0) return 1;
+  const int64_t wanted = (2 * num_cus() + groups - 1) / groups, most = std::max(1, c.tk / 256);
+  return (int)std::min<int64_t>(wanted, most);
+}
+
+}  // namespace
+
+extern "C" int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle value, const DLArrayHandle spans,
+                                     const DLArrayHandle slopes, DLArrayHandle output, DLArrayHandle statistics, int batch, int heads,
+                                     int key_heads, float scale, float cap, int causal, int *memorytoSaving, void **stream) {
+  Call c = {};
+  if (describe(__func__, c, query, key, value, spans, slopes, batch, heads, key_heads, scale, cap, causal) != 0) return -1;
+  TF_REQUIRE(output || statistics, "no result is asked for");
+  TF_REQUIRE(!output || (on_gpu(output) && same_shape(output, query)), "output must live on the GPU and have the query's shape");
+  TF_REQUIRE(!statistics || (on_gpu(statistics) && numel(statistics) == (int64_t)batch * heads * c.tq),
+             "statistics must hold [batch, heads, queries] values and live on the GPU");
+  TF_REQUIRE(same_device({query, output, statistics}), "arrays must live on one device");
+  for (const DLArray *read : {(const DLArray *)query, (const DLArray *)key, (const DLArray *)value, (const DLArray *)spans, (const DLArray *)slopes})
+    TF_REQUIRE(!overlaps(read, output) && !overlaps(read, statistics), "results must not overlap what they are computed from");
+  TF_REQUIRE(!overlaps(output, statistics), "results must not overlap");
+  const int64_t all_rows = (int64_t)batch * c.key_heads * c.rows;
+  hipStream_t s = stream_of(stream);
+  if (all_rows == 0) return 0;
+  float *out = output ? (float *)output->data : nullptr, *stat = statistics ? (float *)statistics->data : nullptr;
+  const int64_t head_pairs = (int64_t)batch * c.key_heads;
+  const bool few = c.rows <= 32 && !(c.rows > 16 && c.dim > 128);
+  int64_t groups;
+  int tiles = 0, keys_a_piece = 0;
+  Pieces pieces = {};
+  pieces.rows = all_rows;
+  if (few) {
+    // about four workgroups a CU; a wave's share of a piece is a multiple of its step
+    const int64_t wanted = std::max<int64_t>(1, (4 * num_cus() + head_pairs - 1) / head_pairs);
+    keys_a_piece = std::max<int>(64, (int)(((c.tk + wanted - 1) / wanted + 63) / 64 * 64));
+    pieces.count = std::max(1, (c.tk + keys_a_piece - 1) / keys_a_piece);
+    groups = head_pairs * pieces.count;
+  } else {
+    tiles = (c.rows + kRows - 1) / kRows;
+    pieces.count = row_pieces(c, head_pairs * tiles);
+    groups = head_pairs * tiles * pieces.count;
+  }
+  TF_REQUIRE(groups < kMaxGroups, "too many sequences, heads and queries for a launch");
+  const bool scratch = pieces.count > 1;
+  TF_REQUIRE(!scratch || !being_captured(s), "this many keys for few queries take scratch, which a captured stream cannot give back");
+  announce_write(output);
+  announce_write(statistics);
+  void *block = nullptr;
+  if (scratch) {
+    const size_t sums = (size_t)pieces.count * all_rows * c.dim * sizeof(float), marks = (size_t)pieces.count * all_rows * sizeof(float2);
+    block = device_alloc(sums + marks, s);
+    if (!block) {
+      if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(sums + marks));
+      return 0;
+    }
+    pieces.marks = (float2 *)block;
+    pieces.sums = (float *)((char *)block + marks);
+  }
+  if (few) {
+    auto go = [&](auto dp, auto nc) {
+      hipLaunchKernelGGL((few_kernel<decltype(dp)::value, decltype(nc)::value>), dim3((unsigned)groups), dim3(kThreads), 0, s, c, out, stat, pieces, keys_a_piece);
+    };
+    if (c.rows <= 16) {
+      if (c.dim <= 64) go(IC<64>{}, IC<1>{});
+      else if (c.dim <= 128) go(IC<128>{}, IC<1>{});
+      else go(IC<256>{}, IC<1>{});
+    } else {
+      if (c.dim <= 64) go(IC<64>{}, IC<2>{});
+      else go(IC<128>{}, IC<2>{});
+    }
+  } else {
+    with_columns(c.dim, [&](auto dp) {
+      hipLaunchKernelGGL((rows_kernel<decltype(dp)::value>), dim3((unsigned)groups), dim3(kThreads), 0, s, c, out, stat, pieces, tiles);
+    });
+  }
+  if (scratch) {
+    if (pieces.count > 16) hipLaunchKernelGGL((join_kernel<16>), dim3((unsigned)all_rows), dim3(1024), 0, s, c, pieces, out, stat);
+    else hipLaunchKernelGGL((join_kernel<1>), dim3((unsigned)((all_rows + 3) / 4)), dim3(256), 0, s, c, pieces, out, stat);
+    device_free(block, s);
+  }
+  return finish(s, "DLGpuAttentionForward");
+}
+
+extern "C" int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle value, const DLArrayHandle spans,
+                                      const DLArrayHandle slopes, const DLArrayHandle output, const DLArrayHandle statistics,
+                                      const DLArrayHandle doutput, DLArrayHandle dquery, DLArrayHandle dkey, DLArrayHandle dvalue, int batch,
+                                      int heads, int key_heads, float scale, float cap, int causal, int *memorytoSaving, void **stream) {
+  Call c = {};
+  if (describe(__func__, c, query, key, value, spans, slopes, batch, heads, key_heads, scale, cap, causal) != 0) return -1;
+  TF_REQUIRE(on_gpu(output) && on_gpu(doutput) && same_shape(output, query) && same_shape(doutput, query),
+             "output and doutput must live on the GPU and have the query's shape");
+  TF_REQUIRE(on_gpu(statistics) && numel(statistics) == (int64_t)batch * heads * c.tq, "statistics must hold [batch, heads, queries] values and live on the GPU");
+  TF_REQUIRE(dquery || dkey || dvalue, "no gradient is asked for");
+  TF_REQUIRE(!dquery || (on_gpu(dquery) && same_shape(dquery, query)), "dquery must live on the GPU and have the query's shape");
+  TF_REQUIRE(!dkey || (on_gpu(dkey) && same_shape(dkey, key)), "dkey must live on the GPU and have the key's shape");
+  TF_REQUIRE(!dvalue || (on_gpu(dvalue) && same_shape(dvalue, value)), "dvalue must live on the GPU and have the value's shape");
+  TF_REQUIRE(same_device({query, output, statistics, doutput, dquery, dkey, dvalue}), "arrays must live on one device");
+  for (const DLArray *read : {(const DLArray *)query, (const DLArray *)key, (const DLArray *)value, (const DLArray *)spans, (const DLArray *)slopes,
+                              (const DLArray *)output, (const DLArray *)statistics, (const DLArray *)doutput})
+    for (const DLArray *written : {(const DLArray *)dquery, (const DLArray *)dkey, (const DLArray *)dvalue})
+      TF_REQUIRE(!overlaps(read, written), "gradients must not overlap what they are computed from");
+  TF_REQUIRE(!overlaps(dquery, dkey) && !overlaps(dquery, dvalue) && !overlaps(dkey, dvalue), "gradients must not overlap");
+  hipStream_t s = stream_of(stream);
+  const int64_t head_pairs = (int64_t)batch * c.key_heads, all_rows = head_pairs * c.rows, all_keys = head_pairs * c.tk;
+  if (all_rows == 0 && all_keys == 0) return 0;
+  const int row_tiles = (c.rows + kRows - 1) / kRows, key_tiles = (c.tk + kRows - 1) / kRows;
+  const int64_t key_groups = head_pairs * key_tiles;
+  int pieces = 1;
+  if ((dkey || dvalue) && key_groups) pieces = (int)std::min<int64_t>((2 * num_cus() + key_groups - 1) / key_groups, std::max(1, c.rows / 256));
+  TF_REQUIRE(head_pairs * row_tiles < kMaxGroups && key_groups * pieces < kMaxGroups && (all_rows + 3) / 4 < kMaxGroups,
+             "too many sequences, heads and queries for a launch");
+  TF_REQUIRE(!being_captured(s), "the backward pass takes scratch, which a captured stream cannot give back");
+  for (const DLArray *written : {(const DLArray *)dquery, (const DLArray *)dkey, (const DLArray *)dvalue}) announce_write(written);
+  const int64_t all = all_keys * c.dim;
+  const size_t row_bytes = (size_t)all_rows * sizeof(Row), part_bytes = pieces > 1 ? (size_t)pieces * 2 * all * sizeof(float) : 0;
+  char *block = (char *)device_alloc(row_bytes + part_bytes, s);
+  if (!block) {
+    if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(row_bytes + part_bytes));
+    return 0;
+  }
+  Row *rows = (Row *)block;
+  float *parts = (float *)(block + row_bytes);
+  const float *dout = (const float *)doutput->data;
+  float *dk = dkey ? (float *)dkey->data : nullptr, *dv = dvalue ? (float *)dvalue->data : nullptr;
+  if (all_rows)
+    hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)((all_rows + 3) / 4)), dim3(kThreads), 0, s, c, (const float *)output->data,
+                       (const float *)statistics->data, dout, rows, all_rows);
+  with_columns(c.dim, [&](auto columns) {
+    constexpr int DP = decltype(columns)::value;
+    if (dquery && all_rows)
+      hipLaunchKernelGGL((dq_kernel<DP>), dim3((unsigned)(head_pairs * row_tiles)), dim3(kThreads), 0, s, c, dout, rows, (float *)dquery->data, row_tiles);
+    if (!key_groups) return;
+    const dim3 grid((unsigned)(key_groups * pieces));
+    if constexpr (DP <= 128) {
+      if (dk && dv) {
+        hipLaunchKernelGGL((dkv_kernel<DP, true, true>), grid, dim3(kThreads), 0, s, c, dout, rows, dk, dv, parts, key_tiles, pieces);
+        return;
+      }
+    }
+    // heads of more than 128 columns: the operands and sums of one gradient fill the registers
+    if (dk) hipLaunchKernelGGL((dkv_kernel<DP, true, false>), grid, dim3(kThreads), 0, s, c, dout, rows, dk, nullptr, parts, key_tiles, pieces);
+    if (dv) hipLaunchKernelGGL((dkv_kernel<DP, false, true>), grid, dim3(kThreads), 0, s, c, dout, rows, nullptr, dv, parts, key_tiles, pieces);
+  });
+  if (pieces > 1)
+    hipLaunchKernelGGL(sum_kernel, dim3((unsigned)std::min<int64_t>((all / 4 + kThreads) / kThreads, 4 * num_cus()), 2), dim3(kThreads), 0, s, parts, dk, dv, all,
+                       pieces);
+  device_free(block, s);
+  return finish(s, "DLGpuAttentionBackward");
+}

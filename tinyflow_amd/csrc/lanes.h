@@ -44,6 +44,26 @@ __device__ inline float sum(float v) {
                               return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
                             }));
 }
+// The sum over each run of T lanes, 8, 16, 32 or 64, in all of them.
+template <int T>
+__device__ inline float sum_over(float v) {
+  static_assert(T == 8 || T == 16 || T == 32 || T == 64, "a power of two of lanes");
+  auto add = [](float a, uint32_t b) { return a + __builtin_bit_cast(float, b); };
+  auto bits = [](float a) { return __builtin_bit_cast(uint32_t, a); };
+  v = add(v, moved<0xB1>(bits(v)));
+  v = add(v, moved<0x4E>(bits(v)));
+  v = add(v, moved<0x141>(bits(v)));
+  if (T > 8) v = add(v, moved<0x140>(bits(v)));
+  if (T > 16) {
+    auto halves = __builtin_amdgcn_permlane16_swap(bits(v), bits(v), false, false);
+    v = add(__builtin_bit_cast(float, halves[0]), halves[1]);
+  }
+  if (T > 32) {
+    auto halves = __builtin_amdgcn_permlane32_swap(bits(v), bits(v), false, false);
+    v = add(__builtin_bit_cast(float, halves[0]), halves[1]);
+  }
+  return v;
+}
 template <int WIDTH>
 __device__ inline uint32_t largest(uint32_t v) {
   return reduce<WIDTH, 1>(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });

@@ -502,6 +502,134 @@ def gated_activation_backward(pre, doutput, dpre, activation, cudaStream):
                                                  cudaStream))
 
 
+# ------------- norm, rotation and placement of heads, attention (no counterparts in the reference)
+
+class HeadPart(ctypes.Structure):
+    """One array of heads of a ``head_rotary`` call; made by ``head_part``."""
+    _fields_ = [("input", _nd.DLArrayHandle), ("gamma", _nd.DLArrayHandle), ("output", _nd.DLArrayHandle),
+                ("heads", ctypes.c_int), ("rotate", ctypes.c_int), ("place", ctypes.c_int)]
+
+
+class HeadGradientPart(ctypes.Structure):
+    """One array of heads of a ``head_rotary_backward`` call; made by ``head_gradient_part``."""
+    _fields_ = [("input", _nd.DLArrayHandle), ("gamma", _nd.DLArrayHandle), ("doutput", _nd.DLArrayHandle),
+                ("dinput", _nd.DLArrayHandle), ("dgamma", _nd.DLArrayHandle), ("heads", ctypes.c_int),
+                ("rotate", ctypes.c_int)]
+
+
+def _part(cls, arrays, **numbers):
+    _nd_args(*[a for a in arrays.values() if a is not None])
+    part = cls(**{name: int(value) for name, value in numbers.items()})
+    for name, a in arrays.items():
+        if a is not None:
+            setattr(part, name, a.handle)
+    part.arrays = arrays   # a handle alone does not keep its storage
+    return part
+
+
+def head_part(input, gamma, output, heads, rotate=True, place=False):
+    """An array of heads as ``head_rotary`` takes it: normed where there is a ``gamma``, rotated with ``rotate``; with
+    ``place`` the output is a cache whose rows ``slots`` names."""
+    return _part(HeadPart, {"input": input, "gamma": gamma, "output": output}, heads=heads, rotate=bool(rotate), place=bool(place))
+
+
+def head_gradient_part(input, gamma, doutput, dinput, dgamma, heads, rotate=True):
+    """An array of heads as ``head_rotary_backward`` takes it.  ``input`` may be None without ``gamma``; one of the two
+    gradients may be None."""
+    return _part(HeadGradientPart, {"input": input, "gamma": gamma, "doutput": doutput, "dinput": dinput, "dgamma": dgamma},
+                 heads=heads, rotate=bool(rotate))
+
+
+def head_rotary(parts, positions, frequencies, amplitude, interleaved, eps, slots, cudaStream):
+    """Norm, rotation and placement of up to four arrays of heads (``head_part``) in one launch."""
+    _nd_args(*[a for a in (positions, frequencies, slots) if a is not None])
+    check_call(_LIB.DLGpuHeadRotary((HeadPart * len(parts))(*parts), len(parts), _handle(positions), _handle(frequencies),
+                                    ctypes.c_float(amplitude), int(bool(interleaved)), ctypes.c_float(eps), _handle(slots),
+                                    cudaStream))
+
+
+def head_rotary_backward(parts, positions, frequencies, amplitude, interleaved, eps, cudaStream):
+    """The gradients of ``head_rotary`` (``head_gradient_part``), from the forward pass's inputs."""
+    _nd_args(*[a for a in (positions, frequencies) if a is not None])
+    wanted = ctypes.c_int(0)
+    check_call(_LIB.DLGpuHeadRotaryBackward((HeadGradientPart * len(parts))(*parts), len(parts), _handle(positions),
+                                            _handle(frequencies), ctypes.c_float(amplitude), int(bool(interleaved)),
+                                            ctypes.c_float(eps), ctypes.byref(wanted), cudaStream))
+    return wanted.value
+
+
+def rotary_frequencies(columns, base=10000.0, factor=1.0, context=None, slow=1.0, fast=32.0):
+    """Frequencies of ``columns`` rotated columns, base ** (-2 i / columns), for ``head_rotary`` (a numpy array).  ``factor``
+    stretches a context: all of them are divided by it; with the ``context`` that they were made for only those that turn at most ``slow`` times
+    over it, none that turns ``fast`` times or more, and those between by parts."""
+    if columns < 2 or columns % 2:
+        raise ValueError("rotary_frequencies: %r columns" % (columns,))
+    f = base ** (-2.0 * np.arange(columns // 2) / columns)
+    kept = 0.0
+    if context is not None:
+        kept = np.clip((context * f / (2 * np.pi) - slow) / (fast - slow), 0.0, 1.0)
+    return (f * (kept + (1.0 - kept) / factor)).astype(np.float32)
+
+
+def attention_spans(queries, keys=None, causal=False, documents=None, prefix=None, window=None, used=None):
+    """The first key that each query sees and the one behind the last, [queries, 2] or [batch, queries, 2], for
+    ``attention_forward`` (a numpy array).  Query i stands at key i + keys - queries, or with ``used`` [batch], the keys of a
+    cache that are filled, at i + used - queries.  ``causal``: none behind the query.  ``documents`` [batch, keys]: numbers that are
+    the same all over a document and nowhere else next to it; only keys of the query's own.  ``prefix`` [batch]: that many first
+    keys (of its document) are seen by every query, whatever ``causal`` says.  ``window``: so many keys up to the query's own."""
+    keys = queries if keys is None else keys
+    end = np.asarray(keys if used is None else used, np.int64).reshape(-1, 1)
+    at = np.arange(queries)[None, :] + end - queries
+    first, last = np.zeros_like(at), np.broadcast_to(end, at.shape)
+    if documents is not None:
+        documents = np.atleast_2d(documents)
+        if documents.shape[1] != keys:
+            raise ValueError("attention_spans: documents %s for %d keys" % (documents.shape, keys))
+        starts = np.ones(documents.shape, bool)
+        starts[:, 1:] = documents[:, 1:] != documents[:, :-1]
+        begin = np.maximum.accumulate(np.where(starts, np.arange(keys), 0), 1)
+        ends = np.ones(documents.shape, bool)
+        ends[:, :-1] = starts[:, 1:]
+        stop = np.minimum.accumulate(np.where(ends, np.arange(keys) + 1, keys)[:, ::-1], 1)[:, ::-1]
+        at = np.broadcast_to(at, (max(len(at), len(documents)), queries))
+        own = np.clip(at, 0, max(keys - 1, 0))
+        first = np.take_along_axis(np.broadcast_to(begin, (len(at), keys)), own, 1)
+        last = np.minimum(last, np.take_along_axis(np.broadcast_to(stop, (len(at), keys)), own, 1))
+    if causal or window is not None:
+        seen = at + 1
+        if prefix is not None:
+            seen = np.maximum(seen, first + np.asarray(prefix, np.int64).reshape(-1, 1))
+        last = np.minimum(last, seen)
+    if window is not None:
+        first = np.maximum(first, at + 1 - window)
+    first, last = np.broadcast_arrays(first, last)
+    spans = np.stack([first, np.maximum(first, last)], 2).astype(np.float32)
+    return spans[0] if len(spans) == 1 else spans
+
+
+def attention_forward(query, key, value, spans, slopes, output, statistics, batch, heads, key_heads, scale, cap, causal, cudaStream):
+    """output = softmax(scores) value; ``statistics`` are what ``attention_backward`` reads.  One of the two may be None, and
+    ``spans`` and ``slopes``."""
+    _nd_args(query, key, value, *[a for a in (spans, slopes, output, statistics) if a is not None])
+    wanted = ctypes.c_int(0)
+    check_call(_LIB.DLGpuAttentionForward(query.handle, key.handle, value.handle, _handle(spans), _handle(slopes), _handle(output),
+                                          _handle(statistics), int(batch), int(heads), int(key_heads), ctypes.c_float(scale),
+                                          ctypes.c_float(cap), int(bool(causal)), ctypes.byref(wanted), cudaStream))
+    return wanted.value
+
+
+def attention_backward(query, key, value, spans, slopes, output, statistics, doutput, dquery, dkey, dvalue, batch, heads, key_heads,
+                       scale, cap, causal, cudaStream):
+    """Those of the three gradients that are not None."""
+    _nd_args(query, key, value, output, statistics, doutput, *[a for a in (spans, slopes, dquery, dkey, dvalue) if a is not None])
+    wanted = ctypes.c_int(0)
+    check_call(_LIB.DLGpuAttentionBackward(query.handle, key.handle, value.handle, _handle(spans), _handle(slopes), output.handle,
+                                           statistics.handle, doutput.handle, _handle(dquery), _handle(dkey), _handle(dvalue),
+                                           int(batch), int(heads), int(key_heads), ctypes.c_float(scale), ctypes.c_float(cap),
+                                           int(bool(causal)), ctypes.byref(wanted), cudaStream))
+    return wanted.value
+
+
 # ------------------------------------------------------------------- optimizers
 
 def sgd_update(output, g, learning_rate, cudaStream):
