@@ -100,5 +100,157 @@ __device__ inline void store4(float *p, int count, f32x4 v) {
   }
 }
 
+// ------------------------------------------------------------------------------ what a wave and a workgroup see
+
+constexpr int kThreads = 256, kRows = 128, kKeys = 32;  // of a workgroup; rows in the forward pass, keys in dkv; steps of the other axis
+constexpr float kNone = -__builtin_inff();
+
+__device__ inline float other_half(float v) {  // lane ^ 32
+  const uint32_t bits = __builtin_bit_cast(uint32_t, v);
+  const auto halves = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+  return __builtin_bit_cast(float, threadIdx.x % 64 < 32 ? halves[1] : halves[0]);
+}
+
+// Row of a 32 x 32 tile that a lane's v-th of 16 values stands for (the layout of the matrix instructions' sums), half = lane / 32.
+constexpr int key_of(int v, int half) { return 8 * (v / 4) + 4 * half + v % 4; }
+
+// The least and the greatest of what a wave's 32 columns, or a workgroup's 128, see, empty ones aside; inner: what all of them see.
+struct Hull {
+  int lo, hi, inner_lo, inner_hi;
+  __device__ inline void of(int lo_, int hi_, bool live) {
+    const bool some = live && lo_ < hi_;
+    lo = some ? lo_ : INT32_MAX;
+    hi = some ? hi_ : 0;
+    inner_lo = some ? lo_ : INT32_MAX;
+    inner_hi = some ? hi_ : 0;
+#pragma unroll
+    for (int step = 1; step < 32; step *= 2) {
+      lo = min(lo, __shfl_xor(lo, step));
+      hi = max(hi, __shfl_xor(hi, step));
+      inner_lo = max(inner_lo, __shfl_xor(inner_lo, step));
+      inner_hi = min(inner_hi, __shfl_xor(inner_hi, step));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    inner_lo = __builtin_amdgcn_readfirstlane(inner_lo);
+    inner_hi = __builtin_amdgcn_readfirstlane(inner_hi);
+  }
+  // over the four waves, through `room`
+  __device__ inline Hull all(int (*room)[4]) const {
+    const int wave = threadIdx.x / 64;
+    if (threadIdx.x % 64 == 0) room[wave][0] = lo, room[wave][1] = hi, room[wave][2] = inner_lo, room[wave][3] = inner_hi;
+    __syncthreads();
+    Hull h = *this;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      h.lo = min(h.lo, room[w][0]);
+      h.hi = max(h.hi, room[w][1]);
+      h.inner_lo = max(h.inner_lo, room[w][2]);
+      h.inner_hi = min(h.inner_hi, room[w][3]);
+    }
+    h.lo = __builtin_amdgcn_readfirstlane(h.lo);
+    h.hi = __builtin_amdgcn_readfirstlane(h.hi);
+    return h;
+  }
+  __device__ inline bool meets(int from, int to) const { return lo < to && hi > from; }
+  __device__ inline bool covers(int from, int to) const { return inner_lo <= from && inner_hi >= to; }
+  // the steps of kKeys keys that it meets: [first, first + steps)
+  __device__ inline int first() const { return lo < hi ? lo / kKeys : 0; }
+  __device__ inline int steps() const { return lo < hi ? (hi + kKeys - 1) / kKeys - first() : 0; }
+};
+
+// Pieces of rows: [piece][row of all][dim] unnormalised sums and [piece][row of all] (maximum, sum); a row of all is (b, key head, row).
+struct Pieces {
+  float *sums;
+  float2 *marks;
+  int count;
+  int64_t rows;  // of all
+};
+
+// Where a row's result or its piece is written, and what it is to be multiplied by.
+__device__ inline float row_end(const Call &c, const Pieces &to, float *out, float *stat, int b, int g, int r, int piece, float top, float total,
+                                bool writes_mark, float *&row) {
+  if (to.count > 1) {
+    const int64_t at = piece * to.rows + ((int64_t)b * c.key_heads + g) * c.rows + r;
+    if (writes_mark) to.marks[at] = make_float2(top, total);
+    row = to.sums + at * c.dim;
+    return 1.f;
+  }
+  if (stat && writes_mark) stat[c.stat_at(b, g, r)] = total == 0.f ? kNone : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  row = out ? out + c.query_at(b, g, r) : nullptr;
+  return total == 0.f ? 0.f : 1.f / total;
+}
+
+// What the backward kernels read of a row: its statistic times log2 e, delta, and the keys that it sees.
+struct Row {
+  float stat, delta;
+  int lo, hi;
+};
+
+// p and ds / scale from the products of queries and keys, and of gradients and values.
+__device__ inline void gradient(const Score &score, float product, float dp, float bias, float stat, float delta, bool seen, float &p, float &ds) {
+  float t = product * score.factor, slope = 1.f;
+  if (score.capped) {
+    t = tanh_of(t);
+    slope = 1.f - t * t;
+    t *= score.top;
+  }
+  p = seen ? __builtin_amdgcn_exp2f(t - bias - stat) : 0.f;
+  ds = seen ? p * (dp - delta) * slope : 0.f;
+}
+
+// The sums of a tile's columns, `blocks` of 32: column 32 d + key_of(v, half) of the lane's row, times `by`.
+template <int BLOCKS>
+__device__ inline void store_sums(const f32x16 (&v)[BLOCKS], float *row, int dim, float by) {
+  const int half = threadIdx.x % 64 / 32;
+#pragma unroll
+  for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = 32 * d + 8 * q + 4 * half;
+      if (c < dim) store4(row + c, dim - c, f32x4{v[d][4 * q] * by, v[d][4 * q + 1] * by, v[d][4 * q + 2] * by, v[d][4 * q + 3] * by});
+    }
+}
+
+// ------------------------------------------------------------------------------ operands split into pairs (attention_pair.hip)
+
+constexpr int kBad = INT32_MIN / 4;  // exponent of a block that cannot be split
+
+// Of blocks of 32 rows, [b, key head][block]: exponents of queries, their gradients, keys and values, and what the block's rows see.  What a call does
+// not have is null.
+struct Exponents {
+  const int *q, *d, *k, *v;
+  const Hull *hulls;
+  int row_blocks, key_blocks;
+
+  // Whether any block of [first, first + n) of a (b, key head) cannot be split, in the lanes that meet one
+  __device__ static inline bool bad(const int *of, int64_t head, int blocks, int first, int n) {
+    bool found = false;
+    if (of)
+      for (int e = threadIdx.x; e < n; e += kThreads) found |= first + e < blocks && of[head * blocks + first + e] == kBad;
+    return found;
+  }
+  __device__ inline bool bad_rows(int64_t head, int first, int n) const { return bad(q, head, row_blocks, first, n) | bad(d, head, row_blocks, first, n); }
+  __device__ inline bool bad_keys(int64_t head, int first, int n) const { return bad(k, head, key_blocks, first, n) | bad(v, head, key_blocks, first, n); }
+  // of the blocks of rows that see one of the keys [from, to)
+  __device__ inline bool bad_rows_of(int64_t head, int from, int to) const {
+    bool found = false;
+    for (int e = threadIdx.x; e < row_blocks; e += kThreads) {
+      const int64_t at = head * row_blocks + e;
+      found |= (q[at] == kBad || d[at] == kBad) && hulls[at].meets(from, to);
+    }
+    return found;
+  }
+};
+
+// Products on pairs where that is faster.  Workgroups that meet a block that cannot be split leave their results to the kernels of attention.hip,
+// which take the exponents that these return.
+bool pair_suits(const Call &c, bool backward);
+size_t pair_bytes(const Call &c, bool backward);  // of scratch
+Exponents pair_forward(const Call &c, float *out, float *stat, const Pieces &pieces, int tiles, char *scratch, hipStream_t s);
+// dq (unless null), dk and dv (unless both are); `parts` as dkv_kernel takes them
+Exponents pair_backward(const Call &c, const float *dout, const Row *rows, float *dq, float *dk, float *dv, float *parts, int row_tiles, int key_tiles,
+                        int pieces, char *scratch, hipStream_t s);
+
 }  // namespace attention
 }  // namespace tf

@@ -19,21 +19,14 @@ using namespace tf::attention;
 
 namespace {
 
-constexpr int kThreads = 256, kRows = 128, kKeys = 32;  // of a workgroup; rows in the forward pass, keys in dkv_kernel; steps of the other axis
-constexpr float kNone = -INFINITY;
-
 template <int V>
 using IC = std::integral_constant<int, V>;
-
-__device__ inline float other_half(float v) { return __shfl_xor(v, 32); }
 
 // ------------------------------------------------------------------------------ tiles of the fp32 instruction
 //
 // v_mfma_f32_32x32x2: a lane supplies A[lane % 32][half] and B[half][lane % 32], half = lane / 32, and holds D[8 (v / 4) + 4 half + v % 4][lane % 32].
 // A score tile is computed with what the lane keeps on the columns: rows in the forward pass and dq, keys in dkv.  Its 16 values are then, as they
 // are, the B operands of the products that follow: step v takes row 8 (v / 4) + 4 half + v % 4 of the tile on the other side.
-
-constexpr int key_of(int v, int half) { return 8 * (v / 4) + 4 * half + v % 4; }
 
 // 32 rows of DP columns in LDS, columns past `dim` and rows past `count` zero.  Four floats more than a row keep the reads apart.
 template <int DP>
@@ -159,82 +152,13 @@ struct Sum {
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d) v[d] *= by;
   }
-  __device__ inline void store(float *row, int dim, float by) const {
-    const int half = threadIdx.x % 64 / 32;
-#pragma unroll
-    for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = 32 * d + 8 * q + 4 * half;
-        if (c < dim) store4(row + c, dim - c, f32x4{v[d][4 * q] * by, v[d][4 * q + 1] * by, v[d][4 * q + 2] * by, v[d][4 * q + 3] * by});
-      }
-  }
 };
-
-// The least and the greatest of what a wave's 32 columns, or a workgroup's 128, see, empty ones aside; inner: what all of them see.
-struct Hull {
-  int lo, hi, inner_lo, inner_hi;
-  __device__ inline void of(int lo_, int hi_, bool live) {
-    const bool some = live && lo_ < hi_;
-    lo = some ? lo_ : INT32_MAX;
-    hi = some ? hi_ : 0;
-    inner_lo = some ? lo_ : INT32_MAX;
-    inner_hi = some ? hi_ : 0;
-#pragma unroll
-    for (int step = 1; step < 32; step *= 2) {
-      lo = min(lo, __shfl_xor(lo, step));
-      hi = max(hi, __shfl_xor(hi, step));
-      inner_lo = max(inner_lo, __shfl_xor(inner_lo, step));
-      inner_hi = min(inner_hi, __shfl_xor(inner_hi, step));
-    }
-  }
-  // over the four waves, through `room`
-  __device__ inline Hull all(int (*room)[4]) const {
-    const int wave = threadIdx.x / 64;
-    if (threadIdx.x % 64 == 0) room[wave][0] = lo, room[wave][1] = hi, room[wave][2] = inner_lo, room[wave][3] = inner_hi;
-    __syncthreads();
-    Hull h = *this;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      h.lo = min(h.lo, room[w][0]);
-      h.hi = max(h.hi, room[w][1]);
-      h.inner_lo = max(h.inner_lo, room[w][2]);
-      h.inner_hi = min(h.inner_hi, room[w][3]);
-    }
-    h.lo = __builtin_amdgcn_readfirstlane(h.lo);
-    h.hi = __builtin_amdgcn_readfirstlane(h.hi);
-    return h;
-  }
-  __device__ inline bool meets(int from, int to) const { return lo < to && hi > from; }
-  __device__ inline bool covers(int from, int to) const { return inner_lo <= from && inner_hi >= to; }
-};
-
-// Pieces of rows: [piece][row of all][dim] unnormalised sums and [piece][row of all] (maximum, sum); a row of all is (b, key head, row).
-struct Pieces {
-  float *sums;
-  float2 *marks;
-  int count;
-  int64_t rows;  // of all
-};
-
-// Writes a row's result or its piece.
-__device__ inline float row_end(const Call &c, const Pieces &to, float *out, float *stat, int b, int g, int r, int piece, float top, float total,
-                                bool writes_mark, float *&row) {
-  if (to.count > 1) {
-    const int64_t at = piece * to.rows + ((int64_t)b * c.key_heads + g) * c.rows + r;
-    if (writes_mark) to.marks[at] = make_float2(top, total);
-    row = to.sums + at * c.dim;
-    return 1.f;
-  }
-  if (stat && writes_mark) stat[c.stat_at(b, g, r)] = total == 0.f ? kNone : (top + __builtin_amdgcn_logf(total)) * kLn2;
-  row = out ? out + c.query_at(b, g, r) : nullptr;
-  return total == 0.f ? 0.f : 1.f / total;
-}
 
 // ------------------------------------------------------------------------------ forward, 128 rows a workgroup
 
 template <int DP>
-__global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out, float *stat, const Pieces pieces, int tiles) {
+__global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out, float *stat, const Pieces pieces, int tiles,
+                                                        const Exponents left) {
   __shared__ __align__(16) Tile<DP> kt, vt;
   __shared__ int room[4][4];
   __shared__ uint32_t found;
@@ -253,7 +177,8 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
   mine.of(lo, hi, live);
   const Hull all = mine.all(room);
   // this piece's steps of the keys that any of the rows sees
-  const int first = all.lo < all.hi ? all.lo / kKeys : 0, steps = all.lo < all.hi ? (all.hi + kKeys - 1) / kKeys - first : 0;
+  const int first = all.first(), steps = all.steps();
+  if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), kRows / 32) | left.bad_keys(bg, first, steps))) return;
   const int begin = first + (int)((int64_t)steps * piece / pieces.count), end = first + (int)((int64_t)steps * (piece + 1) / pieces.count);
   const Score score(c);
   Sum<DP> o;
@@ -297,7 +222,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
   if (!live) return;
   float *row;
   const float by = row_end(c, pieces, out, stat, b, g, r, piece, top, total, half == 0, row);
-  if (row) o.store(row, c.dim, by);
+  if (row) store_sums(o.v, row, c.dim, by);
 }
 
 // ------------------------------------------------------------------------------ forward, few rows
@@ -581,12 +506,6 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void join_kernel(const Call c
 
 // ------------------------------------------------------------------------------ backward
 
-// What the backward kernels read of a row: its statistic times log2 e, delta, and the keys that it sees.
-struct Row {
-  float stat, delta;
-  int lo, hi;
-};
-
 // A wave a row of all.
 __global__ __launch_bounds__(kThreads) void prepare_kernel(const Call c, const float *__restrict__ o, const float *__restrict__ stat,
                                                            const float *__restrict__ dout, Row *__restrict__ rows, int64_t count) {
@@ -607,20 +526,8 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(const Call c, const f
   rows[at] = row;
 }
 
-// p and ds / scale from the products of queries and keys, and of gradients and values.
-__device__ inline void gradient(const Score &score, float product, float dp, float bias, float stat, float delta, bool seen, float &p, float &ds) {
-  float t = product * score.factor, slope = 1.f;
-  if (score.capped) {
-    t = tanh_of(t);
-    slope = 1.f - t * t;
-    t *= score.top;
-  }
-  p = seen ? __builtin_amdgcn_exp2f(t - bias - stat) : 0.f;
-  ds = seen ? p * (dp - delta) * slope : 0.f;
-}
-
 template <int DP>
-__global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float *dout, const Row *rows, float *dq, int tiles) {
+__global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float *dout, const Row *rows, float *dq, int tiles, const Exponents left) {
   __shared__ __align__(16) Tile<DP> kt, vt;
   __shared__ int room[4][4];
   __shared__ uint32_t found;
@@ -639,10 +546,11 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
   Hull mine;
   mine.of(row.lo, row.hi, live);
   const Hull all = mine.all(room);
+  const int begin = all.first(), end = begin + all.steps();
+  if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), kRows / 32) | left.bad_keys(bg, begin, end - begin))) return;
   const Score score(c);
   Sum<DP> sum;
   sum.zero();
-  const int begin = all.lo < all.hi ? all.lo / kKeys : 0, end = all.lo < all.hi ? (all.hi + kKeys - 1) / kKeys : 0;
 #pragma unroll 1
   for (int step = begin; step < end; ++step) {
     const int j0 = step * kKeys, count = min(kKeys, c.tk - j0);
@@ -667,14 +575,14 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
     sum.add(kt, ds);
     if (clean && found) sum.add_back(found, [&](int n) { return c.k + c.key_at(b, g, j0 + n); }, c.dim, ds);
   }
-  if (live) sum.store(dq + at, c.dim, c.scale);
+  if (live) store_sums(sum.v, dq + at, c.dim, c.scale);
 }
 
 // 128 keys a workgroup, 32 a wave, which walks the rows of piece blockIdx.x / (tiles * heads).  Results go to dk and dv, or piece by piece to
 // [piece][2][b, key, key head][dim].
 template <int DP, bool DK, bool DV>
 __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float *dout, const Row *rows, float *dk, float *dv, float *parts,
-                                                       int tiles, int pieces) {
+                                                       int tiles, int pieces, const Exponents left) {
   __shared__ __align__(16) Tile<DP> qt, dt;
   __shared__ Row info[32];
   __shared__ float slopes[32];
@@ -685,6 +593,7 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float
   const int lane = threadIdx.x % 64, half = lane / 32;
   const int tile_lo = tile * kRows, tile_hi = min(c.tk, tile_lo + kRows);
   const int j = tile_lo + threadIdx.x / 64 * 32 + lane % 32;
+  if (left.q && !__syncthreads_or(left.bad_rows_of(bg, tile_lo, tile_hi) | left.bad_keys(bg, tile_lo / 32, kRows / 32))) return;
   const bool live = j < c.tk;
   const int64_t at = c.key_at(b, g, live ? j : 0);
   Operand<DP> k, v;
@@ -749,8 +658,8 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float
   }
   if (!live) return;
   const int64_t all = (int64_t)c.batch * c.tk * c.key_heads * c.dim;
-  if (DK) dks.store((pieces > 1 ? parts + (int64_t)piece * 2 * all : dk) + at, c.dim, c.scale);
-  if (DV) dvs.store((pieces > 1 ? parts + ((int64_t)piece * 2 + 1) * all : dv) + at, c.dim, 1.f);
+  if (DK) store_sums(dks.v, (pieces > 1 ? parts + (int64_t)piece * 2 * all : dk) + at, c.dim, c.scale);
+  if (DV) store_sums(dvs.v, (pieces > 1 ? parts + ((int64_t)piece * 2 + 1) * all : dv) + at, c.dim, 1.f);
 }
 
 // dk and dv from their pieces, in order; half blockIdx.y.
@@ -871,6 +780,7 @@ extern "C" int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHan
   float *out = output ? (float *)output->data : nullptr, *stat = statistics ? (float *)statistics->data : nullptr;
   const int64_t head_pairs = (int64_t)batch * c.key_heads;
   const bool few = c.rows <= 32 && !(c.rows > 16 && c.dim > 128);
+  const bool pairs = !few && pair_suits(c, false);
   int64_t groups;
   int tiles = 0, keys_a_piece = 0;
   Pieces pieces = {};
@@ -887,20 +797,20 @@ extern "C" int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHan
     groups = head_pairs * tiles * pieces.count;
   }
   TF_REQUIRE(groups < kMaxGroups, "too many sequences, heads and queries for a launch");
-  const bool scratch = pieces.count > 1;
-  TF_REQUIRE(!scratch || !being_captured(s), "this many keys for few queries take scratch, which a captured stream cannot give back");
+  const size_t planes = pairs ? pair_bytes(c, false) : 0;
+  TF_REQUIRE((pieces.count == 1 && !planes) || !being_captured(s), "a pass of this size takes scratch, which a captured stream cannot give back");
   announce_write(output);
   announce_write(statistics);
-  void *block = nullptr;
-  if (scratch) {
-    const size_t sums = (size_t)pieces.count * all_rows * c.dim * sizeof(float), marks = (size_t)pieces.count * all_rows * sizeof(float2);
-    block = device_alloc(sums + marks, s);
+  char *block = nullptr;
+  if (pieces.count > 1 || planes) {
+    const size_t marks = pieces.count > 1 ? (size_t)pieces.count * all_rows * sizeof(float2) : 0, sums = marks / sizeof(float2) * c.dim * sizeof(float);
+    block = (char *)device_alloc(planes + marks + sums, s);
     if (!block) {
-      if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(sums + marks));
+      if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(planes + marks + sums));
       return 0;
     }
-    pieces.marks = (float2 *)block;
-    pieces.sums = (float *)((char *)block + marks);
+    pieces.marks = (float2 *)(block + planes);
+    pieces.sums = (float *)(block + planes + marks);
   }
   if (few) {
     auto go = [&](auto dp, auto nc) {
@@ -915,15 +825,16 @@ extern "C" int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHan
       else go(IC<128>{}, IC<2>{});
     }
   } else {
+    const Exponents left = pairs ? pair_forward(c, out, stat, pieces, tiles, block, s) : Exponents{};
     with_columns(c.dim, [&](auto dp) {
-      hipLaunchKernelGGL((rows_kernel<decltype(dp)::value>), dim3((unsigned)groups), dim3(kThreads), 0, s, c, out, stat, pieces, tiles);
+      hipLaunchKernelGGL((rows_kernel<decltype(dp)::value>), dim3((unsigned)groups), dim3(kThreads), 0, s, c, out, stat, pieces, tiles, left);
     });
   }
-  if (scratch) {
+  if (pieces.count > 1) {
     if (pieces.count > 16) hipLaunchKernelGGL((join_kernel<16>), dim3((unsigned)all_rows), dim3(1024), 0, s, c, pieces, out, stat);
     else hipLaunchKernelGGL((join_kernel<1>), dim3((unsigned)((all_rows + 3) / 4)), dim3(256), 0, s, c, pieces, out, stat);
-    device_free(block, s);
   }
+  if (block) device_free(block, s);
   return finish(s, "DLGpuAttentionForward");
 }
 
@@ -959,33 +870,37 @@ extern "C" int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHa
   for (const DLArray *written : {(const DLArray *)dquery, (const DLArray *)dkey, (const DLArray *)dvalue}) announce_write(written);
   const int64_t all = all_keys * c.dim;
   const size_t row_bytes = (size_t)all_rows * sizeof(Row), part_bytes = pieces > 1 ? (size_t)pieces * 2 * all * sizeof(float) : 0;
-  char *block = (char *)device_alloc(row_bytes + part_bytes, s);
+  const bool pairs = all_rows && all_keys && pair_suits(c, true);
+  const size_t planes = pairs ? pair_bytes(c, true) : 0, bytes = planes + part_bytes + row_bytes;
+  char *block = (char *)device_alloc(bytes, s);
   if (!block) {
-    if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(row_bytes + part_bytes));
+    if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(bytes));
     return 0;
   }
-  Row *rows = (Row *)block;
-  float *parts = (float *)(block + row_bytes);
+  float *parts = (float *)(block + planes);
+  Row *rows = (Row *)(block + planes + part_bytes);
   const float *dout = (const float *)doutput->data;
   float *dk = dkey ? (float *)dkey->data : nullptr, *dv = dvalue ? (float *)dvalue->data : nullptr;
   if (all_rows)
     hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)((all_rows + 3) / 4)), dim3(kThreads), 0, s, c, (const float *)output->data,
                        (const float *)statistics->data, dout, rows, all_rows);
+  const Exponents left = pairs ? pair_backward(c, dout, rows, dquery ? (float *)dquery->data : nullptr, dk, dv, parts, row_tiles, key_tiles, pieces, block, s)
+                               : Exponents{};
   with_columns(c.dim, [&](auto columns) {
     constexpr int DP = decltype(columns)::value;
     if (dquery && all_rows)
-      hipLaunchKernelGGL((dq_kernel<DP>), dim3((unsigned)(head_pairs * row_tiles)), dim3(kThreads), 0, s, c, dout, rows, (float *)dquery->data, row_tiles);
+      hipLaunchKernelGGL((dq_kernel<DP>), dim3((unsigned)(head_pairs * row_tiles)), dim3(kThreads), 0, s, c, dout, rows, (float *)dquery->data, row_tiles, left);
     if (!key_groups) return;
     const dim3 grid((unsigned)(key_groups * pieces));
     if constexpr (DP <= 128) {
       if (dk && dv) {
-        hipLaunchKernelGGL((dkv_kernel<DP, true, true>), grid, dim3(kThreads), 0, s, c, dout, rows, dk, dv, parts, key_tiles, pieces);
+        hipLaunchKernelGGL((dkv_kernel<DP, true, true>), grid, dim3(kThreads), 0, s, c, dout, rows, dk, dv, parts, key_tiles, pieces, left);
         return;
       }
     }
     // heads of more than 128 columns: the operands and sums of one gradient fill the registers
-    if (dk) hipLaunchKernelGGL((dkv_kernel<DP, true, false>), grid, dim3(kThreads), 0, s, c, dout, rows, dk, nullptr, parts, key_tiles, pieces);
-    if (dv) hipLaunchKernelGGL((dkv_kernel<DP, false, true>), grid, dim3(kThreads), 0, s, c, dout, rows, nullptr, dv, parts, key_tiles, pieces);
+    if (dk) hipLaunchKernelGGL((dkv_kernel<DP, true, false>), grid, dim3(kThreads), 0, s, c, dout, rows, dk, nullptr, parts, key_tiles, pieces, left);
+    if (dv) hipLaunchKernelGGL((dkv_kernel<DP, false, true>), grid, dim3(kThreads), 0, s, c, dout, rows, nullptr, dv, parts, key_tiles, pieces, left);
   });
   if (pieces > 1)
     hipLaunchKernelGGL(sum_kernel, dim3((unsigned)std::min<int64_t>((all / 4 + kThreads) / kThreads, 4 * num_cus()), 2), dim3(kThreads), 0, s, parts, dk, dv, all,

@@ -1,0 +1,842 @@
+// Attention on fp16 pairs: forward_kernel, dq_kernel and dkv_kernel, and pack_kernel, which splits their operands.
+//
+// A block of 32 rows of an operand (queries, their gradients, keys or values of one head) is multiplied by the power of two that brings its
+// largest value into [2^14, 2^15), and each element is made of two fp16 numbers, h its nearest one and l the nearest to what is left: three
+// products of the fp16 instruction, h h' + h l' + l h', take the place of one of the fp32 instruction, which has a sixteenth of its rate (gemm_pair.h
+// has the argument; what is left off is 2^-23 of an element, or a fixed part of its block's largest value where that is more).
+//   Where l is held 2^11 times larger (operands of scores and of their gradients, both sides), that part is 2^-50, and products with an l have sums of
+//   their own.  Where it is not (p and what p multiplies), it is 2^-39, and one sum takes all three: twice the sums of o or dv would not leave room
+//   for two waves a SIMD, or for the operands of dk.  p is at most 4, and held times 2^12 or 2^13.
+// Scales are a block's, so a product's scale is known for a whole tile and costs nothing: it is part of the factor of a score, of the
+// exponent of p, of ds.  A sum over several blocks has the scale of the largest one so far (`unit`); when a larger one comes the sum is multiplied.
+//
+// A block with an infinity or a NaN, one whose values pass 2^55, or one of keys or values with a row smaller than 2^-16 of its largest (it would
+// lose its digits) has kBad for its exponent, and workgroups that meet one leave their rows to the fp32 kernels.  Rows that see nothing and keys
+// that nothing sees are packed as zeros, whatever they hold.
+#include "attention.h"
+#include "internal.h"
+
+#include <algorithm>
+#include <type_traits>
+#include <utility>
+
+namespace tf {
+namespace attention {
+namespace {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+template <int V>
+using IC = std::integral_constant<int, V>;
+
+template <int N, class F, int... I>
+__device__ __forceinline__ void static_for_impl(F &&f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void static_for(F &&f) {
+  static_for_impl<N>(f, std::make_integer_sequence<int, N>{});
+}
+
+constexpr int kFragment = 1024;  // bytes: 32 rows x 16 of fp16, a wave's lanes one behind the other
+constexpr int kInfoBytes = 1024;  // of a block of rows: eight arrays of 32, see Info
+constexpr float kLowScale = 0x1p11f, kLowUnscale = 0x1p-11f;
+constexpr int kSmallest = 110;   // exponents above it stand for values that no sum notices
+constexpr int kLargest = -40;
+
+// Bytes of a block of 32 rows: DP columns of h and l.
+__host__ __device__ constexpr int64_t block_size(int dp) { return dp * 128; }
+
+// ------------------------------------------------------------------------------ splitting
+
+// By value: a bit cast of an element of a vector takes the vector's first one, whichever it is.
+__device__ inline uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
+
+enum Info { kStat = 0, kDelta, kLo, kHi, kSlope, kAhead };
+
+struct Job {
+  const float *src;
+  bool of_rows;
+  float low;         // factor of l in the transposed form
+  char *plain, *transposed;
+  int *exponents;
+  int first;         // workgroup
+};
+struct Pack {
+  Job jobs[4];
+  int n_jobs, row_blocks, key_blocks;
+  const Row *rows;   // backward: of all rows
+  float *info;       // backward: [b, key head][block of rows][8][32]
+  Hull *hulls;
+  int *delta_exponents;  // |delta| of the block is below 2^this
+};
+
+__device__ inline void split(float x, float low, _Float16 &h, _Float16 &l) {
+  h = (_Float16)x;
+  l = (_Float16)((x - (float)h) * low);
+}
+
+// A workgroup a block.  Plain form: step s of 16 columns, h then l, lane: row lane % 32, columns 16 s + 8 (lane / 32) + 0..7.  Transposed: columns 32 d
+// + lane % 32, rows 16 t + key_of's order, so that a tile's probabilities are the other operand as they lie.
+template <int DP>
+__global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack p) {
+  __shared__ __align__(16) float tile[32][DP + 4];
+  __shared__ uint32_t most[32];
+  __shared__ int hull[2];
+  int which = 0;
+  for (int i = 1; i < p.n_jobs; ++i) which = (int)blockIdx.x >= p.jobs[i].first ? i : which;
+  const Job &job = p.jobs[which];
+  const int blocks = job.of_rows ? p.row_blocks : p.key_blocks;
+  const int at = (int)blockIdx.x - job.first, head = at / blocks, block = at % blocks, b = head / c.key_heads, g = head % c.key_heads;
+  const int tid = threadIdx.x, row = tid / 8, n = block * 32 + row;
+  bool used;
+  Row info = {0.f, 0.f, 0, 0};
+  if (job.of_rows) {
+    used = n < c.rows;
+    if (used && p.rows) info = p.rows[(int64_t)head * c.rows + n];
+    else if (used) c.seen(b, n / c.group, info.lo, info.hi);
+    used = used && info.lo < info.hi;
+  } else {
+    // keys that any query sees lie between the first and the last of them
+    int lo = 0, hi = c.tk;
+    if (c.spans) {
+      if (tid == 0) hull[0] = c.tk, hull[1] = 0;
+      __syncthreads();
+      lo = c.tk, hi = 0;
+      for (int i = tid; i < c.tq; i += kThreads) {
+        int l, h;
+        c.seen(b, i, l, h);
+        if (l < h) lo = min(lo, l), hi = max(hi, h);
+      }
+      atomicMin(&hull[0], lo);
+      atomicMax(&hull[1], hi);
+      __syncthreads();
+      lo = hull[0], hi = hull[1];
+    }
+    used = n < c.tk && n >= lo && n < hi;
+  }
+  const float *src = job.src + (used ? job.of_rows ? c.query_at(b, g, n) : c.key_at(b, g, n) : 0);
+  f32x4 x[DP / 32];
+  uint32_t top = 0;
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) {
+    const int col = 32 * e + tid % 8 * 4;
+    x[e] = used && col < c.dim ? load4(src + col, c.dim - col) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = max(top, bits_of(x[e][i]) & 0x7fffffffu);
+  }
+#pragma unroll
+  for (int step = 1; step < 8; step *= 2) top = max(top, (uint32_t)__shfl_xor((int)top, step));
+  if (tid % 8 == 0) most[row] = top;
+  __syncthreads();
+  uint32_t largest = 0, least = 0x7f800000u;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const uint32_t v = most[i];
+    largest = max(largest, v);
+    least = v ? min(least, v) : least;
+  }
+  const int field = (int)(largest >> 23);
+  int exponent = min(kSmallest, 141 - field);
+  if (largest >= 0x7f800000u || exponent < kLargest || (!job.of_rows && largest && (int)(least >> 23) < field - 16 && exponent < kSmallest)) exponent = kBad;
+  if (tid == 0) job.exponents[(int64_t)head * blocks + block] = exponent;
+  if (job.of_rows && p.info && which == 0) {  // what the backward kernels read of the rows
+    const int64_t of_block = (int64_t)head * blocks + block;
+    if (tid < 64) {
+      const int r = block * 32 + tid % 32;
+      const bool is = r < c.rows;
+      Row mine = {0.f, 0.f, 0, 0};
+      if (is) mine = p.rows[(int64_t)head * c.rows + r];
+      if (mine.lo >= mine.hi) mine.stat = mine.delta = 0.f;
+      Hull seen;
+      seen.of(mine.lo, mine.hi, is);
+      if (seen.lo >= seen.hi) seen.lo = seen.hi = 0;
+      // rows that see nothing, or that are none, keep the block from covering anything
+      if (__any(mine.lo >= mine.hi)) seen.inner_lo = INT32_MAX, seen.inner_hi = 0;
+      uint32_t delta = bits_of(mine.delta) & 0x7fffffffu;
+#pragma unroll
+      for (int step = 1; step < 32; step *= 2) delta = max(delta, (uint32_t)__shfl_xor((int)delta, step));
+      if (tid < 32) {
+        float *to = p.info + of_block * (kInfoBytes / 4) + tid;
+        to[32 * kStat] = mine.stat;
+        to[32 * kDelta] = mine.delta;
+        to[32 * kLo] = __builtin_bit_cast(float, mine.lo);
+        to[32 * kHi] = __builtin_bit_cast(float, mine.hi);
+        to[32 * kSlope] = c.slopes && is ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
+        to[32 * kAhead] = (float)(r / c.group + c.tk - c.tq);
+      }
+      if (tid == 0) {
+        p.hulls[of_block] = seen;
+        p.delta_exponents[of_block] = (int)(delta >> 23) - 126;
+      }
+    }
+  }
+  if (exponent == kBad) return;
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[e][i] = __builtin_ldexpf(x[e][i], exponent);
+    *reinterpret_cast<f32x4 *>(&tile[row][32 * e + tid % 8 * 4]) = x[e];
+  }
+  __syncthreads();
+  const int64_t to = ((int64_t)head * blocks + block) * block_size(DP);
+  if (job.plain)
+#pragma unroll
+    for (int u = tid; u < DP * 4; u += kThreads) {
+      const int r = u % 32, eighth = u / 32;
+      f16x8 h, l;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        _Float16 a, d;
+        split(tile[r][8 * eighth + e], kLowScale, a, d);
+        h[e] = a;
+        l[e] = d;
+      }
+      char *out = job.plain + to + eighth / 2 * 2 * kFragment + (eighth % 2 * 32 + r) * 16;
+      *reinterpret_cast<f16x8 *>(out) = h;
+      *reinterpret_cast<f16x8 *>(out + kFragment) = l;
+    }
+  if (job.transposed)
+#pragma unroll
+    for (int u = tid; u < DP * 4; u += kThreads) {
+      const int col = u % DP, t = u / DP / 2, half = u / DP % 2;
+      f16x8 h, l;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        _Float16 a, d;
+        split(tile[16 * t + key_of(e, half)][col], job.low, a, d);
+        h[e] = a;
+        l[e] = d;
+      }
+      char *out = job.transposed + to + (col / 32 * 2 + t) * 2 * kFragment + (half * 32 + col % 32) * 16;
+      *reinterpret_cast<f16x8 *>(out) = h;
+      *reinterpret_cast<f16x8 *>(out + kFragment) = l;
+    }
+}
+
+// ------------------------------------------------------------------------------ what the products share
+
+__device__ inline f16x8 fragment(const char *at) { return *reinterpret_cast<const f16x8 *>(at); }
+__device__ inline f32x16 mfma(f16x8 a, f16x8 b, f32x16 sum) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, sum, 0, 0, 0); }
+__device__ inline f32x16 zeros() {
+  f32x16 z;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) z[v] = 0.f;
+  return z;
+}
+
+// A wave's operand of 32 rows or keys in the plain form, in registers.
+template <int DP>
+struct Held {
+  f16x8 h[DP / 16], l[DP / 16];
+  __device__ inline void load(const char *block) {
+    const int lane = threadIdx.x % 64;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+      h[s] = fragment(block + 2 * s * kFragment + lane * 16);
+      l[s] = fragment(block + (2 * s + 1) * kFragment + lane * 16);
+    }
+  }
+  // Waits for them, before loads that the compiler does not count are under way.
+  __device__ inline void wait() {
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) asm volatile("" : "+v"(h[s]), "+v"(l[s]));
+  }
+};
+
+// The product of a block in LDS, in the plain form, with what the wave holds.
+template <int DP>
+__device__ __forceinline__ f32x16 product(const char *block, const Held<DP> &b) {
+  const char *at = block + threadIdx.x % 64 * 16;
+  f32x16 sum = zeros(), low = zeros();
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const f16x8 h = fragment(at + 2 * s * kFragment), l = fragment(at + (2 * s + 1) * kFragment);
+    low = mfma(l, b.h[s], low);
+    sum = mfma(h, b.h[s], sum);
+    low = mfma(h, b.l[s], low);
+  }
+#pragma unroll
+  for (int v = 0; v < 16; ++v) sum[v] = __builtin_fmaf(low[v], kLowUnscale, sum[v]);
+  return sum;
+}
+
+// 16 values of a tile as the other operand of a product over its rows.
+struct Weights {
+  f16x8 h[2], l[2];
+  template <bool SCALED>
+  __device__ __forceinline__ void set(const float (&w)[16]) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const f32x2 x = {w[8 * t + e], w[8 * t + e + 1]};
+        const f16x2 top = __builtin_convertvector(x, f16x2);
+        // x - h is a number of 32 bits, and so is 2^11 times that
+        f32x2 left;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          left[i] = SCALED ? __builtin_fmaf((float)top[i], -kLowScale, x[i] * kLowScale) : __builtin_fmaf((float)top[i], -1.f, x[i]);
+        const f16x2 rest = __builtin_convertvector(left, f16x2);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          h[t][e + i] = top[i];
+          l[t][e + i] = rest[i];
+        }
+      }
+  }
+};
+
+// sum[d] += of a transposed block with l as it is
+template <int DP>
+__device__ __forceinline__ void add_product(f32x16 (&sum)[DP / 32], const char *block, const Weights &w) {
+  const char *at = block + threadIdx.x % 64 * 16;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const f16x8 h = fragment(at + (2 * d + t) * 2 * kFragment), l = fragment(at + ((2 * d + t) * 2 + 1) * kFragment);
+      sum[d] = mfma(l, w.h[t], sum[d]);
+      sum[d] = mfma(h, w.l[t], sum[d]);
+      sum[d] = mfma(h, w.h[t], sum[d]);
+    }
+}
+// the same with both l scaled: their products have sums of their own
+template <int DP>
+__device__ __forceinline__ void add_product(f32x16 (&sum)[DP / 32], f32x16 (&low)[DP / 32], const char *block, const Weights &w) {
+  const char *at = block + threadIdx.x % 64 * 16;
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const f16x8 h = fragment(at + (2 * d + t) * 2 * kFragment), l = fragment(at + ((2 * d + t) * 2 + 1) * kFragment);
+      low[d] = mfma(l, w.h[t], low[d]);
+      sum[d] = mfma(h, w.h[t], sum[d]);
+      low[d] = mfma(h, w.l[t], low[d]);
+    }
+}
+template <int N>
+__device__ inline void multiply(f32x16 (&sum)[N], float by) {
+#pragma unroll
+  for (int d = 0; d < N; ++d) sum[d] *= by;
+}
+
+// Brings 1 KB from `from` to LDS at `to`, 16 bytes a lane.  Written out because the compiler takes every read of LDS for a reader of the loads
+// into it that are under way, and waits for them; `arrived` is the wait that they need.  It writes no register.
+__device__ __forceinline__ void fetch(uint32_t to, const char *from) {
+  const uint32_t at = __builtin_amdgcn_readfirstlane(to), lane = threadIdx.x % 64 * 16u;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane), "s"(from) : "memory");
+}
+// Everything that this wave has fetched, and read from LDS, has arrived, in all waves.
+__device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ inline uint32_t lds_address(const char *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p; }
+
+__device__ inline const char *uniform(const char *p) {
+  const uint64_t v = (uint64_t)p;
+  return (const char *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)v) | (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32);
+}
+
+// What the launch before has written and this one only reads, at an address that the wave shares: by a scalar load, which leaves the count of
+// the vector loads under way alone.
+__device__ inline int scalar(const int *p) { return *(const __attribute__((address_space(4))) int *)uniform((const char *)p); }
+// 2^-(a + b) factor, for scores: not below 2^-80 of it, where a score is nothing, so that it times the -infinity of a masked one is that
+__device__ inline float unscaled(float factor, int a, int b) { return __builtin_ldexpf(factor, max(-(a + b), -80)); }
+
+
+// Fetches block `index` of each of N operands, one behind the other in LDS from `to` on, a wave every fourth fragment.
+template <int DP, int N>
+__device__ __forceinline__ void fetch_blocks(uint32_t to, const char *const (&of)[N], int64_t index) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  static_for<N>([&](auto n) {
+    const char *from = uniform(of[decltype(n)::value] + index * block_size(DP)) + wave * kFragment;
+#pragma unroll
+    for (int f = 0; f < DP / 32; ++f) fetch(to + (uint32_t)(decltype(n)::value * block_size(DP) + (4 * f + wave) * kFragment), from + 4 * f * kFragment);
+  });
+}
+
+// ------------------------------------------------------------------------------ forward
+
+// 128 rows a workgroup, 32 a wave; steps of 32 keys, the next one on its way into LDS while one is worked on.  PLAIN: neither cap nor bias.
+template <int DP, bool PLAIN>
+__global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Call c, const char *qs, const char *ks, const char *vs, const Exponents ex, float *out,
+                                                              float *stat, const Pieces pieces, int tiles) {
+  constexpr int BLOCK = (int)block_size(DP);
+  __shared__ __align__(16) char lds[2][2 * BLOCK];
+  __shared__ int room[4][4];
+  const int heads = c.batch * c.key_heads;
+  const int bg = (int)blockIdx.x % heads, rest = (int)blockIdx.x / heads;
+  const int b = bg / c.key_heads, g = bg % c.key_heads, tile = tiles - 1 - rest % tiles, piece = rest / tiles;
+  const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int r = tile * kRows + wave * 32 + lane % 32;
+  const bool live = r < c.rows;
+  const int i = (live ? r : c.rows - 1) / c.group, ahead = i + c.tk - c.tq;
+  int lo, hi;
+  c.seen(b, i, lo, hi);
+  Hull mine;
+  mine.of(lo, hi, live);
+  const Hull all = mine.all(room);
+  const int first = all.first(), steps = all.steps();
+  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32) | ex.bad_keys(bg, first, steps))) return;
+  const int begin = first + (int)((int64_t)steps * piece / pieces.count), end = first + (int)((int64_t)steps * (piece + 1) / pieces.count);
+  const int block = min(tile * (kRows / 32) + wave, ex.row_blocks - 1);
+  const int64_t row_block = (int64_t)bg * ex.row_blocks + block, key_block = (int64_t)bg * ex.key_blocks;
+  const int eq = scalar(ex.q + row_block);
+  const float slope = !PLAIN && c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
+  Held<DP> q;
+  q.load(qs + row_block * BLOCK);
+  q.wait();
+  const Score score(c);
+  f32x16 o[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d) o[d] = zeros();
+  float top = kNone, total = 0.f;   // total times 2^12
+  int unit = kSmallest;             // o is times 2^(12 + unit)
+  const char *const from[2] = {ks, vs};
+  const uint32_t to = lds_address(&lds[0][0]);
+  if (begin < end) fetch_blocks<DP, 2>(to, from, key_block + begin);
+#pragma unroll 1
+  for (int step = begin; step < end; ++step) {
+    const int slot = (step - begin) & 1, j0 = step * kKeys;
+    const int ek = scalar(ex.k + key_block + step), ev = scalar(ex.v + key_block + step);
+    arrived();
+    if (step + 1 < end) fetch_blocks<DP, 2>(to + (uint32_t)((1 - slot) * 2 * BLOCK), from, key_block + step + 1);
+    if (!mine.meets(j0, j0 + kKeys)) continue;
+    const char *const keys = lds[slot], *const values = lds[slot] + BLOCK;
+    const f32x16 s = product<DP>(keys, q);
+    const float factor = unscaled(score.factor, eq, ek);
+    const bool whole = mine.covers(j0, j0 + kKeys);
+    float p[16], most = kNone;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      p[v] = s[v];
+      if (!PLAIN) {
+        p[v] *= factor;
+        if (score.capped) p[v] = score.top * tanh_of(p[v]);
+        p[v] -= slope * fabsf((float)(ahead - (j0 + key_of(v, half))));
+      }
+    }
+    if (!whole)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int j = j0 + key_of(v, half);
+        p[v] = j >= lo && j < hi ? p[v] : kNone;
+      }
+#pragma unroll
+    for (int v = 0; v < 16; ++v) most = fmaxf(most, p[v]);
+    most = fmaxf(most, other_half(most));
+    if (PLAIN) most = most == kNone ? kNone : most * factor;
+    // The sums' exponent follows the maximum only where it grows by more than 2: p is at most 4 then, and most steps leave the sums alone.
+    const float next = most > top + 2.f ? most : top, base = next == kNone ? 0.f : next;
+    if (__any(next != top)) {
+      const float fade = __builtin_amdgcn_exp2f(top - base);
+      total *= fade;
+      multiply(o, fade);
+    }
+    top = next;
+    if (ev < unit) {
+      multiply(o, __builtin_ldexpf(1.f, ev - unit));
+      unit = ev;
+    }
+    // p times 2^12 and the values' distance to the unit, up to 2^-20 of it here
+    const int apart = unit - ev, near = max(apart, -20);
+    const float shift = (float)(12 + near) - base;
+    float sum = 0.f;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      p[v] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(p[v], factor, shift) : p[v] + shift);
+      sum += p[v];
+    }
+    total = __builtin_fmaf(sum, __builtin_ldexpf(1.f, -near), total);
+    if (apart < near)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) p[v] = __builtin_ldexpf(p[v], apart - near);
+    Weights w;
+    w.set<false>(p);
+    add_product<DP>(o, values, w);
+  }
+  if (!live) return;
+  total = (total + other_half(total)) * 0x1p-12f;
+  float *row;
+  const float by = row_end(c, pieces, out, stat, b, g, r, piece, top, total, half == 0, row);
+  if (row) {
+    multiply(o, __builtin_ldexpf(1.f, -12 - unit));
+    store_sums(o, row, c.dim, by);
+  }
+}
+
+// ------------------------------------------------------------------------------ backward
+
+// |dp - delta| of a tile is below 2^this: a product of DP columns of less than 2^15 each, and delta, of which one more bit is a sum.
+template <int DP>
+__device__ inline int gradient_exponent(int ed, int ev, int delta) {
+  constexpr int LOG = DP <= 32 ? 5 : DP <= 64 ? 6 : 7;
+  return max(LOG + 30 - ed - ev, delta) + 1;
+}
+
+// p times 2^13 (0 where a mask says so) and the derivative of the cap, from a product.
+template <bool PLAIN>
+__device__ __forceinline__ float weight(const Score &score, float product, float factor, float bias, float stat, float &slope) {
+  if (PLAIN) return __builtin_amdgcn_exp2f(__builtin_fmaf(product, factor, 13.f - stat));
+  float t = product * factor;
+  slope = 1.f;
+  if (score.capped) {
+    t = tanh_of(t);
+    slope = __builtin_fmaf(-t, t, 1.f);
+    t *= score.top;
+  }
+  return __builtin_amdgcn_exp2f((t - bias) - (stat - 13.f));
+}
+
+// 128 rows a workgroup, as forward_kernel; in LDS a step's keys, values and keys transposed.
+template <int DP, bool PLAIN>
+__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Call c, const char *qs, const char *ds_, const char *ks, const char *vs, const char *kts,
+                                                                        const Exponents ex, const Row *rows, const int *delta_exponents, float *dq, int tiles) {
+  constexpr int BLOCK = (int)block_size(DP);
+  __shared__ __align__(16) char lds[2][3 * BLOCK];
+  __shared__ int room[4][4];
+  const int heads = c.batch * c.key_heads;
+  const int bg = (int)blockIdx.x % heads, tile = tiles - 1 - (int)blockIdx.x / heads;
+  const int b = bg / c.key_heads, g = bg % c.key_heads;
+  const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int r = tile * kRows + wave * 32 + lane % 32;
+  const bool live = r < c.rows;
+  const Row row = rows[(int64_t)bg * c.rows + (live ? r : 0)];
+  const int ahead = (live ? r : 0) / c.group + c.tk - c.tq;
+  Hull mine;
+  mine.of(row.lo, row.hi, live);
+  const Hull all = mine.all(room);
+  const int begin = all.first(), end = begin + all.steps();
+  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32) | ex.bad_keys(bg, begin, end - begin))) return;
+  const int block = min(tile * (kRows / 32) + wave, ex.row_blocks - 1);
+  const int64_t row_block = (int64_t)bg * ex.row_blocks + block, key_block = (int64_t)bg * ex.key_blocks;
+  const int eq = scalar(ex.q + row_block), ed = scalar(ex.d + row_block), edelta = scalar(delta_exponents + row_block);
+  const float slope = !PLAIN && c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
+  // a row that sees nothing has whatever statistic
+  const bool some = live && row.lo < row.hi;
+  const float stat = some ? row.stat : 0.f, delta = some ? row.delta : 0.f;
+  Held<DP> q, d;
+  q.load(qs + row_block * BLOCK);
+  d.load(ds_ + row_block * BLOCK);
+  q.wait();
+  d.wait();
+  const Score score(c);
+  f32x16 sum[DP / 32], low[DP / 32];
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) sum[e] = low[e] = zeros();
+  int unit = INT32_MAX / 2;  // sum is times 2^unit
+  const char *const from[3] = {ks, vs, kts};
+  const uint32_t to = lds_address(&lds[0][0]);
+  if (begin < end) fetch_blocks<DP, 3>(to, from, key_block + begin);
+#pragma unroll 1
+  for (int step = begin; step < end; ++step) {
+    const int slot = (step - begin) & 1, j0 = step * kKeys;
+    const int ek = scalar(ex.k + key_block + step), ev = scalar(ex.v + key_block + step);
+    arrived();
+    if (step + 1 < end) fetch_blocks<DP, 3>(to + (uint32_t)((1 - slot) * 3 * BLOCK), from, key_block + step + 1);
+    if (!mine.meets(j0, j0 + kKeys)) continue;
+    const f32x16 s = product<DP>(lds[slot], q), dp = product<DP>(lds[slot] + BLOCK, d);
+    const int new_unit = min(unit, 14 - gradient_exponent<DP>(ed, ev, edelta) + ek);
+    if (new_unit < unit) {
+      if (step > begin) {
+        const float by = __builtin_ldexpf(1.f, new_unit - unit);
+        multiply(sum, by);
+        multiply(low, by);
+      }
+      unit = new_unit;
+    }
+    const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(1.f, -(ed + ev));
+    const int shift = unit - ek - 13;  // of ds, from p times 2^13
+    const bool whole = mine.covers(j0, j0 + kKeys);
+    float ds[16];
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const int j = j0 + key_of(v, half);
+      float cap = 1.f;
+      const float p = weight<PLAIN>(score, s[v], factor, PLAIN ? 0.f : slope * fabsf((float)(ahead - j)), stat, cap);
+      ds[v] = p * __builtin_fmaf(dp[v], d_factor, -delta);
+      if (!PLAIN) ds[v] *= cap;
+      ds[v] = __builtin_ldexpf(ds[v], shift);
+    }
+    if (!whole)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) {
+        const int j = j0 + key_of(v, half);
+        ds[v] = j >= row.lo && j < row.hi ? ds[v] : 0.f;
+      }
+    Weights w;
+    w.set<true>(ds);
+    add_product<DP>(sum, low, lds[slot] + 2 * BLOCK, w);
+  }
+  if (!live) return;
+  if (begin >= end) unit = 0;
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) sum[e][v] = __builtin_ldexpf(__builtin_fmaf(low[e][v], kLowUnscale, sum[e][v]), -unit);
+  store_sums(sum, dq + c.query_at(b, g, r), c.dim, c.scale);
+}
+
+// 128 keys a workgroup, 32 a wave; steps of 32 rows: in LDS queries, gradients, both transposed, and what Info says of the rows.
+template <int DP, bool PLAIN>
+__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const Call c, const char *qs, const char *ds_, const char *qts, const char *dts, const char *ks,
+                                                                         const char *vs, const Exponents ex, const char *info, const int *delta_exponents,
+                                                                         float *dk, float *dv, float *parts, int tiles, int pieces) {
+  constexpr int BLOCK = (int)block_size(DP), SLOT = 4 * BLOCK + kInfoBytes;
+  __shared__ __align__(16) char lds[2][SLOT];
+  __shared__ int range[2];
+  const int heads = c.batch * c.key_heads;
+  const int bg = (int)blockIdx.x % heads, rest = (int)blockIdx.x / heads;
+  const int b = bg / c.key_heads, g = bg % c.key_heads, tile = rest % tiles, piece = rest / tiles;
+  const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int tile_lo = tile * kRows, tile_hi = min(c.tk, tile_lo + kRows);
+  if (__syncthreads_or(ex.bad_rows_of(bg, tile_lo, tile_hi) | ex.bad_keys(bg, tile_lo / 32, kRows / 32))) return;
+  const int64_t row_block = (int64_t)bg * ex.row_blocks;
+  // the blocks of rows that see one of the keys
+  if (threadIdx.x == 0) range[0] = ex.row_blocks, range[1] = 0;
+  __syncthreads();
+  {
+    int lo = ex.row_blocks, hi = 0;
+    for (int e = threadIdx.x; e < ex.row_blocks; e += kThreads)
+      if (ex.hulls[row_block + e].meets(tile_lo, tile_hi)) lo = min(lo, e), hi = max(hi, e + 1);
+    atomicMin(&range[0], lo);
+    atomicMax(&range[1], hi);
+  }
+  __syncthreads();
+  const int first = __builtin_amdgcn_readfirstlane(range[0]), steps = max(0, __builtin_amdgcn_readfirstlane(range[1]) - first);
+  const int begin = first + (int)((int64_t)steps * piece / pieces), end = first + (int)((int64_t)steps * (piece + 1) / pieces);
+  const int j0 = tile_lo + wave * 32, j = j0 + lane % 32;
+  const bool live = j < c.tk;
+  const int64_t key_block = (int64_t)bg * ex.key_blocks + min(tile * (kRows / 32) + wave, ex.key_blocks - 1);
+  const int ek = scalar(ex.k + key_block), ev = scalar(ex.v + key_block);
+  Held<DP> k, v;
+  k.load(ks + key_block * BLOCK);
+  v.load(vs + key_block * BLOCK);
+  k.wait();
+  v.wait();
+  const Score score(c);
+  f32x16 dks[DP / 32], low[DP / 32], dvs[DP / 32];
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e) dks[e] = low[e] = dvs[e] = zeros();
+  int unit = INT32_MAX / 2, unit_v = kSmallest;  // of dks and low; of dvs, which are times 2^13 more
+  const char *const from[4] = {qs, ds_, qts, dts};
+  const uint32_t to = lds_address(&lds[0][0]);
+  auto fetch_step = [&](int step, int slot) {
+    fetch_blocks<DP, 4>(to + (uint32_t)(slot * SLOT), from, row_block + step);
+    if (wave == 0) fetch(to + (uint32_t)(slot * SLOT + 4 * BLOCK), uniform(info + (row_block + step) * kInfoBytes));
+  };
+  if (begin < end) fetch_step(begin, 0);
+#pragma unroll 1
+  for (int step = begin; step < end; ++step) {
+    const int slot = (step - begin) & 1;
+    const int eq = scalar(ex.q + row_block + step), ed = scalar(ex.d + row_block + step), edelta = scalar(delta_exponents + row_block + step);
+    Hull seen;
+    seen.lo = scalar(&ex.hulls[row_block + step].lo);
+    seen.hi = scalar(&ex.hulls[row_block + step].hi);
+    seen.inner_lo = scalar(&ex.hulls[row_block + step].inner_lo);
+    seen.inner_hi = scalar(&ex.hulls[row_block + step].inner_hi);
+    arrived();
+    if (step + 1 < end) fetch_step(step + 1, 1 - slot);
+    if (!seen.meets(j0, j0 + 32)) continue;
+    const char *const at = lds[slot];
+    const f32x16 s = product<DP>(at, k), dp = product<DP>(at + BLOCK, v);
+    const int new_unit = min(unit, 14 - gradient_exponent<DP>(ed, ev, edelta) + eq);
+    if (new_unit < unit) {
+      const float by = __builtin_ldexpf(1.f, max(new_unit - unit, -200));
+      multiply(dks, by);
+      multiply(low, by);
+      unit = new_unit;
+    }
+    if (ed < unit_v) {
+      multiply(dvs, __builtin_ldexpf(1.f, ed - unit_v));
+      unit_v = ed;
+    }
+    const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(1.f, -(ed + ev));
+    const int shift = unit - eq - 13;
+    const float p_factor = __builtin_ldexpf(1.f, unit_v - ed);
+    const bool whole = seen.covers(j0, j0 + 32);
+    const float *const of = reinterpret_cast<const float *>(at + 4 * BLOCK);
+    float p[16], ds[16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int n = 8 * q + 4 * half;
+      const f32x4 stat = *reinterpret_cast<const f32x4 *>(of + 32 * kStat + n), delta = *reinterpret_cast<const f32x4 *>(of + 32 * kDelta + n);
+      f32x4 slope = {0.f, 0.f, 0.f, 0.f}, ahead = slope;
+      if (!PLAIN && c.slopes) {
+        slope = *reinterpret_cast<const f32x4 *>(of + 32 * kSlope + n);
+        ahead = *reinterpret_cast<const f32x4 *>(of + 32 * kAhead + n);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int x = 4 * q + e;
+        float cap = 1.f;
+        p[x] = weight<PLAIN>(score, s[x], factor, PLAIN ? 0.f : slope[e] * fabsf(ahead[e] - (float)j), stat[e], cap);
+        ds[x] = p[x] * __builtin_fmaf(dp[x], d_factor, -delta[e]);
+        if (!PLAIN) ds[x] *= cap;
+        ds[x] = __builtin_ldexpf(ds[x], shift);
+        p[x] *= p_factor;
+      }
+      if (!whole) {
+        const f32x4 lo = *reinterpret_cast<const f32x4 *>(of + 32 * kLo + n), hi = *reinterpret_cast<const f32x4 *>(of + 32 * kHi + n);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool sees = j >= (int)bits_of(lo[e]) && j < (int)bits_of(hi[e]);
+          p[4 * q + e] = sees ? p[4 * q + e] : 0.f;
+          ds[4 * q + e] = sees ? ds[4 * q + e] : 0.f;
+        }
+      }
+    }
+    Weights w;
+    w.set<false>(p);
+    add_product<DP>(dvs, at + 3 * BLOCK, w);
+    w.set<true>(ds);
+    add_product<DP>(dks, low, at + 2 * BLOCK, w);
+  }
+  if (!live) return;
+  if (unit == INT32_MAX / 2) unit = 0;
+#pragma unroll
+  for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      dks[e][x] = __builtin_ldexpf(__builtin_fmaf(low[e][x], kLowUnscale, dks[e][x]), -unit);
+      dvs[e][x] = __builtin_ldexpf(dvs[e][x], -13 - unit_v);
+    }
+  const int64_t all = (int64_t)c.batch * c.tk * c.key_heads * c.dim, key = c.key_at(b, g, j);
+  float *const to_k = pieces > 1 ? parts + (int64_t)piece * 2 * all : dk, *const to_v = pieces > 1 ? parts + ((int64_t)piece * 2 + 1) * all : dv;
+  if (to_k) store_sums(dks, to_k + key, c.dim, c.scale);
+  if (to_v) store_sums(dvs, to_v + key, c.dim, 1.f);
+}
+
+// ------------------------------------------------------------------------------ host
+
+int columns_of(int dim) { return (dim + 31) / 32 * 32; }
+
+template <class F>
+void with_columns(int dim, const F &f) {
+  if (dim <= 32) f(IC<32>{});
+  else if (dim <= 64) f(IC<64>{});
+  else if (dim <= 96) f(IC<96>{});
+  else f(IC<128>{});
+}
+int blocks_of(int64_t rows) { return (int)((rows + 31) / 32); }
+
+// Scratch, handed out piece by piece on 256-byte bounds.
+struct Scratch {
+  char *at;
+  size_t used;
+  char *take(size_t bytes) {
+    char *p = at + used;
+    used += (bytes + 255) / 256 * 256;
+    return p;
+  }
+};
+
+struct Layout {
+  char *q, *d, *k, *v, *qt, *dt, *kt, *vt, *info;
+  int *eq, *ed, *ek, *ev, *edelta;
+  Hull *hulls;
+  Layout(const Call &c, bool backward, Scratch &s) {
+    const int64_t heads = (int64_t)c.batch * c.key_heads, rows = heads * blocks_of(c.rows), keys = heads * blocks_of(c.tk);
+    const size_t row_bytes = (size_t)rows * block_size(columns_of(c.dim)), key_bytes = (size_t)keys * block_size(columns_of(c.dim));
+    q = s.take(row_bytes);
+    k = s.take(key_bytes);
+    d = backward ? s.take(row_bytes) : nullptr;
+    v = backward ? s.take(key_bytes) : nullptr;
+    qt = backward ? s.take(row_bytes) : nullptr;
+    dt = backward ? s.take(row_bytes) : nullptr;
+    kt = backward ? s.take(key_bytes) : nullptr;
+    vt = backward ? nullptr : s.take(key_bytes);
+    info = backward ? s.take((size_t)rows * kInfoBytes) : nullptr;
+    eq = (int *)s.take(rows * 4);
+    ek = (int *)s.take(keys * 4);
+    ev = (int *)s.take(keys * 4);
+    ed = backward ? (int *)s.take(rows * 4) : nullptr;
+    edelta = backward ? (int *)s.take(rows * 4) : nullptr;
+    hulls = backward ? (Hull *)s.take(rows * sizeof(Hull)) : nullptr;
+  }
+};
+
+void pack(const Call &c, Pack &p, hipStream_t s) {
+  const int heads = c.batch * c.key_heads;
+  int groups = 0;
+  p.row_blocks = blocks_of(c.rows);
+  p.key_blocks = blocks_of(c.tk);
+  for (int i = 0; i < p.n_jobs; ++i) {
+    p.jobs[i].first = groups;
+    groups += heads * (p.jobs[i].of_rows ? p.row_blocks : p.key_blocks);
+  }
+  with_columns(c.dim, [&](auto dp) { hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3((unsigned)groups), dim3(kThreads), 0, s, c, p); });
+}
+
+}  // namespace
+
+bool pair_suits(const Call &c, bool backward) {
+  static const char *off = getenv("TINYFLOW_SPLIT");
+  if (off && off[0] == '0') return false;
+  const float factor = c.cap > 0.f ? c.scale / c.cap : c.scale;
+  if (c.dim > 128 || !(factor > 0x1p-40f && factor < 0x1p40f)) return false;
+  if (c.rows < 32 || c.tk < 32) return false;
+  // the planes are written by one launch, a block a workgroup
+  if ((int64_t)c.batch * c.key_heads * (blocks_of(c.rows) + (int64_t)blocks_of(c.tk)) * 2 >= 1 << 24) return false;
+  return true;
+}
+
+size_t pair_bytes(const Call &c, bool backward) {
+  Scratch s = {nullptr, 0};
+  Layout l(c, backward, s);
+  return s.used;
+}
+
+Exponents pair_forward(const Call &c, float *out, float *stat, const Pieces &pieces, int tiles, char *scratch, hipStream_t s) {
+  Scratch of = {scratch, 0};
+  const Layout l(c, false, of);
+  Pack p = {};
+  p.n_jobs = 3;
+  p.jobs[0] = Job{c.q, true, 1.f, l.q, nullptr, l.eq, 0};
+  p.jobs[1] = Job{c.k, false, 1.f, l.k, nullptr, l.ek, 0};
+  p.jobs[2] = Job{c.v, false, 1.f, nullptr, l.vt, l.ev, 0};
+  pack(c, p, s);
+  const Exponents ex = {l.eq, nullptr, l.ek, l.ev, nullptr, p.row_blocks, p.key_blocks};
+  const unsigned groups = (unsigned)((int64_t)c.batch * c.key_heads * tiles * pieces.count);
+  const bool plain = !c.slopes && c.cap == 0.f;
+  with_columns(c.dim, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    hipLaunchKernelGGL((plain ? forward_kernel<DP, true> : forward_kernel<DP, false>), dim3(groups), dim3(kThreads), 0, s, c, l.q, l.k, l.vt, ex, out, stat, pieces, tiles);
+  });
+  return ex;
+}
+
+Exponents pair_backward(const Call &c, const float *dout, const Row *rows, float *dq, float *dk, float *dv, float *parts, int row_tiles, int key_tiles,
+                        int pieces, char *scratch, hipStream_t s) {
+  Scratch of = {scratch, 0};
+  const Layout l(c, true, of);
+  Pack p = {};
+  p.n_jobs = 4;
+  const bool keys = dk || dv;
+  p.jobs[0] = Job{c.q, true, kLowScale, l.q, keys ? l.qt : nullptr, l.eq, 0};
+  p.jobs[1] = Job{dout, true, 1.f, l.d, keys ? l.dt : nullptr, l.ed, 0};
+  p.jobs[2] = Job{c.k, false, kLowScale, l.k, dq ? l.kt : nullptr, l.ek, 0};
+  p.jobs[3] = Job{c.v, false, 1.f, l.v, nullptr, l.ev, 0};
+  p.rows = rows;
+  p.info = (float *)l.info;
+  p.hulls = l.hulls;
+  p.delta_exponents = l.edelta;
+  pack(c, p, s);
+  const Exponents ex = {l.eq, l.ed, l.ek, l.ev, l.hulls, p.row_blocks, p.key_blocks};
+  const bool plain = !c.slopes && c.cap == 0.f;
+  const int heads = c.batch * c.key_heads;
+  with_columns(c.dim, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    if (dq)
+      hipLaunchKernelGGL((plain ? dq_kernel<DP, true> : dq_kernel<DP, false>), dim3((unsigned)(heads * row_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.k, l.v, l.kt, ex,
+                         rows, l.edelta, dq, row_tiles);
+    if (keys)
+      hipLaunchKernelGGL((plain ? dkv_kernel<DP, true> : dkv_kernel<DP, false>), dim3((unsigned)(heads * key_tiles * pieces)), dim3(kThreads), 0, s, c, l.q, l.d, l.qt, l.dt,
+                         l.k, l.v, ex, l.info, l.edelta, dk, dv, parts, key_tiles, pieces);
+  });
+  return ex;
+}
+
+}  // namespace attention
+}  // namespace tf
