@@ -135,14 +135,15 @@ struct Hull {
     inner_lo = __builtin_amdgcn_readfirstlane(inner_lo);
     inner_hi = __builtin_amdgcn_readfirstlane(inner_hi);
   }
-  // over the four waves, through `room`
-  __device__ inline Hull all(int (*room)[4]) const {
+  // over a workgroup's waves, through `room`
+  template <int WAVES>
+  __device__ inline Hull all(int (&room)[WAVES][4]) const {
     const int wave = threadIdx.x / 64;
     if (threadIdx.x % 64 == 0) room[wave][0] = lo, room[wave][1] = hi, room[wave][2] = inner_lo, room[wave][3] = inner_hi;
     __syncthreads();
     Hull h = *this;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       h.lo = min(h.lo, room[w][0]);
       h.hi = max(h.hi, room[w][1]);
       h.inner_lo = max(h.inner_lo, room[w][2]);
@@ -227,7 +228,7 @@ struct Exponents {
   __device__ static inline bool bad(const int *of, int64_t head, int blocks, int first, int n) {
     bool found = false;
     if (of)
-      for (int e = threadIdx.x; e < n; e += kThreads) found |= first + e < blocks && of[head * blocks + first + e] == kBad;
+      for (int e = threadIdx.x; e < n; e += blockDim.x) found |= first + e < blocks && of[head * blocks + first + e] == kBad;
     return found;
   }
   __device__ inline bool bad_rows(int64_t head, int first, int n) const { return bad(q, head, row_blocks, first, n) | bad(d, head, row_blocks, first, n); }
@@ -235,7 +236,7 @@ struct Exponents {
   // of the blocks of rows that see one of the keys [from, to)
   __device__ inline bool bad_rows_of(int64_t head, int from, int to) const {
     bool found = false;
-    for (int e = threadIdx.x; e < row_blocks; e += kThreads) {
+    for (int e = threadIdx.x; e < row_blocks; e += blockDim.x) {
       const int64_t at = head * row_blocks + e;
       found |= (q[at] == kBad || d[at] == kBad) && hulls[at].meets(from, to);
     }
@@ -248,9 +249,9 @@ struct Exponents {
 bool pair_suits(const Call &c, bool backward);
 size_t pair_bytes(const Call &c, bool backward);  // of scratch
 Exponents pair_forward(const Call &c, float *out, float *stat, const Pieces &pieces, int tiles, char *scratch, hipStream_t s);
-// dq (unless null), dk and dv (unless both are); `parts` as dkv_kernel takes them
-Exponents pair_backward(const Call &c, const float *dout, const Row *rows, float *dq, float *dk, float *dv, float *parts, int row_tiles, int key_tiles,
-                        int pieces, char *scratch, hipStream_t s);
+// Also what prepare_kernel writes to `rows`; dq (unless null), dk and dv (unless both are); `parts` as dkv_kernel takes them
+Exponents pair_backward(const Call &c, const float *out, const float *stat, const float *dout, Row *rows, float *dq, float *dk, float *dv, float *parts,
+                        int row_tiles, int key_tiles, int pieces, char *scratch, hipStream_t s);
 
 }  // namespace attention
 }  // namespace tf

@@ -171,14 +171,14 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
   int lo, hi;
   c.seen(b, i, lo, hi);
   const float slope = c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
-  Operand<DP> q;
-  q.load(c.q + c.query_at(b, g, live ? r : 0), c.dim, live);
   Hull mine;
   mine.of(lo, hi, live);
   const Hull all = mine.all(room);
   // this piece's steps of the keys that any of the rows sees
   const int first = all.first(), steps = all.steps();
   if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), kRows / 32) | left.bad_keys(bg, first, steps))) return;
+  Operand<DP> q;
+  q.load(c.q + c.query_at(b, g, live ? r : 0), c.dim, live);
   const int begin = first + (int)((int64_t)steps * piece / pieces.count), end = first + (int)((int64_t)steps * (piece + 1) / pieces.count);
   const Score score(c);
   Sum<DP> o;
@@ -451,57 +451,81 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Call c, float *out,
   }
 }
 
-// Rows of all from their pieces, in the pieces' order: a row to W waves, each with a run of the pieces.
+// Rows of all from their pieces, in the pieces' order: a row to W waves, each with a run of the pieces.  The pieces' factors are in LDS before their
+// sums are read, eight loads of a lane under way: with each sum behind the branch on its mark 512 pieces of 16 rows of 128 took 44 us.
+constexpr int kMostPieces = 2048;
 template <int W>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void join_kernel(const Call c, const Pieces pieces, float *out, float *stat) {
-  constexpr int ROWS = W > 4 ? 1 : 4 / W;
-  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, sub = wave % W;
+  constexpr int ROWS = W > 4 ? 1 : 4 / W, LANES = 64 * W, MOST = 4, UNDER_WAY = 8;  // MOST: columns of a lane
+  __shared__ float by[ROWS][W > 1 ? kMostPieces : 16];
+  __shared__ float parts[W > 1 ? W : 1][MOST][64];
+  __shared__ float tops[W], totals[W];
+  const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, sub = wave % W, own = threadIdx.x % LANES;
   const int64_t row = (int64_t)blockIdx.x * ROWS + wave / W;
-  if (W <= 1 && row >= pieces.rows) return;
-  const int64_t at = row < pieces.rows ? row : pieces.rows - 1;
-  float top = kNone;
-  for (int p = lane; p < pieces.count; p += 64) top = fmaxf(top, pieces.marks[p * pieces.rows + at].x);
+  if (row >= pieces.rows) return;  // with one wave a row
+  float *const weights = by[wave / W];
+  float top = kNone, total = 0.f;
+  for (int p = own; p < pieces.count; p += LANES) top = fmaxf(top, pieces.marks[p * pieces.rows + row].x);
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) top = fmaxf(top, __shfl_xor(top, step));
+  if constexpr (W > 1) {
+    if (lane == 0) tops[sub] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < W; ++w) top = fmaxf(top, tops[w]);
+  }
   const float from = top == kNone ? 0.f : top;
-  float total = 0.f;
-  for (int p = lane; p < pieces.count; p += 64) {
-    const float2 mark = pieces.marks[p * pieces.rows + at];
-    total += mark.y * __builtin_amdgcn_exp2f(mark.x - from);
+  for (int p = own; p < pieces.count; p += LANES) {
+    const float2 mark = pieces.marks[p * pieces.rows + row];
+    const float factor = __builtin_amdgcn_exp2f(mark.x - from);
+    total += mark.y * factor;
+    weights[p] = mark.y == 0.f ? 0.f : factor;  // nothing seen: nothing stored that counts
   }
 #pragma unroll
   for (int step = 1; step < 64; step *= 2) total += __shfl_xor(total, step);
-  const int each = (pieces.count + W - 1) / W, begin = min(pieces.count, sub * each), end = min(pieces.count, begin + each);
-  constexpr int MOST = 4;  // columns of a lane
-  float sum[MOST] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int p = begin; p < end; ++p) {
-    const float2 mark = pieces.marks[p * pieces.rows + at];
-    if (mark.y == 0.f) continue;  // nothing seen: nothing stored that counts
-    const float by = __builtin_amdgcn_exp2f(mark.x - from);
-    const float *from_row = pieces.sums + (p * pieces.rows + at) * c.dim;
+  if constexpr (W > 1) {
+    if (lane == 0) totals[sub] = total;
+    __syncthreads();
+    total = 0.f;
 #pragma unroll
-    for (int e = 0; e < MOST; ++e)
-      if (lane + 64 * e < c.dim) sum[e] += from_row[lane + 64 * e] * by;
+    for (int w = 0; w < W; ++w) total += totals[w];
+  } else {
+    __builtin_amdgcn_wave_barrier();
+  }
+  const int each = (pieces.count + W - 1) / W, begin = min(pieces.count, sub * each), end = min(pieces.count, begin + each);
+  float sum[MOST] = {0.f, 0.f, 0.f, 0.f};
+  for (int p0 = begin; p0 < end; p0 += UNDER_WAY) {
+#pragma unroll
+    for (int e = 0; e < MOST; ++e) {
+      if (64 * e >= c.dim) break;
+      float v[UNDER_WAY];
+#pragma unroll
+      for (int u = 0; u < UNDER_WAY; ++u)
+        v[u] = pieces.sums[((int64_t)min(p0 + u, end - 1) * pieces.rows + row) * c.dim + min(lane + 64 * e, c.dim - 1)];
+#pragma unroll
+      for (int u = 0; u < UNDER_WAY; ++u) {
+        const float factor = p0 + u < end ? weights[p0 + u] : 0.f;
+        sum[e] += factor != 0.f ? v[u] * factor : 0.f;
+      }
+    }
   }
   if constexpr (W > 1) {
-    __shared__ float parts[ROWS][W][MOST][64];
 #pragma unroll
-    for (int e = 0; e < MOST; ++e) parts[wave / W][sub][e][lane] = sum[e];
+    for (int e = 0; e < MOST; ++e) parts[sub][e][lane] = sum[e];
     __syncthreads();
-    if (sub > 0 || row >= pieces.rows) return;
+    if (sub > 0) return;
 #pragma unroll
     for (int e = 0; e < MOST; ++e)
-      for (int w = 1; w < W; ++w) sum[e] += parts[wave / W][w][e][lane];
+      for (int w = 1; w < W; ++w) sum[e] += parts[w][e][lane];
   }
   const int r = (int)(row % c.rows), g = (int)(row / c.rows % c.key_heads), b = (int)(row / c.rows / c.key_heads);
   if (stat && lane == 0) stat[c.stat_at(b, g, r)] = total == 0.f ? kNone : (top + __builtin_amdgcn_logf(total)) * kLn2;
   if (!out) return;
-  const float by = total == 0.f ? 0.f : 1.f / total;
+  const float scale = total == 0.f ? 0.f : 1.f / total;
   float *to = out + c.query_at(b, g, r);
 #pragma unroll
   for (int e = 0; e < MOST; ++e)
-    if (lane + 64 * e < c.dim) to[lane + 64 * e] = sum[e] * by;
+    if (lane + 64 * e < c.dim) to[lane + 64 * e] = sum[e] * scale;
 }
 
 // ------------------------------------------------------------------------------ backward
@@ -540,14 +564,14 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
   const int ahead = (live ? r : 0) / c.group + c.tk - c.tq;
   const float slope = c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
   const int64_t at = c.query_at(b, g, live ? r : 0);
-  Operand<DP> q, d;
-  q.load(c.q + at, c.dim, live);
-  d.load(dout + at, c.dim, live);
   Hull mine;
   mine.of(row.lo, row.hi, live);
   const Hull all = mine.all(room);
   const int begin = all.first(), end = begin + all.steps();
   if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), kRows / 32) | left.bad_keys(bg, begin, end - begin))) return;
+  Operand<DP> q, d;
+  q.load(c.q + at, c.dim, live);
+  d.load(dout + at, c.dim, live);
   const Score score(c);
   Sum<DP> sum;
   sum.zero();
@@ -755,7 +779,7 @@ void with_columns(int dim, const F &f) {
 // Pieces of rows_kernel along the keys: as many as it takes for two workgroups a CU, of 256 keys at least.
 int row_pieces(const Call &c, int64_t groups) {
   if (groups == 0) return 1;
-  const int64_t wanted = (2 * num_cus() + groups - 1) / groups, most = std::max(1, c.tk / 256);
+  const int64_t wanted = (2 * num_cus() + groups - 1) / groups, most = std::min(kMostPieces, std::max(1, c.tk / 256));
   return (int)std::min<int64_t>(wanted, most);
 }
 
@@ -787,7 +811,7 @@ extern "C" int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHan
   pieces.rows = all_rows;
   if (few) {
     // about four workgroups a CU; a wave's share of a piece is a multiple of its step
-    const int64_t wanted = std::max<int64_t>(1, (4 * num_cus() + head_pairs - 1) / head_pairs);
+    const int64_t wanted = std::min<int64_t>(kMostPieces, std::max<int64_t>(1, (4 * num_cus() + head_pairs - 1) / head_pairs));
     keys_a_piece = std::max<int>(64, (int)(((c.tk + wanted - 1) / wanted + 63) / 64 * 64));
     pieces.count = std::max(1, (c.tk + keys_a_piece - 1) / keys_a_piece);
     groups = head_pairs * pieces.count;
@@ -881,10 +905,10 @@ extern "C" int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHa
   Row *rows = (Row *)(block + planes + part_bytes);
   const float *dout = (const float *)doutput->data;
   float *dk = dkey ? (float *)dkey->data : nullptr, *dv = dvalue ? (float *)dvalue->data : nullptr;
-  if (all_rows)
+  if (all_rows && !pairs)
     hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)((all_rows + 3) / 4)), dim3(kThreads), 0, s, c, (const float *)output->data,
                        (const float *)statistics->data, dout, rows, all_rows);
-  const Exponents left = pairs ? pair_backward(c, dout, rows, dquery ? (float *)dquery->data : nullptr, dk, dv, parts, row_tiles, key_tiles, pieces, block, s)
+  const Exponents left = pairs ? pair_backward(c, (const float *)output->data, (const float *)statistics->data, dout, rows, dquery ? (float *)dquery->data : nullptr, dk, dv, parts, row_tiles, key_tiles, pieces, block, s)
                                : Exponents{};
   with_columns(c.dim, [&](auto columns) {
     constexpr int DP = decltype(columns)::value;

@@ -15,6 +15,7 @@
 // that nothing sees are packed as zeros, whatever they hold.
 #include "attention.h"
 #include "internal.h"
+#include "lanes.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -45,6 +46,7 @@ constexpr int kInfoBytes = 1024;  // of a block of rows: eight arrays of 32, see
 constexpr float kLowScale = 0x1p11f, kLowUnscale = 0x1p-11f;
 constexpr int kSmallest = 110;   // exponents above it stand for values that no sum notices
 constexpr int kLargest = -40;
+constexpr int kNoUnit = INT32_MAX / 2;  // of a sum of nothing
 
 // Bytes of a block of 32 rows: DP columns of h and l.
 __host__ __device__ constexpr int64_t block_size(int dp) { return dp * 128; }
@@ -59,7 +61,6 @@ enum Info { kStat = 0, kDelta, kLo, kHi, kSlope, kAhead };
 struct Job {
   const float *src;
   bool of_rows;
-  float low;         // factor of l in the transposed form
   char *plain, *transposed;
   int *exponents;
   int first;         // workgroup
@@ -67,10 +68,11 @@ struct Job {
 struct Pack {
   Job jobs[4];
   int n_jobs, row_blocks, key_blocks;
-  const Row *rows;   // backward: of all rows
-  float *info;       // backward: [b, key head][block of rows][8][32]
+  // backward, by job 1, the gradients of the output:
+  const float *out, *stat;
+  Row *rows;         // of all
+  float *info;       // [b, key head][block of rows][8][32]
   Hull *hulls;
-  int *delta_exponents;  // |delta| of the block is below 2^this
 };
 
 __device__ inline void split(float x, float low, _Float16 &h, _Float16 &l) {
@@ -94,10 +96,8 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
   bool used;
   Row info = {0.f, 0.f, 0, 0};
   if (job.of_rows) {
-    used = n < c.rows;
-    if (used && p.rows) info = p.rows[(int64_t)head * c.rows + n];
-    else if (used) c.seen(b, n / c.group, info.lo, info.hi);
-    used = used && info.lo < info.hi;
+    if (n < c.rows) c.seen(b, n / c.group, info.lo, info.hi);
+    used = info.lo < info.hi;
   } else {
     // keys that any query sees lie between the first and the last of them
     int lo = 0, hi = c.tk;
@@ -142,35 +142,44 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
   int exponent = min(kSmallest, 141 - field);
   if (largest >= 0x7f800000u || exponent < kLargest || (!job.of_rows && largest && (int)(least >> 23) < field - 16 && exponent < kSmallest)) exponent = kBad;
   if (tid == 0) job.exponents[(int64_t)head * blocks + block] = exponent;
-  if (job.of_rows && p.info && which == 0) {  // what the backward kernels read of the rows
-    const int64_t of_block = (int64_t)head * blocks + block;
+  if (p.info && which == 1) {  // what the backward kernels read of the rows
+    __shared__ Row of_rows[32];
+    float delta = 0.f;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e) {
+      const int col = 32 * e + tid % 8 * 4;
+      if (!used || col >= c.dim) continue;
+      const f32x4 o = load4(p.out + (src - job.src) + col, c.dim - col);
+      delta += (x[e][0] * o[0] + x[e][1] * o[1]) + (x[e][2] * o[2] + x[e][3] * o[3]);
+    }
+    delta = lanes::sum_over<8>(delta);
+    if (tid % 8 == 0) {
+      if (used) info.stat = p.stat[c.stat_at(b, g, n)] * kLog2e;
+      if (!used || info.stat == kNone) info = Row{0.f, 0.f, 0, 0};
+      else info.delta = delta;
+      if (n < c.rows) p.rows[(int64_t)head * c.rows + n] = info;
+      of_rows[row] = info;
+    }
+    __syncthreads();
     if (tid < 64) {
       const int r = block * 32 + tid % 32;
-      const bool is = r < c.rows;
-      Row mine = {0.f, 0.f, 0, 0};
-      if (is) mine = p.rows[(int64_t)head * c.rows + r];
-      if (mine.lo >= mine.hi) mine.stat = mine.delta = 0.f;
+      const Row mine = of_rows[tid % 32];
       Hull seen;
-      seen.of(mine.lo, mine.hi, is);
+      seen.of(mine.lo, mine.hi, true);
       if (seen.lo >= seen.hi) seen.lo = seen.hi = 0;
       // rows that see nothing, or that are none, keep the block from covering anything
       if (__any(mine.lo >= mine.hi)) seen.inner_lo = INT32_MAX, seen.inner_hi = 0;
-      uint32_t delta = bits_of(mine.delta) & 0x7fffffffu;
-#pragma unroll
-      for (int step = 1; step < 32; step *= 2) delta = max(delta, (uint32_t)__shfl_xor((int)delta, step));
+      const int64_t of_block = (int64_t)head * blocks + block;
       if (tid < 32) {
         float *to = p.info + of_block * (kInfoBytes / 4) + tid;
         to[32 * kStat] = mine.stat;
         to[32 * kDelta] = mine.delta;
         to[32 * kLo] = __builtin_bit_cast(float, mine.lo);
         to[32 * kHi] = __builtin_bit_cast(float, mine.hi);
-        to[32 * kSlope] = c.slopes && is ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
+        to[32 * kSlope] = c.slopes && r < c.rows ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
         to[32 * kAhead] = (float)(r / c.group + c.tk - c.tq);
       }
-      if (tid == 0) {
-        p.hulls[of_block] = seen;
-        p.delta_exponents[of_block] = (int)(delta >> 23) - 126;
-      }
+      if (tid == 0) p.hulls[of_block] = seen;
     }
   }
   if (exponent == kBad) return;
@@ -206,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         _Float16 a, d;
-        split(tile[16 * t + key_of(e, half)][col], job.low, a, d);
+        split(tile[16 * t + key_of(e, half)][col], 1.f, a, d);
         h[e] = a;
         l[e] = d;
       }
@@ -266,7 +275,6 @@ __device__ __forceinline__ f32x16 product(const char *block, const Held<DP> &b) 
 // 16 values of a tile as the other operand of a product over its rows.
 struct Weights {
   f16x8 h[2], l[2];
-  template <bool SCALED>
   __device__ __forceinline__ void set(const float (&w)[16]) {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
@@ -274,11 +282,9 @@ struct Weights {
       for (int e = 0; e < 8; e += 2) {
         const f32x2 x = {w[8 * t + e], w[8 * t + e + 1]};
         const f16x2 top = __builtin_convertvector(x, f16x2);
-        // x - h is a number of 32 bits, and so is 2^11 times that
         f32x2 left;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          left[i] = SCALED ? __builtin_fmaf((float)top[i], -kLowScale, x[i] * kLowScale) : __builtin_fmaf((float)top[i], -1.f, x[i]);
+        for (int i = 0; i < 2; ++i) left[i] = x[i] - (float)top[i];
         const f16x2 rest = __builtin_convertvector(left, f16x2);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -289,7 +295,7 @@ struct Weights {
   }
 };
 
-// sum[d] += of a transposed block with l as it is
+// sum[d] += of a transposed block
 template <int DP>
 __device__ __forceinline__ void add_product(f32x16 (&sum)[DP / 32], const char *block, const Weights &w) {
   const char *at = block + threadIdx.x % 64 * 16;
@@ -301,20 +307,6 @@ __device__ __forceinline__ void add_product(f32x16 (&sum)[DP / 32], const char *
       sum[d] = mfma(l, w.h[t], sum[d]);
       sum[d] = mfma(h, w.l[t], sum[d]);
       sum[d] = mfma(h, w.h[t], sum[d]);
-    }
-}
-// the same with both l scaled: their products have sums of their own
-template <int DP>
-__device__ __forceinline__ void add_product(f32x16 (&sum)[DP / 32], f32x16 (&low)[DP / 32], const char *block, const Weights &w) {
-  const char *at = block + threadIdx.x % 64 * 16;
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const f16x8 h = fragment(at + (2 * d + t) * 2 * kFragment), l = fragment(at + ((2 * d + t) * 2 + 1) * kFragment);
-      low[d] = mfma(l, w.h[t], low[d]);
-      sum[d] = mfma(h, w.h[t], sum[d]);
-      low[d] = mfma(h, w.l[t], low[d]);
     }
 }
 template <int N>
@@ -345,10 +337,11 @@ __device__ inline int scalar(const int *p) { return *(const __attribute__((addre
 __device__ inline float unscaled(float factor, int a, int b) { return __builtin_ldexpf(factor, max(-(a + b), -80)); }
 
 
-// Fetches block `index` of each of N operands, one behind the other in LDS from `to` on, a wave every fourth fragment.
+// Fetches block `index` of each of N operands, one behind the other in LDS from `to` on, each of four waves every fourth
+// fragment.
 template <int DP, int N>
 __device__ __forceinline__ void fetch_blocks(uint32_t to, const char *const (&of)[N], int64_t index) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % 4);
   static_for<N>([&](auto n) {
     const char *from = uniform(of[decltype(n)::value] + index * block_size(DP)) + wave * kFragment;
 #pragma unroll
@@ -358,17 +351,22 @@ __device__ __forceinline__ void fetch_blocks(uint32_t to, const char *const (&of
 
 // ------------------------------------------------------------------------------ forward
 
-// 128 rows a workgroup, 32 a wave; steps of 32 keys, the next one on its way into LDS while one is worked on.  PLAIN: neither cap nor bias.
+// 128 rows a workgroup, of two groups of four waves with 32 rows each: one group takes the even steps of 32 keys, one the odd ones, and the
+// second's sums join the first's through LDS at the end.  While a step is worked on the next one is on its way into LDS.  Two waves a SIMD then
+// belong to one workgroup, which takes half as long, and a causal pass, whose workgroups differ as the rows do, ends with
+// light ones on every CU.  PLAIN: neither cap nor bias.
 template <int DP, bool PLAIN>
-__global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Call c, const char *qs, const char *ks, const char *vs, const Exponents ex, float *out,
-                                                              float *stat, const Pieces pieces, int tiles) {
+__global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel(const Call c, const char *qs, const char *ks, const char *vs, const Exponents ex,
+                                                                                 float *out, float *stat, const Pieces pieces, int tiles) {
   constexpr int BLOCK = (int)block_size(DP);
-  __shared__ __align__(16) char lds[2][2 * BLOCK];
-  __shared__ int room[4][4];
+  __shared__ __align__(16) char lds[2][2][2 * BLOCK];  // [parity][group]
+  __shared__ int room[8][4];
+  __shared__ float marks[2][kRows];
   const int heads = c.batch * c.key_heads;
   const int bg = (int)blockIdx.x % heads, rest = (int)blockIdx.x / heads;
   const int b = bg / c.key_heads, g = bg % c.key_heads, tile = tiles - 1 - rest % tiles, piece = rest / tiles;
-  const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % 4);
+  const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
   const int r = tile * kRows + wave * 32 + lane % 32;
   const bool live = r < c.rows;
   const int i = (live ? r : c.rows - 1) / c.group, ahead = i + c.tk - c.tq;
@@ -376,7 +374,7 @@ __global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Call c, cons
   c.seen(b, i, lo, hi);
   Hull mine;
   mine.of(lo, hi, live);
-  const Hull all = mine.all(room);
+  const Hull all = mine.all(room);  // the second group's waves have the first's rows
   const int first = all.first(), steps = all.steps();
   if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32) | ex.bad_keys(bg, first, steps))) return;
   const int begin = first + (int)((int64_t)steps * piece / pieces.count), end = first + (int)((int64_t)steps * (piece + 1) / pieces.count);
@@ -394,16 +392,17 @@ __global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Call c, cons
   float top = kNone, total = 0.f;   // total times 2^12
   int unit = kSmallest;             // o is times 2^(12 + unit)
   const char *const from[2] = {ks, vs};
-  const uint32_t to = lds_address(&lds[0][0]);
-  if (begin < end) fetch_blocks<DP, 2>(to, from, key_block + begin);
+  const uint32_t to = lds_address(&lds[0][group][0]);
+  if (begin + group < end) fetch_blocks<DP, 2>(to, from, key_block + begin + group);
+  int parity = 0;
 #pragma unroll 1
-  for (int step = begin; step < end; ++step) {
-    const int slot = (step - begin) & 1, j0 = step * kKeys;
-    const int ek = scalar(ex.k + key_block + step), ev = scalar(ex.v + key_block + step);
+  for (int pair = begin; pair < end; pair += 2, parity ^= 1) {
+    const int step = pair + group, j0 = step * kKeys;
     arrived();
-    if (step + 1 < end) fetch_blocks<DP, 2>(to + (uint32_t)((1 - slot) * 2 * BLOCK), from, key_block + step + 1);
-    if (!mine.meets(j0, j0 + kKeys)) continue;
-    const char *const keys = lds[slot], *const values = lds[slot] + BLOCK;
+    if (step + 2 < end) fetch_blocks<DP, 2>(to + (uint32_t)((1 - parity) * 4 * BLOCK), from, key_block + step + 2);
+    if (step >= end || !mine.meets(j0, j0 + kKeys)) continue;
+    const int ek = scalar(ex.k + key_block + step), ev = scalar(ex.v + key_block + step);
+    const char *const keys = lds[parity][group], *const values = keys + BLOCK;
     const f32x16 s = product<DP>(keys, q);
     const float factor = unscaled(score.factor, eq, ek);
     const bool whole = mine.covers(j0, j0 + kKeys);
@@ -453,26 +452,49 @@ __global__ __launch_bounds__(kThreads, 2) void forward_kernel(const Call c, cons
 #pragma unroll
       for (int v = 0; v < 16; ++v) p[v] = __builtin_ldexpf(p[v], apart - near);
     Weights w;
-    w.set<false>(p);
+    w.set(p);
     add_product<DP>(o, values, w);
   }
-  if (!live) return;
   total = (total + other_half(total)) * 0x1p-12f;
-  float *row;
-  const float by = row_end(c, pieces, out, stat, b, g, r, piece, top, total, half == 0, row);
-  if (row) {
-    multiply(o, __builtin_ldexpf(1.f, -12 - unit));
-    store_sums(o, row, c.dim, by);
+  multiply(o, __builtin_ldexpf(1.f, -12 - unit));
+  // the second group's rows to the first
+  __syncthreads();
+  f32x4 *const room_o = reinterpret_cast<f32x4 *>(&lds[0][0][0]) + wave * (DP / 8 * 64);
+  if (group == 1) {
+    if (half == 0) {
+      marks[0][wave * 32 + lane] = top;
+      marks[1][wave * 32 + lane] = total;
+    }
+#pragma unroll
+    for (int e = 0; e < DP / 8; ++e)
+      room_o[e * 64 + lane] = f32x4{o[e / 4][e % 4 * 4], o[e / 4][e % 4 * 4 + 1], o[e / 4][e % 4 * 4 + 2], o[e / 4][e % 4 * 4 + 3]};
   }
+  __syncthreads();
+  if (group == 1 || !live) return;
+  const float other_top = marks[0][wave * 32 + lane % 32], other_total = marks[1][wave * 32 + lane % 32];
+  const float joined = fmaxf(top, other_top), base = joined == kNone ? 0.f : joined;
+  const float mine_by = __builtin_amdgcn_exp2f(top - base), other_by = __builtin_amdgcn_exp2f(other_top - base);
+  total = total * mine_by + other_total * other_by;
+#pragma unroll
+  for (int e = 0; e < DP / 8; ++e) {
+    const f32x4 x = room_o[e * 64 + lane];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) o[e / 4][e % 4 * 4 + n] = o[e / 4][e % 4 * 4 + n] * mine_by + x[n] * other_by;
+  }
+  float *row;
+  const float by = row_end(c, pieces, out, stat, b, g, r, piece, joined, total, half == 0, row);
+  if (row) store_sums(o, row, c.dim, by);
 }
 
 // ------------------------------------------------------------------------------ backward
 
-// |dp - delta| of a tile is below 2^this: a product of DP columns of less than 2^15 each, and delta, of which one more bit is a sum.
-template <int DP>
-__device__ inline int gradient_exponent(int ed, int ev, int delta) {
-  constexpr int LOG = DP <= 32 ? 5 : DP <= 64 ? 6 : 7;
-  return max(LOG + 30 - ed - ev, delta) + 1;
+// The exponent that brings the tile's largest gradient to 2^13 or below 2^14; that of a sum so far, `unit` less `other`, unless it is smaller.
+__device__ __forceinline__ int gradient_unit(const float (&ds)[16], int other, int unit) {
+  float most = 0.f;
+#pragma unroll
+  for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(ds[v]));
+  const int field = __builtin_amdgcn_readfirstlane((int)(lanes::largest<64>(bits_of(most)) >> 23));
+  return field == 0 || field == 255 ? unit : min(unit, 140 - field + other);
 }
 
 // p times 2^13 (0 where a mask says so) and the derivative of the cap, from a product.
@@ -492,7 +514,7 @@ __device__ __forceinline__ float weight(const Score &score, float product, float
 // 128 rows a workgroup, as forward_kernel; in LDS a step's keys, values and keys transposed.
 template <int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Call c, const char *qs, const char *ds_, const char *ks, const char *vs, const char *kts,
-                                                                        const Exponents ex, const Row *rows, const int *delta_exponents, float *dq, int tiles) {
+                                                                        const Exponents ex, const Row *rows, float *dq, int tiles) {
   constexpr int BLOCK = (int)block_size(DP);
   __shared__ __align__(16) char lds[2][3 * BLOCK];
   __shared__ int room[4][4];
@@ -511,7 +533,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
   if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32) | ex.bad_keys(bg, begin, end - begin))) return;
   const int block = min(tile * (kRows / 32) + wave, ex.row_blocks - 1);
   const int64_t row_block = (int64_t)bg * ex.row_blocks + block, key_block = (int64_t)bg * ex.key_blocks;
-  const int eq = scalar(ex.q + row_block), ed = scalar(ex.d + row_block), edelta = scalar(delta_exponents + row_block);
+  const int eq = scalar(ex.q + row_block), ed = scalar(ex.d + row_block);
   const float slope = !PLAIN && c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
   // a row that sees nothing has whatever statistic
   const bool some = live && row.lo < row.hi;
@@ -522,10 +544,10 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
   q.wait();
   d.wait();
   const Score score(c);
-  f32x16 sum[DP / 32], low[DP / 32];
+  f32x16 sum[DP / 32];
 #pragma unroll
-  for (int e = 0; e < DP / 32; ++e) sum[e] = low[e] = zeros();
-  int unit = INT32_MAX / 2;  // sum is times 2^unit
+  for (int e = 0; e < DP / 32; ++e) sum[e] = zeros();
+  int unit = kNoUnit;  // sum is times 2^unit
   const char *const from[3] = {ks, vs, kts};
   const uint32_t to = lds_address(&lds[0][0]);
   if (begin < end) fetch_blocks<DP, 3>(to, from, key_block + begin);
@@ -537,27 +559,15 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
     if (step + 1 < end) fetch_blocks<DP, 3>(to + (uint32_t)((1 - slot) * 3 * BLOCK), from, key_block + step + 1);
     if (!mine.meets(j0, j0 + kKeys)) continue;
     const f32x16 s = product<DP>(lds[slot], q), dp = product<DP>(lds[slot] + BLOCK, d);
-    const int new_unit = min(unit, 14 - gradient_exponent<DP>(ed, ev, edelta) + ek);
-    if (new_unit < unit) {
-      if (step > begin) {
-        const float by = __builtin_ldexpf(1.f, new_unit - unit);
-        multiply(sum, by);
-        multiply(low, by);
-      }
-      unit = new_unit;
-    }
     const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(1.f, -(ed + ev));
-    const int shift = unit - ek - 13;  // of ds, from p times 2^13
     const bool whole = mine.covers(j0, j0 + kKeys);
     float ds[16];
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
-      const int j = j0 + key_of(v, half);
       float cap = 1.f;
-      const float p = weight<PLAIN>(score, s[v], factor, PLAIN ? 0.f : slope * fabsf((float)(ahead - j)), stat, cap);
+      const float p = weight<PLAIN>(score, s[v], factor, PLAIN ? 0.f : slope * fabsf((float)(ahead - (j0 + key_of(v, half)))), stat, cap);
       ds[v] = p * __builtin_fmaf(dp[v], d_factor, -delta);
       if (!PLAIN) ds[v] *= cap;
-      ds[v] = __builtin_ldexpf(ds[v], shift);
     }
     if (!whole)
 #pragma unroll
@@ -565,23 +575,30 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
         const int j = j0 + key_of(v, half);
         ds[v] = j >= row.lo && j < row.hi ? ds[v] : 0.f;
       }
+    const int new_unit = gradient_unit(ds, ek, unit);
+    if (new_unit < unit) {
+      multiply(sum, __builtin_ldexpf(1.f, max(new_unit - unit, -200)));
+      unit = new_unit;
+    }
+    if (unit == kNoUnit) continue;  // nothing but zeros so far
+#pragma unroll
+    for (int v = 0; v < 16; ++v) ds[v] = __builtin_ldexpf(ds[v], unit - ek);
     Weights w;
-    w.set<true>(ds);
-    add_product<DP>(sum, low, lds[slot] + 2 * BLOCK, w);
+    w.set(ds);
+    add_product<DP>(sum, lds[slot] + 2 * BLOCK, w);
   }
   if (!live) return;
-  if (begin >= end) unit = 0;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) sum[e][v] = __builtin_ldexpf(__builtin_fmaf(low[e][v], kLowUnscale, sum[e][v]), -unit);
+    for (int v = 0; v < 16; ++v) sum[e][v] = unit == kNoUnit ? 0.f : __builtin_ldexpf(sum[e][v], -13 - unit);
   store_sums(sum, dq + c.query_at(b, g, r), c.dim, c.scale);
 }
 
 // 128 keys a workgroup, 32 a wave; steps of 32 rows: in LDS queries, gradients, both transposed, and what Info says of the rows.
 template <int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const Call c, const char *qs, const char *ds_, const char *qts, const char *dts, const char *ks,
-                                                                         const char *vs, const Exponents ex, const char *info, const int *delta_exponents,
+                                                                         const char *vs, const Exponents ex, const char *info,
                                                                          float *dk, float *dv, float *parts, int tiles, int pieces) {
   constexpr int BLOCK = (int)block_size(DP), SLOT = 4 * BLOCK + kInfoBytes;
   __shared__ __align__(16) char lds[2][SLOT];
@@ -616,10 +633,10 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   k.wait();
   v.wait();
   const Score score(c);
-  f32x16 dks[DP / 32], low[DP / 32], dvs[DP / 32];
+  f32x16 dks[DP / 32], dvs[DP / 32];
 #pragma unroll
-  for (int e = 0; e < DP / 32; ++e) dks[e] = low[e] = dvs[e] = zeros();
-  int unit = INT32_MAX / 2, unit_v = kSmallest;  // of dks and low; of dvs, which are times 2^13 more
+  for (int e = 0; e < DP / 32; ++e) dks[e] = dvs[e] = zeros();
+  int unit = kNoUnit, unit_v = kSmallest;  // both are times 2^(13 + unit)
   const char *const from[4] = {qs, ds_, qts, dts};
   const uint32_t to = lds_address(&lds[0][0]);
   auto fetch_step = [&](int step, int slot) {
@@ -630,7 +647,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
 #pragma unroll 1
   for (int step = begin; step < end; ++step) {
     const int slot = (step - begin) & 1;
-    const int eq = scalar(ex.q + row_block + step), ed = scalar(ex.d + row_block + step), edelta = scalar(delta_exponents + row_block + step);
+    const int eq = scalar(ex.q + row_block + step), ed = scalar(ex.d + row_block + step);
     Hull seen;
     seen.lo = scalar(&ex.hulls[row_block + step].lo);
     seen.hi = scalar(&ex.hulls[row_block + step].hi);
@@ -641,19 +658,11 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
     if (!seen.meets(j0, j0 + 32)) continue;
     const char *const at = lds[slot];
     const f32x16 s = product<DP>(at, k), dp = product<DP>(at + BLOCK, v);
-    const int new_unit = min(unit, 14 - gradient_exponent<DP>(ed, ev, edelta) + eq);
-    if (new_unit < unit) {
-      const float by = __builtin_ldexpf(1.f, max(new_unit - unit, -200));
-      multiply(dks, by);
-      multiply(low, by);
-      unit = new_unit;
-    }
     if (ed < unit_v) {
       multiply(dvs, __builtin_ldexpf(1.f, ed - unit_v));
       unit_v = ed;
     }
     const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(1.f, -(ed + ev));
-    const int shift = unit - eq - 13;
     const float p_factor = __builtin_ldexpf(1.f, unit_v - ed);
     const bool whole = seen.covers(j0, j0 + 32);
     const float *const of = reinterpret_cast<const float *>(at + 4 * BLOCK);
@@ -674,7 +683,6 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
         p[x] = weight<PLAIN>(score, s[x], factor, PLAIN ? 0.f : slope[e] * fabsf(ahead[e] - (float)j), stat[e], cap);
         ds[x] = p[x] * __builtin_fmaf(dp[x], d_factor, -delta[e]);
         if (!PLAIN) ds[x] *= cap;
-        ds[x] = __builtin_ldexpf(ds[x], shift);
         p[x] *= p_factor;
       }
       if (!whole) {
@@ -688,18 +696,25 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
       }
     }
     Weights w;
-    w.set<false>(p);
+    w.set(p);
     add_product<DP>(dvs, at + 3 * BLOCK, w);
-    w.set<true>(ds);
-    add_product<DP>(dks, low, at + 2 * BLOCK, w);
+    const int new_unit = gradient_unit(ds, eq, unit);
+    if (new_unit < unit) {
+      multiply(dks, __builtin_ldexpf(1.f, max(new_unit - unit, -200)));
+      unit = new_unit;
+    }
+    if (unit == kNoUnit) continue;  // nothing but zeros so far
+#pragma unroll
+    for (int x = 0; x < 16; ++x) ds[x] = __builtin_ldexpf(ds[x], unit - eq);
+    w.set(ds);
+    add_product<DP>(dks, at + 2 * BLOCK, w);
   }
   if (!live) return;
-  if (unit == INT32_MAX / 2) unit = 0;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
-      dks[e][x] = __builtin_ldexpf(__builtin_fmaf(low[e][x], kLowUnscale, dks[e][x]), -unit);
+      dks[e][x] = unit == kNoUnit ? 0.f : __builtin_ldexpf(dks[e][x], -13 - unit);
       dvs[e][x] = __builtin_ldexpf(dvs[e][x], -13 - unit_v);
     }
   const int64_t all = (int64_t)c.batch * c.tk * c.key_heads * c.dim, key = c.key_at(b, g, j);
@@ -734,7 +749,7 @@ struct Scratch {
 
 struct Layout {
   char *q, *d, *k, *v, *qt, *dt, *kt, *vt, *info;
-  int *eq, *ed, *ek, *ev, *edelta;
+  int *eq, *ed, *ek, *ev;
   Hull *hulls;
   Layout(const Call &c, bool backward, Scratch &s) {
     const int64_t heads = (int64_t)c.batch * c.key_heads, rows = heads * blocks_of(c.rows), keys = heads * blocks_of(c.tk);
@@ -752,7 +767,6 @@ struct Layout {
     ek = (int *)s.take(keys * 4);
     ev = (int *)s.take(keys * 4);
     ed = backward ? (int *)s.take(rows * 4) : nullptr;
-    edelta = backward ? (int *)s.take(rows * 4) : nullptr;
     hulls = backward ? (Hull *)s.take(rows * sizeof(Hull)) : nullptr;
   }
 };
@@ -793,35 +807,36 @@ Exponents pair_forward(const Call &c, float *out, float *stat, const Pieces &pie
   const Layout l(c, false, of);
   Pack p = {};
   p.n_jobs = 3;
-  p.jobs[0] = Job{c.q, true, 1.f, l.q, nullptr, l.eq, 0};
-  p.jobs[1] = Job{c.k, false, 1.f, l.k, nullptr, l.ek, 0};
-  p.jobs[2] = Job{c.v, false, 1.f, nullptr, l.vt, l.ev, 0};
+  p.jobs[0] = Job{c.q, true, l.q, nullptr, l.eq, 0};
+  p.jobs[1] = Job{c.k, false, l.k, nullptr, l.ek, 0};
+  p.jobs[2] = Job{c.v, false, nullptr, l.vt, l.ev, 0};
   pack(c, p, s);
   const Exponents ex = {l.eq, nullptr, l.ek, l.ev, nullptr, p.row_blocks, p.key_blocks};
   const unsigned groups = (unsigned)((int64_t)c.batch * c.key_heads * tiles * pieces.count);
   const bool plain = !c.slopes && c.cap == 0.f;
   with_columns(c.dim, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    hipLaunchKernelGGL((plain ? forward_kernel<DP, true> : forward_kernel<DP, false>), dim3(groups), dim3(kThreads), 0, s, c, l.q, l.k, l.vt, ex, out, stat, pieces, tiles);
+    hipLaunchKernelGGL((plain ? forward_kernel<DP, true> : forward_kernel<DP, false>), dim3(groups), dim3(2 * kThreads), 0, s, c, l.q, l.k, l.vt, ex, out, stat, pieces, tiles);
   });
   return ex;
 }
 
-Exponents pair_backward(const Call &c, const float *dout, const Row *rows, float *dq, float *dk, float *dv, float *parts, int row_tiles, int key_tiles,
+Exponents pair_backward(const Call &c, const float *out, const float *stat, const float *dout, Row *rows, float *dq, float *dk, float *dv, float *parts, int row_tiles, int key_tiles,
                         int pieces, char *scratch, hipStream_t s) {
   Scratch of = {scratch, 0};
   const Layout l(c, true, of);
   Pack p = {};
   p.n_jobs = 4;
   const bool keys = dk || dv;
-  p.jobs[0] = Job{c.q, true, kLowScale, l.q, keys ? l.qt : nullptr, l.eq, 0};
-  p.jobs[1] = Job{dout, true, 1.f, l.d, keys ? l.dt : nullptr, l.ed, 0};
-  p.jobs[2] = Job{c.k, false, kLowScale, l.k, dq ? l.kt : nullptr, l.ek, 0};
-  p.jobs[3] = Job{c.v, false, 1.f, l.v, nullptr, l.ev, 0};
+  p.jobs[0] = Job{c.q, true, l.q, keys ? l.qt : nullptr, l.eq, 0};
+  p.jobs[1] = Job{dout, true, l.d, keys ? l.dt : nullptr, l.ed, 0};
+  p.jobs[2] = Job{c.k, false, l.k, dq ? l.kt : nullptr, l.ek, 0};
+  p.jobs[3] = Job{c.v, false, l.v, nullptr, l.ev, 0};
+  p.out = out;
+  p.stat = stat;
   p.rows = rows;
   p.info = (float *)l.info;
   p.hulls = l.hulls;
-  p.delta_exponents = l.edelta;
   pack(c, p, s);
   const Exponents ex = {l.eq, l.ed, l.ek, l.ev, l.hulls, p.row_blocks, p.key_blocks};
   const bool plain = !c.slopes && c.cap == 0.f;
@@ -830,10 +845,10 @@ Exponents pair_backward(const Call &c, const float *dout, const Row *rows, float
     constexpr int DP = decltype(dp)::value;
     if (dq)
       hipLaunchKernelGGL((plain ? dq_kernel<DP, true> : dq_kernel<DP, false>), dim3((unsigned)(heads * row_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.k, l.v, l.kt, ex,
-                         rows, l.edelta, dq, row_tiles);
+                         rows, dq, row_tiles);
     if (keys)
       hipLaunchKernelGGL((plain ? dkv_kernel<DP, true> : dkv_kernel<DP, false>), dim3((unsigned)(heads * key_tiles * pieces)), dim3(kThreads), 0, s, c, l.q, l.d, l.qt, l.dt,
-                         l.k, l.v, ex, l.info, l.edelta, dk, dv, parts, key_tiles, pieces);
+                         l.k, l.v, ex, l.info, dk, dv, parts, key_tiles, pieces);
   });
   return ex;
 }

@@ -302,8 +302,15 @@ __global__ __launch_bounds__(1024) void sum_pieces_kernel(const Sums of, int dim
   const int along = threadIdx.x % 32, slice = threadIdx.x / 32, c = blockIdx.x * 32 + along;
   const float *partial = of.partial[blockIdx.y];
   float s = 0.f;
+  const int pieces = of.pieces[blockIdx.y];
   if (c < dim)
-    for (int p = slice; p < of.pieces[blockIdx.y]; p += 32) s += partial[(int64_t)p * dim + c];
+    for (int p = slice; p < pieces; p += 32 * 8) {  // eight loads under way
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = partial[(int64_t)min(p + 32 * e, pieces - 1) * dim + c];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s += p + 32 * e < pieces ? v[e] : 0.f;
+    }
   sums[slice][along] = s;
   __syncthreads();
   if (slice > 0 || c >= dim) return;

@@ -517,27 +517,20 @@ class HeadGradientPart(ctypes.Structure):
                 ("rotate", ctypes.c_int)]
 
 
-def _part(cls, arrays, **numbers):
-    _nd_args(*[a for a in arrays.values() if a is not None])
-    part = cls(**{name: int(value) for name, value in numbers.items()})
-    for name, a in arrays.items():
-        if a is not None:
-            setattr(part, name, a.handle)
-    part.arrays = arrays   # a handle alone does not keep its storage
-    return part
-
-
 def head_part(input, gamma, output, heads, rotate=True, place=False):
     """An array of heads as ``head_rotary`` takes it: normed where there is a ``gamma``, rotated with ``rotate``; with
     ``place`` the output is a cache whose rows ``slots`` names."""
-    return _part(HeadPart, {"input": input, "gamma": gamma, "output": output}, heads=heads, rotate=bool(rotate), place=bool(place))
+    part = HeadPart(input.handle, None if gamma is None else gamma.handle, output.handle, heads, rotate, place)
+    part.arrays = input, gamma, output   # a handle alone does not keep its storage
+    return part
 
 
 def head_gradient_part(input, gamma, doutput, dinput, dgamma, heads, rotate=True):
     """An array of heads as ``head_rotary_backward`` takes it.  ``input`` may be None without ``gamma``; one of the two
     gradients may be None."""
-    return _part(HeadGradientPart, {"input": input, "gamma": gamma, "doutput": doutput, "dinput": dinput, "dgamma": dgamma},
-                 heads=heads, rotate=bool(rotate))
+    part = HeadGradientPart(_handle(input), _handle(gamma), doutput.handle, _handle(dinput), _handle(dgamma), heads, rotate)
+    part.arrays = input, gamma, doutput, dinput, dgamma
+    return part
 
 
 def head_rotary(parts, positions, frequencies, amplitude, interleaved, eps, slots, cudaStream):
