@@ -887,14 +887,21 @@ extern "C" int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHa
   const int row_tiles = (c.rows + kRows - 1) / kRows, key_tiles = (c.tk + kRows - 1) / kRows;
   const int64_t key_groups = head_pairs * key_tiles;
   int pieces = 1;
-  if ((dkey || dvalue) && key_groups) pieces = (int)std::min<int64_t>((2 * num_cus() + key_groups - 1) / key_groups, std::max(1, c.rows / 256));
+  const bool pairs = all_rows && all_keys && pair_suits(c, true);
+  if ((dkey || dvalue) && key_groups) pieces = (int)std::min<int64_t>(((pairs && c.dim <= 64 ? 4 : 2) * num_cus() + key_groups - 1) / key_groups, std::max(1, c.rows / 256));
+  // on pairs whole (b, key head, piece)s are dealt to the eight XCDs: a multiple of eight of them where that takes at most half as many again
+  if (pairs)
+    for (int more = pieces; more <= pieces + pieces / 2 && more <= std::max(1, c.rows / 256); ++more)
+      if (head_pairs * more % 8 == 0) {
+        pieces = more;
+        break;
+      }
   TF_REQUIRE(head_pairs * row_tiles < kMaxGroups && key_groups * pieces < kMaxGroups && (all_rows + 3) / 4 < kMaxGroups,
              "too many sequences, heads and queries for a launch");
   TF_REQUIRE(!being_captured(s), "the backward pass takes scratch, which a captured stream cannot give back");
   for (const DLArray *written : {(const DLArray *)dquery, (const DLArray *)dkey, (const DLArray *)dvalue}) announce_write(written);
   const int64_t all = all_keys * c.dim;
   const size_t row_bytes = (size_t)all_rows * sizeof(Row), part_bytes = pieces > 1 ? (size_t)pieces * 2 * all * sizeof(float) : 0;
-  const bool pairs = all_rows && all_keys && pair_suits(c, true);
   const size_t planes = pairs ? pair_bytes(c, true) : 0, bytes = planes + part_bytes + row_bytes;
   char *block = (char *)device_alloc(bytes, s);
   if (!block) {

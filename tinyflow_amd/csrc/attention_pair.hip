@@ -2,11 +2,9 @@
 //
 // A block of 32 rows of an operand (queries, their gradients, keys or values of one head) is multiplied by the power of two that brings its
 // largest value into [2^14, 2^15), and each element is made of two fp16 numbers, h its nearest one and l the nearest to what is left: three
-// products of the fp16 instruction, h h' + h l' + l h', take the place of one of the fp32 instruction, which has a sixteenth of its rate (gemm_pair.h
-// has the argument; what is left off is 2^-23 of an element, or a fixed part of its block's largest value where that is more).
-//   Where l is held 2^11 times larger (operands of scores and of their gradients, both sides), that part is 2^-50, and products with an l have sums of
-//   their own.  Where it is not (p and what p multiplies), it is 2^-39, and one sum takes all three: twice the sums of o or dv would not leave room
-//   for two waves a SIMD, or for the operands of dk.  p is at most 4, and held times 2^12 or 2^13.
+// products of the fp16 instruction, h h' + h l' + l h', take the place of one of the fp32 instruction, which has a sixteenth of its rate.  What is
+// left off is 2^-23 of an element, or 2^-40 of its block's largest value where that is more, and l l', up to 2^-22 of a product.  p is at most 4, and
+// split times 2^12 or 2^13, so what is left off there is 2^-37 of 1 at most.
 // Scales are a block's, so a product's scale is known for a whole tile and costs nothing: it is part of the factor of a score, of the
 // exponent of p, of ds.  A sum over several blocks has the scale of the largest one so far (`unit`); when a larger one comes the sum is multiplied.
 //
@@ -43,7 +41,6 @@ __device__ __forceinline__ void static_for(F &&f) {
 
 constexpr int kFragment = 1024;  // bytes: 32 rows x 16 of fp16, a wave's lanes one behind the other
 constexpr int kInfoBytes = 1024;  // of a block of rows: eight arrays of 32, see Info
-constexpr float kLowScale = 0x1p11f, kLowUnscale = 0x1p-11f;
 constexpr int kSmallest = 110;   // exponents above it stand for values that no sum notices
 constexpr int kLargest = -40;
 constexpr int kNoUnit = INT32_MAX / 2;  // of a sum of nothing
@@ -75,9 +72,9 @@ struct Pack {
   Hull *hulls;
 };
 
-__device__ inline void split(float x, float low, _Float16 &h, _Float16 &l) {
+__device__ inline void split(float x, _Float16 &h, _Float16 &l) {
   h = (_Float16)x;
-  l = (_Float16)((x - (float)h) * low);
+  l = (_Float16)(x - (float)h);
 }
 
 // A workgroup a block.  Plain form: step s of 16 columns, h then l, lane: row lane % 32, columns 16 s + 8 (lane / 32) + 0..7.  Transposed: columns 32 d
@@ -199,7 +196,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         _Float16 a, d;
-        split(tile[r][8 * eighth + e], kLowScale, a, d);
+        split(tile[r][8 * eighth + e], a, d);
         h[e] = a;
         l[e] = d;
       }
@@ -215,7 +212,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         _Float16 a, d;
-        split(tile[16 * t + key_of(e, half)][col], 1.f, a, d);
+        split(tile[16 * t + key_of(e, half)][col], a, d);
         h[e] = a;
         l[e] = d;
       }
@@ -248,71 +245,120 @@ struct Held {
       l[s] = fragment(block + (2 * s + 1) * kFragment + lane * 16);
     }
   }
-  // Waits for them, before loads that the compiler does not count are under way.
+  // Waits for them, before loads that the compiler does not count are under way.  APART: in the registers that only matrix instructions
+  // read, where the others are too few for what they are needed for.
+  template <bool APART>
   __device__ inline void wait() {
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) asm volatile("" : "+v"(h[s]), "+v"(l[s]));
+    for (int s = 0; s < DP / 16; ++s)
+      if constexpr (APART) asm volatile("" : "+a"(h[s]), "+a"(l[s]));
+      else asm volatile("" : "+v"(h[s]), "+v"(l[s]));
   }
 };
 
-// The product of a block in LDS, in the plain form, with what the wave holds.
-template <int DP>
-__device__ __forceinline__ f32x16 product(const char *block, const Held<DP> &b) {
-  const char *at = block + threadIdx.x % 64 * 16;
-  f32x16 sum = zeros(), low = zeros();
-#pragma unroll
-  for (int s = 0; s < DP / 16; ++s) {
-    const f16x8 h = fragment(at + 2 * s * kFragment), l = fragment(at + (2 * s + 1) * kFragment);
-    low = mfma(l, b.h[s], low);
-    sum = mfma(h, b.h[s], sum);
-    low = mfma(h, b.l[s], low);
-  }
-#pragma unroll
-  for (int v = 0; v < 16; ++v) sum[v] = __builtin_fmaf(low[v], kLowUnscale, sum[v]);
-  return sum;
+// Products of blocks that lie one behind the other in LDS, in the plain form, with what the wave holds for each.  The fragments are read READ_AHEAD
+// steps before they are multiplied, and `between(n)` is what is computed while the n-th instruction runs, of which a step has three: a wave issues
+// in order, so only what stands behind a single matrix instruction, before the next, runs beside it (five vector instructions do in the 34 cycles of
+// one; from the eighth on each costs five cycles).  The order is kept as it stands here; left to itself the compiler reads a fragment, waits
+// for it and multiplies.
+template <int DP, int N, int READ_AHEAD, class Between>
+__device__ __forceinline__ void products(const char *blocks, const Held<DP> *const (&held)[N], f32x16 (&sum)[N], const Between &between) {
+  constexpr int STEPS = DP / 16, ALL = N * STEPS, AHEAD = READ_AHEAD < ALL ? READ_AHEAD : ALL;
+  const char *const at = blocks + threadIdx.x % 64 * 16;
+  f16x8 h[ALL], l[ALL];
+  auto read = [&](auto n_c) {
+    constexpr int n = decltype(n_c)::value;
+    h[n] = fragment(at + 2 * n * kFragment);
+    l[n] = fragment(at + (2 * n + 1) * kFragment);
+  };
+  static_for<AHEAD>([&](auto n) { read(n); });
+  __builtin_amdgcn_sched_barrier(0);
+  static_for<ALL>([&](auto n_c) {
+    constexpr int n = decltype(n_c)::value, block = n / STEPS, step = n % STEPS;
+    if constexpr (step == 0) sum[block] = zeros();
+    if constexpr (n + AHEAD < ALL) read(IC<n + AHEAD>{});
+    sum[block] = mfma(l[n], held[block]->h[step], sum[block]);
+    between(IC<3 * n>{});
+    __builtin_amdgcn_sched_barrier(0);
+    sum[block] = mfma(h[n], held[block]->l[step], sum[block]);
+    between(IC<3 * n + 1>{});
+    __builtin_amdgcn_sched_barrier(0);
+    sum[block] = mfma(h[n], held[block]->h[step], sum[block]);
+    between(IC<3 * n + 2>{});
+    __builtin_amdgcn_sched_barrier(0);
+  });
 }
 
-// 16 values of a tile as the other operand of a product over its rows.
+// 16 values of a tile as the other operand of a product over its rows: instruction t takes values 8 t .. 8 t + 7.
 struct Weights {
   f16x8 h[2], l[2];
-  __device__ __forceinline__ void set(const float (&w)[16]) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const f32x2 x = {w[8 * t + e], w[8 * t + e + 1]};
-        const f16x2 top = __builtin_convertvector(x, f16x2);
-        f32x2 left;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) left[i] = x[i] - (float)top[i];
-        const f16x2 rest = __builtin_convertvector(left, f16x2);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          h[t][e + i] = top[i];
-          l[t][e + i] = rest[i];
-        }
-      }
+  // values 2 n and 2 n + 1
+  template <int n>
+  __device__ __forceinline__ void set(float a, float b) {
+    constexpr int t = n / 4, e = 2 * (n % 4);
+    const f32x2 x = {a, b};
+    const f16x2 top = __builtin_convertvector(x, f16x2);
+    const f32x2 left = {a - (float)top[0], b - (float)top[1]};
+    const f16x2 rest = __builtin_convertvector(left, f16x2);
+    h[t][e] = top[0];
+    h[t][e + 1] = top[1];
+    l[t][e] = rest[0];
+    l[t][e + 1] = rest[1];
   }
 };
 
-// sum[d] += of a transposed block
-template <int DP>
-__device__ __forceinline__ void add_product(f32x16 (&sum)[DP / 32], const char *block, const Weights &w) {
-  const char *at = block + threadIdx.x % 64 * 16;
-#pragma unroll
-  for (int d = 0; d < DP / 32; ++d)
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const f16x8 h = fragment(at + (2 * d + t) * 2 * kFragment), l = fragment(at + ((2 * d + t) * 2 + 1) * kFragment);
-      sum[d] = mfma(l, w.h[t], sum[d]);
-      sum[d] = mfma(h, w.l[t], sum[d]);
-      sum[d] = mfma(h, w.h[t], sum[d]);
-    }
+// sum[d] += of a transposed block, `between` as above.  The weights' second halves may be set in it, before the instruction 3 DP / 32.
+template <int DP, int READ_AHEAD, class Between>
+__device__ __forceinline__ void add_product(f32x16 (&sum)[DP / 32], const char *block, const Weights &w, const Between &between) {
+  constexpr int D = DP / 32, ALL = 2 * D, AHEAD = READ_AHEAD < ALL ? READ_AHEAD : ALL;
+  const char *const at = block + threadIdx.x % 64 * 16;
+  f16x8 h[ALL], l[ALL];
+  auto read = [&](auto n_c) {
+    constexpr int n = decltype(n_c)::value, index = n % D * 2 + n / D;
+    h[n] = fragment(at + index * 2 * kFragment);
+    l[n] = fragment(at + (index * 2 + 1) * kFragment);
+  };
+  static_for<AHEAD>([&](auto n) { read(n); });
+  __builtin_amdgcn_sched_barrier(0);
+  static_for<ALL>([&](auto n_c) {
+    constexpr int n = decltype(n_c)::value, t = n / D, d = n % D;
+    if constexpr (n + AHEAD < ALL) read(IC<n + AHEAD>{});
+    sum[d] = mfma(l[n], w.h[t], sum[d]);
+    between(IC<3 * n>{});
+    __builtin_amdgcn_sched_barrier(0);
+    sum[d] = mfma(h[n], w.l[t], sum[d]);
+    between(IC<3 * n + 1>{});
+    __builtin_amdgcn_sched_barrier(0);
+    sum[d] = mfma(h[n], w.h[t], sum[d]);
+    between(IC<3 * n + 2>{});
+    __builtin_amdgcn_sched_barrier(0);
+  });
 }
+// COUNT pieces of work over the places [FIRST, FIRST + PLACES): do_piece(k) at place n.
+template <int n, int FIRST, int PLACES, int COUNT, class F>
+__device__ __forceinline__ void spread(const F &do_piece) {
+  if constexpr (n >= FIRST && n < FIRST + PLACES)
+    static_for<COUNT>([&](auto k_c) {
+      if constexpr (decltype(k_c)::value * PLACES / COUNT == n - FIRST) do_piece(k_c);
+    });
+}
+struct Nothing {
+  template <class T>
+  __device__ __forceinline__ void operator()(T) const {}
+};
+
 template <int N>
 __device__ inline void multiply(f32x16 (&sum)[N], float by) {
 #pragma unroll
   for (int d = 0; d < N; ++d) sum[d] *= by;
+}
+// Keeps sums in the registers that only matrix instructions work on: where a branch multiplies them, the compiler otherwise holds them in the
+// others and moves all of them there and back at every step.
+template <bool APART, int N>
+__device__ __forceinline__ void keep(f32x16 (&sum)[N]) {
+  if constexpr (APART)
+#pragma unroll
+    for (int d = 0; d < N; ++d) asm volatile("" : "+a"(sum[d]));
 }
 
 // Brings 1 KB from `from` to LDS at `to`, 16 bytes a lane.  Written out because the compiler takes every read of LDS for a reader of the loads
@@ -337,17 +383,25 @@ __device__ inline int scalar(const int *p) { return *(const __attribute__((addre
 __device__ inline float unscaled(float factor, int a, int b) { return __builtin_ldexpf(factor, max(-(a + b), -80)); }
 
 
-// Fetches block `index` of each of N operands, one behind the other in LDS from `to` on, each of four waves every fourth
-// fragment.
+// Block `index` of each of N operands, one behind the other in LDS from `to` on: N DP / 32 fetches of each of four waves, every fourth fragment.
 template <int DP, int N>
-__device__ __forceinline__ void fetch_blocks(uint32_t to, const char *const (&of)[N], int64_t index) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % 4);
-  static_for<N>([&](auto n) {
-    const char *from = uniform(of[decltype(n)::value] + index * block_size(DP)) + wave * kFragment;
-#pragma unroll
-    for (int f = 0; f < DP / 32; ++f) fetch(to + (uint32_t)(decltype(n)::value * block_size(DP) + (4 * f + wave) * kFragment), from + 4 * f * kFragment);
-  });
-}
+struct Blocks {
+  const char *from[N];
+  uint32_t to;
+  int wave;
+  __device__ __forceinline__ Blocks(const char *const (&of)[N], int64_t index, uint32_t at) : to(at), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / 64 % 4)) {
+    static_for<N>([&](auto n) { from[decltype(n)::value] = uniform(of[decltype(n)::value] + index * block_size(DP)) + wave * kFragment; });
+  }
+  template <int f>
+  __device__ __forceinline__ void one() const {
+    constexpr int n = f / (DP / 32), i = f % (DP / 32);
+    fetch(to + (uint32_t)(n * block_size(DP) + (4 * i + wave) * kFragment), from[n] + 4 * i * kFragment);
+  }
+  static constexpr int kCount = N * DP / 32;
+  __device__ __forceinline__ void all() const {
+    static_for<kCount>([&](auto f) { one<decltype(f)::value>(); });
+  }
+};
 
 // ------------------------------------------------------------------------------ forward
 
@@ -359,6 +413,7 @@ template <int DP, bool PLAIN>
 __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel(const Call c, const char *qs, const char *ks, const char *vs, const Exponents ex,
                                                                                  float *out, float *stat, const Pieces pieces, int tiles) {
   constexpr int BLOCK = (int)block_size(DP);
+  constexpr int AHEAD = DP <= 64 ? 1 : 3;
   __shared__ __align__(16) char lds[2][2][2 * BLOCK];  // [parity][group]
   __shared__ int room[8][4];
   __shared__ float marks[2][kRows];
@@ -384,7 +439,7 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
   const float slope = !PLAIN && c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
   Held<DP> q;
   q.load(qs + row_block * BLOCK);
-  q.wait();
+  q.template wait<false>();
   const Score score(c);
   f32x16 o[DP / 32];
 #pragma unroll
@@ -393,23 +448,24 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
   int unit = kSmallest;             // o is times 2^(12 + unit)
   const char *const from[2] = {ks, vs};
   const uint32_t to = lds_address(&lds[0][group][0]);
-  if (begin + group < end) fetch_blocks<DP, 2>(to, from, key_block + begin + group);
+  if (begin + group < end) Blocks<DP, 2>(from, key_block + begin + group, to).all();
   int parity = 0;
 #pragma unroll 1
   for (int pair = begin; pair < end; pair += 2, parity ^= 1) {
     const int step = pair + group, j0 = step * kKeys;
     arrived();
-    if (step + 2 < end) fetch_blocks<DP, 2>(to + (uint32_t)((1 - parity) * 4 * BLOCK), from, key_block + step + 2);
+    if (step + 2 < end) Blocks<DP, 2>(from, key_block + step + 2, to + (uint32_t)((1 - parity) * 4 * BLOCK)).all();
     if (step >= end || !mine.meets(j0, j0 + kKeys)) continue;
     const int ek = scalar(ex.k + key_block + step), ev = scalar(ex.v + key_block + step);
     const char *const keys = lds[parity][group], *const values = keys + BLOCK;
-    const f32x16 s = product<DP>(keys, q);
+    f32x16 s[1];
+    products<DP, 1, AHEAD>(keys, {&q}, s, Nothing{});
     const float factor = unscaled(score.factor, eq, ek);
     const bool whole = mine.covers(j0, j0 + kKeys);
     float p[16], most = kNone;
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
-      p[v] = s[v];
+      p[v] = s[0][v];
       if (!PLAIN) {
         p[v] *= factor;
         if (score.capped) p[v] = score.top * tanh_of(p[v]);
@@ -451,9 +507,15 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
     if (apart < near)
 #pragma unroll
       for (int v = 0; v < 16; ++v) p[v] = __builtin_ldexpf(p[v], apart - near);
+    // the second half's operands while the first half is multiplied
     Weights w;
-    w.set(p);
-    add_product<DP>(o, values, w);
+    static_for<4>([&](auto n) { w.set<decltype(n)::value>(p[2 * decltype(n)::value], p[2 * decltype(n)::value + 1]); });
+    add_product<DP, AHEAD>(o, values, w, [&](auto place) {
+      spread<decltype(place)::value, 0, 3 * DP / 32 - 1, 4>([&](auto k) {
+        constexpr int n = 4 + decltype(k)::value;
+        w.set<n>(p[2 * n], p[2 * n + 1]);
+      });
+    });
   }
   total = (total + other_half(total)) * 0x1p-12f;
   multiply(o, __builtin_ldexpf(1.f, -12 - unit));
@@ -488,19 +550,20 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
 
 // ------------------------------------------------------------------------------ backward
 
-// The exponent that brings the tile's largest gradient to 2^13 or below 2^14; that of a sum so far, `unit` less `other`, unless it is smaller.
-__device__ __forceinline__ int gradient_unit(const float (&ds)[16], int other, int unit) {
+// The unit of a sum of gradients times what has exponent `other`: the tile's largest gradient, held times 2^held, becomes less than 2^14 in it, unless
+// an earlier tile's was larger.
+__device__ __forceinline__ int gradient_unit(const float (&ds)[16], int held, int other, int unit) {
   float most = 0.f;
 #pragma unroll
   for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(ds[v]));
   const int field = __builtin_amdgcn_readfirstlane((int)(lanes::largest<64>(bits_of(most)) >> 23));
-  return field == 0 || field == 255 ? unit : min(unit, 140 - field + other);
+  return field == 0 || field == 255 ? unit : min(unit, 140 - field + held + other);
 }
 
-// p times 2^13 (0 where a mask says so) and the derivative of the cap, from a product.
+// p times 2^x, for shift = x - the row's statistic, and the derivative of the cap, from a product.
 template <bool PLAIN>
-__device__ __forceinline__ float weight(const Score &score, float product, float factor, float bias, float stat, float &slope) {
-  if (PLAIN) return __builtin_amdgcn_exp2f(__builtin_fmaf(product, factor, 13.f - stat));
+__device__ __forceinline__ float weight(const Score &score, float product, float factor, float bias, float shift, float &slope) {
+  if (PLAIN) return __builtin_amdgcn_exp2f(__builtin_fmaf(product, factor, shift));
   float t = product * factor;
   slope = 1.f;
   if (score.capped) {
@@ -508,14 +571,14 @@ __device__ __forceinline__ float weight(const Score &score, float product, float
     slope = __builtin_fmaf(-t, t, 1.f);
     t *= score.top;
   }
-  return __builtin_amdgcn_exp2f((t - bias) - (stat - 13.f));
+  return __builtin_amdgcn_exp2f((t - bias) + shift);
 }
 
 // 128 rows a workgroup, as forward_kernel; in LDS a step's keys, values and keys transposed.
 template <int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Call c, const char *qs, const char *ds_, const char *ks, const char *vs, const char *kts,
                                                                         const Exponents ex, const Row *rows, float *dq, int tiles) {
-  constexpr int BLOCK = (int)block_size(DP);
+  constexpr int BLOCK = (int)block_size(DP), AHEAD = 3;
   __shared__ __align__(16) char lds[2][3 * BLOCK];
   __shared__ int room[4][4];
   const int heads = c.batch * c.key_heads;
@@ -541,8 +604,8 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
   Held<DP> q, d;
   q.load(qs + row_block * BLOCK);
   d.load(ds_ + row_block * BLOCK);
-  q.wait();
-  d.wait();
+  q.template wait<(DP > 64)>();
+  d.template wait<(DP > 64)>();
   const Score score(c);
   f32x16 sum[DP / 32];
 #pragma unroll
@@ -550,48 +613,64 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
   int unit = kNoUnit;  // sum is times 2^unit
   const char *const from[3] = {ks, vs, kts};
   const uint32_t to = lds_address(&lds[0][0]);
-  if (begin < end) fetch_blocks<DP, 3>(to, from, key_block + begin);
+  if (begin < end) Blocks<DP, 3>(from, key_block + begin, to).all();
 #pragma unroll 1
   for (int step = begin; step < end; ++step) {
     const int slot = (step - begin) & 1, j0 = step * kKeys;
     const int ek = scalar(ex.k + key_block + step), ev = scalar(ex.v + key_block + step);
     arrived();
-    if (step + 1 < end) fetch_blocks<DP, 3>(to + (uint32_t)((1 - slot) * 3 * BLOCK), from, key_block + step + 1);
-    if (!mine.meets(j0, j0 + kKeys)) continue;
-    const f32x16 s = product<DP>(lds[slot], q), dp = product<DP>(lds[slot] + BLOCK, d);
+    // the last step fetches itself again
+    const Blocks<DP, 3> next(from, key_block + min(step + 1, end - 1), to + (uint32_t)((1 - slot) * 3 * BLOCK));
+    if (DP <= 64 && !mine.meets(j0, j0 + kKeys)) {  // longer heads: the sums would move at every step for it
+      next.all();
+      continue;
+    }
+    keep<(DP > 64)>(sum);
     const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(1.f, -(ed + ev));
-    const bool whole = mine.covers(j0, j0 + kKeys);
-    float ds[16];
+    float p[16], cap[16], ds[16];
+    f32x16 s[2];
+    auto tile = [&](auto whole_c) {
+      constexpr bool WHOLE = decltype(whole_c)::value;
+      products<DP, 2, AHEAD>(lds[slot], {&q, &d}, s, [&](auto place) {
+        constexpr int FIRST = 3 * DP / 16;
+        spread<decltype(place)::value, 0, FIRST, decltype(next)::kCount>([&](auto f) { next.template one<decltype(f)::value>(); });
+        spread<decltype(place)::value, FIRST + 2, FIRST - 2, 16>([&](auto v_c) {
+          constexpr int v = decltype(v_c)::value;
+          const int j = j0 + key_of(v, half);
+          p[v] = weight<PLAIN>(score, s[0][v], factor, PLAIN ? 0.f : slope * fabsf((float)(ahead - j)), -stat, cap[v]);
+          if (!WHOLE) p[v] = ((j >= row.lo) & (j < row.hi)) ? p[v] : 0.f;
+        });
+      });
+    };
+    if (mine.covers(j0, j0 + kKeys)) tile(std::true_type{});
+    else tile(std::false_type{});
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
-      float cap = 1.f;
-      const float p = weight<PLAIN>(score, s[v], factor, PLAIN ? 0.f : slope * fabsf((float)(ahead - (j0 + key_of(v, half)))), stat, cap);
-      ds[v] = p * __builtin_fmaf(dp[v], d_factor, -delta);
-      if (!PLAIN) ds[v] *= cap;
+      ds[v] = p[v] * __builtin_fmaf(s[1][v], d_factor, -delta);
+      if (!PLAIN) ds[v] *= cap[v];
     }
-    if (!whole)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int j = j0 + key_of(v, half);
-        ds[v] = j >= row.lo && j < row.hi ? ds[v] : 0.f;
-      }
-    const int new_unit = gradient_unit(ds, ek, unit);
+    const int new_unit = gradient_unit(ds, 0, ek, unit);
     if (new_unit < unit) {
       multiply(sum, __builtin_ldexpf(1.f, max(new_unit - unit, -200)));
+      keep<(DP > 64)>(sum);
       unit = new_unit;
     }
-    if (unit == kNoUnit) continue;  // nothing but zeros so far
-#pragma unroll
-    for (int v = 0; v < 16; ++v) ds[v] = __builtin_ldexpf(ds[v], unit - ek);
+    const int shift = unit == kNoUnit ? 0 : unit - ek;  // nothing but zeros so far
     Weights w;
-    w.set(ds);
-    add_product<DP>(sum, lds[slot] + 2 * BLOCK, w);
+    auto set = [&](auto n_c) {
+      constexpr int n = decltype(n_c)::value;
+      w.set<n>(__builtin_ldexpf(ds[2 * n], shift), __builtin_ldexpf(ds[2 * n + 1], shift));
+    };
+    static_for<4>(set);
+    add_product<DP, AHEAD>(sum, lds[slot] + 2 * BLOCK, w,
+                           [&](auto place) { spread<decltype(place)::value, 0, 3 * DP / 32 - 1, 4>([&](auto k) { set(IC<4 + decltype(k)::value>{}); }); });
   }
+  arrived();  // what the last step has fetched
   if (!live) return;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) sum[e][v] = unit == kNoUnit ? 0.f : __builtin_ldexpf(sum[e][v], -13 - unit);
+    for (int v = 0; v < 16; ++v) sum[e][v] = unit == kNoUnit ? 0.f : __builtin_ldexpf(sum[e][v], -unit);
   store_sums(sum, dq + c.query_at(b, g, r), c.dim, c.scale);
 }
 
@@ -600,29 +679,40 @@ template <int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const Call c, const char *qs, const char *ds_, const char *qts, const char *dts, const char *ks,
                                                                          const char *vs, const Exponents ex, const char *info,
                                                                          float *dk, float *dv, float *parts, int tiles, int pieces) {
-  constexpr int BLOCK = (int)block_size(DP), SLOT = 4 * BLOCK + kInfoBytes;
+  constexpr int BLOCK = (int)block_size(DP), SLOT = 4 * BLOCK + kInfoBytes, AHEAD = DP <= 64 ? 1 : 3;
   __shared__ __align__(16) char lds[2][SLOT];
   __shared__ int range[2];
-  const int heads = c.batch * c.key_heads;
-  const int bg = (int)blockIdx.x % heads, rest = (int)blockIdx.x / heads;
-  const int b = bg / c.key_heads, g = bg % c.key_heads, tile = rest % tiles, piece = rest / tiles;
+  // A (b, key head) and a piece of its rows belong to one XCD, whose workgroups then walk the same rows at the same time: the rows come
+  // from its L2 for all but the first.  XCDs take them back and forth, later rows, which see more keys in a causal pass, first; earlier keys, which
+  // more rows see, come first.
+  const int heads = c.batch * c.key_heads, turns = (heads * pieces + 7) / 8, xcd = (int)blockIdx.x % 8;
+  const int turn = (int)blockIdx.x / 8 % turns, tile = (int)blockIdx.x / 8 / turns, of_xcd = 8 * turn + (turn % 2 ? 7 - xcd : xcd);
+  if (of_xcd >= heads * pieces) return;
+  const int bg = of_xcd % heads, piece = pieces - 1 - of_xcd / heads, b = bg / c.key_heads, g = bg % c.key_heads;
   const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int tile_lo = tile * kRows, tile_hi = min(c.tk, tile_lo + kRows);
   if (__syncthreads_or(ex.bad_rows_of(bg, tile_lo, tile_hi) | ex.bad_keys(bg, tile_lo / 32, kRows / 32))) return;
   const int64_t row_block = (int64_t)bg * ex.row_blocks;
-  // the blocks of rows that see one of the keys
-  if (threadIdx.x == 0) range[0] = ex.row_blocks, range[1] = 0;
+  // The blocks of rows that see one of the keys.  Without spans pieces are the same rows for all keys; with them they may be few of all rows, and
+  // are cut as they are.
+  const int from_block = c.spans ? 0 : (int)((int64_t)ex.row_blocks * piece / pieces);
+  const int to_block = c.spans ? ex.row_blocks : (int)((int64_t)ex.row_blocks * (piece + 1) / pieces);
+  if (threadIdx.x == 0) range[0] = to_block, range[1] = 0;
   __syncthreads();
   {
-    int lo = ex.row_blocks, hi = 0;
-    for (int e = threadIdx.x; e < ex.row_blocks; e += kThreads)
+    int lo = to_block, hi = 0;
+    for (int e = from_block + threadIdx.x; e < to_block; e += kThreads)
       if (ex.hulls[row_block + e].meets(tile_lo, tile_hi)) lo = min(lo, e), hi = max(hi, e + 1);
     atomicMin(&range[0], lo);
     atomicMax(&range[1], hi);
   }
   __syncthreads();
-  const int first = __builtin_amdgcn_readfirstlane(range[0]), steps = max(0, __builtin_amdgcn_readfirstlane(range[1]) - first);
-  const int begin = first + (int)((int64_t)steps * piece / pieces), end = first + (int)((int64_t)steps * (piece + 1) / pieces);
+  int begin = __builtin_amdgcn_readfirstlane(range[0]), end = __builtin_amdgcn_readfirstlane(range[1]);
+  if (c.spans) {
+    const int first = begin, steps = max(0, end - begin);
+    begin = first + (int)((int64_t)steps * piece / pieces);
+    end = first + (int)((int64_t)steps * (piece + 1) / pieces);
+  }
   const int j0 = tile_lo + wave * 32, j = j0 + lane % 32;
   const bool live = j < c.tk;
   const int64_t key_block = (int64_t)bg * ex.key_blocks + min(tile * (kRows / 32) + wave, ex.key_blocks - 1);
@@ -630,91 +720,125 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   Held<DP> k, v;
   k.load(ks + key_block * BLOCK);
   v.load(vs + key_block * BLOCK);
-  k.wait();
-  v.wait();
+  k.template wait<(DP > 64)>();
+  v.template wait<(DP > 64)>();
   const Score score(c);
   f32x16 dks[DP / 32], dvs[DP / 32];
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e) dks[e] = dvs[e] = zeros();
-  int unit = kNoUnit, unit_v = kSmallest;  // both are times 2^(13 + unit)
+  int unit = kNoUnit, unit_v = kSmallest;  // dks are times 2^unit, dvs times 2^(13 + unit_v)
   const char *const from[4] = {qs, ds_, qts, dts};
   const uint32_t to = lds_address(&lds[0][0]);
-  auto fetch_step = [&](int step, int slot) {
-    fetch_blocks<DP, 4>(to + (uint32_t)(slot * SLOT), from, row_block + step);
+  auto fetch_info = [&](int step, int slot) {
     if (wave == 0) fetch(to + (uint32_t)(slot * SLOT + 4 * BLOCK), uniform(info + (row_block + step) * kInfoBytes));
   };
-  if (begin < end) fetch_step(begin, 0);
-#pragma unroll 1
-  for (int step = begin; step < end; ++step) {
-    const int slot = (step - begin) & 1;
-    const int eq = scalar(ex.q + row_block + step), ed = scalar(ex.d + row_block + step);
-    Hull seen;
+  auto hull_of = [&](int step, Hull &seen) {
     seen.lo = scalar(&ex.hulls[row_block + step].lo);
     seen.hi = scalar(&ex.hulls[row_block + step].hi);
     seen.inner_lo = scalar(&ex.hulls[row_block + step].inner_lo);
     seen.inner_hi = scalar(&ex.hulls[row_block + step].inner_hi);
+  };
+  // the first block from `step` on that sees one of the workgroup's keys; others may be some that cannot be split, of which nothing is stored
+  auto next_of = [&](int step) {
+    Hull seen;
+    for (; step < end; ++step) {
+      hull_of(step, seen);
+      if (seen.meets(tile_lo, tile_hi)) break;
+    }
+    return step;
+  };
+  int step = next_of(begin), slot = 0;
+  if (step < end) {
+    Blocks<DP, 4>(from, row_block + step, to).all();
+    fetch_info(step, 0);
+  }
+#pragma unroll 1
+  for (int next; step < end; step = next, slot ^= 1) {
+    const int eq = scalar(ex.q + row_block + step), ed = scalar(ex.d + row_block + step);
+    Hull seen;
+    hull_of(step, seen);
+    next = next_of(step + 1);
     arrived();
-    if (step + 1 < end) fetch_step(step + 1, 1 - slot);
-    if (!seen.meets(j0, j0 + 32)) continue;
+    // the last step fetches itself again
+    const Blocks<DP, 4> coming(from, row_block + (next < end ? next : step), to + (uint32_t)((1 - slot) * SLOT));
+    fetch_info(next < end ? next : step, 1 - slot);
+    keep<(DP > 64)>(dks);
+    keep<(DP > 64)>(dvs);
+    if (DP <= 64 && !seen.meets(j0, j0 + 32)) {  // longer heads: the sums would move at every step for it
+      coming.all();
+      continue;
+    }
     const char *const at = lds[slot];
-    const f32x16 s = product<DP>(at, k), dp = product<DP>(at + BLOCK, v);
     if (ed < unit_v) {
       multiply(dvs, __builtin_ldexpf(1.f, ed - unit_v));
+      keep<(DP > 64)>(dvs);
       unit_v = ed;
     }
     const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(1.f, -(ed + ev));
-    const float p_factor = __builtin_ldexpf(1.f, unit_v - ed);
-    const bool whole = seen.covers(j0, j0 + 32);
-    const float *const of = reinterpret_cast<const float *>(at + 4 * BLOCK);
-    float p[16], ds[16];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int n = 8 * q + 4 * half;
-      const f32x4 stat = *reinterpret_cast<const f32x4 *>(of + 32 * kStat + n), delta = *reinterpret_cast<const f32x4 *>(of + 32 * kDelta + n);
-      f32x4 slope = {0.f, 0.f, 0.f, 0.f}, ahead = slope;
-      if (!PLAIN && c.slopes) {
-        slope = *reinterpret_cast<const f32x4 *>(of + 32 * kSlope + n);
-        ahead = *reinterpret_cast<const f32x4 *>(of + 32 * kAhead + n);
-      }
+    const int held = 13 + max(unit_v - ed, -60);  // p is held times 2^this, as the sum of dv needs it
+    const float *const of = reinterpret_cast<const float *>(at + 4 * BLOCK) + 4 * half;
+    auto four = [&](int array, int q) { return *reinterpret_cast<const f32x4 *>(of + 32 * array + 8 * q); };
+    float p[16], cap[16], ds[16];
+    f32x16 s[2];
+    Weights w;
+    auto tile = [&](auto whole_c) {
+      constexpr bool WHOLE = decltype(whole_c)::value;
+      f32x4 shift[4];
+      static_for<4>([&](auto q) { shift[decltype(q)::value] = (float)held - four(kStat, decltype(q)::value); });
+      products<DP, 2, AHEAD>(at, {&k, &v}, s, [&](auto place) {
+        constexpr int FIRST = 3 * DP / 16;
+        spread<decltype(place)::value, 0, FIRST, decltype(coming)::kCount>([&](auto f) { coming.template one<decltype(f)::value>(); });
+        spread<decltype(place)::value, FIRST + 2, FIRST - 4, 16>([&](auto x_c) {
+          constexpr int x = decltype(x_c)::value, q = x / 4, e = x % 4;
+          float bias = 0.f;
+          if (!PLAIN && c.slopes) bias = of[32 * kSlope + 8 * q + e] * fabsf(of[32 * kAhead + 8 * q + e] - (float)j);
+          p[x] = weight<PLAIN>(score, s[0][x], factor, bias, shift[q][e], cap[x]);
+          if (!WHOLE) {
+            const int lo = (int)bits_of(of[32 * kLo + 8 * q + e]), hi = (int)bits_of(of[32 * kHi + 8 * q + e]);
+            p[x] = ((j >= lo) & (j < hi)) ? p[x] : 0.f;
+          }
+        });
+        // two values behind
+        spread<decltype(place)::value, FIRST + 4, FIRST - 4, 8>([&](auto n_c) {
+          constexpr int n = decltype(n_c)::value;
+          w.set<n>(p[2 * n], p[2 * n + 1]);
+        });
+      });
+    };
+    if (seen.covers(j0, j0 + 32)) tile(std::true_type{});
+    else tile(std::false_type{});
+    static_for<4>([&](auto q) {
+      const f32x4 delta = four(kDelta, decltype(q)::value);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int x = 4 * q + e;
-        float cap = 1.f;
-        p[x] = weight<PLAIN>(score, s[x], factor, PLAIN ? 0.f : slope[e] * fabsf(ahead[e] - (float)j), stat[e], cap);
-        ds[x] = p[x] * __builtin_fmaf(dp[x], d_factor, -delta[e]);
-        if (!PLAIN) ds[x] *= cap;
-        p[x] *= p_factor;
+        const int x = 4 * decltype(q)::value + e;
+        ds[x] = p[x] * __builtin_fmaf(s[1][x], d_factor, -delta[e]);
+        if (!PLAIN) ds[x] *= cap[x];
       }
-      if (!whole) {
-        const f32x4 lo = *reinterpret_cast<const f32x4 *>(of + 32 * kLo + n), hi = *reinterpret_cast<const f32x4 *>(of + 32 * kHi + n);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool sees = j >= (int)bits_of(lo[e]) && j < (int)bits_of(hi[e]);
-          p[4 * q + e] = sees ? p[4 * q + e] : 0.f;
-          ds[4 * q + e] = sees ? ds[4 * q + e] : 0.f;
-        }
-      }
-    }
-    Weights w;
-    w.set(p);
-    add_product<DP>(dvs, at + 3 * BLOCK, w);
-    const int new_unit = gradient_unit(ds, eq, unit);
+    });
+    const int new_unit = gradient_unit(ds, held, eq, unit);
     if (new_unit < unit) {
       multiply(dks, __builtin_ldexpf(1.f, max(new_unit - unit, -200)));
+      keep<(DP > 64)>(dks);
       unit = new_unit;
     }
-    if (unit == kNoUnit) continue;  // nothing but zeros so far
-#pragma unroll
-    for (int x = 0; x < 16; ++x) ds[x] = __builtin_ldexpf(ds[x], unit - eq);
-    w.set(ds);
-    add_product<DP>(dks, at + 2 * BLOCK, w);
+    Weights wd;
+    const int shift = unit == kNoUnit ? 0 : unit - eq - held;  // nothing but zeros so far
+    add_product<DP, AHEAD>(dvs, at + 3 * BLOCK, w, [&](auto place) {
+      spread<decltype(place)::value, 0, 3 * DP / 16, 8>([&](auto n_c) {
+        constexpr int n = decltype(n_c)::value;
+        wd.set<n>(__builtin_ldexpf(ds[2 * n], shift), __builtin_ldexpf(ds[2 * n + 1], shift));
+      });
+    });
+    add_product<DP, AHEAD>(dks, at + 2 * BLOCK, wd, Nothing{});
   }
+  arrived();  // what the last step has fetched
   if (!live) return;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
-      dks[e][x] = unit == kNoUnit ? 0.f : __builtin_ldexpf(dks[e][x], -13 - unit);
+      dks[e][x] = unit == kNoUnit ? 0.f : __builtin_ldexpf(dks[e][x], -unit);
       dvs[e][x] = __builtin_ldexpf(dvs[e][x], -13 - unit_v);
     }
   const int64_t all = (int64_t)c.batch * c.tk * c.key_heads * c.dim, key = c.key_at(b, g, j);
@@ -847,7 +971,7 @@ Exponents pair_backward(const Call &c, const float *out, const float *stat, cons
       hipLaunchKernelGGL((plain ? dq_kernel<DP, true> : dq_kernel<DP, false>), dim3((unsigned)(heads * row_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.k, l.v, l.kt, ex,
                          rows, dq, row_tiles);
     if (keys)
-      hipLaunchKernelGGL((plain ? dkv_kernel<DP, true> : dkv_kernel<DP, false>), dim3((unsigned)(heads * key_tiles * pieces)), dim3(kThreads), 0, s, c, l.q, l.d, l.qt, l.dt,
+      hipLaunchKernelGGL((plain ? dkv_kernel<DP, true> : dkv_kernel<DP, false>), dim3((unsigned)((heads * pieces + 7) / 8 * 8 * key_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.qt, l.dt,
                          l.k, l.v, ex, l.info, dk, dv, parts, key_tiles, pieces);
   });
   return ex;
