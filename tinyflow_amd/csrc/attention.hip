@@ -889,13 +889,6 @@ extern "C" int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHa
   int pieces = 1;
   const bool pairs = all_rows && all_keys && pair_suits(c, true);
   if ((dkey || dvalue) && key_groups) pieces = (int)std::min<int64_t>(((pairs && c.dim <= 64 ? 4 : 2) * num_cus() + key_groups - 1) / key_groups, std::max(1, c.rows / 256));
-  // on pairs whole (b, key head, piece)s are dealt to the eight XCDs: a multiple of eight of them where that takes at most half as many again
-  if (pairs)
-    for (int more = pieces; more <= pieces + pieces / 2 && more <= std::max(1, c.rows / 256); ++more)
-      if (head_pairs * more % 8 == 0) {
-        pieces = more;
-        break;
-      }
   TF_REQUIRE(head_pairs * row_tiles < kMaxGroups && key_groups * pieces < kMaxGroups && (all_rows + 3) / 4 < kMaxGroups,
              "too many sequences, heads and queries for a launch");
   TF_REQUIRE(!being_captured(s), "the backward pass takes scratch, which a captured stream cannot give back");

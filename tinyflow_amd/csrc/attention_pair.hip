@@ -298,7 +298,10 @@ struct Weights {
     constexpr int t = n / 4, e = 2 * (n % 4);
     const f32x2 x = {a, b};
     const f16x2 top = __builtin_convertvector(x, f16x2);
-    const f32x2 left = {a - (float)top[0], b - (float)top[1]};
+    // what is left, from the fp16 number as it lies: the compiler would widen it first
+    f32x2 left;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(left[0]) : "v"(top), "v"(a));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(left[1]) : "v"(top), "v"(b));
     const f16x2 rest = __builtin_convertvector(left, f16x2);
     h[t][e] = top[0];
     h[t][e + 1] = top[1];
@@ -361,11 +364,17 @@ __device__ __forceinline__ void keep(f32x16 (&sum)[N]) {
     for (int d = 0; d < N; ++d) asm volatile("" : "+a"(sum[d]));
 }
 
-// Brings 1 KB from `from` to LDS at `to`, 16 bytes a lane.  Written out because the compiler takes every read of LDS for a reader of the loads
-// into it that are under way, and waits for them; `arrived` is the wait that they need.  It writes no register.
+// Brings one or two KB from `from` + OFFSET to LDS at `to` + OFFSET, 16 bytes a lane.  Written out because the compiler takes every read of LDS for a
+// reader of the loads into it that are under way, and waits for them; `arrived` is the wait that they need.  They write no register.
+template <int OFFSET, bool TWO>
 __device__ __forceinline__ void fetch(uint32_t to, const char *from) {
-  const uint32_t at = __builtin_amdgcn_readfirstlane(to), lane = threadIdx.x % 64 * 16u;
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(at), "v"(lane), "s"(from) : "memory");
+  const uint32_t lane = threadIdx.x % 64 * 16u;
+  if constexpr (TWO)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3\n\tglobal_load_lds_dwordx4 %1, %2 offset:%4" ::"s"(to), "v"(lane),
+                 "s"(from), "n"(OFFSET), "n"(OFFSET + 1024)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3" ::"s"(to), "v"(lane), "s"(from), "n"(OFFSET) : "memory");
 }
 // Everything that this wave has fetched, and read from LDS, has arrived, in all waves.
 __device__ __forceinline__ void arrived() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -383,21 +392,22 @@ __device__ inline int scalar(const int *p) { return *(const __attribute__((addre
 __device__ inline float unscaled(float factor, int a, int b) { return __builtin_ldexpf(factor, max(-(a + b), -80)); }
 
 
-// Block `index` of each of N operands, one behind the other in LDS from `to` on: N DP / 32 fetches of each of four waves, every fourth fragment.
+// Block `index` of each of N operands, one behind the other in LDS from `to` on: each of four waves fetches a quarter of each.
 template <int DP, int N>
 struct Blocks {
+  static constexpr int QUARTER = DP / 32, EACH = (QUARTER + 1) / 2, kCount = N * EACH;  // fragments, fetches
   const char *from[N];
   uint32_t to;
-  int wave;
-  __device__ __forceinline__ Blocks(const char *const (&of)[N], int64_t index, uint32_t at) : to(at), wave(__builtin_amdgcn_readfirstlane(threadIdx.x / 64 % 4)) {
-    static_for<N>([&](auto n) { from[decltype(n)::value] = uniform(of[decltype(n)::value] + index * block_size(DP)) + wave * kFragment; });
+  __device__ __forceinline__ Blocks(const char *const (&of)[N], int64_t index, uint32_t at) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64 % 4);
+    to = __builtin_amdgcn_readfirstlane(at + (uint32_t)(wave * QUARTER * kFragment));
+    static_for<N>([&](auto n) { from[decltype(n)::value] = uniform(of[decltype(n)::value] + index * block_size(DP) + wave * QUARTER * kFragment); });
   }
   template <int f>
   __device__ __forceinline__ void one() const {
-    constexpr int n = f / (DP / 32), i = f % (DP / 32);
-    fetch(to + (uint32_t)(n * block_size(DP) + (4 * i + wave) * kFragment), from[n] + 4 * i * kFragment);
+    constexpr int n = f / EACH, i = f % EACH * 2;
+    fetch<i * kFragment, (i + 1 < QUARTER)>(to + (uint32_t)(n * block_size(DP)), from[n]);
   }
-  static constexpr int kCount = N * DP / 32;
   __device__ __forceinline__ void all() const {
     static_for<kCount>([&](auto f) { one<decltype(f)::value>(); });
   }
@@ -682,37 +692,28 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   constexpr int BLOCK = (int)block_size(DP), SLOT = 4 * BLOCK + kInfoBytes, AHEAD = DP <= 64 ? 1 : 3;
   __shared__ __align__(16) char lds[2][SLOT];
   __shared__ int range[2];
-  // A (b, key head) and a piece of its rows belong to one XCD, whose workgroups then walk the same rows at the same time: the rows come
-  // from its L2 for all but the first.  XCDs take them back and forth, later rows, which see more keys in a causal pass, first; earlier keys, which
-  // more rows see, come first.
-  const int heads = c.batch * c.key_heads, turns = (heads * pieces + 7) / 8, xcd = (int)blockIdx.x % 8;
-  const int turn = (int)blockIdx.x / 8 % turns, tile = (int)blockIdx.x / 8 / turns, of_xcd = 8 * turn + (turn % 2 ? 7 - xcd : xcd);
-  if (of_xcd >= heads * pieces) return;
-  const int bg = of_xcd % heads, piece = pieces - 1 - of_xcd / heads, b = bg / c.key_heads, g = bg % c.key_heads;
+  // Earlier keys, which more rows see in a causal pass, first.
+  const int heads = c.batch * c.key_heads, bg = (int)blockIdx.x % heads, piece = (int)blockIdx.x / heads % pieces, tile = (int)blockIdx.x / heads / pieces;
+  const int b = bg / c.key_heads, g = bg % c.key_heads;
   const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int tile_lo = tile * kRows, tile_hi = min(c.tk, tile_lo + kRows);
   if (__syncthreads_or(ex.bad_rows_of(bg, tile_lo, tile_hi) | ex.bad_keys(bg, tile_lo / 32, kRows / 32))) return;
   const int64_t row_block = (int64_t)bg * ex.row_blocks;
-  // The blocks of rows that see one of the keys.  Without spans pieces are the same rows for all keys; with them they may be few of all rows, and
-  // are cut as they are.
-  const int from_block = c.spans ? 0 : (int)((int64_t)ex.row_blocks * piece / pieces);
-  const int to_block = c.spans ? ex.row_blocks : (int)((int64_t)ex.row_blocks * (piece + 1) / pieces);
-  if (threadIdx.x == 0) range[0] = to_block, range[1] = 0;
+  // The blocks of rows that see one of the keys, cut in pieces.  (The same rows for all tiles in a piece, one (b, key head, piece) to an XCD, came from
+  // its L2 and left a third of the CUs without work in a causal pass: causal 4096 x 16 heads of 128 685 us, or 475 with tiles from both ends in one
+  // workgroup; these 420.)
+  if (threadIdx.x == 0) range[0] = ex.row_blocks, range[1] = 0;
   __syncthreads();
   {
-    int lo = to_block, hi = 0;
-    for (int e = from_block + threadIdx.x; e < to_block; e += kThreads)
+    int lo = ex.row_blocks, hi = 0;
+    for (int e = threadIdx.x; e < ex.row_blocks; e += kThreads)
       if (ex.hulls[row_block + e].meets(tile_lo, tile_hi)) lo = min(lo, e), hi = max(hi, e + 1);
     atomicMin(&range[0], lo);
     atomicMax(&range[1], hi);
   }
   __syncthreads();
-  int begin = __builtin_amdgcn_readfirstlane(range[0]), end = __builtin_amdgcn_readfirstlane(range[1]);
-  if (c.spans) {
-    const int first = begin, steps = max(0, end - begin);
-    begin = first + (int)((int64_t)steps * piece / pieces);
-    end = first + (int)((int64_t)steps * (piece + 1) / pieces);
-  }
+  const int first = __builtin_amdgcn_readfirstlane(range[0]), steps = max(0, __builtin_amdgcn_readfirstlane(range[1]) - first);
+  const int begin = first + (int)((int64_t)steps * piece / pieces), end = first + (int)((int64_t)steps * (piece + 1) / pieces);
   const int j0 = tile_lo + wave * 32, j = j0 + lane % 32;
   const bool live = j < c.tk;
   const int64_t key_block = (int64_t)bg * ex.key_blocks + min(tile * (kRows / 32) + wave, ex.key_blocks - 1);
@@ -730,7 +731,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   const char *const from[4] = {qs, ds_, qts, dts};
   const uint32_t to = lds_address(&lds[0][0]);
   auto fetch_info = [&](int step, int slot) {
-    if (wave == 0) fetch(to + (uint32_t)(slot * SLOT + 4 * BLOCK), uniform(info + (row_block + step) * kInfoBytes));
+    if (wave == 0) fetch<0, false>(__builtin_amdgcn_readfirstlane(to + (uint32_t)(slot * SLOT + 4 * BLOCK)), uniform(info + (row_block + step) * kInfoBytes));
   };
   auto hull_of = [&](int step, Hull &seen) {
     seen.lo = scalar(&ex.hulls[row_block + step].lo);
@@ -971,7 +972,7 @@ Exponents pair_backward(const Call &c, const float *out, const float *stat, cons
       hipLaunchKernelGGL((plain ? dq_kernel<DP, true> : dq_kernel<DP, false>), dim3((unsigned)(heads * row_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.k, l.v, l.kt, ex,
                          rows, dq, row_tiles);
     if (keys)
-      hipLaunchKernelGGL((plain ? dkv_kernel<DP, true> : dkv_kernel<DP, false>), dim3((unsigned)((heads * pieces + 7) / 8 * 8 * key_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.qt, l.dt,
+      hipLaunchKernelGGL((plain ? dkv_kernel<DP, true> : dkv_kernel<DP, false>), dim3((unsigned)(heads * pieces * key_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.qt, l.dt,
                          l.k, l.v, ex, l.info, dk, dv, parts, key_tiles, pieces);
   });
   return ex;
