@@ -230,10 +230,24 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
 // v_mfma_f32_16x16x4: a lane supplies A[lane % 16][lane / 16] and B[lane / 16][lane % 16] and holds D[4 (lane / 16) + v][lane % 16].  Scores: keys by
 // rows, columns 16 g + 4 (lane / 16) + e of both.  The values' product takes key 4 (lane / 16) + v at step v, as the scores lie,
 // and sums column 64 d + 4 (row of D) + e into sum[d][e]: both operands are 16-byte loads from where they lie in memory, 16 lanes side by side.
+// What bounds it is HBM as long as a wave's next step is on its way all the time that one is worked on: with the next keys fetched behind the
+// scores and the next values behind their product, and loads behind branches, of which all are waited for, 100 003 keys of 2 heads of 128 took 49 us,
+// and so 35-39 (5.2-5.9 TB/s).
 constexpr int kFewKeys = 16;  // of a wave's step
 
+// op over the four lanes with the same lane % 16
+template <class Op>
+__device__ inline float over_quarters(float v, const Op &op) {
+  uint32_t bits = __builtin_bit_cast(uint32_t, v);
+  auto halves = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);
+  v = op(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+  bits = __builtin_bit_cast(uint32_t, v);
+  halves = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+  return op(__uint_as_float(halves[0]), __uint_as_float(halves[1]));
+}
+
 template <int DP, int NC>
-__global__ __launch_bounds__(kThreads) void few_kernel(const Call c, float *out, float *stat, const Pieces pieces, int keys_a_piece) {
+__global__ __launch_bounds__(kThreads, DP * NC <= 128 ? 2 : 1) void few_kernel(const Call c, float *out, float *stat, const Pieces pieces, int keys_a_piece) {
   constexpr int GD = DP / 16, VD = DP / 64;
   const int bg = (int)blockIdx.x % (c.batch * c.key_heads), piece = (int)blockIdx.x / (c.batch * c.key_heads);
   const int b = bg / c.key_heads, g = bg % c.key_heads;
@@ -292,30 +306,43 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Call c, float *out,
   }
   const int64_t key_step = (int64_t)c.key_heads * c.dim;
   const float *k0 = c.k + c.key_at(b, g, 0), *v0 = c.v + c.key_at(b, g, 0);
-  f32x4 k[GD], vals[4][VD];
-  auto load_keys = [&](int j0) {  // keys behind the last are the last again
-    const float *row = k0 + (int64_t)min(j0 + col, end - 1) * key_step;
-#pragma unroll
-    for (int e = 0; e < GD; ++e) {
-      const int d = 16 * e + 4 * quarter;
-      k[e] = d < c.dim ? load4(row + d, c.dim - d) : f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+  // Loads without a branch, so that it is known how many are under way: columns that are none have an offset behind the buffer and read as zero, and
+  // keys behind the last are the last again.
+  typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned u32x4;
+  f32x4 keys[2][GD], values[2][4][VD];
+  auto fetch = [&](const float *base, int row, int column) {
+    const uint32_t at = (uint32_t)row * (uint32_t)(key_step * 4) + (uint32_t)column * 4u;
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(base), 0, 0x7fffffff, 0x00020000);
+    f32x4 x = __builtin_bit_cast(f32x4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(r, (int)(column < c.dim ? at : 0x80000000u), 0, 0));
+    return x;
   };
-  auto load_values = [&](int j0) {
+  auto load = [&](auto parity, int j0) {
+    j0 = __builtin_amdgcn_readfirstlane(min(j0, end - 1));
+    const float *kb = k0 + j0 * key_step, *vb = v0 + j0 * key_step;
+    const int last = end - 1 - j0;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const float *row = v0 + (int64_t)min(j0 + 4 * quarter + v, end - 1) * key_step;
+    for (int e = 0; e < GD; ++e) keys[decltype(parity)::value][e] = fetch(kb, min(col, last), 16 * e + 4 * quarter);
 #pragma unroll
-      for (int d = 0; d < VD; ++d) {
-        const int at = 64 * d + 4 * col;
-        vals[v][d] = at < c.dim ? load4(row + at, c.dim - at) : f32x4{0.f, 0.f, 0.f, 0.f};
-      }
-    }
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int d = 0; d < VD; ++d) values[decltype(parity)::value][v][d] = fetch(vb, min(4 * quarter + v, last), 64 * d + 4 * col);
   };
-  int j0 = begin + kFewKeys * wave;
-  if (j0 < end) load_keys(j0), load_values(j0);
-#pragma unroll 1
-  for (; j0 < end; j0 += 4 * kFewKeys) {
+  // rows whose length is no multiple of four: what a load brought from behind their end
+  auto cut = [&](f32x4 &x, int column) {
+#pragma unroll
+    for (int i = 1; i < 4; ++i) x[i] = column + i < c.dim ? x[i] : 0.f;
+  };
+  auto step = [&](auto parity, int j0) {
+    auto &k = keys[decltype(parity)::value];
+    auto &vals = values[decltype(parity)::value];
+    if (c.dim % 4) {
+#pragma unroll
+      for (int e = 0; e < GD; ++e) cut(k[e], 16 * e + 4 * quarter);
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+#pragma unroll
+        for (int d = 0; d < VD; ++d) cut(vals[v][d], 64 * d + 4 * col);
+    }
     const bool whole = inner_lo <= j0 && inner_hi >= j0 + kFewKeys && end >= j0 + kFewKeys;
     float p[NC][4];
 #pragma unroll
@@ -333,8 +360,7 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Call c, float *out,
         if (!whole) p[n][v] = j >= lo[n] && j < hi[n] && j < end ? p[n][v] : kNone;
         most = fmaxf(most, p[n][v]);
       }
-      most = fmaxf(most, __shfl_xor(most, 16));
-      most = fmaxf(most, other_half(most));
+      most = over_quarters(most, [](float a, float b) { return fmaxf(a, b); });
       const float next = fmaxf(top[n], most), from = next == kNone ? 0.f : next;
       const float fade = __builtin_amdgcn_exp2f(top[n] - from);
       top[n] = next;
@@ -352,8 +378,6 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Call c, float *out,
           for (int e = 0; e < 4; ++e) o[n][d][e] *= fade;
       }
     }
-    const int next = j0 + 4 * kFewKeys;
-    if (next < end) load_keys(next);
     if (!whole) {
       // values that are not finite: only to the rows that see them
       bool ok = true;
@@ -400,7 +424,17 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Call c, float *out,
         for (int d = 0; d < VD; ++d)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[n][d][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vals[v][d][e], p[n][v], o[n][d][e], 0, 0, 0);
-    if (next < end) load_values(next);
+  };
+  constexpr int STEP = 4 * kFewKeys;
+  int j0 = begin + kFewKeys * wave;
+  if (j0 < end) load(IC<0>{}, j0);
+#pragma unroll 1
+  for (; j0 < end; j0 += 2 * STEP) {
+    load(IC<1>{}, j0 + STEP);
+    step(IC<0>{}, j0);
+    if (j0 + STEP >= end) break;
+    load(IC<0>{}, j0 + 2 * STEP);
+    step(IC<1>{}, j0 + STEP);
   }
 
   // the four waves' sums, through LDS in their order
@@ -408,8 +442,7 @@ __global__ __launch_bounds__(kThreads) void few_kernel(const Call c, float *out,
   __shared__ f32x4 parts[3][VD * 4][64];
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
-    total[n] += __shfl_xor(total[n], 16);
-    total[n] += other_half(total[n]);
+    total[n] = over_quarters(total[n], [](float a, float b) { return a + b; });
     if (n) __syncthreads();
     if (quarter == 0) {
       marks[wave][col][0] = top[n];
@@ -803,15 +836,15 @@ extern "C" int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHan
   if (all_rows == 0) return 0;
   float *out = output ? (float *)output->data : nullptr, *stat = statistics ? (float *)statistics->data : nullptr;
   const int64_t head_pairs = (int64_t)batch * c.key_heads;
-  const bool few = c.rows <= 32 && !(c.rows > 16 && c.dim > 128);
+  const bool few = c.rows <= 32 && !(c.rows > 16 && c.dim > 128) && (int64_t)c.key_heads * c.dim < 1 << 24;  // 16 rows are less than 2^31 bytes apart
   const bool pairs = !few && pair_suits(c, false);
   int64_t groups;
   int tiles = 0, keys_a_piece = 0;
   Pieces pieces = {};
   pieces.rows = all_rows;
   if (few) {
-    // about four workgroups a CU; a wave's share of a piece is a multiple of its step
-    const int64_t wanted = std::min<int64_t>(kMostPieces, std::max<int64_t>(1, (4 * num_cus() + head_pairs - 1) / head_pairs));
+    // about two workgroups a CU (one each of 2 / 4 / 8: eight sequences of up to 8 192 keys 48 / 53 / 62 us, one of 100 003 51 / 58 / 68); a wave's share of a piece is a multiple of its step
+    const int64_t wanted = std::min<int64_t>(kMostPieces, std::max<int64_t>(1, (2 * num_cus() + head_pairs - 1) / head_pairs));
     keys_a_piece = std::max<int>(64, (int)(((c.tk + wanted - 1) / wanted + 63) / 64 * 64));
     pieces.count = std::max(1, (c.tk + keys_a_piece - 1) / keys_a_piece);
     groups = head_pairs * pieces.count;
