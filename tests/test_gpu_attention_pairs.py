@@ -1,0 +1,120 @@
+"""Attention on fp16 pairs where splitting could go wrong: blocks of unlike magnitude, of zeros, of rows too unlike for one exponent, and what is not
+finite; both engines against float64."""
+import numpy as np
+import pytest
+
+import attention_ref as ref
+from test_gpu_attention import _check, _data, _run
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("d", [24, 64, 96, 128])
+def test_both_engines(rt, monkeypatch, split, d):
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    _check(rt, *_data(2, 333, 290, 4, 2, d, d), causal=True)
+    _check(rt, *_data(1, 200, 700, 2, 1, d, d), slopes=np.array([0.5, 0.01]), cap=8.0)
+
+
+def test_the_engines_are_two(rt, monkeypatch):
+    """TINYFLOW_SPLIT=0 reaches the calls: the bits differ."""
+    outs = []
+    for split in ("0", "1"):
+        monkeypatch.setenv("TINYFLOW_SPLIT", split)
+        outs.append(_run(rt, *_data(1, 600, 600, 4, 2, 64, 3), causal=True))
+    assert (outs[0][0] != outs[1][0]).any() and (outs[0][2][0] != outs[1][2][0]).any()
+
+
+@pytest.mark.parametrize("which", range(4))
+@pytest.mark.parametrize("power", [-30, -8, 8, 25])
+def test_blocks_of_unlike_magnitude(rt, which, power):
+    """Every other block of 32 rows of one operand by a power of two: sums change their unit on the way, up and down.  (Bounds are of the call's
+    largest values, so the small blocks are compared by themselves below.)"""
+    a = _data(2, 300, 300, 2, 1, 64, 4)
+    x = a[which].reshape(2, 300, -1)
+    blocks = np.arange(300) // 32 % 2 == 1
+    x[:, blocks] *= np.float32(2.0 ** (power if which > 1 else np.clip(power, -8, 3)))   # scores stay in the exponential's range
+    _check(rt, *a, causal=True)
+
+
+def test_small_blocks_by_themselves(rt):
+    """Gradients of documents that are 2^-40 of their neighbours': each document's results have their own digits."""
+    from tinyflow_amd import gpu_op
+    q, k, v, do = _data(1, 320, 320, 2, 2, 64, 5)
+    documents = np.arange(320) // 80
+    small = documents % 2 == 1
+    do[:, small] *= np.float32(2.0 ** -40)
+    v[:, small] *= np.float32(2.0 ** -20)
+    spans = gpu_op.attention_spans(320, documents=documents, causal=True)
+    out, stat, grads = _run(rt, q, k, v, do, spans=spans)
+    for n in range(4):
+        own = documents == n
+        want = ref.Attention(q[:, own], k[:, own], v[:, own], None, None, 0.125, causal=True)
+        ref.assert_within(out[:, own], want.out, want.out_tol, "out of document %d" % n)
+        values = want.backward(out[:, own], stat[:, :, own], do[:, own])
+        for what, got, (value, tol) in zip(("dq", "dk", "dv"), grads, values):
+            off = np.linalg.norm(got[:, own] - value) / np.linalg.norm(value)
+            # blocks of 32 rows span two documents: 2^-39 of the larger one's values is left off, 2^-19 of the smaller one's values
+            # for dv, and for the products of both (2^-60 apart) what the fp32 kernels give
+            assert off <= 2.0 ** -15, "%s of document %d is %.2g off" % (what, n, off)
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_zeros(rt, which):
+    a = _data(1, 160, 200, 2, 1, 40, 6)
+    a[which][:, 30:130] = 0
+    _check(rt, *a, causal=True)
+    a[which][...] = 0
+    _check(rt, *a, causal=True)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e12, 1e30])
+def test_values_and_gradients_at_the_ends_of_the_range(rt, scale):
+    """Values of 1e30 pass what a block may have and take the fp32 kernels; 1e-30 is held as it is."""
+    q, k, v, do = _data(1, 150, 150, 2, 1, 32, 7)
+    _check(rt, q, k, v * np.float32(scale), do / np.float32(max(scale, 1.0)), causal=True)
+
+
+@pytest.mark.parametrize("which", [1, 2])
+def test_rows_too_unlike_for_one_exponent(rt, which):
+    """A key or value of 2^30 times its neighbours: its block is left to the fp32 kernels, in the tiles that see it."""
+    a = _data(1, 400, 400, 2, 1, 64, 8)
+    a[which][0, 210] *= np.float32(2.0 ** 30)
+    if which == 1:
+        a[0][0, :, :, :] *= np.float32(2.0 ** -26)   # scores stay in the exponential's range
+    _check(rt, *a, causal=True)
+
+
+@pytest.mark.parametrize("tq,tk", [(40, 3000), (128, 1100), (33, 257)])
+def test_cut_along_the_keys(rt, tq, tk):
+    """Few rows over many keys: pieces of their own units, joined."""
+    q, k, v, do = _data(1, tq, tk, 2, 2, 48, 9)
+    v[:, tk // 2:] *= np.float32(64)
+    k[:, : tk // 3] *= np.float32(0.01)
+    spans = np.zeros((tq, 2), np.float32)
+    spans[:, 1] = tk - np.arange(tq)
+    spans[::5] = 0
+    _check(rt, q, k, v, do, spans=spans)
+
+
+def test_one_bad_gradient_row(rt):
+    """A gradient that is not finite reaches the keys that its query sees, and no others."""
+    q, k, v, do = _data(1, 300, 300, 1, 1, 64, 10)
+    out, stat, _ = clean = _run(rt, q, k, v, do, causal=True)
+    do[0, 170, 0, 3] = np.inf
+    dq, dk, dv = _run(rt, q, k, v, do, causal=True)[2]
+    assert not np.isfinite(dv[0, :171, 0, 3]).any() and np.isfinite(dv[0, 171:]).all() and np.isfinite(dk[0, 171:]).all()
+    assert np.isnan(dq[0, 170]).all() and np.isfinite(np.delete(dq[0], 170, 0)).all()
+    for got, was in zip((dk, dv), clean[2][1:]):
+        np.testing.assert_allclose(got[0, 171:], was[0, 171:], rtol=1e-4, atol=1e-6 * np.abs(was).max())
+
+
+def test_more_rows_than_one_workgroup_a_cu(rt):
+    """Tiles, pieces and heads beyond what is resident at once; the same bits again."""
+    a = _data(3, 700, 700, 6, 3, 64, 11)
+    first = _check(rt, *a, causal=True)
+    again = _run(rt, *a, causal=True)
+    np.testing.assert_array_equal(first[0], again[0])
+    for x, y in zip(first[2], again[2]):
+        np.testing.assert_array_equal(x, y)

@@ -557,7 +557,7 @@ class SwapExecutor(object):
             self.swap_out_at, self.swap_in_at, self.release_at, self.recompute_at = by_node
             return
         cheap = (ad.BNForwardOp, ad.ActivationForwardOp, ad.ReluOp, ad.LayerNormForwardOp, ad.GatedActivationOp,
-                 ad.CounterDropoutOp)
+                 ad.CounterDropoutOp, ad.HeadRotaryOp)
         again = (lambda n: isinstance(n.op, cheap)) if (self.swap and self.recompute) else None
         timing = {}
         if self.host_link_bytes_per_second:
@@ -601,6 +601,14 @@ class SwapExecutor(object):
             # both projections; dx, or one of the two weights' gradients
             rows, (width, inner) = self.tensors[node.inputs[0]].shape[0], self.tensors[node.inputs[1]].shape
             flops, rate = (2.0 if getattr(node, "type", 0) else 4.0) * rows * width * inner, 300e12
+        elif isinstance(node.op, (ad.AttentionForwardOp, ad.AttentionStatisticsOp, ad.AttentionBackwardOp)):
+            # a product of queries and keys and one of the weights and the values; backward both again, and one a gradient
+            queries, keys = node.op.geometry(node, [self.tensors[i].shape for i in node.inputs[:3]])
+            products = 3.0 if isinstance(node.op, ad.AttentionBackwardOp) else 2.0
+            flops = 2.0 * products * np.prod(self.tensors[node.inputs[0]].shape, dtype=np.float64) * keys
+            rate = 300e12
+            if node.numbers[-1]:
+                flops *= 0.5
         elif isinstance(node.op, ad.MatMulOp):
             a = self.tensors[node.inputs[0]].shape
             flops = 2.0 * np.prod(self.tensors[node].shape, dtype=np.float64) * (a[0] if node.matmul_attr_trans_A

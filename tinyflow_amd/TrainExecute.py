@@ -543,8 +543,8 @@ def find_groups(topo_order, shapes, unavailable, roles, joins):
 
 
 def find_siblings(topo_order, unavailable):
-    """Nodes that one call computes: the gradients of a layer norm or of a gated feed-forward product, which have the same
-    inputs, and a gated product with the projections that it is made of.  Returns first node -> all of them, in order; they
+    """Nodes that one call computes: the gradients of a layer norm, of a gated feed-forward product, of a head's norm and rotation or of
+    an attention, which have the same inputs, a gated product with the projections that it is made of, and an attention with its statistics.  Returns first node -> all of them, in order; they
     run at the first one's place, where its inputs are there and no parameter that they read has been updated, since updates stand behind
     the last reader.  Every array holds what it would."""
     siblings, first_of = {}, {}
@@ -553,6 +553,12 @@ def find_siblings(topo_order, unavailable):
             continue
         if isinstance(n.op, (ad.LayerNormBackwardOp, ad.GatedBackwardOp)):
             key = (n.op, tuple(n.inputs), n.eps if isinstance(n.op, ad.LayerNormBackwardOp) else n.activation)
+        elif isinstance(n.op, ad.HeadRotaryBackwardOp):
+            key = (n.op, tuple(n.inputs), n.heads, n.has, n.turn)
+        elif isinstance(n.op, ad.AttentionBackwardOp):
+            key = (n.op, tuple(n.inputs), n.numbers, n.has)
+        elif isinstance(n.op, (ad.AttentionForwardOp, ad.AttentionStatisticsOp)):
+            key = ("attention", tuple(n.inputs), n.numbers, n.has)
         elif isinstance(n.op, ad.GatedProjectionOp):
             key = n
         elif isinstance(n.op, ad.GatedActivationOp) and n.inputs[0] in first_of:
@@ -572,6 +578,11 @@ def _sibling_compute(members):
     if isinstance(members[0].op, ad.GatedProjectionOp):
         def compute(node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream):
             return gpu_op.gated_feed_forward(*input_vals, *output_val, members[1].activation, cudaStream)
+    elif isinstance(members[0].op, (ad.AttentionForwardOp, ad.AttentionStatisticsOp)):
+        kinds = [type(n.op) for n in members]
+
+        def compute(node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream):
+            return ad.AttentionForwardOp.compute_several(dict(zip(kinds, output_val)), node, input_vals, cudaStream)
     else:
         types = [n.type for n in members]
 

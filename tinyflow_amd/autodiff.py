@@ -13,6 +13,7 @@ graph, which decides which C entry points run, in which order, on which shapes.
 Every ``compute`` goes through ``gpu_op`` into libc_runtime_api.so; there is no
 numpy branch (the reference keeps one for a subset of ops, autodiff.py:312-779).
 """
+import math
 import random
 from functools import reduce
 from operator import add
@@ -1020,6 +1021,187 @@ class CounterDropoutBackwardOp(Op):
 
 # -------------------------------------------------------------------- optimizer
 
+# ------------------------- norm, rotation of heads, attention (no counterparts in the reference)
+
+def _head_columns(shape, heads):
+    """Columns of a head of an array of heads: [.., heads * D], or [.., .., heads, D]."""
+    columns = shape[-1] if len(shape) == 4 else shape[-1] // heads
+    if columns < 1 or (shape[2] != heads if len(shape) == 4 else shape[-1] % heads):
+        raise ValueError("%d heads of an array %s" % (heads, shape))
+    return columns
+
+
+class HeadRotaryOp(Op):
+    """x / sqrt(mean(x^2) + eps) * gamma of every head, its first columns turned by position * frequency; without ``gamma`` no norm,
+    without ``frequencies`` no rotation (gpu_op.head_rotary).  Positions and frequencies have no gradient.  Keeps nothing for
+    the backward nodes."""
+
+    def __call__(self, node_A, heads, gamma=None, positions=None, frequencies=None, amplitude=1.0, interleaved=False, eps=1e-6):
+        if (positions is None) != (frequencies is None):
+            raise ValueError("head_rotary_op: positions and frequencies go together")
+        node = Op.__call__(self)
+        node.inputs = [node_A] + [n for n in (gamma, positions, frequencies) if n is not None]
+        node.name = "HeadRotary"
+        node.heads = heads
+        node.has = gamma is not None, frequencies is not None
+        node.turn = amplitude, interleaved, eps
+        return node
+
+    @staticmethod
+    def operands(node, values):
+        """(gamma, positions, frequencies) of what stands behind the input, None for those that are not there."""
+        norm, rotates = node.has
+        return (values[0] if norm else None,) + (tuple(values[int(norm):int(norm) + 2]) if rotates else (None, None))
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        gamma, positions, frequencies = self.operands(node, input_vals[1:])
+        amplitude, interleaved, eps = node.turn
+        gpu_op.head_rotary([gpu_op.head_part(input_vals[0], gamma, output_val, node.heads, rotate=frequencies is not None)],
+                           positions, frequencies, amplitude, interleaved, eps, None, cudaStream)
+        return 0
+
+    def gradient(self, node, output_grad):
+        norm, _ = node.has
+        grads = [head_rotary_backward_op(node, output_grad, type) for type in range(1 + norm)]
+        return grads + [zeroslike_op(n) for n in node.inputs[1 + norm:]]
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        columns = _head_columns(input_shapes[0], node.heads)
+        gamma, _, frequencies = self.operands(node, input_shapes[1:])
+        if gamma is not None and tuple(gamma) != (columns,):
+            raise ValueError("head_rotary_op: gamma %s for heads of %d columns" % (gamma, columns))
+        if frequencies is not None and (len(frequencies) != 1 or 2 * frequencies[0] > columns):
+            raise ValueError("head_rotary_op: frequencies %s for heads of %d columns" % (frequencies, columns))
+        return input_shapes[0]
+
+
+class HeadRotaryBackwardOp(Op):
+    """inputs: those of the forward node, dy; type 0: gradient w.r.t. x, 1: gamma"""
+
+    def __call__(self, forward, output_grad, type):
+        node = Op.__call__(self)
+        node.inputs = list(forward.inputs) + [output_grad]
+        node.name = "HeadRotaryBackward"
+        node.heads, node.has, node.turn = forward.heads, forward.has, forward.turn
+        node.type = type
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        return self.compute_several({node.type: output_val}, node, input_vals, cudaStream)
+
+    @staticmethod
+    def compute_several(outputs, node, input_vals, cudaStream):
+        """Those of the two gradients that ``outputs`` has, by type, in one call."""
+        gamma, positions, frequencies = HeadRotaryOp.operands(node, input_vals[1:-1])
+        amplitude, interleaved, eps = node.turn
+        part = gpu_op.head_gradient_part(input_vals[0], gamma, input_vals[-1], outputs.get(0), outputs.get(1), node.heads,
+                                         rotate=frequencies is not None)
+        return gpu_op.head_rotary_backward([part], positions, frequencies, amplitude, interleaved, eps, cudaStream)
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[node.type]
+
+
+class _AttentionNodes(Op):
+    """What the nodes of an attention share.  node.numbers: batch, heads, key_heads, scale (None: 1 / sqrt(columns)), cap, causal;
+    node.has: whether there are spans and slopes among the inputs."""
+
+    def make(self, inputs, name, numbers, has):
+        node = Op.__call__(self)
+        node.inputs, node.name, node.numbers, node.has = inputs, name, numbers, has
+        return node
+
+    @staticmethod
+    def arguments(node, values):
+        """(query, key, value, spans, slopes), the values behind them, and the numbers of the call."""
+        rest = list(values[3:])
+        masks = [rest.pop(0) if there else None for there in node.has]
+        batch, heads, key_heads, scale, cap, causal = node.numbers
+        if scale is None:
+            scale = _head_columns(values[0].shape, heads) ** -0.5
+        return list(values[:3]) + masks, rest, (batch, heads, key_heads, scale, cap, causal)
+
+    @staticmethod
+    def geometry(node, shapes):
+        """(queries, keys) of a sequence"""
+        batch, heads, key_heads = node.numbers[:3]
+        query, key, value = shapes[:3]
+        columns = _head_columns(query, heads)
+        if tuple(key) != tuple(value) or _head_columns(key, key_heads) != columns or heads % key_heads:
+            raise ValueError("attention: %d heads of %s, %d of %s and %s" % (heads, query, key_heads, key, value))
+        rows = [int(math.prod(s)) // (n * columns) for s, n in ((query, heads), (key, key_heads))]
+        if any(r % batch for r in rows):
+            raise ValueError("attention: %d and %d rows of %d sequences" % (rows[0], rows[1], batch))
+        return rows[0] // batch, rows[1] // batch
+
+
+class AttentionForwardOp(_AttentionNodes):
+    """softmax(scores) value (gpu_op.attention_forward); spans and slopes, nodes that may be None, have no gradient."""
+
+    def __call__(self, query, key, value, batch, heads, key_heads=None, scale=None, cap=0.0, causal=False, spans=None, slopes=None):
+        numbers = batch, heads, heads if key_heads is None else key_heads, scale, cap, bool(causal)
+        masks = [n for n in (spans, slopes) if n is not None]
+        return self.make([query, key, value] + masks, "AttentionForward", numbers, (spans is not None, slopes is not None))
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        return self.compute_several({AttentionForwardOp: output_val}, node, input_vals, cudaStream)
+
+    @staticmethod
+    def compute_several(outputs, node, input_vals, cudaStream):
+        """Output and statistics, those that ``outputs`` has, by the class of their node, in one call."""
+        operands, _, numbers = _AttentionNodes.arguments(node, input_vals)
+        return gpu_op.attention_forward(*operands, outputs.get(AttentionForwardOp), outputs.get(AttentionStatisticsOp), *numbers,
+                                        cudaStream)
+
+    def gradient(self, node, output_grad):
+        statistics = attention_statistics_op(node)
+        grads = [attention_backward_op(node, statistics, output_grad, type) for type in range(3)]
+        return grads + [zeroslike_op(n) for n in node.inputs[3:]]
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        self.geometry(node, input_shapes)
+        return input_shapes[0]
+
+
+class AttentionStatisticsOp(_AttentionNodes):
+    """The logarithm of each query's sum of exponentials, which the backward nodes read: (batch, heads, queries)."""
+
+    def __call__(self, forward):
+        return self.make(list(forward.inputs), "AttentionStatistics", forward.numbers, forward.has)
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        return AttentionForwardOp.compute_several({AttentionStatisticsOp: output_val}, node, input_vals, cudaStream)
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return node.numbers[0], node.numbers[1], self.geometry(node, input_shapes)[0]
+
+
+class AttentionBackwardOp(_AttentionNodes):
+    """inputs: those of the forward node, its output, the statistics, dy; type 0: gradient w.r.t. query, 1: key, 2: value"""
+
+    def __call__(self, forward, statistics, output_grad, type):
+        node = self.make(list(forward.inputs) + [forward, statistics, output_grad], "AttentionBackward", forward.numbers, forward.has)
+        node.type = type
+        return node
+
+    def compute(self, node, input_vals, output_val, cudnnHandle, cublasHandle, cudaStream, use_numpy=False):
+        _no_numpy(use_numpy)
+        return self.compute_several({node.type: output_val}, node, input_vals, cudaStream)
+
+    @staticmethod
+    def compute_several(outputs, node, input_vals, cudaStream):
+        """Those of the three gradients that ``outputs`` has, by type, in one call."""
+        operands, rest, numbers = _AttentionNodes.arguments(node, input_vals)
+        return gpu_op.attention_backward(*operands, *rest, *[outputs.get(type) for type in range(3)], *numbers, cudaStream)
+
+    def infer_shape(self, node, input_shapes, cudnnHandle):
+        return input_shapes[node.type]
+
+
 class SgdOp(Op):
     """In-place w -= lr * g; produces no value of its own (reference autodiff.py:2028-2047)."""
 
@@ -1075,6 +1257,21 @@ def dense(X, W, b):
 def gated_feed_forward(X, gate, up, activation="silu"):
     """activation(X gate) * (X up), "sigmoid", "relu", "silu" or "gelu" (no counterpart in the reference)"""
     return gated_activation_op(gated_projection_op(X, gate, up), activation)
+
+
+def self_attention(X, Wq, Wk, Wv, Wo, batch, heads, key_heads=None, gammas=None, positions=None, frequencies=None, spans=None,
+                   slopes=None, cap=0.0, causal=True):
+    """attention(rotated(X Wq), rotated(X Wk), X Wv) Wo for X [batch * tokens, width]; ``gammas``, if given, norm the heads of queries and
+    keys.  No counterpart in the reference."""
+    key_heads = heads if key_heads is None else key_heads
+    gammas = gammas or (None, None)
+    q, k = matmul_op(X, Wq), matmul_op(X, Wk)
+    if gammas[0] is not None or frequencies is not None:
+        q = head_rotary_op(q, heads, gammas[0], positions, frequencies)
+    if gammas[1] is not None or frequencies is not None:
+        k = head_rotary_op(k, key_heads, gammas[1], positions, frequencies)
+    return matmul_op(attention_forward_op(q, k, matmul_op(X, Wv), batch, heads, key_heads, cap=cap, causal=causal, spans=spans,
+                                          slopes=slopes), Wo)
 
 
 def conv2withbias(input, filter, bias, dataformat, padding, strideh, stridew):
@@ -1260,6 +1457,11 @@ gated_activation_backward_op = GatedActivationBackwardOp()
 gated_backward_op = GatedBackwardOp()
 counter_dropout_op = CounterDropoutOp()
 counter_dropout_backward_op = CounterDropoutBackwardOp()
+head_rotary_op = HeadRotaryOp()
+head_rotary_backward_op = HeadRotaryBackwardOp()
+attention_forward_op = AttentionForwardOp()
+attention_statistics_op = AttentionStatisticsOp()
+attention_backward_op = AttentionBackwardOp()
 sgd_op = SgdOp()
 adam_op = AdamOp()
 dropout_forward_op = DropoutForwardOp()

@@ -911,8 +911,8 @@ void pack(const Call &c, Pack &p, hipStream_t s) {
 }  // namespace
 
 bool pair_suits(const Call &c, bool backward) {
-  static const char *off = getenv("TINYFLOW_SPLIT");
-  if (off && off[0] == '0') return false;
+  const char *e = getenv("TINYFLOW_SPLIT");
+  if (e && e[0] == '0') return false;
   const float factor = c.cap > 0.f ? c.scale / c.cap : c.scale;
   if (c.dim > 128 || !(factor > 0x1p-40f && factor < 0x1p40f)) return false;
   if (c.rows < 32 || c.tk < 32) return false;
