@@ -118,3 +118,16 @@ def test_more_rows_than_one_workgroup_a_cu(rt):
     np.testing.assert_array_equal(first[0], again[0])
     for x, y in zip(first[2], again[2]):
         np.testing.assert_array_equal(x, y)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_errors_of_rows_do_not_add_up(rt, d):
+    """Of n independent errors with no mean the sum is beyond six times the root of their squares' sum once in 10^9.  What is summed here is what a gain
+    of all queries, or of all keys, would have for its gradient."""
+    q, k, v, do = _data(1, 1024, 1024, 8, 8, d, 12)
+    out, stat, grads = _run(rt, q, k, v, do, causal=True)
+    values = ref.Attention(q, k, v, None, None, 1 / np.sqrt(d), causal=True).backward(out, stat, do)
+    for what, x, got, (want, _) in (("queries", q, grads[0], values[0]), ("keys", k, grads[1], values[1])):
+        off = ((got - want) * x).sum(3)
+        z = off.sum() / np.sqrt((off * off).sum())
+        assert abs(z) <= 6, "the errors of the %s add up: %.1f" % (what, z)
