@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import attention_ref as ref
+from parity import stable_seed
 from test_gpu_attention import _check, _data, _run
 
 pytestmark = pytest.mark.gpu
@@ -131,3 +132,14 @@ def test_errors_of_rows_do_not_add_up(rt, d):
         off = ((got - want) * x).sum(3)
         z = off.sum() / np.sqrt((off * off).sum())
         assert abs(z) <= 6, "the errors of the %s add up: %.1f" % (what, z)
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("tq,tk", [(1, 1200), (7, 2500), (40, 1500), (150, 1030)])
+def test_gradients_of_few_queries(rt, monkeypatch, split, tq, tk):
+    """The keys are cut; one key of another magnitude leaves its tile, all pieces of it, to the fp32 kernels."""
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    a = _data(2, tq, tk, 2, 2, 48, stable_seed((tq, tk)))
+    _check(rt, *a, causal=True)
+    a[2][1, 700] *= np.float32(2.0 ** 30)
+    _check(rt, *a, causal=True)

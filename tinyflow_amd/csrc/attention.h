@@ -249,9 +249,15 @@ struct Exponents {
 bool pair_suits(const Call &c, bool backward);
 size_t pair_bytes(const Call &c, bool backward);  // of scratch
 Exponents pair_forward(const Call &c, float *out, float *stat, const Pieces &pieces, int tiles, char *scratch, hipStream_t s);
-// Also what prepare_kernel writes to `rows`; dq (unless null), dk and dv (unless both are); `parts` as dkv_kernel takes them
-Exponents pair_backward(const Call &c, const float *out, const float *stat, const float *dout, Row *rows, float *dq, float *dk, float *dv, float *parts,
-                        int row_tiles, int key_tiles, int pieces, char *scratch, hipStream_t s);
+// Where a backward pass writes: dq, or its pieces `row_stride` apart; dk and dv, or `parts` as dkv_kernel takes them.
+struct Gradients {
+  float *dq, *dk, *dv, *parts;
+  int64_t row_stride;
+  int row_pieces, pieces;
+};
+// Also what prepare_kernel writes to `rows`; dq (unless null), dk and dv (unless both are)
+Exponents pair_backward(const Call &c, const float *out, const float *stat, const float *dout, Row *rows, const Gradients &to, int row_tiles, int key_tiles,
+                        char *scratch, hipStream_t s);
 
 }  // namespace attention
 }  // namespace tf

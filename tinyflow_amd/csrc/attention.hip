@@ -5,7 +5,7 @@
 //   rows_kernel    128 rows a workgroup, the fp32 matrix instruction
 // Both can be cut along the keys: pieces write their unnormalised sums with their maximum, join_kernel adds them up in their order.
 // Backward: prepare_kernel (delta, what each row sees), dq_kernel (128 rows a workgroup, walks the keys), dkv_kernel (128 keys a workgroup, walks the
-// rows; cut along the rows where keys are few, sum_kernel adds the pieces).  Both compute the scores again; no sum goes
+// rows); where that leaves CUs without work the walks are cut, and sum_kernel adds the pieces.  Both compute the scores again; no sum goes
 // through atomics, so the bits do not depend on the order in which workgroups run.
 #include "attention.h"
 #include "internal.h"
@@ -583,13 +583,14 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(const Call c, const f
   rows[at] = row;
 }
 
+// 128 rows a workgroup, 32 a wave, and of the keys that they see piece blockIdx.x / (tiles * heads); a piece's results are `stride` behind the one's before.
 template <int DP>
-__global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float *dout, const Row *rows, float *dq, int tiles, const Exponents left) {
+__global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float *dout, const Row *rows, float *dq, int64_t stride, int tiles, int pieces, const Exponents left) {
   __shared__ __align__(16) Tile<DP> kt, vt;
   __shared__ int room[4][4];
   __shared__ uint32_t found;
-  const int bg = (int)blockIdx.x % (c.batch * c.key_heads), tile = tiles - 1 - (int)blockIdx.x / (c.batch * c.key_heads);
-  const int b = bg / c.key_heads, g = bg % c.key_heads;
+  const int bg = (int)blockIdx.x % (c.batch * c.key_heads), rest = (int)blockIdx.x / (c.batch * c.key_heads);
+  const int b = bg / c.key_heads, g = bg % c.key_heads, tile = tiles - 1 - rest % tiles, piece = rest / tiles;
   const int lane = threadIdx.x % 64, half = lane / 32;
   const int r = tile * kRows + threadIdx.x / 64 * 32 + lane % 32;
   const bool live = r < c.rows;
@@ -600,8 +601,9 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
   Hull mine;
   mine.of(row.lo, row.hi, live);
   const Hull all = mine.all(room);
-  const int begin = all.first(), end = begin + all.steps();
-  if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), kRows / 32) | left.bad_keys(bg, begin, end - begin))) return;
+  const int first = all.first(), steps = all.steps();
+  if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), kRows / 32) | left.bad_keys(bg, first, steps))) return;
+  const int begin = first + (int)((int64_t)steps * piece / pieces), end = first + (int)((int64_t)steps * (piece + 1) / pieces);
   Operand<DP> q, d;
   q.load(c.q + at, c.dim, live);
   d.load(dout + at, c.dim, live);
@@ -632,7 +634,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
     sum.add(kt, ds);
     if (clean && found) sum.add_back(found, [&](int n) { return c.k + c.key_at(b, g, j0 + n); }, c.dim, ds);
   }
-  if (live) store_sums(sum.v, dq + at, c.dim, c.scale);
+  if (live) store_sums(sum.v, dq + piece * stride + at, c.dim, c.scale);
 }
 
 // 128 keys a workgroup, 32 a wave, which walks the rows of piece blockIdx.x / (tiles * heads).  Results go to dk and dv, or piece by piece to
@@ -719,14 +721,14 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float
   if (DV) store_sums(dvs.v, (pieces > 1 ? parts + ((int64_t)piece * 2 + 1) * all : dv) + at, c.dim, 1.f);
 }
 
-// dk and dv from their pieces, in order; half blockIdx.y.
-__global__ __launch_bounds__(kThreads) void sum_kernel(const float *__restrict__ parts, float *__restrict__ dk, float *__restrict__ dv, int64_t all, int pieces) {
-  float *to = blockIdx.y ? dv : dk;
+// Gradients from their pieces [piece][gradient][all], in order: blockIdx.y says which, of gridDim.y.
+__global__ __launch_bounds__(kThreads) void sum_kernel(const float *__restrict__ parts, float *__restrict__ first, float *__restrict__ second, int64_t all, int pieces) {
+  float *to = blockIdx.y ? second : first;
   if (!to) return;
   for (int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4; e < all; e += (int64_t)gridDim.x * kThreads * 4) {
     const int n = (int)(all - e < 4 ? all - e : 4);
     f32x4 s = load4(parts + blockIdx.y * all + e, n);
-    for (int p = 1; p < pieces; ++p) s += load4(parts + (2 * p + blockIdx.y) * all + e, n);
+    for (int p = 1; p < pieces; ++p) s += load4(parts + ((int64_t)gridDim.y * p + blockIdx.y) * all + e, n);
     store4(to + e, n, s);
   }
 }
@@ -812,7 +814,7 @@ void with_columns(int dim, const F &f) {
 // Pieces of rows_kernel along the keys: as many as it takes for two workgroups a CU, of 256 keys at least.
 int row_pieces(const Call &c, int64_t groups) {
   if (groups == 0) return 1;
-  const int64_t wanted = (2 * num_cus() + groups - 1) / groups, most = std::min(kMostPieces, std::max(1, c.tk / 256));
+  const int64_t wanted = (2 * num_cus() + groups - 1) / groups, most = std::min(kMostPieces, std::max(1, c.tk / 128));
   return (int)std::min<int64_t>(wanted, most);
 }
 
@@ -919,34 +921,41 @@ extern "C" int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHa
   if (all_rows == 0 && all_keys == 0) return 0;
   const int row_tiles = (c.rows + kRows - 1) / kRows, key_tiles = (c.tk + kRows - 1) / kRows;
   const int64_t key_groups = head_pairs * key_tiles;
-  int pieces = 1;
   const bool pairs = all_rows && all_keys && pair_suits(c, true);
-  if ((dkey || dvalue) && key_groups) pieces = (int)std::min<int64_t>(((pairs && c.dim <= 64 ? 4 : 2) * num_cus() + key_groups - 1) / key_groups, std::max(1, c.rows / 256));
-  TF_REQUIRE(head_pairs * row_tiles < kMaxGroups && key_groups * pieces < kMaxGroups && (all_rows + 3) / 4 < kMaxGroups,
+  // Where the tiles leave CUs without work their walks are cut, in pieces of 128 or more rows or keys (of 256: one head of 64, backward, 256 x 256 47.5 us and
+  // here 44.5, 300 x 1000 60 and 49).  Cutting dq as well took 8 queries over 8 192 keys from 320 us to 55, and from 1 288 to 59 on the fp32 instruction.
+  // Four workgroups a CU instead of two gain dk and dv of short heads something, two fit one, but not dq: 1024 x 4096, 8 heads of 64, 143 us, 150 with it.
+  int pieces = 1, row_pieces = 1;
+  const int64_t row_groups = head_pairs * row_tiles;
+  if ((dkey || dvalue) && key_groups) pieces = (int)std::min<int64_t>(((pairs && c.dim <= 64 ? 4 : 2) * num_cus() + key_groups - 1) / key_groups, std::max(1, c.rows / 128));
+  if (dquery && row_groups) row_pieces = (int)std::min<int64_t>((2 * num_cus() + row_groups - 1) / row_groups, std::max(1, c.tk / 128));
+  TF_REQUIRE(row_groups * row_pieces < kMaxGroups && key_groups * pieces < kMaxGroups && (all_rows + 3) / 4 < kMaxGroups,
              "too many sequences, heads and queries for a launch");
   TF_REQUIRE(!being_captured(s), "the backward pass takes scratch, which a captured stream cannot give back");
   for (const DLArray *written : {(const DLArray *)dquery, (const DLArray *)dkey, (const DLArray *)dvalue}) announce_write(written);
-  const int64_t all = all_keys * c.dim;
-  const size_t row_bytes = (size_t)all_rows * sizeof(Row), part_bytes = pieces > 1 ? (size_t)pieces * 2 * all * sizeof(float) : 0;
-  const size_t planes = pairs ? pair_bytes(c, true) : 0, bytes = planes + part_bytes + row_bytes;
+  const int64_t all = all_keys * c.dim, all_queries = all_rows * c.dim;
+  const size_t row_bytes = (size_t)all_rows * sizeof(Row), row_part_bytes = row_pieces > 1 ? (size_t)row_pieces * all_queries * sizeof(float) : 0;
+  const size_t part_bytes = pieces > 1 ? (size_t)pieces * 2 * all * sizeof(float) : 0;
+  const size_t planes = pairs ? pair_bytes(c, true) : 0, bytes = planes + row_bytes + row_part_bytes + part_bytes;
   char *block = (char *)device_alloc(bytes, s);
   if (!block) {
     if (memorytoSaving) *memorytoSaving = shortfall(block_bytes(bytes));
     return 0;
   }
-  float *parts = (float *)(block + planes);
-  Row *rows = (Row *)(block + planes + part_bytes);
+  Row *rows = (Row *)(block + planes);
+  float *row_parts = (float *)(block + planes + row_bytes), *parts = (float *)(block + planes + row_bytes + row_part_bytes);
   const float *dout = (const float *)doutput->data;
-  float *dk = dkey ? (float *)dkey->data : nullptr, *dv = dvalue ? (float *)dvalue->data : nullptr;
+  float *dq = dquery ? (float *)dquery->data : nullptr, *dk = dkey ? (float *)dkey->data : nullptr, *dv = dvalue ? (float *)dvalue->data : nullptr;
+  const Gradients to = {row_pieces > 1 ? row_parts : dq, dk, dv, parts, row_pieces > 1 ? all_queries : 0, row_pieces, pieces};
   if (all_rows && !pairs)
     hipLaunchKernelGGL(prepare_kernel, dim3((unsigned)((all_rows + 3) / 4)), dim3(kThreads), 0, s, c, (const float *)output->data,
                        (const float *)statistics->data, dout, rows, all_rows);
-  const Exponents left = pairs ? pair_backward(c, (const float *)output->data, (const float *)statistics->data, dout, rows, dquery ? (float *)dquery->data : nullptr, dk, dv, parts, row_tiles, key_tiles, pieces, block, s)
-                               : Exponents{};
+  const Exponents left =
+      pairs ? pair_backward(c, (const float *)output->data, (const float *)statistics->data, dout, rows, to, row_tiles, key_tiles, block, s) : Exponents{};
   with_columns(c.dim, [&](auto columns) {
     constexpr int DP = decltype(columns)::value;
-    if (dquery && all_rows)
-      hipLaunchKernelGGL((dq_kernel<DP>), dim3((unsigned)(head_pairs * row_tiles)), dim3(kThreads), 0, s, c, dout, rows, (float *)dquery->data, row_tiles, left);
+    if (dq && all_rows)
+      hipLaunchKernelGGL((dq_kernel<DP>), dim3((unsigned)(row_groups * row_pieces)), dim3(kThreads), 0, s, c, dout, rows, to.dq, to.row_stride, row_tiles, row_pieces, left);
     if (!key_groups) return;
     const dim3 grid((unsigned)(key_groups * pieces));
     if constexpr (DP <= 128) {
@@ -959,9 +968,12 @@ extern "C" int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHa
     if (dk) hipLaunchKernelGGL((dkv_kernel<DP, true, false>), grid, dim3(kThreads), 0, s, c, dout, rows, dk, nullptr, parts, key_tiles, pieces, left);
     if (dv) hipLaunchKernelGGL((dkv_kernel<DP, false, true>), grid, dim3(kThreads), 0, s, c, dout, rows, nullptr, dv, parts, key_tiles, pieces, left);
   });
-  if (pieces > 1)
-    hipLaunchKernelGGL(sum_kernel, dim3((unsigned)std::min<int64_t>((all / 4 + kThreads) / kThreads, 4 * num_cus()), 2), dim3(kThreads), 0, s, parts, dk, dv, all,
-                       pieces);
+  auto sum = [&](const float *from, float *first, float *second, int64_t n, int of) {
+    const unsigned groups = (unsigned)std::min<int64_t>((n / 4 + kThreads) / kThreads, 4 * num_cus());
+    hipLaunchKernelGGL(sum_kernel, dim3(groups, from == parts ? 2 : 1), dim3(kThreads), 0, s, from, first, second, n, of);
+  };
+  if (row_pieces > 1) sum(row_parts, dq, nullptr, all_queries, row_pieces);
+  if (pieces > 1) sum(parts, dk, dv, all, pieces);
   device_free(block, s);
   return finish(s, "DLGpuAttentionBackward");
 }

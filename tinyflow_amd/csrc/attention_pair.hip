@@ -600,13 +600,13 @@ __device__ __forceinline__ float weight(const Score &score, float product, float
 // 128 rows a workgroup, as forward_kernel; in LDS a step's keys, values and keys transposed.
 template <int DP, bool PLAIN>
 __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Call c, const char *qs, const char *ds_, const char *ks, const char *vs, const char *kts,
-                                                                        const Exponents ex, const Row *rows, float *dq, int tiles) {
+                                                                        const Exponents ex, const Row *rows, float *dq, int64_t stride, int tiles, int pieces) {
   constexpr int BLOCK = (int)block_size(DP), AHEAD = 3;
   __shared__ __align__(16) char lds[2][3 * BLOCK];
   __shared__ int room[4][4];
   const int heads = c.batch * c.key_heads;
-  const int bg = (int)blockIdx.x % heads, tile = tiles - 1 - (int)blockIdx.x / heads;
-  const int b = bg / c.key_heads, g = bg % c.key_heads;
+  const int bg = (int)blockIdx.x % heads, rest = (int)blockIdx.x / heads;
+  const int b = bg / c.key_heads, g = bg % c.key_heads, tile = tiles - 1 - rest % tiles, piece = rest / tiles;
   const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int r = tile * kRows + wave * 32 + lane % 32;
   const bool live = r < c.rows;
@@ -615,8 +615,9 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
   Hull mine;
   mine.of(row.lo, row.hi, live);
   const Hull all = mine.all(room);
-  const int begin = all.first(), end = begin + all.steps();
-  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32) | ex.bad_keys(bg, begin, end - begin))) return;
+  const int first = all.first(), steps = all.steps();
+  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32) | ex.bad_keys(bg, first, steps))) return;
+  const int begin = first + (int)((int64_t)steps * piece / pieces), end = first + (int)((int64_t)steps * (piece + 1) / pieces);
   const int block = min(tile * (kRows / 32) + wave, ex.row_blocks - 1);
   const int64_t row_block = (int64_t)bg * ex.row_blocks + block, key_block = (int64_t)bg * ex.key_blocks;
   const int eq = scalar(ex.q + row_block), ed = scalar(ex.d + row_block);
@@ -696,7 +697,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
   for (int e = 0; e < DP / 32; ++e)
 #pragma unroll
     for (int v = 0; v < 16; ++v) sum[e][v] = unit == kNoUnit ? 0.f : __builtin_ldexpf(sum[e][v], -unit);
-  store_sums(sum, dq + c.query_at(b, g, r), c.dim, c.scale);
+  store_sums(sum, dq + piece * stride + c.query_at(b, g, r), c.dim, c.scale);
 }
 
 // 128 keys a workgroup, 32 a wave; steps of 32 rows: in LDS queries, gradients, both transposed, and what Info says of the rows.
@@ -932,7 +933,11 @@ bool pair_suits(const Call &c, bool backward) {
   if (e && e[0] == '0') return false;
   const float factor = c.cap > 0.f ? c.scale / c.cap : c.scale;
   if (c.dim > 128 || !(factor > 0x1p-40f && factor < 0x1p40f)) return false;
-  if (c.rows < 32 || c.tk < 32) return false;
+  // Below these splitting costs more than it saves.  Microseconds of a call, fp32 kernels / these, one head: forward, 33 x 33 of 64 12 / 16, 128 x 128 of 32
+  // 13 / 15, 33 x 257 of 32 24 / 18, 128 x 128 of 64 21 / 17, 64 x 64 of 128 20 / 18; backward, 64 x 64 of 32 25 / 30, 33 x 33 of 64 36 / 32, 33 x 257 of 32
+  // 36 / 34, 8 x 1024 of 32 30 / 35 and of 64 43 / 37.
+  if (!backward && (int64_t)c.tk * c.dim < 8192) return false;
+  if (backward && ((int64_t)std::max(c.rows, c.tk) * c.dim <= 2048 || (c.dim <= 32 && std::min(c.rows, c.tk) < 32))) return false;
   // the planes are written by one launch, a block a workgroup
   if ((int64_t)c.batch * c.key_heads * (blocks_of(c.rows) + (int64_t)blocks_of(c.tk)) * 2 >= 1 << 24) return false;
   return true;
@@ -963,16 +968,16 @@ Exponents pair_forward(const Call &c, float *out, float *stat, const Pieces &pie
   return ex;
 }
 
-Exponents pair_backward(const Call &c, const float *out, const float *stat, const float *dout, Row *rows, float *dq, float *dk, float *dv, float *parts, int row_tiles, int key_tiles,
-                        int pieces, char *scratch, hipStream_t s) {
+Exponents pair_backward(const Call &c, const float *out, const float *stat, const float *dout, Row *rows, const Gradients &to, int row_tiles, int key_tiles,
+                        char *scratch, hipStream_t s) {
   Scratch of = {scratch, 0};
   const Layout l(c, true, of);
   Pack p = {};
   p.n_jobs = 4;
-  const bool keys = dk || dv;
+  const bool keys = to.dk || to.dv;
   p.jobs[0] = Job{c.q, true, l.q, keys ? l.qt : nullptr, l.eq, 0};
   p.jobs[1] = Job{dout, true, l.d, keys ? l.dt : nullptr, l.ed, 0};
-  p.jobs[2] = Job{c.k, false, l.k, dq ? l.kt : nullptr, l.ek, 0};
+  p.jobs[2] = Job{c.k, false, l.k, to.dq ? l.kt : nullptr, l.ek, 0};
   p.jobs[3] = Job{c.v, false, l.v, nullptr, l.ev, 0};
   p.out = out;
   p.stat = stat;
@@ -985,12 +990,12 @@ Exponents pair_backward(const Call &c, const float *out, const float *stat, cons
   const int heads = c.batch * c.key_heads;
   with_columns(c.dim, [&](auto dp) {
     constexpr int DP = decltype(dp)::value;
-    if (dq)
-      hipLaunchKernelGGL((plain ? dq_kernel<DP, true> : dq_kernel<DP, false>), dim3((unsigned)(heads * row_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.k, l.v, l.kt, ex,
-                         rows, dq, row_tiles);
+    if (to.dq)
+      hipLaunchKernelGGL((plain ? dq_kernel<DP, true> : dq_kernel<DP, false>), dim3((unsigned)(heads * row_tiles * to.row_pieces)), dim3(kThreads), 0, s, c, l.q, l.d, l.k,
+                         l.v, l.kt, ex, rows, to.dq, to.row_stride, row_tiles, to.row_pieces);
     if (keys)
-      hipLaunchKernelGGL((plain ? dkv_kernel<DP, true> : dkv_kernel<DP, false>), dim3((unsigned)(heads * pieces * key_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.qt, l.dt,
-                         l.k, l.v, ex, l.info, dk, dv, parts, key_tiles, pieces);
+      hipLaunchKernelGGL((plain ? dkv_kernel<DP, true> : dkv_kernel<DP, false>), dim3((unsigned)(heads * to.pieces * key_tiles)), dim3(kThreads), 0, s, c, l.q, l.d, l.qt,
+                         l.dt, l.k, l.v, ex, l.info, to.dk, to.dv, to.parts, key_tiles, to.pieces);
   });
   return ex;
 }
