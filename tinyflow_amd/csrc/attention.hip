@@ -838,6 +838,7 @@ extern "C" int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHan
   if (all_rows == 0) return 0;
   float *out = output ? (float *)output->data : nullptr, *stat = statistics ? (float *)statistics->data : nullptr;
   const int64_t head_pairs = (int64_t)batch * c.key_heads;
+  // (32 rows, 8 heads of 64 over 512 keys, 12 us, by the other forms 21; 5 queries of 4 heads over 4 096 keys, eight sequences, 76 and 177)
   const bool few = c.rows <= 32 && !(c.rows > 16 && c.dim > 128) && (int64_t)c.key_heads * c.dim < 1 << 24;  // 16 rows are less than 2^31 bytes apart
   const bool pairs = !few && pair_suits(c, false);
   int64_t groups;
@@ -890,6 +891,7 @@ extern "C" int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHan
     });
   }
   if (pieces.count > 1) {
+    // one wave a row where the pieces are few: 4 096 keys, eight sequences, 16 pieces, 75 us, with sixteen waves 89
     if (pieces.count > 16) hipLaunchKernelGGL((join_kernel<16>), dim3((unsigned)all_rows), dim3(1024), 0, s, c, pieces, out, stat);
     else hipLaunchKernelGGL((join_kernel<1>), dim3((unsigned)((all_rows + 3) / 4)), dim3(256), 0, s, c, pieces, out, stat);
   }
@@ -924,10 +926,10 @@ extern "C" int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHa
   const bool pairs = all_rows && all_keys && pair_suits(c, true);
   // Where the tiles leave CUs without work their walks are cut, in pieces of 128 or more rows or keys (of 256: one head of 64, backward, 256 x 256 47.5 us and
   // here 44.5, 300 x 1000 60 and 49).  Cutting dq as well took 8 queries over 8 192 keys from 320 us to 55, and from 1 288 to 59 on the fp32 instruction.
-  // Four workgroups a CU instead of two gain dk and dv of short heads something, two fit one, but not dq: 1024 x 4096, 8 heads of 64, 143 us, 150 with it.
+  // Two workgroups a CU: with four, two of which fit one with short heads, 4 x 1 024 tokens of 16 heads of 64 took 200 us, with two 177.
   int pieces = 1, row_pieces = 1;
   const int64_t row_groups = head_pairs * row_tiles;
-  if ((dkey || dvalue) && key_groups) pieces = (int)std::min<int64_t>(((pairs && c.dim <= 64 ? 4 : 2) * num_cus() + key_groups - 1) / key_groups, std::max(1, c.rows / 128));
+  if ((dkey || dvalue) && key_groups) pieces = (int)std::min<int64_t>((2 * num_cus() + key_groups - 1) / key_groups, std::max(1, c.rows / 128));
   if (dquery && row_groups) row_pieces = (int)std::min<int64_t>((2 * num_cus() + row_groups - 1) / row_groups, std::max(1, c.tk / 128));
   TF_REQUIRE(row_groups * row_pieces < kMaxGroups && key_groups * pieces < kMaxGroups && (all_rows + 3) / 4 < kMaxGroups,
              "too many sequences, heads and queries for a launch");
