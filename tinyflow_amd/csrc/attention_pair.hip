@@ -715,9 +715,10 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   const int tile_lo = tile * kRows, tile_hi = min(c.tk, tile_lo + kRows);
   if (__syncthreads_or(ex.bad_rows_of(bg, tile_lo, tile_hi) | ex.bad_keys(bg, tile_lo / 32, kRows / 32))) return;
   const int64_t row_block = (int64_t)bg * ex.row_blocks;
-  // The blocks of rows that see one of the keys, cut in pieces.  (The same rows for all tiles in a piece, one (b, key head, piece) to an XCD, came from
-  // its L2 and left a third of the CUs without work in a causal pass: causal 4096 x 16 heads of 128 685 us, or 475 with tiles from both ends in one
-  // workgroup; these 420.)
+  // The blocks of rows that see one of the keys; a piece has every pieces-th of them, from the last on, which in a causal pass all tiles see: a piece's tiles
+  // of one head, on one XCD where heads times pieces are a multiple of 8, go through the same blocks together and find them in its L2.  (4 096 x 16
+  // heads of 128 on 4, causal: 443 MiB from memory and 408 us; pieces one behind the other, of each tile's rows, 1 985 MiB and 426, the whole backward pass 789 us and 747;
+  // pieces one behind the other, of all rows, leave a third of the CUs without work: 685, or 475 with tiles from both ends in one workgroup.)
   if (threadIdx.x == 0) range[0] = ex.row_blocks, range[1] = 0;
   __syncthreads();
   {
@@ -729,7 +730,6 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   }
   __syncthreads();
   const int first = __builtin_amdgcn_readfirstlane(range[0]), steps = max(0, __builtin_amdgcn_readfirstlane(range[1]) - first);
-  const int begin = first + (int)((int64_t)steps * piece / pieces), end = first + (int)((int64_t)steps * (piece + 1) / pieces);
   const int j0 = tile_lo + wave * 32, j = j0 + lane % 32;
   const bool live = j < c.tk;
   const int64_t key_block = (int64_t)bg * ex.key_blocks + min(tile * (kRows / 32) + wave, ex.key_blocks - 1);
@@ -760,27 +760,28 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   // the first block from `step` on that sees one of the workgroup's keys; others may be some that cannot be split, of which nothing is stored
   auto next_of = [&](int step) {
     Hull seen;
-    for (; step < end; ++step) {
+    for (; step >= first; step -= pieces) {
       hull_of(step, seen);
       if (seen.meets(tile_lo, tile_hi)) break;
     }
     return step;
   };
-  int step = next_of(begin), slot = 0;
-  if (step < end) {
+  const int last = first + steps - 1;
+  int step = next_of(last - (last + pieces - piece) % pieces), slot = 0;
+  if (step >= first) {
     Blocks<DP, 4>(from, row_block + step, to).all();
     fetch_info(step, 0);
   }
 #pragma unroll 1
-  for (int next; step < end; step = next, slot ^= 1) {
+  for (int next; step >= first; step = next, slot ^= 1) {
     const int eq = scalar(ex.q + row_block + step), ed = scalar(ex.d + row_block + step);
     Hull seen;
     hull_of(step, seen);
-    next = next_of(step + 1);
+    next = next_of(step - pieces);
     arrived();
     // the last step fetches itself again
-    const Blocks<DP, 4> coming(from, row_block + (next < end ? next : step), to + (uint32_t)((1 - slot) * SLOT));
-    fetch_info(next < end ? next : step, 1 - slot);
+    const Blocks<DP, 4> coming(from, row_block + (next >= first ? next : step), to + (uint32_t)((1 - slot) * SLOT));
+    fetch_info(next >= first ? next : step, 1 - slot);
     keep<(DP > 64)>(dks);
     keep<(DP > 64)>(dvs);
     if (DP <= 64 && !seen.meets(j0, j0 + 32)) {  // longer heads: the sums would move at every step for it
