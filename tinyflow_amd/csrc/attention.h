@@ -233,6 +233,8 @@ struct Exponents {
   }
   __device__ inline bool bad_rows(int64_t head, int first, int n) const { return bad(q, head, row_blocks, first, n) | bad(d, head, row_blocks, first, n); }
   __device__ inline bool bad_keys(int64_t head, int first, int n) const { return bad(k, head, key_blocks, first, n) | bad(v, head, key_blocks, first, n); }
+  // Any of a (b, key head).  The fp32 kernels ask this first: of a head without one they only see its exponents (dq of 4 096 x 16 heads of 128 5.3 us, 7.9 without).
+  __device__ inline bool bad_head(int64_t head) const { return bad_rows(head, 0, row_blocks) | bad_keys(head, 0, key_blocks); }
   // of the blocks of rows that see one of the keys [from, to)
   __device__ inline bool bad_rows_of(int64_t head, int from, int to) const {
     bool found = false;

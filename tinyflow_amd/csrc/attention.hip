@@ -164,6 +164,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
   __shared__ uint32_t found;
   const int bg = (int)blockIdx.x % (c.batch * c.key_heads), rest = (int)blockIdx.x / (c.batch * c.key_heads);
   const int b = bg / c.key_heads, g = bg % c.key_heads, tile = tiles - 1 - rest % tiles, piece = rest / tiles;
+  if (left.q && !__syncthreads_or(left.bad_head(bg))) return;
   const int lane = threadIdx.x % 64, half = lane / 32;
   const int r = tile * kRows + threadIdx.x / 64 * 32 + lane % 32;
   const bool live = r < c.rows;
@@ -591,6 +592,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
   __shared__ uint32_t found;
   const int bg = (int)blockIdx.x % (c.batch * c.key_heads), rest = (int)blockIdx.x / (c.batch * c.key_heads);
   const int b = bg / c.key_heads, g = bg % c.key_heads, tile = tiles - 1 - rest % tiles, piece = rest / tiles;
+  if (left.q && !__syncthreads_or(left.bad_head(bg))) return;
   const int lane = threadIdx.x % 64, half = lane / 32;
   const int r = tile * kRows + threadIdx.x / 64 * 32 + lane % 32;
   const bool live = r < c.rows;
@@ -721,15 +723,25 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float
   if (DV) store_sums(dvs.v, (pieces > 1 ? parts + ((int64_t)piece * 2 + 1) * all : dv) + at, c.dim, 1.f);
 }
 
-// Gradients from their pieces [piece][gradient][all], in order: blockIdx.y says which, of gridDim.y.
-__global__ __launch_bounds__(kThreads) void sum_kernel(const float *__restrict__ parts, float *__restrict__ first, float *__restrict__ second, int64_t all, int pieces) {
-  float *to = blockIdx.y ? second : first;
-  if (!to) return;
-  for (int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4; e < all; e += (int64_t)gridDim.x * kThreads * 4) {
-    const int n = (int)(all - e < 4 ? all - e : 4);
-    f32x4 s = load4(parts + blockIdx.y * all + e, n);
-    for (int p = 1; p < pieces; ++p) s += load4(parts + ((int64_t)gridDim.y * p + blockIdx.y) * all + e, n);
-    store4(to + e, n, s);
+// Gradients from their pieces, in order: blockIdx.y says which, `stride` is from one piece to the next.
+struct Job {
+  const float *from;
+  float *to;
+  int64_t all, stride;
+  int pieces;
+};
+struct Jobs {
+  Job job[3];
+  int n;
+};
+__global__ __launch_bounds__(kThreads) void sum_kernel(const Jobs jobs) {
+  const Job &job = jobs.job[blockIdx.y];
+  const float *__restrict__ from = job.from;
+  for (int64_t e = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4; e < job.all; e += (int64_t)gridDim.x * kThreads * 4) {
+    const int n = (int)(job.all - e < 4 ? job.all - e : 4);
+    f32x4 s = load4(from + e, n);
+    for (int p = 1; p < job.pieces; ++p) s += load4(from + p * job.stride + e, n);
+    store4(job.to + e, n, s);
   }
 }
 
@@ -970,12 +982,14 @@ extern "C" int DLGpuAttentionBackward(const DLArrayHandle query, const DLArrayHa
     if (dk) hipLaunchKernelGGL((dkv_kernel<DP, true, false>), grid, dim3(kThreads), 0, s, c, dout, rows, dk, nullptr, parts, key_tiles, pieces, left);
     if (dv) hipLaunchKernelGGL((dkv_kernel<DP, false, true>), grid, dim3(kThreads), 0, s, c, dout, rows, nullptr, dv, parts, key_tiles, pieces, left);
   });
-  auto sum = [&](const float *from, float *first, float *second, int64_t n, int of) {
-    const unsigned groups = (unsigned)std::min<int64_t>((n / 4 + kThreads) / kThreads, 4 * num_cus());
-    hipLaunchKernelGGL(sum_kernel, dim3(groups, from == parts ? 2 : 1), dim3(kThreads), 0, s, from, first, second, n, of);
-  };
-  if (row_pieces > 1) sum(row_parts, dq, nullptr, all_queries, row_pieces);
-  if (pieces > 1) sum(parts, dk, dv, all, pieces);
+  Jobs sums = {};
+  if (row_pieces > 1) sums.job[sums.n++] = Job{row_parts, dq, all_queries, all_queries, row_pieces};
+  if (pieces > 1 && dk) sums.job[sums.n++] = Job{parts, dk, all, 2 * all, pieces};
+  if (pieces > 1 && dv) sums.job[sums.n++] = Job{parts + all, dv, all, 2 * all, pieces};
+  if (sums.n) {
+    const int64_t most = std::max(row_pieces > 1 ? all_queries : 0, pieces > 1 ? all : 0);
+    hipLaunchKernelGGL(sum_kernel, dim3((unsigned)std::min<int64_t>((most / 4 + kThreads) / kThreads, 4 * num_cus()), sums.n), dim3(kThreads), 0, s, sums);
+  }
   device_free(block, s);
   return finish(s, "DLGpuAttentionBackward");
 }
