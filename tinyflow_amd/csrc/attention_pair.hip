@@ -597,11 +597,18 @@ __device__ __forceinline__ float weight(const Score &score, float product, float
   return __builtin_amdgcn_exp2f((t - bias) + shift);
 }
 
+// Whether two waves share a SIMD, in 256 registers each; longer heads have all 512, their sums and held operands among those that only matrix instructions work on.  With
+// 96 columns two are faster where cap or bias are vector work to hide (2 x 1 777 tokens, documents, 6 heads on 3 of 72, the whole backward pass 145 us and 155), and slower
+// without (4 096 tokens, 16 heads on 4 of 96, 626 and 611).
+template <int DP, bool PLAIN>
+constexpr bool kTwoWaves = DP <= 64 || (DP <= 96 && !PLAIN);
+
 // 128 rows a workgroup, as forward_kernel; in LDS a step's keys, values and keys transposed.
 template <int DP, bool PLAIN>
-__global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Call c, const char *qs, const char *ds_, const char *ks, const char *vs, const char *kts,
+__global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_kernel(const Call c, const char *qs, const char *ds_, const char *ks, const char *vs, const char *kts,
                                                                         const Exponents ex, const Row *rows, float *dq, int64_t stride, int tiles, int pieces) {
-  constexpr int BLOCK = (int)block_size(DP), AHEAD = 3;
+  constexpr int BLOCK = (int)block_size(DP), AHEAD = DP > 64 && kTwoWaves<DP, PLAIN> ? 2 : 3;
+  constexpr bool TWO = kTwoWaves<DP, PLAIN>;
   __shared__ __align__(16) char lds[2][3 * BLOCK];
   __shared__ int room[4][4];
   const int heads = c.batch * c.key_heads;
@@ -630,8 +637,8 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
   d.load(ds_ + row_block * BLOCK);
   d.alternate();
   const float sign = lane % 2 ? -1.f : 1.f;
-  q.template wait<(DP > 64)>();
-  d.template wait<(DP > 64)>();
+  q.template wait<!TWO>();
+  d.template wait<!TWO>();
   const Score score(c);
   f32x16 sum[DP / 32];
 #pragma unroll
@@ -647,11 +654,11 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
     arrived();
     // the last step fetches itself again
     const Blocks<DP, 3> next(from, key_block + min(step + 1, end - 1), to + (uint32_t)((1 - slot) * 3 * BLOCK));
-    if (DP <= 64 && !mine.meets(j0, j0 + kKeys)) {  // longer heads: the sums would move at every step for it
+    if (TWO && !mine.meets(j0, j0 + kKeys)) {  // longer heads: the sums would move at every step for it
       next.all();
       continue;
     }
-    keep<(DP > 64)>(sum);
+    keep<!TWO>(sum);
     const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(sign, -(ed + ev));
     float p[16], cap[16], ds[16];
     f32x16 s[2];
@@ -678,7 +685,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dq_kernel(const Ca
     const int new_unit = gradient_unit(ds, 0, ek, unit);
     if (new_unit < unit) {
       multiply(sum, __builtin_ldexpf(1.f, max(new_unit - unit, -200)));
-      keep<(DP > 64)>(sum);
+      keep<!TWO>(sum);
       unit = new_unit;
     }
     const int shift = unit == kNoUnit ? 0 : unit - ek;  // nothing but zeros so far
