@@ -56,8 +56,8 @@ def test_small_blocks_by_themselves(rt):
         values = want.backward(out[:, own], stat[:, :, own], do[:, own])
         for what, got, (value, tol) in zip(("dq", "dk", "dv"), grads, values):
             off = np.linalg.norm(got[:, own] - value) / np.linalg.norm(value)
-            # blocks of 32 rows span two documents: 2^-39 of the larger one's values is left off, 2^-19 of the smaller one's values
-            # for dv, and for the products of both (2^-60 apart) what the fp32 kernels give
+            # a block of 32 rows that spans two documents is left to the fp32 kernels: sums of up to 80 rows or keys and 64 columns of products, each rounding
+            # 2^-24 of a magnitude that cancellation makes up to four times the result's: 2^-24 (80 + 64) 4 < 2^-14.8
             assert off <= 2.0 ** -15, "%s of document %d is %.2g off" % (what, n, off)
 
 
@@ -143,3 +143,15 @@ def test_gradients_of_few_queries(rt, monkeypatch, split, tq, tk):
     _check(rt, *a, causal=True)
     a[2][1, 700] *= np.float32(2.0 ** 30)
     _check(rt, *a, causal=True)
+
+
+def test_a_small_gradient_among_large_ones(rt):
+    """Every 40th row's gradient is 2^-30 of the others': its dq has its own digits."""
+    q, k, v, do = _data(1, 300, 300, 2, 1, 64, 13)
+    rows = np.arange(300) % 40 == 7
+    do[:, rows] *= np.float32(2.0 ** -30)
+    out, stat, grads = _run(rt, q, k, v, do, causal=True)
+    want = ref.Attention(q, k, v, None, None, 0.125, causal=True).backward(out, stat, do)[0][0]
+    off = np.linalg.norm((grads[0] - want)[:, rows]) / np.linalg.norm(want[:, rows])
+    # sums of up to 300 keys and 64 columns, each rounding 2^-24 of up to four times the result's magnitude: 2^-24 (300 + 64) 4 < 2^-13.4
+    assert off <= 2.0 ** -13.4, "%.2g off" % off

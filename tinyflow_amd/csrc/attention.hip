@@ -1,8 +1,10 @@
 // Attention, forward and backward (no counterpart in the reference).  attention.h has the formulas and what rows are.
 //
-// Forms of the forward pass, and which one runs (choose_forward):
-//   few_kernel     up to 32 rows of a key head: every wave streams its own keys from memory to registers, nothing is staged; bound by HBM
-//   rows_kernel    128 rows a workgroup, the fp32 matrix instruction
+// Forms of the forward pass (which one runs: DLGpuAttentionForward, pair_suits):
+//   few_kernel     up to 32 rows of a key head: every wave streams its own keys from memory to registers, nothing is staged; bound by HBM: 100 003 keys of 2
+//                  heads of 128, 205 MB, 39 us, 5.2 TB/s
+//   rows_kernel    128 rows a workgroup, the fp32 matrix instruction, which bounds it: 4 096 causal tokens of 16 heads on 4 of 128, 69 GFLOP, 1.09 ms
+//   attention_pair.hip    the same rows on fp16 pairs, 0.2 ms; rows_kernel then takes what cannot be split
 // Both can be cut along the keys: pieces write their unnormalised sums with their maximum, join_kernel adds them up in their order.
 // Backward: prepare_kernel (delta, what each row sees), dq_kernel (128 rows a workgroup, walks the keys), dkv_kernel (128 keys a workgroup, walks the
 // rows); where that leaves CUs without work the walks are cut, and sum_kernel adds the pieces.  Both compute the scores again; no sum goes
