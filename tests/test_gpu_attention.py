@@ -255,3 +255,20 @@ def test_array_shapes(rt, shape):
     got = _empty(rt, shaped(q).shape)
     assert gpu_op.attention_forward(*a, None, None, got, None, 2, 4, 2, 0.25, 0.0, False, rt.stream) == 0
     np.testing.assert_array_equal(got.asnumpy().reshape(out.shape), out)
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("tq,tk", [(3, 900), (700, 900), (700, 20)])
+def test_each_gradient_alone_in_pieces(rt, monkeypatch, split, tq, tk):
+    """One gradient of three, where walks are cut along the keys, the rows or both; an array of another gradient stays as it was."""
+    from tinyflow_amd import gpu_op
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    q, k, v, do = _data(2, tq, tk, 2, 1, 80, 15)
+    out, stat, grads = _run(rt, q, k, v, do)
+    a = _device(rt, q, k, v) + [None, None] + _device(rt, out, stat, do)
+    numbers = (2, 2, 1, 80 ** -0.5, 0.0, False, rt.stream)
+    for some in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        g = [_empty(rt, grads[n].shape) if n in some else None for n in range(3)]
+        assert gpu_op.attention_backward(*a, *g, *numbers) == 0
+        for n in some:
+            np.testing.assert_array_equal(g[n].asnumpy(), grads[n])

@@ -229,3 +229,26 @@ def test_in_a_captured_graph(rt):
         for g, a in zip(got, (y, cache, dx)):
             np.testing.assert_array_equal(g, a.asnumpy())
     gpu_op.destroy_cudaStream(stream)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rows,dim,rotary", [(9, 64, 8), (9, 128, 64), (4100, 128, 32), (3, 256, 248), (5, 512, 8)])
+def test_whole_units_partly_rotated(rt, rows, dim, rotary, interleaved):
+    _check(rt, rows, 2 if rows < 4000 else 8, dim, rotary, interleaved, True)
+
+
+@pytest.mark.parametrize("heads,dim", [(17, 64), (18, 40)])
+def test_in_place_of_many_rows(rt, heads, dim):
+    """Several heads one behind the other in a lane, the last run of them shorter."""
+    from tinyflow_amd import gpu_op
+    rows = 4001
+    x, gamma, dy = _data(rows, heads, dim, 14)
+    f, positions = _frequencies(dim), np.arange(rows, dtype=np.float32)
+    ax, ag, ady, ap, af = _device(rt, x.reshape(rows, -1), gamma, dy.reshape(rows, -1), positions, f)
+    y, dx, dg, dg2 = (_empty(rt, s) for s in ((rows, heads * dim), (rows, heads * dim), (dim,), (dim,)))
+    gpu_op.head_rotary([gpu_op.head_part(ax, ag, y, heads)], ap, af, 1.0, False, EPS, None, rt.stream)
+    assert gpu_op.head_rotary_backward([gpu_op.head_gradient_part(ax, ag, ady, dx, dg, heads)], ap, af, 1.0, False, EPS, rt.stream) == 0
+    assert gpu_op.head_rotary_backward([gpu_op.head_gradient_part(ax, ag, ady, ady, dg2, heads)], ap, af, 1.0, False, EPS, rt.stream) == 0
+    gpu_op.head_rotary([gpu_op.head_part(ax, ag, ax, heads)], ap, af, 1.0, False, EPS, None, rt.stream)
+    for a, b in ((y, ax), (dx, ady), (dg, dg2)):
+        np.testing.assert_array_equal(a.asnumpy(), b.asnumpy())

@@ -825,7 +825,7 @@ void with_columns(int dim, const F &f) {
   else f(IC<256>{});
 }
 
-// Pieces of rows_kernel along the keys: as many as it takes for two workgroups a CU, of 256 keys at least.
+// Pieces of a forward tile's walk along the keys: as many as it takes for two workgroups a CU, of 128 keys at least.
 int row_pieces(const Call &c, int64_t groups) {
   if (groups == 0) return 1;
   const int64_t wanted = (2 * num_cus() + groups - 1) / groups, most = std::min(kMostPieces, std::max(1, c.tk / 128));

@@ -406,7 +406,7 @@ void with_lanes(const Launch &l, const F &f) {
   else if (units <= 16) go(std::integral_constant<int, 16>{}, std::integral_constant<int, 1>{});
   else if (units <= 32) go(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
   else if (units <= 64) go(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-  else go(std::integral_constant<int, 64>{}, std::integral_constant<int, 3>{});
+  else f(std::integral_constant<int, 64>{}, std::integral_constant<int, 3>{}, std::false_type{});  // up to 1 024 of 1 536 columns
 }
 
 // Heads that share a row's angles: one where lanes are few, up to four where there are enough of them.  Microseconds with one, two and four, forward /
