@@ -838,29 +838,33 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
     };
     if (seen.covers(j0, j0 + 32)) tile(std::true_type{});
     else tile(std::false_type{});
-    static_for<4>([&](auto q) {
-      const f32x4 delta = four(kDelta, decltype(q)::value);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int x = 4 * decltype(q)::value + e;
-        ds[x] = p[x] * __builtin_fmaf(s[1][x], d_factor, -delta[e]);
+    // While dv is summed: ds, the unit that dk's sum takes for it, and ds as that product's operand.
+    f32x4 delta[4];
+    static_for<4>([&](auto q) { delta[decltype(q)::value] = four(kDelta, decltype(q)::value); });
+    constexpr int PLACES = 3 * DP / 16, HALF = PLACES / 2;
+    int new_unit = unit, shift = 0;
+    Weights wd;
+    add_product<DP, AHEAD>(dvs, at + 3 * BLOCK, w, [&](auto place) {
+      constexpr int at_place = decltype(place)::value;
+      spread<at_place, 0, HALF - 1, 16>([&](auto x_c) {
+        constexpr int x = decltype(x_c)::value;
+        ds[x] = p[x] * __builtin_fmaf(s[1][x], d_factor, -delta[x / 4][x % 4]);
         if (!PLAIN) ds[x] *= cap[x];
+      });
+      if constexpr (at_place == HALF - 1) {
+        new_unit = gradient_unit(ds, held, eq, unit);
+        shift = new_unit == kNoUnit ? 0 : new_unit - eq - held;  // nothing but zeros so far
       }
+      spread<at_place, HALF, PLACES - HALF, 8>([&](auto n_c) {
+        constexpr int n = decltype(n_c)::value;
+        wd.set<n>(__builtin_ldexpf(ds[2 * n], shift), __builtin_ldexpf(ds[2 * n + 1], shift));
+      });
     });
-    const int new_unit = gradient_unit(ds, held, eq, unit);
     if (new_unit < unit) {
       multiply(dks, __builtin_ldexpf(1.f, max(new_unit - unit, -200)));
       keep<(DP > 64)>(dks);
       unit = new_unit;
     }
-    Weights wd;
-    const int shift = unit == kNoUnit ? 0 : unit - eq - held;  // nothing but zeros so far
-    add_product<DP, AHEAD>(dvs, at + 3 * BLOCK, w, [&](auto place) {
-      spread<decltype(place)::value, 0, 3 * DP / 16, 8>([&](auto n_c) {
-        constexpr int n = decltype(n_c)::value;
-        wd.set<n>(__builtin_ldexpf(ds[2 * n], shift), __builtin_ldexpf(ds[2 * n + 1], shift));
-      });
-    });
     add_product<DP, AHEAD>(dks, at + 2 * BLOCK, wd, Nothing{});
   }
   arrived();  // what the last step has fetched
