@@ -155,3 +155,21 @@ def test_a_small_gradient_among_large_ones(rt):
     off = np.linalg.norm((grads[0] - want)[:, rows]) / np.linalg.norm(want[:, rows])
     # sums of up to 300 keys and 64 columns, each rounding 2^-24 of up to four times the result's magnitude: 2^-24 (300 + 64) 4 < 2^-13.4
     assert off <= 2.0 ** -13.4, "%.2g off" % off
+
+
+@pytest.mark.parametrize("tq", [2048, 2049])
+def test_spans_of_many_queries(rt, tq):
+    """Keys in front of the first span and behind the last hold NaN, and those that a gap leaves out numbers that no product has."""
+    q, k, v, do = _data(2, tq, 2300, 1, 1, 32, 16)
+    first = 100 + np.arange(tq) // 700 * 400
+    spans = np.stack([first, np.minimum(first + 350, 2250)], 1).astype(np.float32)
+    spans[5] = 7, 7
+    want = ref.Attention(q, k, v, spans, None, 32 ** -0.5)
+    for x in (k, v):
+        x[:, :100] = x[:, 2250:] = np.nan
+        x[0, 451:499] = 3e4
+    out, stat, grads = _run(rt, q, k, v, do, spans=spans)
+    ref.assert_within(out, want.out, want.out_tol, "out")
+    ref.assert_within(stat, want.stat, want.stat_tol, "statistics")
+    for what, got, (value, tol) in zip(("dq", "dk", "dv"), grads, want.backward(out, stat, do)):
+        ref.assert_within(got, value, tol, what)

@@ -48,6 +48,7 @@ constexpr int kFragment = 1024;  // bytes: 32 rows x 16 of fp16, a wave's lanes 
 constexpr int kInfoBytes = 1024;  // of a block of rows: eight arrays of 32, see Info
 constexpr int kSmallest = 110;   // exponents above it stand for values that no sum notices
 constexpr int kLargest = -40;
+constexpr int kSpansReadByAll = 2048;
 constexpr int kNoUnit = INT32_MAX / 2;  // of a sum of nothing
 
 // Bytes of a block of 32 rows: DP columns of h and l.
@@ -70,6 +71,7 @@ struct Job {
 struct Pack {
   Job jobs[4];
   int n_jobs, row_blocks, key_blocks;
+  int2 *seen;        // of each sequence, the keys between the first and the last that any query sees; null: each workgroup finds out
   // backward, by job 1, the gradients of the output:
   const float *out, *stat;
   Row *rows;         // of all
@@ -80,6 +82,27 @@ struct Pack {
 __device__ inline void split(float x, _Float16 &h, _Float16 &l) {
   h = (_Float16)x;
   l = (_Float16)(x - (float)h);
+}
+
+// The first key that any of a sequence's queries sees, and the one behind the last, by THREADS threads.
+template <int THREADS>
+__device__ inline void span_hull(const Call &c, int b, int (&hull)[2]) {
+  if (threadIdx.x == 0) hull[0] = c.tk, hull[1] = 0;
+  __syncthreads();
+  int lo = c.tk, hi = 0;
+  for (int i = threadIdx.x; i < c.tq; i += THREADS) {
+    int l, h;
+    c.seen(b, i, l, h);
+    if (l < h) lo = min(lo, l), hi = max(hi, h);
+  }
+  atomicMin(&hull[0], lo);
+  atomicMax(&hull[1], hi);
+  __syncthreads();
+}
+__global__ __launch_bounds__(1024) void seen_kernel(const Call c, int2 *seen) {
+  __shared__ int hull[2];
+  span_hull<1024>(c, (int)blockIdx.x, hull);
+  if (threadIdx.x == 0) seen[blockIdx.x] = make_int2(hull[0], hull[1]);
 }
 
 // A workgroup a block; bound by HBM, 5.0 to 5.4 TB/s with long heads.  Plain form: step s of 16 columns, h then l, lane: row lane % 32, columns 16 s + 8 (lane / 32) + 0..7.  Transposed: columns 32 d
@@ -104,18 +127,12 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
     // keys that any query sees lie between the first and the last of them
     int lo = 0, hi = c.tk;
     if (c.spans) {
-      if (tid == 0) hull[0] = c.tk, hull[1] = 0;
-      __syncthreads();
-      lo = c.tk, hi = 0;
-      for (int i = tid; i < c.tq; i += kThreads) {
-        int l, h;
-        c.seen(b, i, l, h);
-        if (l < h) lo = min(lo, l), hi = max(hi, h);
+      if (p.seen) {
+        lo = p.seen[b].x, hi = p.seen[b].y;
+      } else {
+        span_hull<kThreads>(c, b, hull);
+        lo = hull[0], hi = hull[1];
       }
-      atomicMin(&hull[0], lo);
-      atomicMax(&hull[1], hi);
-      __syncthreads();
-      lo = hull[0], hi = hull[1];
     }
     used = n < c.tk && n >= lo && n < hi;
   }
@@ -910,6 +927,7 @@ struct Layout {
   char *q, *d, *k, *v, *qt, *dt, *kt, *vt, *info;
   int *eq, *ed, *ek, *ev;
   Hull *hulls;
+  int2 *seen;
   Layout(const Call &c, bool backward, Scratch &s) {
     const int64_t heads = (int64_t)c.batch * c.key_heads, rows = heads * blocks_of(c.rows), keys = heads * blocks_of(c.tk);
     const size_t row_bytes = (size_t)rows * block_size(columns_of(c.dim)), key_bytes = (size_t)keys * block_size(columns_of(c.dim));
@@ -927,10 +945,15 @@ struct Layout {
     ev = (int *)s.take(keys * 4);
     ed = backward ? (int *)s.take(rows * 4) : nullptr;
     hulls = backward ? (Hull *)s.take(rows * sizeof(Hull)) : nullptr;
+    // All spans in every workgroup of keys are quadratic: forward, documents of 1 024, 131 072 tokens of 4 heads of 64 3 134 us and here 570; of 512, 4 096 tokens
+    // 59.9 and 57.7, 2 048 tokens 63.8 and with the launch 65.9.
+    seen = c.spans && c.tq > kSpansReadByAll ? (int2 *)s.take(c.batch * sizeof(int2)) : nullptr;
   }
 };
 
-void pack(const Call &c, Pack &p, hipStream_t s) {
+void pack(const Call &c, Pack &p, int2 *seen, hipStream_t s) {
+  p.seen = seen;
+  if (seen) hipLaunchKernelGGL(seen_kernel, dim3((unsigned)c.batch), dim3(1024), 0, s, c, seen);
   const int heads = c.batch * c.key_heads;
   int groups = 0;
   p.row_blocks = blocks_of(c.rows);
@@ -973,7 +996,7 @@ Exponents pair_forward(const Call &c, float *out, float *stat, const Pieces &pie
   p.jobs[0] = Job{c.q, true, l.q, nullptr, l.eq, 0};
   p.jobs[1] = Job{c.k, false, l.k, nullptr, l.ek, 0};
   p.jobs[2] = Job{c.v, false, nullptr, l.vt, l.ev, 0};
-  pack(c, p, s);
+  pack(c, p, l.seen, s);
   const Exponents ex = {l.eq, nullptr, l.ek, l.ev, nullptr, p.row_blocks, p.key_blocks};
   const unsigned groups = (unsigned)((int64_t)c.batch * c.key_heads * tiles * pieces.count);
   const bool plain = !c.slopes && c.cap == 0.f;
@@ -1000,7 +1023,7 @@ Exponents pair_backward(const Call &c, const float *out, const float *stat, cons
   p.rows = rows;
   p.info = (float *)l.info;
   p.hulls = l.hulls;
-  pack(c, p, s);
+  pack(c, p, l.seen, s);
   const Exponents ex = {l.eq, l.ed, l.ek, l.ev, l.hulls, p.row_blocks, p.key_blocks};
   const bool plain = !c.slopes && c.cap == 0.f;
   const int heads = c.batch * c.key_heads;
