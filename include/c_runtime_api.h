@@ -490,7 +490,8 @@ int DLGpuHeadRotaryBackward(const DLHeadGradientPart *parts, int n_parts, const 
  * them those with j <= i + keys - queries.  A query that sees none has the output 0 and the statistic -inf.  What a query does not see counts for nothing, whatever
  * it holds.  statistics [batch, heads, queries] are what the backward pass reads; one of output and statistics may be NULL.
  * Results must not overlap what they are computed from.  A call that takes scratch is refused on a stream that is being captured
- * into a graph: TINYFLOW_SPLIT=0 in the environment keeps the products on the fp32 instruction, where only few queries over many keys take some. */
+ * into a graph: TINYFLOW_SPLIT=0 in the environment keeps the products on the fp32 instruction, where only queries too few
+ * to give every CU work take some, over many keys. */
 int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle value, const DLArrayHandle spans,
                           const DLArrayHandle slopes, DLArrayHandle output, DLArrayHandle statistics, int batch, int heads,
                           int key_heads, float scale, float cap, int causal, int *memorytoSaving, void **stream);
