@@ -488,7 +488,10 @@ int DLGpuHeadRotaryBackward(const DLHeadGradientPart *parts, int n_parts, const 
  *   output_i = sum_j exp(s_ij - statistics_i) v_j, statistics_i = log sum_j exp(s_ij), over the keys j that query i sees.
  * These are spans[i] = (first, last): first <= j < last, spans [batch, queries, 2] or [queries, 2]; without spans all.  With `causal` of
  * them those with j <= i + keys - queries.  A query that sees none has the output 0 and the statistic -inf.  What a query does not see counts for nothing, whatever
- * it holds.  statistics [batch, heads, queries] are what the backward pass reads; one of output and statistics may be NULL.
+ * it holds.
+ * (The second term has the rounding of its size, 1e-3 at 1e4, and counts from the end of the keys, also where spans
+ * leave the end out.)
+ * statistics [batch, heads, queries] are what the backward pass reads; one of output and statistics may be NULL.
  * Results must not overlap what they are computed from.  A call that takes scratch is refused on a stream that is being captured
  * into a graph: TINYFLOW_SPLIT=0 in the environment keeps the products on the fp32 instruction, where only queries too few
  * to give every CU work take some, over many keys. */
