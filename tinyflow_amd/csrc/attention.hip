@@ -10,6 +10,7 @@
 // rows); where that leaves CUs without work the walks are cut, and sum_kernel adds the pieces.  Both compute the scores again; no sum goes
 // through atomics, so the bits do not depend on the order in which workgroups run.
 #include "attention.h"
+#include "few_rows.h"
 #include "internal.h"
 
 #include <algorithm>
@@ -310,18 +311,21 @@ __global__ __launch_bounds__(kThreads, DP * NC <= 128 ? 2 : 1) void few_kernel(c
   const int64_t key_step = (int64_t)c.key_heads * c.dim;
   const float *k0 = c.k + c.key_at(b, g, 0), *v0 = c.v + c.key_at(b, g, 0);
   // Loads without a branch, so that it is known how many are under way: columns that are none have an offset behind the buffer and read as zero, and
-  // keys behind the last are the last again.
+  // keys behind the last are the last again.  The buffer ends with the array: four columns of a head whose length is no multiple of four may reach
+  // behind the last one.
   typedef __attribute__((__vector_size__(4 * sizeof(unsigned)))) unsigned u32x4;
   f32x4 keys[2][GD], values[2][4][VD];
+  const int64_t in_array = (int64_t)c.batch * c.tk * key_step, head_at = c.key_at(b, g, 0);
+  int bytes;
   auto fetch = [&](const float *base, int row, int column) {
-    const uint32_t at = (uint32_t)row * (uint32_t)(key_step * 4) + (uint32_t)column * 4u;
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(base), 0, 0x7fffffff, 0x00020000);
-    f32x4 x = __builtin_bit_cast(f32x4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(r, (int)(column < c.dim ? at : 0x80000000u), 0, 0));
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(base), 0, bytes, 0x00020000);
+    f32x4 x = __builtin_bit_cast(f32x4, (u32x4)__builtin_amdgcn_raw_buffer_load_b128(r, (int)buffer_offset(row, key_step, column, c.dim), 0, 0));
     return x;
   };
   auto load = [&](auto parity, int j0) {
     j0 = __builtin_amdgcn_readfirstlane(min(j0, end - 1));
     const float *kb = k0 + j0 * key_step, *vb = v0 + j0 * key_step;
+    bytes = buffer_bytes(in_array, head_at + j0 * key_step);
     const int last = end - 1 - j0;
 #pragma unroll
     for (int e = 0; e < GD; ++e) keys[decltype(parity)::value][e] = fetch(kb, min(col, last), 16 * e + 4 * quarter);
