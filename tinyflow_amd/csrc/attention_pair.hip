@@ -12,7 +12,7 @@
 // forward: pack 19 us, forward 195 to 208 (344 TFLOP/s; the fp32 instruction 1 094); backward: pack 53, dq 291 to 321 (343, three products), dkv 408 to 458
 // (320, four).  A product of the library on the fp16 instruction reaches a third of 1 178 to 1 347.
 //
-// A block with an infinity or a NaN, one whose values pass 2^55, or one of anything but queries with a row smaller than 2^-16 of its largest (it would
+// A block with an infinity or a NaN, one of gradients with a row whose statistic or delta is not finite, one whose values pass 2^55, or one of anything but queries with a row smaller than 2^-16 of its largest (it would
 // lose its digits; of a query only the scores count, which need none below that) has kBad for its exponent, and workgroups that meet one leave their
 // rows to the fp32 kernels.  Rows that see nothing and keys that nothing sees are packed as zeros, whatever they hold.
 #include "attention.h"
@@ -160,7 +160,6 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
   const int field = (int)(largest >> 23);
   int exponent = min(kSmallest, 141 - field);
   if (largest >= 0x7f800000u || exponent < kLargest || (which && largest && (int)(least >> 23) < field - 16 && exponent < kSmallest)) exponent = kBad;
-  if (tid == 0) job.exponents[(int64_t)head * blocks + block] = exponent;
   if (p.info && which == 1) {  // what the backward kernels read of the rows
     __shared__ Row of_rows[32];
     float delta = 0.f;
@@ -179,7 +178,9 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
       if (n < c.rows) p.rows[(int64_t)head * c.rows + n] = info;
       of_rows[row] = info;
     }
-    __syncthreads();
+    // A row that has seen an infinity or a NaN has passed it to its statistic or to delta, and 0 times that is no gradient of the keys that it
+    // does not see: the fp32 kernels choose by mask.
+    if (__syncthreads_or(tid % 8 == 0 && !(finite(info.stat) && finite(info.delta)))) exponent = kBad;
     if (tid < 64) {
       const int r = block * 32 + tid % 32;
       const Row mine = of_rows[tid % 32];
@@ -201,6 +202,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
       if (tid == 0) p.hulls[of_block] = seen;
     }
   }
+  if (tid == 0) job.exponents[(int64_t)head * blocks + block] = exponent;
   if (exponent == kBad) return;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e) {
