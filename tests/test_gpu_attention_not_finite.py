@@ -49,3 +49,19 @@ def test_no_gradient_becomes_zero(rt, monkeypatch, split, d):
     k[0, 5, 0, 3] = np.nan
     _, _, (dq, dk, dv) = _run(rt, q, k, clean, do, causal=True)
     assert np.isnan(dk).all() and np.isnan(dv).all() and np.isnan(dq[:, 5:]).any(3).all() and np.isfinite(dq[:, :5]).all()
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_shares_past_the_largest_number(rt, monkeypatch, split, d):
+    """Statistics far below the scores' make every share infinite: so are the gradients, not 0."""
+    from tinyflow_amd import gpu_op
+    from test_gpu_attention import _device, _empty
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    q, k, v, do = _data(1, 300, 300, 2, 1, d, 23)
+    out, stat, _ = _run(rt, q, k, v, do, backward=False)
+    grads = [_empty(rt, x.shape) for x in (q, k, v)]
+    a = _device(rt, q, k, v) + [None, None] + _device(rt, out, stat - 300, do)
+    assert gpu_op.attention_backward(*a, *grads, 1, 2, 1, d ** -0.5, 0.0, False, rt.stream) == 0
+    for g in grads:
+        assert not np.isfinite(g.asnumpy()).any()

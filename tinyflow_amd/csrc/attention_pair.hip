@@ -726,7 +726,7 @@ __global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_k
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e)
 #pragma unroll
-    for (int v = 0; v < 16; ++v) sum[e][v] = unit == kNoUnit ? 0.f : __builtin_ldexpf(sum[e][v], -unit);
+    for (int v = 0; v < 16; ++v) sum[e][v] = __builtin_ldexpf(sum[e][v], unit == kNoUnit ? 0 : -unit);
   store_sums(sum, dq + piece * stride + c.query_at(b, g, r), c.dim, c.scale);
 }
 
@@ -892,7 +892,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   for (int e = 0; e < DP / 32; ++e)
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
-      dks[e][x] = unit == kNoUnit ? 0.f : __builtin_ldexpf(dks[e][x], -unit);
+      dks[e][x] = __builtin_ldexpf(dks[e][x], unit == kNoUnit ? 0 : -unit);
       dvs[e][x] = __builtin_ldexpf(dvs[e][x], -13 - unit_v);
     }
   const int64_t all = (int64_t)c.batch * c.tk * c.key_heads * c.dim, key = c.key_at(b, g, j);
