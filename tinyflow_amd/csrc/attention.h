@@ -224,24 +224,47 @@ struct Exponents {
   const Hull *hulls;
   int row_blocks, key_blocks;
 
-  // Whether any block of [first, first + n) of a (b, key head) cannot be split, in the lanes that meet one
-  __device__ static inline bool bad(const int *of, int64_t head, int blocks, int first, int n) {
+  // An element is off by up to 2^-39 of its block's largest value, which moves a score by up to 2^-39 of scale times the columns times the largest of both
+  // blocks: what two exponents must add up to for a bound of 2^18 on that product, so 2^-21 on the error.  Queries and keys of a few units pass it by
+  // 2^8 with 128 columns.
+  int least_sum;
+
+  // Whether what a (b, key head) has in the blocks of a tile cannot be computed on pairs, in the lanes that find out: the tile's `n` blocks of rows from
+  // `first` on and the blocks of keys that they see.
+  __device__ inline bool bad_rows(int64_t head, int first, int n, int first_key, int n_keys) const {
     bool found = false;
-    if (of)
-      for (int e = threadIdx.x; e < n; e += blockDim.x) found |= first + e < blocks && of[head * blocks + first + e] == kBad;
+    int least = INT32_MAX / 2;
+    for (int e = first; e < first + n && e < row_blocks; ++e) {
+      least = min(least, q[head * row_blocks + e]);
+      if (d) found |= n_keys > 0 && d[head * row_blocks + e] == kBad;
+    }
+    for (int e = threadIdx.x; e < n_keys; e += blockDim.x) {
+      const int64_t at = head * key_blocks + first_key + e;
+      found |= first_key + e < key_blocks && (least + k[at] < least_sum || v[at] == kBad);
+    }
     return found;
   }
-  __device__ inline bool bad_rows(int64_t head, int first, int n) const { return bad(q, head, row_blocks, first, n) | bad(d, head, row_blocks, first, n); }
-  __device__ inline bool bad_keys(int64_t head, int first, int n) const { return bad(k, head, key_blocks, first, n) | bad(v, head, key_blocks, first, n); }
-  // Any of a (b, key head).  The fp32 kernels ask this first: of a head without one they only see its exponents (dq of 4 096 x 16 heads of 128 5.3 us, 7.9 without).
-  __device__ inline bool bad_head(int64_t head) const { return bad_rows(head, 0, row_blocks) | bad_keys(head, 0, key_blocks); }
-  // of the blocks of rows that see one of the keys [from, to)
-  __device__ inline bool bad_rows_of(int64_t head, int from, int to) const {
-    bool found = false;
+  // A tile's `n` blocks of keys from `first` on, the keys [from, to), and the blocks of rows that see one of them.
+  __device__ inline bool bad_keys(int64_t head, int first, int n, int from, int to) const {
+    bool bad_value = false, found = false;
+    int least = INT32_MAX / 2;
+    for (int e = first; e < first + n && e < key_blocks; ++e) {
+      least = min(least, k[head * key_blocks + e]);
+      bad_value |= v[head * key_blocks + e] == kBad;
+    }
     for (int e = threadIdx.x; e < row_blocks; e += blockDim.x) {
       const int64_t at = head * row_blocks + e;
-      found |= (q[at] == kBad || d[at] == kBad) && hulls[at].meets(from, to);
+      found |= (least + q[at] < least_sum || d[at] == kBad || bad_value) && hulls[at].meets(from, to);
     }
+    return found;
+  }
+  // Whether any tile of a (b, key head) may be such: either a query's or a key's exponent is below its share of the sum.  The fp32 kernels ask this first: of a head
+  // without one they only see its exponents (dq of 4 096 x 16 heads of 128 5.3 us, 7.9 without).
+  __device__ inline bool bad_head(int64_t head) const {
+    const int share = least_sum >> 1;
+    bool found = false;
+    for (int e = threadIdx.x; e < row_blocks; e += blockDim.x) found |= q[head * row_blocks + e] < share || (d && d[head * row_blocks + e] == kBad);
+    for (int e = threadIdx.x; e < key_blocks; e += blockDim.x) found |= k[head * key_blocks + e] < least_sum - share || v[head * key_blocks + e] == kBad;
     return found;
   }
 };

@@ -12,14 +12,16 @@
 // forward: pack 19 us, forward 195 to 208 (344 TFLOP/s; the fp32 instruction 1 094); backward: pack 53, dq 291 to 321 (343, three products), dkv 408 to 458
 // (320, four).  A product of the library on the fp16 instruction reaches a third of 1 178 to 1 347.
 //
-// A block with an infinity or a NaN, one of gradients with a row whose statistic or delta is not finite, one whose values pass 2^55, or one of anything but queries with a row smaller than 2^-16 of its largest (it would
-// lose its digits; of a query only the scores count, which need none below that) has kBad for its exponent, and workgroups that meet one leave their
-// rows to the fp32 kernels.  Rows that see nothing and keys that nothing sees are packed as zeros, whatever they hold.
+// A block with an infinity or a NaN, one of gradients with a row whose statistic or delta is not finite, one whose values pass 2^55, or one of anything
+// but queries with a row smaller than 2^-16 of its largest (it would lose its digits) has kBad for its exponent.  Workgroups that meet one, or blocks of queries and keys
+// so large that what is left off would show in a score (Exponents::least_sum), leave their rows to the fp32 kernels.  Rows that see nothing and keys that
+// nothing sees are packed as zeros, whatever they hold.
 #include "attention.h"
 #include "internal.h"
 #include "lanes.h"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -477,7 +479,7 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
   mine.of(lo, hi, live);
   const Hull all = mine.all(room);  // the second group's waves have the first's rows
   const int first = all.first(), steps = all.steps();
-  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32) | ex.bad_keys(bg, first, steps))) return;
+  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32, first, steps))) return;
   const int begin = first + (int)((int64_t)steps * piece / pieces.count), end = first + (int)((int64_t)steps * (piece + 1) / pieces.count);
   const int block = min(tile * (kRows / 32) + wave, ex.row_blocks - 1);
   const int64_t row_block = (int64_t)bg * ex.row_blocks + block, key_block = (int64_t)bg * ex.key_blocks;
@@ -646,7 +648,7 @@ __global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_k
   mine.of(row.lo, row.hi, live);
   const Hull all = mine.all(room);
   const int first = all.first(), steps = all.steps();
-  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32) | ex.bad_keys(bg, first, steps))) return;
+  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32, first, steps))) return;
   const int begin = first + (int)((int64_t)steps * piece / pieces), end = first + (int)((int64_t)steps * (piece + 1) / pieces);
   const int block = min(tile * (kRows / 32) + wave, ex.row_blocks - 1);
   const int64_t row_block = (int64_t)bg * ex.row_blocks + block, key_block = (int64_t)bg * ex.key_blocks;
@@ -743,7 +745,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   const int b = bg / c.key_heads, g = bg % c.key_heads;
   const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int tile_lo = tile * kRows, tile_hi = min(c.tk, tile_lo + kRows);
-  if (__syncthreads_or(ex.bad_rows_of(bg, tile_lo, tile_hi) | ex.bad_keys(bg, tile_lo / 32, kRows / 32))) return;
+  if (__syncthreads_or(ex.bad_keys(bg, tile_lo / 32, kRows / 32, tile_lo, tile_hi))) return;
   const int64_t row_block = (int64_t)bg * ex.row_blocks;
   // The blocks of rows that see one of the keys; a piece has every pieces-th of them, from the last on, which in a causal pass all tiles see: a piece's tiles
   // of one head, on one XCD where heads times pieces are a multiple of 8, go through the same blocks together and find them in its L2.  (4 096 x 16
@@ -967,6 +969,13 @@ void pack(const Call &c, Pack &p, int2 *seen, hipStream_t s) {
   with_columns(c.dim, [&](auto dp) { hipLaunchKernelGGL((pack_kernel<decltype(dp)::value>), dim3((unsigned)groups), dim3(kThreads), 0, s, c, p); });
 }
 
+// Exponents::least_sum: elements of a block are less than 2^15 times 2^-exponent
+int least_sum(const Call &c) {
+  int exponent;
+  (void)frexpf(c.scale * (float)c.dim, &exponent);   // 2^exponent is more
+  return exponent + 30 - 18;
+}
+
 }  // namespace
 
 bool pair_suits(const Call &c, bool backward) {
@@ -999,7 +1008,7 @@ Exponents pair_forward(const Call &c, float *out, float *stat, const Pieces &pie
   p.jobs[1] = Job{c.k, false, l.k, nullptr, l.ek, 0};
   p.jobs[2] = Job{c.v, false, nullptr, l.vt, l.ev, 0};
   pack(c, p, l.seen, s);
-  const Exponents ex = {l.eq, nullptr, l.ek, l.ev, nullptr, p.row_blocks, p.key_blocks};
+  const Exponents ex = {l.eq, nullptr, l.ek, l.ev, nullptr, p.row_blocks, p.key_blocks, least_sum(c)};
   const unsigned groups = (unsigned)((int64_t)c.batch * c.key_heads * tiles * pieces.count);
   const bool plain = !c.slopes && c.cap == 0.f;
   with_columns(c.dim, [&](auto dp) {
@@ -1026,7 +1035,7 @@ Exponents pair_backward(const Call &c, const float *out, const float *stat, cons
   p.info = (float *)l.info;
   p.hulls = l.hulls;
   pack(c, p, l.seen, s);
-  const Exponents ex = {l.eq, l.ed, l.ek, l.ev, l.hulls, p.row_blocks, p.key_blocks};
+  const Exponents ex = {l.eq, l.ed, l.ek, l.ev, l.hulls, p.row_blocks, p.key_blocks, least_sum(c)};
   const bool plain = !c.slopes && c.cap == 0.f;
   const int heads = c.batch * c.key_heads;
   with_columns(c.dim, [&](auto dp) {
