@@ -77,3 +77,24 @@ def test_scores_that_pass_every_digit(rt, monkeypatch, split, scale):
     assert np.abs(out.asnumpy()[0, :, 0] - p @ v[0, :, 0]).max() <= 2.0 ** -18   # sums of a few values of up to 4
     for got in (dq, dk, dv):
         assert np.isfinite(got.asnumpy()).all()
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("small,scale", [((-60, -20), 38), ((-50, -35), 39), ((-20, -15), 35), ((20, 10), -30)])
+def test_scales_that_make_up_for_small_operands(rt, monkeypatch, split, small, scale):
+    """Queries and keys of 2^small with a scale of 2^scale."""
+    from tinyflow_amd import gpu_op, ndarray
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    q, k, v, do = _data(1, 300, 300, 2, 1, 64, 39)
+    q, k = q * np.float32(2.0 ** small[0]), k * np.float32(2.0 ** small[1])
+    scale = 2.0 ** scale
+    a = [ndarray.array(x, ctx=rt.ctx) for x in (q, k, v, do)]
+    out, stat, *grads = (ndarray.array(np.full(s, 7.25, np.float32), ctx=rt.ctx) for s in (q.shape, (1, 2, 300), q.shape, k.shape, v.shape))
+    numbers = (1, 2, 1, scale, 0.0, False, rt.stream)
+    assert gpu_op.attention_forward(*a[:3], None, None, out, stat, *numbers) == 0
+    assert gpu_op.attention_backward(*a[:3], None, None, out, stat, a[3], *grads, *numbers) == 0
+    want = ref.Attention(q, k, v, None, None, scale)
+    ref.assert_within(out.asnumpy(), want.out, want.out_tol, "out")
+    ref.assert_within(stat.asnumpy(), want.stat, want.stat_tol, "statistics")
+    for what, got, (value, tol) in zip(("dq", "dk", "dv"), grads, want.backward(out.asnumpy(), stat.asnumpy(), do)):
+        ref.assert_within(got.asnumpy(), value, tol, what)

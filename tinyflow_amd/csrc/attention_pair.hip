@@ -426,8 +426,8 @@ __device__ inline const char *uniform(const char *p) {
 // What the launch before has written and this one only reads, at an address that the wave shares: by a scalar load, which leaves the count of
 // the vector loads under way alone.
 __device__ inline int scalar(const int *p) { return *(const __attribute__((address_space(4))) int *)uniform((const char *)p); }
-// 2^-(a + b) factor, for scores: not below 2^-80 of it, where a score is nothing, so that it times the -infinity of a masked one is that
-__device__ inline float unscaled(float factor, int a, int b) { return __builtin_ldexpf(factor, max(-(a + b), -80)); }
+// 2^-(a + b) factor, for scores: not below 2^-120, where a product of less than 2^37 is no score, so that it times the -infinity of a masked one is that
+__device__ inline float unscaled(float factor, int a, int b) { return fmaxf(__builtin_ldexpf(factor, -(a + b)), 0x1p-120f); }
 
 
 // Block `index` of each of N operands, one behind the other in LDS from `to` on: each of four waves fetches a quarter of each.
