@@ -35,6 +35,23 @@ def test_a_query_among_larger_ones(rt, monkeypatch, split, power):
 
 
 @pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("power", [-12, -30, -60])
+def test_queries_of_documents(rt, monkeypatch, split, power):
+    """Documents that end inside of blocks, every other one with queries of 2^power: their keys' gradients are as small."""
+    from tinyflow_amd import gpu_op
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    q, k, v, do = _data(1, 320, 320, 2, 2, 64, 32)
+    documents = np.arange(320) // 80
+    q[:, documents % 2 == 1] *= np.float32(2.0 ** power)
+    spans = gpu_op.attention_spans(320, documents=documents)
+    out, stat, (_, dk, _) = _run(rt, q, k, v, do, spans=spans)
+    for n in range(4):
+        own = documents == n
+        want = ref.Attention(q[:, own], k[:, own], v[:, own], None, None, 0.125).backward(out[:, own], stat[:, :, own], do[:, own])[1][0]
+        assert _off(dk[:, own], want) <= ROW, "dk of document %d" % n
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
 @pytest.mark.parametrize("power", [14, 24, 30, 40])
 @pytest.mark.parametrize("which", ["query", "key"])
 def test_a_large_column_that_meets_zeros(rt, monkeypatch, split, power, which):

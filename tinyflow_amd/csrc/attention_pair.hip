@@ -12,10 +12,10 @@
 // forward: pack 19 us, forward 195 to 208 (344 TFLOP/s; the fp32 instruction 1 094); backward: pack 53, dq 291 to 321 (343, three products), dkv 408 to 458
 // (320, four).  A product of the library on the fp16 instruction reaches a third of 1 178 to 1 347.
 //
-// A block with an infinity or a NaN, one of gradients with a row whose statistic or delta is not finite, one whose values pass 2^55, or one of anything
-// but queries with a row smaller than 2^-16 of its largest (it would lose its digits) has kBad for its exponent.  Workgroups that meet one, or blocks of queries and keys
-// so large that what is left off would show in a score (Exponents::least_sum), leave their rows to the fp32 kernels.  Rows that see nothing and keys that
-// nothing sees are packed as zeros, whatever they hold.
+// A block with an infinity or a NaN, one of gradients with a row whose statistic or delta is not finite, one whose values pass 2^55, or one with a row
+// smaller than 2^-16 of its largest (it would lose its digits; of queries and keys in the forward pass only the scores count) has kBad for its
+// exponent.  Workgroups that meet one, or blocks of queries and keys so large that what is left off would show in a score (Exponents::least_sum), leave their rows
+// to the fp32 kernels.  Rows that see nothing and keys that nothing sees are packed as zeros, whatever they hold.
 #include "attention.h"
 #include "internal.h"
 #include "lanes.h"
@@ -66,6 +66,7 @@ enum Info { kStat = 0, kDelta, kLo, kHi, kSlope, kAhead };
 struct Job {
   const float *src;
   bool of_rows;
+  bool digits;       // whether every row's own digits count, not only the scores'
   char *plain, *transposed;
   int *exponents;
   int first;         // workgroup
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
   }
   const int field = (int)(largest >> 23);
   int exponent = min(kSmallest, 141 - field);
-  if (largest >= 0x7f800000u || exponent < kLargest || (which && largest && (int)(least >> 23) < field - 16 && exponent < kSmallest)) exponent = kBad;
+  if (largest >= 0x7f800000u || exponent < kLargest || (job.digits && largest && (int)(least >> 23) < field - 16 && exponent < kSmallest)) exponent = kBad;
   if (p.info && which == 1) {  // what the backward kernels read of the rows
     __shared__ Row of_rows[32];
     float delta = 0.f;
@@ -1004,9 +1005,9 @@ Exponents pair_forward(const Call &c, float *out, float *stat, const Pieces &pie
   const Layout l(c, false, of);
   Pack p = {};
   p.n_jobs = 3;
-  p.jobs[0] = Job{c.q, true, l.q, nullptr, l.eq, 0};
-  p.jobs[1] = Job{c.k, false, l.k, nullptr, l.ek, 0};
-  p.jobs[2] = Job{c.v, false, nullptr, l.vt, l.ev, 0};
+  p.jobs[0] = Job{c.q, true, false, l.q, nullptr, l.eq, 0};
+  p.jobs[1] = Job{c.k, false, false, l.k, nullptr, l.ek, 0};
+  p.jobs[2] = Job{c.v, false, true, nullptr, l.vt, l.ev, 0};
   pack(c, p, l.seen, s);
   const Exponents ex = {l.eq, nullptr, l.ek, l.ev, nullptr, p.row_blocks, p.key_blocks, least_sum(c)};
   const unsigned groups = (unsigned)((int64_t)c.batch * c.key_heads * tiles * pieces.count);
@@ -1025,10 +1026,10 @@ Exponents pair_backward(const Call &c, const float *out, const float *stat, cons
   Pack p = {};
   p.n_jobs = 4;
   const bool keys = to.dk || to.dv;
-  p.jobs[0] = Job{c.q, true, l.q, keys ? l.qt : nullptr, l.eq, 0};
-  p.jobs[1] = Job{dout, true, l.d, keys ? l.dt : nullptr, l.ed, 0};
-  p.jobs[2] = Job{c.k, false, l.k, to.dq ? l.kt : nullptr, l.ek, 0};
-  p.jobs[3] = Job{c.v, false, l.v, nullptr, l.ev, 0};
+  p.jobs[0] = Job{c.q, true, true, l.q, keys ? l.qt : nullptr, l.eq, 0};
+  p.jobs[1] = Job{dout, true, true, l.d, keys ? l.dt : nullptr, l.ed, 0};
+  p.jobs[2] = Job{c.k, false, true, l.k, to.dq ? l.kt : nullptr, l.ek, 0};
+  p.jobs[3] = Job{c.v, false, true, l.v, nullptr, l.ev, 0};
   p.out = out;
   p.stat = stat;
   p.rows = rows;
