@@ -72,6 +72,43 @@ def test_a_large_column_that_meets_zeros(rt, monkeypatch, split, power, which):
 
 
 @pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("power", [14, 24, 30, 40])
+def test_a_large_column_of_values(rt, monkeypatch, split, power):
+    """The other columns' outputs, and with no gradient in the large column all other gradients."""
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    q, k, v, do = _data(1, 300, 300, 2, 1, 64, 34)
+    v[..., 5] *= np.float32(2.0 ** power)
+    do[..., 5] = 0
+    out, stat, grads = _run(rt, q, k, v, do, causal=True)
+    rest = np.arange(64) != 5
+    want = ref.Attention(q, k, v[..., rest], None, None, 0.125, causal=True)
+    ref.assert_within(out[..., rest], want.out, want.out_tol, "out")
+    # scores are of 64 columns, dp of the 63 that count
+    assert _off(out[..., 5], ref.Attention(q, k, v[..., 5:6], None, None, 0.125, causal=True).out[..., 0]) <= ROW
+    small = want.backward(out[..., rest], stat, do[..., rest])
+    for what, got, (value, tol) in zip(("dq", "dk"), grads, small):
+        ref.assert_within(got, value, tol, what)
+    ref.assert_within(grads[2][..., rest], *small[2], "dv")
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("power", [-24, -34, -44])
+@pytest.mark.parametrize("which", range(4))
+def test_a_small_column(rt, monkeypatch, split, power, which):
+    """Its own gradient (of a query's or key's column, from the other's; of a value's, from the output's) or output has its digits."""
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    a = _data(1, 300, 300, 2, 1, 64, 35)
+    a[which][..., 7] *= np.float32(2.0 ** power)
+    q, k, v, do = a
+    out, stat, grads = _run(rt, q, k, v, do, causal=True)
+    want = ref.Attention(q, k, v, None, None, 0.125, causal=True)
+    values = [value for value, _ in want.backward(out, stat, do)]
+    pairs = {0: (grads[1], values[1]), 1: (grads[0], values[0]), 2: (out, want.out), 3: (grads[2], values[2])}
+    got, value = pairs[which]
+    assert _off(got[..., 7], value[..., 7]) <= ROW
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
 @pytest.mark.parametrize("scale", [1e3, 1e6, 1e9])
 def test_scores_that_pass_every_digit(rt, monkeypatch, split, scale):
     """Every query has one key that takes all: scores of up to 1e10, whose differences are what they are."""

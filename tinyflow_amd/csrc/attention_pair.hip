@@ -13,7 +13,7 @@
 // (320, four).  A product of the library on the fp16 instruction reaches a third of 1 178 to 1 347.
 //
 // A block with an infinity or a NaN, one of gradients with a row whose statistic or delta is not finite, one whose values pass 2^55, or one with a row
-// smaller than 2^-16 of its largest (it would lose its digits; of queries and keys in the forward pass only the scores count) has kBad for its
+// or a column smaller than 2^-16 of its largest (it would lose its digits; of queries and keys in the forward pass only the scores count) has kBad for its
 // exponent.  Workgroups that meet one, or blocks of queries and keys so large that what is left off would show in a score (Exponents::least_sum), leave their rows
 // to the fp32 kernels.  Rows that see nothing and keys that nothing sees are packed as zeros, whatever they hold.
 #include "attention.h"
@@ -66,7 +66,7 @@ enum Info { kStat = 0, kDelta, kLo, kHi, kSlope, kAhead };
 struct Job {
   const float *src;
   bool of_rows;
-  bool digits;       // whether every row's own digits count, not only the scores'
+  bool digits;       // whether every row's and column's own digits count, not only the scores'
   char *plain, *transposed;
   int *exponents;
   int first;         // workgroup
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(1024) void seen_kernel(const Call c, int2 *seen) {
 template <int DP>
 __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack p) {
   __shared__ __align__(16) float tile[32][DP + 4];
-  __shared__ uint32_t most[32];
+  __shared__ uint32_t most[32], columns[4][8];
   __shared__ int hull[2];
   int which = 0;
   for (int i = 1; i < p.n_jobs; ++i) which = (int)blockIdx.x >= p.jobs[i].first ? i : which;
@@ -154,11 +154,13 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
   if (tid % 8 == 0) most[row] = top;
   __syncthreads();
   uint32_t largest = 0, least = 0x7f800000u;
+  int rows = 0;  // with anything but zeros
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const uint32_t v = most[i];
     largest = max(largest, v);
     least = v ? min(least, v) : least;
+    rows += v != 0;
   }
   const int field = (int)(largest >> 23);
   int exponent = min(kSmallest, 141 - field);
@@ -205,15 +207,29 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
       if (tid == 0) p.hulls[of_block] = seen;
     }
   }
-  if (tid == 0) job.exponents[(int64_t)head * blocks + block] = exponent;
-  if (exponent == kBad) return;
+  // Columns that are smaller than 2^-16 of the block's largest in all rows, and not all zeros: a bit for each of the lane's columns with an element
+  // that is not smaller, and one with any.  (Of a single row they are no column yet: its elements are what they are beside its largest.)
+  static_assert(DP <= 128, "16 columns a lane");
+  const uint32_t not_small = (uint32_t)max(field - 16, 0) << 23;
+  uint32_t marks = 0;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[e][i] = __builtin_ldexpf(x[e][i], exponent);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t size = bits_of(x[e][i]) & 0x7fffffffu;
+      marks |= (size >= not_small ? 1u << (4 * e + i) : 0u) | (size ? 0x10000u << (4 * e + i) : 0u);
+      x[e][i] = __builtin_ldexpf(x[e][i], exponent);
+    }
     *reinterpret_cast<f32x4 *>(&tile[row][32 * e + tid % 8 * 4]) = x[e];
   }
+#pragma unroll
+  for (int step = 8; step < 64; step *= 2) marks |= (uint32_t)__shfl_xor((int)marks, step);
+  if (tid % 64 < 8) columns[tid / 64][tid % 8] = marks;
   __syncthreads();
+  marks = columns[0][tid % 8] | columns[1][tid % 8] | columns[2][tid % 8] | columns[3][tid % 8];
+  if (job.digits && rows > 1 && __any((marks >> 16 & ~marks) != 0)) exponent = kBad;
+  if (tid == 0) job.exponents[(int64_t)head * blocks + block] = exponent;
+  if (exponent == kBad) return;
   const int64_t to = ((int64_t)head * blocks + block) * block_size(DP);
   if (job.plain)
 #pragma unroll
