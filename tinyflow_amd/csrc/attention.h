@@ -229,14 +229,16 @@ struct Exponents {
   // 2^8 with 128 columns.
   int least_sum;
 
-  // Whether what a (b, key head) has in the blocks of a tile cannot be computed on pairs, in the lanes that find out: the tile's `n` blocks of rows from
+  // Whether what a (b, key head) has in the blocks of a tile cannot be computed on pairs, in the lanes that find out: the tile's four blocks of rows from
   // `first` on and the blocks of keys that they see.
-  __device__ inline bool bad_rows(int64_t head, int first, int n, int first_key, int n_keys) const {
+  __device__ inline bool bad_rows(int64_t head, int first, int first_key, int n_keys) const {
     bool found = false;
     int least = INT32_MAX / 2;
-    for (int e = first; e < first + n && e < row_blocks; ++e) {
-      least = min(least, q[head * row_blocks + e]);
-      if (d) found |= n_keys > 0 && d[head * row_blocks + e] == kBad;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t at = head * row_blocks + min(first + e, row_blocks - 1);
+      least = min(least, q[at]);
+      if (d) found |= n_keys > 0 && d[at] == kBad;
     }
     for (int e = threadIdx.x; e < n_keys; e += blockDim.x) {
       const int64_t at = head * key_blocks + first_key + e;
@@ -244,13 +246,15 @@ struct Exponents {
     }
     return found;
   }
-  // A tile's `n` blocks of keys from `first` on, the keys [from, to), and the blocks of rows that see one of them.
-  __device__ inline bool bad_keys(int64_t head, int first, int n, int from, int to) const {
+  // A tile's four blocks of keys from `first` on, the keys [from, to), and the blocks of rows that see one of them.
+  __device__ inline bool bad_keys(int64_t head, int first, int from, int to) const {
     bool bad_value = false, found = false;
     int least = INT32_MAX / 2;
-    for (int e = first; e < first + n && e < key_blocks; ++e) {
-      least = min(least, k[head * key_blocks + e]);
-      bad_value |= v[head * key_blocks + e] == kBad;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t at = head * key_blocks + min(first + e, key_blocks - 1);
+      least = min(least, k[at]);
+      bad_value |= v[at] == kBad;
     }
     for (int e = threadIdx.x; e < row_blocks; e += blockDim.x) {
       const int64_t at = head * row_blocks + e;

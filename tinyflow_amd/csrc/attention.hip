@@ -180,7 +180,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
   const Hull all = mine.all(room);
   // this piece's steps of the keys that any of the rows sees
   const int first = all.first(), steps = all.steps();
-  if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), kRows / 32, first, steps))) return;
+  if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), first, steps))) return;
   Operand<DP> q;
   q.load(c.q + c.query_at(b, g, live ? r : 0), c.dim, live);
   const int begin = first + (int)((int64_t)steps * piece / pieces.count), end = first + (int)((int64_t)steps * (piece + 1) / pieces.count);
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
   mine.of(row.lo, row.hi, live);
   const Hull all = mine.all(room);
   const int first = all.first(), steps = all.steps();
-  if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), kRows / 32, first, steps))) return;
+  if (left.q && !__syncthreads_or(left.bad_rows(bg, tile * (kRows / 32), first, steps))) return;
   const int begin = first + (int)((int64_t)steps * piece / pieces), end = first + (int)((int64_t)steps * (piece + 1) / pieces);
   Operand<DP> q, d;
   q.load(c.q + at, c.dim, live);
@@ -660,7 +660,7 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float
   const int lane = threadIdx.x % 64, half = lane / 32;
   const int tile_lo = tile * kRows, tile_hi = min(c.tk, tile_lo + kRows);
   const int j = tile_lo + threadIdx.x / 64 * 32 + lane % 32;
-  if (left.q && !__syncthreads_or(left.bad_keys(bg, tile_lo / 32, kRows / 32, tile_lo, tile_hi))) return;
+  if (left.q && !__syncthreads_or(left.bad_keys(bg, tile_lo / 32, tile_lo, tile_hi))) return;
   const bool live = j < c.tk;
   const int64_t at = c.key_at(b, g, live ? j : 0);
   Operand<DP> k, v;

@@ -211,23 +211,31 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
   // that is not smaller, and one with any.  (Of a single row they are no column yet: its elements are what they are beside its largest.)
   static_assert(DP <= 128, "16 columns a lane");
   const uint32_t not_small = (uint32_t)max(field - 16, 0) << 23;
-  uint32_t marks = 0;
+  const bool judged = job.digits && rows > 1;
+  if (judged) {
+    uint32_t marks = 0;
+#pragma unroll
+    for (int e = 0; e < DP / 32; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t size = bits_of(x[e][i]) & 0x7fffffffu;
+        marks |= (size >= not_small ? 1u << (4 * e + i) : 0u) | (size ? 0x10000u << (4 * e + i) : 0u);
+      }
+#pragma unroll
+    for (int step = 8; step < 64; step *= 2) marks |= (uint32_t)__shfl_xor((int)marks, step);
+    if (tid % 64 < 8) columns[tid / 64][tid % 8] = marks;
+  }
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t size = bits_of(x[e][i]) & 0x7fffffffu;
-      marks |= (size >= not_small ? 1u << (4 * e + i) : 0u) | (size ? 0x10000u << (4 * e + i) : 0u);
-      x[e][i] = __builtin_ldexpf(x[e][i], exponent);
-    }
+    for (int i = 0; i < 4; ++i) x[e][i] = __builtin_ldexpf(x[e][i], exponent);
     *reinterpret_cast<f32x4 *>(&tile[row][32 * e + tid % 8 * 4]) = x[e];
   }
-#pragma unroll
-  for (int step = 8; step < 64; step *= 2) marks |= (uint32_t)__shfl_xor((int)marks, step);
-  if (tid % 64 < 8) columns[tid / 64][tid % 8] = marks;
   __syncthreads();
-  marks = columns[0][tid % 8] | columns[1][tid % 8] | columns[2][tid % 8] | columns[3][tid % 8];
-  if (job.digits && rows > 1 && __any((marks >> 16 & ~marks) != 0)) exponent = kBad;
+  if (judged) {
+    const uint32_t marks = columns[0][tid % 8] | columns[1][tid % 8] | columns[2][tid % 8] | columns[3][tid % 8];
+    if (__any((marks >> 16 & ~marks) != 0)) exponent = kBad;
+  }
   if (tid == 0) job.exponents[(int64_t)head * blocks + block] = exponent;
   if (exponent == kBad) return;
   const int64_t to = ((int64_t)head * blocks + block) * block_size(DP);
@@ -496,7 +504,7 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
   mine.of(lo, hi, live);
   const Hull all = mine.all(room);  // the second group's waves have the first's rows
   const int first = all.first(), steps = all.steps();
-  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32, first, steps))) return;
+  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), first, steps))) return;
   const int begin = first + (int)((int64_t)steps * piece / pieces.count), end = first + (int)((int64_t)steps * (piece + 1) / pieces.count);
   const int block = min(tile * (kRows / 32) + wave, ex.row_blocks - 1);
   const int64_t row_block = (int64_t)bg * ex.row_blocks + block, key_block = (int64_t)bg * ex.key_blocks;
@@ -665,7 +673,7 @@ __global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_k
   mine.of(row.lo, row.hi, live);
   const Hull all = mine.all(room);
   const int first = all.first(), steps = all.steps();
-  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), kRows / 32, first, steps))) return;
+  if (__syncthreads_or(ex.bad_rows(bg, tile * (kRows / 32), first, steps))) return;
   const int begin = first + (int)((int64_t)steps * piece / pieces), end = first + (int)((int64_t)steps * (piece + 1) / pieces);
   const int block = min(tile * (kRows / 32) + wave, ex.row_blocks - 1);
   const int64_t row_block = (int64_t)bg * ex.row_blocks + block, key_block = (int64_t)bg * ex.key_blocks;
@@ -762,7 +770,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   const int b = bg / c.key_heads, g = bg % c.key_heads;
   const int lane = threadIdx.x % 64, half = lane / 32, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int tile_lo = tile * kRows, tile_hi = min(c.tk, tile_lo + kRows);
-  if (__syncthreads_or(ex.bad_keys(bg, tile_lo / 32, kRows / 32, tile_lo, tile_hi))) return;
+  if (__syncthreads_or(ex.bad_keys(bg, tile_lo / 32, tile_lo, tile_hi))) return;
   const int64_t row_block = (int64_t)bg * ex.row_blocks;
   // The blocks of rows that see one of the keys; a piece has every pieces-th of them, from the last on, which in a causal pass all tiles see: a piece's tiles
   // of one head, on one XCD where heads times pieces are a multiple of 8, go through the same blocks together and find them in its L2.  (4 096 x 16
