@@ -109,6 +109,23 @@ def test_a_small_column(rt, monkeypatch, split, power, which):
 
 
 @pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("power", [-90, -105, -116])
+def test_small_values_everywhere(rt, monkeypatch, split, power):
+    """All values, or all gradients, near the smallest that fp32 has."""
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    q, k, v, do = _data(1, 300, 300, 2, 1, 64, 37)
+    small = np.float32(2.0 ** power)
+    tiny = 300 * 2.0 ** -149   # what is lost below the normal numbers
+    want = ref.Attention(q, k, v * small, None, None, 0.125, causal=True)
+    out, stat, grads = _run(rt, q, k, v * small, do * np.float32(64), causal=True)
+    ref.assert_within(out, want.out, want.out_tol + tiny, "out")
+    want = ref.Attention(q, k, v, None, None, 0.125, causal=True)
+    out, stat, grads = _run(rt, q, k, v, do * small, causal=True)
+    for what, got, (value, tol) in zip(("dq", "dk", "dv"), grads, want.backward(out, stat, do * small)):
+        ref.assert_within(got, value, tol + 64 * tiny, what)
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
 @pytest.mark.parametrize("scale", [1e3, 1e6, 1e9])
 def test_scores_that_pass_every_digit(rt, monkeypatch, split, scale):
     """Every query has one key that takes all: scores of up to 1e10, whose differences are what they are."""

@@ -12,10 +12,10 @@
 // forward: pack 19 us, forward 195 to 208 (344 TFLOP/s; the fp32 instruction 1 094); backward: pack 53, dq 291 to 321 (343, three products), dkv 408 to 458
 // (320, four).  A product of the library on the fp16 instruction reaches a third of 1 178 to 1 347.
 //
-// A block with an infinity or a NaN, one of gradients with a row whose statistic or delta is not finite, one whose values pass 2^55, or one with a row
-// or a column smaller than 2^-16 of its largest (it would lose its digits; of queries and keys in the forward pass only the scores count) has kBad for its
-// exponent.  Workgroups that meet one, or blocks of queries and keys so large that what is left off would show in a score (Exponents::least_sum), leave their rows
-// to the fp32 kernels.  Rows that see nothing and keys that nothing sees are packed as zeros, whatever they hold.
+// A block has kBad for its exponent if it holds an infinity or a NaN, or gradients with a row whose statistic or delta is not finite, if its values pass
+// 2^55 or stay below 2^-96, or if a row or a column of it is smaller than 2^-16 of its largest value and would lose its digits (of queries and keys in the forward
+// pass only the scores count).  Workgroups that meet one, or blocks of queries and keys so large that what is left off would show in a score
+// (Exponents::least_sum), leave their rows to the fp32 kernels.  Rows that see nothing and keys that nothing sees are packed as zeros, whatever they hold.
 #include "attention.h"
 #include "internal.h"
 #include "lanes.h"
@@ -48,7 +48,7 @@ __device__ __forceinline__ void static_for(F &&f) {
 
 constexpr int kFragment = 1024;  // bytes: 32 rows x 16 of fp16, a wave's lanes one behind the other
 constexpr int kInfoBytes = 1024;  // of a block of rows: eight arrays of 32, see Info
-constexpr int kSmallest = 110;   // exponents above it stand for values that no sum notices
+constexpr int kSmallest = 110;   // the largest exponent: of zeros, and of queries and keys that no score notices
 constexpr int kLargest = -40;
 constexpr int kSpansReadByAll = 2048;
 constexpr int kNoUnit = INT32_MAX / 2;  // of a sum of nothing
@@ -164,7 +164,8 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
   }
   const int field = (int)(largest >> 23);
   int exponent = min(kSmallest, 141 - field);
-  if (largest >= 0x7f800000u || exponent < kLargest || (job.digits && largest && (int)(least >> 23) < field - 16 && exponent < kSmallest)) exponent = kBad;
+  if (largest >= 0x7f800000u || exponent < kLargest) exponent = kBad;
+  if (job.digits && largest && ((int)(least >> 23) < field - 16 || 141 - field > kSmallest)) exponent = kBad;
   if (p.info && which == 1) {  // what the backward kernels read of the rows
     __shared__ Row of_rows[32];
     float delta = 0.f;
