@@ -109,6 +109,25 @@ def test_a_small_column(rt, monkeypatch, split, power, which):
 
 
 @pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("d", [48, 64, 128])
+@pytest.mark.parametrize("power", [20, 32, 40, 60])
+def test_keys_that_every_query_gives_little(rt, monkeypatch, split, d, power):
+    """A share of about 2^-power each: their values' and their own gradients are as small, and have their digits."""
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    q, k, v, do = _data(1, 300, 300, 2, 1, d, 36)
+    low = np.arange(300) // 7 % 3 == 1
+    q[..., 0] = 4
+    k[..., 0] = 0
+    k[:, low, :, 0] = -power * np.log(2) * np.sqrt(d) / 4
+    out, stat, (_, dk, dv) = _run(rt, q, k, v, do)
+    want = ref.Attention(q, k, v, None, None, d ** -0.5).backward(out, stat, do)
+    # Scores of up to 42 and 10 are sums of up to 128 products in chains of 40: 2^-24 40 52 off, and as much of the share: 2^-13; the sums themselves as
+    # above.
+    for what, got, value in (("dk", dk, want[1][0]), ("dv", dv, want[2][0])):
+        assert _off(got[:, low], value[:, low]) <= 2.0 ** -12.4, what
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
 @pytest.mark.parametrize("power", [-90, -105, -116])
 def test_small_values_everywhere(rt, monkeypatch, split, power):
     """All values, or all gradients, near the smallest that fp32 has."""
@@ -169,3 +188,48 @@ def test_scales_that_make_up_for_small_operands(rt, monkeypatch, split, small, s
     ref.assert_within(stat.asnumpy(), want.stat, want.stat_tol, "statistics")
     for what, got, (value, tol) in zip(("dq", "dk", "dv"), grads, want.backward(out.asnumpy(), stat.asnumpy(), do)):
         ref.assert_within(got.asnumpy(), value, tol, what)
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("power", [12, 30, 50])
+@pytest.mark.parametrize("which", ["values", "gradients"])
+def test_neighbours_with_larger_numbers(rt, monkeypatch, split, power, which):
+    """Two documents whose border is no border of a block of queries (of keys), the first with values (gradients) of 2^power of the second's: the
+    second's results are those that it has alone."""
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    tq, tk, rows, keys = (300, 320, 40, 64) if which == "values" else (320, 300, 64, 40)
+    q, k, v, do = _data(1, tq, tk, 2, 2, 64, 40)
+    spans = np.zeros((tq, 2), np.float32)
+    spans[:rows, 1] = keys
+    spans[rows:] = keys, tk
+    if which == "values":
+        v[:, :keys] *= np.float32(2.0 ** power)
+    else:
+        do[:, :rows] *= np.float32(2.0 ** power)
+    out, stat, (dq, dk, dv) = _run(rt, q, k, v, do, spans=spans)
+    want = ref.Attention(q[:, rows:], k[:, keys:], v[:, keys:], None, None, 0.125)
+    ref.assert_within(out[:, rows:], want.out, want.out_tol, "out")
+    ref.assert_within(stat[..., rows:], want.stat, want.stat_tol, "statistics")
+    values = want.backward(out[:, rows:], stat[..., rows:], do[:, rows:])
+    for what, got, (value, tol) in zip(("dq", "dk", "dv"), (dq[:, rows:], dk[:, keys:], dv[:, keys:]), values):
+        ref.assert_within(got, value, tol, what)
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("power", [12, 30, 50])
+@pytest.mark.parametrize("first", [True, False])
+def test_large_values_of_which_little_is_taken(rt, monkeypatch, split, power, first):
+    """A block of keys with values of 2^power, and a share of 2^-power 2^-12 for each of its keys: outputs and gradients come from the others."""
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    q, k, v, do = _data(1, 200, 320, 2, 1, 64, 41)
+    block = slice(0, 32) if first else slice(224, 256)
+    q[..., 0], k[..., 0] = 4, 0
+    k[:, block, :, 0] = -(power + 12) * np.log(2) * 8 / 4
+    v[:, block] *= np.float32(2.0 ** power)
+    out, stat, grads = _run(rt, q, k, v, do)
+    want = ref.Attention(q, k, v, None, None, 0.125)
+    for what, got, value in zip(("out", "dq", "dk", "dv"), [out] + grads, [want.out] + [x for x, _ in want.backward(out, stat, do)]):
+        # the shares of the block are of scores of up to 44: 2^-24 40 52 off, and so are their dk and dv
+        assert _off(got, value) <= 2.0 ** -12.4, what
+        if what in ("dk", "dv"):
+            assert _off(got[:, block], value[:, block]) <= 2.0 ** -12.4, what

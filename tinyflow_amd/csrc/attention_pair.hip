@@ -3,10 +3,11 @@
 // A block of 32 rows of an operand (queries, their gradients, keys or values of one head) is multiplied by the power of two that brings its
 // largest value into [2^14, 2^15), and each element is made of two fp16 numbers, h its nearest one and l the nearest to what is left: three
 // products of the fp16 instruction, h h' + h l' + l h', take the place of one of the fp32 instruction, which has a sixteenth of its rate.  What is
-// left off is 2^-23 of an element, or 2^-40 of its block's largest value where that is more, and l l', up to 2^-22 of a product.  p is at most 4, and
-// split times 2^12 or 2^13, so what is left off there is 2^-37 of 1 at most.
+// left off is 2^-23 of an element, or 2^-40 of its block's largest value where that is more, and l l', up to 2^-22 of a product.
 // Scales are a block's, so a product's scale is known for a whole tile and costs nothing: it is part of the factor of a score, of the
-// exponent of p, of ds.  A sum over several blocks has the scale of the largest one so far (`unit`); when a larger one comes the sum is multiplied.
+// exponent of p, of ds.  The sum over blocks has a scale of its own for each row (out, dq) or key (dk, dv): that of the largest p v, ds k, ds q or p do that it
+// has had, so that what is left off p or ds is 2^-30 of that at most, whatever lies beside the row or was next to nothing in it.  When a larger one comes the
+// sum is multiplied; a lane holds one row's or key's, so that is one factor a lane.
 //
 // Bound: the part's power and, with one or two waves a SIMD, the vector work between the products.  4 096 causal tokens, 16 heads on 4 of 128, 69 GFLOP
 // forward: pack 19 us, forward 195 to 208 (344 TFLOP/s; the fp32 instruction 1 094); backward: pack 53, dq 291 to 321 (343, three products), dkv 408 to 458
@@ -52,6 +53,7 @@ constexpr int kSmallest = 110;   // the largest exponent: of zeros, and of queri
 constexpr int kLargest = -40;
 constexpr int kSpansReadByAll = 2048;
 constexpr int kNoUnit = INT32_MAX / 2;  // of a sum of nothing
+constexpr int kMostHeld = 60;
 
 // Bytes of a block of 32 rows: DP columns of h and l.
 __host__ __device__ constexpr int64_t block_size(int dp) { return dp * 128; }
@@ -154,13 +156,11 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
   if (tid % 8 == 0) most[row] = top;
   __syncthreads();
   uint32_t largest = 0, least = 0x7f800000u;
-  int rows = 0;  // with anything but zeros
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const uint32_t v = most[i];
     largest = max(largest, v);
     least = v ? min(least, v) : least;
-    rows += v != 0;
   }
   const int field = (int)(largest >> 23);
   int exponent = min(kSmallest, 141 - field);
@@ -212,7 +212,8 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
   // that is not smaller, and one with any.  (Of a single row they are no column yet: its elements are what they are beside its largest.)
   static_assert(DP <= 128, "16 columns a lane");
   const uint32_t not_small = (uint32_t)max(field - 16, 0) << 23;
-  const bool judged = job.digits && rows > 1;
+  const uint64_t rows = __ballot(tid % 64 < 32 && most[tid % 32] != 0);  // with anything but zeros
+  const bool judged = job.digits && (rows & (rows - 1)) != 0;
   if (judged) {
     uint32_t marks = 0;
 #pragma unroll
@@ -222,8 +223,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
         const uint32_t size = bits_of(x[e][i]) & 0x7fffffffu;
         marks |= (size >= not_small ? 1u << (4 * e + i) : 0u) | (size ? 0x10000u << (4 * e + i) : 0u);
       }
-#pragma unroll
-    for (int step = 8; step < 64; step *= 2) marks |= (uint32_t)__shfl_xor((int)marks, step);
+    marks = lanes::reduce<64, 8>(marks, [](uint32_t a, uint32_t b) { return a | b; });
     if (tid % 64 < 8) columns[tid / 64][tid % 8] = marks;
   }
 #pragma unroll
@@ -518,8 +518,8 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
   f32x16 o[DP / 32];
 #pragma unroll
   for (int d = 0; d < DP / 32; ++d) o[d] = zeros();
-  float top = kNone, total = 0.f;   // total times 2^12
-  int unit = kSmallest;             // o is times 2^(12 + unit)
+  // Of the lane's row: o is sum exp2(s) v times 2^offset, total sum exp2(s) times 2^(offset - 40).
+  float offset = 1e9f, total = 0.f;
   const char *const from[2] = {ks, vs};
   const uint32_t to = lds_address(&lds[0][group][0]);
   if (begin + group < end) Blocks<DP, 2>(from, key_block + begin + group, to).all();
@@ -555,32 +555,25 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
 #pragma unroll
     for (int v = 0; v < 16; ++v) most = fmaxf(most, p[v]);
     most = fmaxf(most, other_half(most));
-    if (PLAIN) most = most == kNone ? kNone : most * factor;
-    // The sums' exponent follows the maximum only where it grows by more than 2: p is at most 4 then, and most steps leave the sums alone.
-    const float next = most > top + 2.f ? most : top, base = next == kNone ? 0.f : next;
-    if (__any(next != top)) {
-      const float fade = __builtin_amdgcn_exp2f(top - base);
+    if (PLAIN) most *= factor;
+    // exp2(s + shift) is the other operand, to the scale of the block's values.  A row's offset follows the largest p v that it has, not what its
+    // neighbours see or a large value of which it takes next to nothing: it is lowered where the operand would pass 2^15, to 2^9, so that most steps leave
+    // the sums alone.
+    float shift = offset - (float)ev;
+    if (__any(most + shift > 15.f)) {
+      const float lower = most + shift > 15.f ? 9.f - most + (float)ev : offset, fade = __builtin_amdgcn_exp2f(fmaxf(lower - offset, -200.f));
       total *= fade;
       multiply(o, fade);
+      offset = lower;
+      shift = offset - (float)ev;
     }
-    top = next;
-    if (ev < unit) {
-      multiply(o, __builtin_ldexpf(1.f, ev - unit));
-      unit = ev;
-    }
-    // p times 2^12 and the values' distance to the unit, up to 2^-20 of it here
-    const int apart = unit - ev, near = max(apart, -20);
-    const float shift = (float)(12 + near) - base;
     float sum = 0.f;
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
       p[v] = __builtin_amdgcn_exp2f(PLAIN ? __builtin_fmaf(p[v], factor, shift) : p[v] + shift);
       sum += p[v];
     }
-    total = __builtin_fmaf(sum, __builtin_ldexpf(1.f, -near), total);
-    if (apart < near)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) p[v] = __builtin_ldexpf(p[v], apart - near);
+    total = __builtin_fmaf(sum, __builtin_ldexpf(1.f, ev - 40), total);
     // the second half's operands while the first half is multiplied
     Weights w;
     static_for<4>([&](auto n) { w.set<decltype(n)::value>(p[2 * decltype(n)::value], p[2 * decltype(n)::value + 1]); });
@@ -591,8 +584,15 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
       });
     });
   }
-  total = (total + other_half(total)) * 0x1p-12f;
-  multiply(o, __builtin_ldexpf(1.f, -12 - unit));
+  total += other_half(total);
+  // to a maximum with total in [1, 2), and o to the same
+  const int above = (int)(bits_of(total) >> 23) - 127;
+  const float top = total == 0.f ? kNone : (float)(40 + above) - offset;
+  total = __builtin_ldexpf(total, -above);
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[d][v] = __builtin_ldexpf(o[d][v], -40 - above);
   // the second group's rows to the first
   __syncthreads();
   f32x4 *const room_o = reinterpret_cast<f32x4 *>(&lds[0][0][0]) + wave * (DP / 8 * 64);
@@ -624,14 +624,12 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
 
 // ------------------------------------------------------------------------------ backward
 
-// The unit of a sum of gradients times what has exponent `other`: the tile's largest gradient, held times 2^held, becomes less than 2^14 in it, unless
-// an earlier tile's was larger.
-__device__ __forceinline__ int gradient_unit(const float (&ds)[16], int held, int other, int unit) {
-  float most = 0.f;
-#pragma unroll
-  for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(ds[v]));
-  const int field = __builtin_amdgcn_readfirstlane((int)(lanes::largest<64>(bits_of(most)) >> 23));
-  return field == 0 || field == 255 ? unit : min(unit, 140 - field + held + other);
+// The unit of the sum of a lane's row or key, of gradients times what has exponent `other`: the step's largest gradient, held times 2^held, has to stay below
+// 2^15 in it.  Where one has to be lowered it becomes less than 2^6, and so do those of more than 2^10, so that it seldom has to.
+__device__ __forceinline__ int gradient_unit(float most, int held, int other, int unit, bool &lowers) {
+  const int field = (int)(bits_of(fmaxf(most, other_half(most))) >> 23), limit = field == 0 || field == 255 ? INT32_MAX : 141 - field + held + other;
+  lowers = __any(unit > limit);
+  return lowers && unit > limit - 5 ? min(unit, limit - 9) : unit;
 }
 
 // p times 2^x, for shift = x - the row's statistic, and the derivative of the cap, from a product.
@@ -694,7 +692,7 @@ __global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_k
   f32x16 sum[DP / 32];
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e) sum[e] = zeros();
-  int unit = kNoUnit;  // sum is times 2^unit
+  int unit = kNoUnit;  // sum is times 2^unit, of the lane's row
   const char *const from[3] = {ks, vs, kts};
   const uint32_t to = lds_address(&lds[0][0]);
   if (begin < end) Blocks<DP, 3>(from, key_block + begin, to).all();
@@ -733,8 +731,12 @@ __global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_k
       ds[v] = p[v] * __builtin_fmaf(s[1][v], d_factor, -delta);
       if (!PLAIN) ds[v] *= cap[v];
     }
-    const int new_unit = gradient_unit(ds, 0, ek, unit);
-    if (new_unit < unit) {
+    float most = 0.f;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(ds[v]));
+    bool lowers;
+    const int new_unit = gradient_unit(most, 0, ek, unit, lowers);
+    if (lowers) {
       multiply(sum, __builtin_ldexpf(1.f, max(new_unit - unit, -200)));
       keep<!TWO>(sum);
       unit = new_unit;
@@ -803,7 +805,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
   f32x16 dks[DP / 32], dvs[DP / 32];
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e) dks[e] = dvs[e] = zeros();
-  int unit = kNoUnit, unit_v = kSmallest;  // dks are times 2^unit, dvs times 2^(13 + unit_v)
+  int unit = kNoUnit, unit_v = kNoUnit;  // dks are times 2^unit, dvs times 2^unit_v, of the lane's key
   const char *const from[4] = {qs, ds_, qts, dts};
   const uint32_t to = lds_address(&lds[0][0]);
   auto fetch_info = [&](int step, int slot) {
@@ -847,34 +849,35 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
       continue;
     }
     const char *const at = lds[slot];
-    if (ed < unit_v) {
-      multiply(dvs, __builtin_ldexpf(1.f, ed - unit_v));
-      keep<(DP > 64)>(dvs);
-      unit_v = ed;
-    }
     const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(sign, -(ed + ev));
-    const int held = 13 + max(unit_v - ed, -60);  // p is held times 2^this, as the sum of dv needs it
+    // p is held times 2^this, as the sum of dv needs it, or 2^60 where that leaves fp32 no room
+    auto held_by = [&](int u) { return min(max(u - ed, -47), kMostHeld); };
+    int held = held_by(unit_v);
     const float *const of = reinterpret_cast<const float *>(at + 4 * BLOCK) + 4 * half;
     auto four = [&](int array, int q) { return *reinterpret_cast<const f32x4 *>(of + 32 * array + 8 * q); };
-    float p[16], cap[16], ds[16];
+    float p[16], cap[16], ds[16], most = 0.f;
     f32x16 s[2];
     Weights w;
     auto tile = [&](auto whole_c) {
       constexpr bool WHOLE = decltype(whole_c)::value;
-      f32x4 shift[4];
-      static_for<4>([&](auto q) { shift[decltype(q)::value] = (float)held - four(kStat, decltype(q)::value); });
+      // all at once, or, where the registers are full, as they are needed
+      constexpr bool LATE = !PLAIN && DP == 64;
+      f32x4 shift[LATE ? 1 : 4];
+      if constexpr (!LATE) static_for<4>([&](auto q) { shift[decltype(q)::value] = (float)held - four(kStat, decltype(q)::value); });
       products<DP, 2, AHEAD>(at, {&k, &v}, s, [&](auto place) {
         constexpr int FIRST = 3 * DP / 16;
         spread<decltype(place)::value, 0, FIRST, decltype(coming)::kCount>([&](auto f) { coming.template one<decltype(f)::value>(); });
         spread<decltype(place)::value, FIRST + 2, FIRST - 4, 16>([&](auto x_c) {
           constexpr int x = decltype(x_c)::value, q = x / 4, e = x % 4;
+          if constexpr (LATE && e == 0) shift[0] = (float)held - four(kStat, q);
           float bias = 0.f;
           if (!PLAIN && c.slopes) bias = of[32 * kSlope + 8 * q + e] * fabsf(of[32 * kAhead + 8 * q + e] - (float)j);
-          p[x] = weight<PLAIN>(score, s[0][x], factor, bias, shift[q][e], cap[x]);
+          p[x] = weight<PLAIN>(score, s[0][x], factor, bias, shift[LATE ? 0 : q][e], cap[x]);
           if (!WHOLE) {
             const int lo = (int)bits_of(of[32 * kLo + 8 * q + e]), hi = (int)bits_of(of[32 * kHi + 8 * q + e]);
             p[x] = ((j >= lo) & (j < hi)) ? p[x] : 0.f;
           }
+          if constexpr (x % 2) most = fmaxf(fmaxf(most, p[x - 1]), p[x]);
         });
         // two values behind
         spread<decltype(place)::value, FIRST + 4, FIRST - 4, 8>([&](auto n_c) {
@@ -885,11 +888,36 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
     };
     if (seen.covers(j0, j0 + 32)) tile(std::true_type{});
     else tile(std::false_type{});
+    // A key's first share sets its unit.  Shares that pass what fp16 holds, or that are not held as the sum needs them, lower it so that they become less than 2^6, and
+    // of the wave's other keys that of those of more than 2^10, so that this is seldom.  A unit follows the largest p do that its key has had, whatever the rows give to
+    // others.
+    most = fmaxf(most, other_half(most));
+    asm("" : "+v"(unit_v));  // what follows from it is computed again, not kept all along
+    held = held_by(unit_v);
+    const float passes = unit_v - ed > kMostHeld && unit_v != kNoUnit ? 0.f : 65000.f;
+    int next_unit = unit_v == kNoUnit && most > 0.f ? held + ed : unit_v;
+    if (__any(most > passes)) {
+      const bool lowers = most > fminf(passes, 1024.f);
+      const int to = lowers ? min(unit_v - ed, held + 132 - (int)(bits_of(most) >> 23)) : held;
+      static_for<8>([&](auto n_c) {
+        constexpr int n = decltype(n_c)::value;
+        p[2 * n] = __builtin_ldexpf(p[2 * n], to - held);
+        p[2 * n + 1] = __builtin_ldexpf(p[2 * n + 1], to - held);
+        w.set<n>(p[2 * n], p[2 * n + 1]);
+      });
+      if (lowers) next_unit = to + ed;
+      multiply(dvs, __builtin_ldexpf(1.f, max(next_unit - unit_v, -200)));
+      keep<(DP > 64)>(dvs);
+      held = to;
+    }
+    unit_v = next_unit;
     // While dv is summed: ds, the unit that dk's sum takes for it, and ds as that product's operand.
     f32x4 delta[4];
     static_for<4>([&](auto q) { delta[decltype(q)::value] = four(kDelta, decltype(q)::value); });
     constexpr int PLACES = 3 * DP / 16, HALF = PLACES / 2;
     int new_unit = unit, shift = 0;
+    float largest = 0.f;
+    bool lowers = false;
     Weights wd;
     add_product<DP, AHEAD>(dvs, at + 3 * BLOCK, w, [&](auto place) {
       constexpr int at_place = decltype(place)::value;
@@ -897,9 +925,10 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
         constexpr int x = decltype(x_c)::value;
         ds[x] = p[x] * __builtin_fmaf(s[1][x], d_factor, -delta[x / 4][x % 4]);
         if (!PLAIN) ds[x] *= cap[x];
+        if constexpr (x % 2) largest = fmaxf(fmaxf(largest, fabsf(ds[x - 1])), fabsf(ds[x]));
       });
       if constexpr (at_place == HALF - 1) {
-        new_unit = gradient_unit(ds, held, eq, unit);
+        new_unit = gradient_unit(largest, held, eq, unit, lowers);
         shift = new_unit == kNoUnit ? 0 : new_unit - eq - held;  // nothing but zeros so far
       }
       spread<at_place, HALF, PLACES - HALF, 8>([&](auto n_c) {
@@ -907,7 +936,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
         wd.set<n>(__builtin_ldexpf(ds[2 * n], shift), __builtin_ldexpf(ds[2 * n + 1], shift));
       });
     });
-    if (new_unit < unit) {
+    if (lowers) {
       multiply(dks, __builtin_ldexpf(1.f, max(new_unit - unit, -200)));
       keep<(DP > 64)>(dks);
       unit = new_unit;
@@ -921,7 +950,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
       dks[e][x] = __builtin_ldexpf(dks[e][x], unit == kNoUnit ? 0 : -unit);
-      dvs[e][x] = __builtin_ldexpf(dvs[e][x], -13 - unit_v);
+      dvs[e][x] = __builtin_ldexpf(dvs[e][x], -unit_v);
     }
   const int64_t all = (int64_t)c.batch * c.tk * c.key_heads * c.dim, key = c.key_at(b, g, j);
   float *const to_k = pieces > 1 ? parts + (int64_t)piece * 2 * all : dk, *const to_v = pieces > 1 ? parts + ((int64_t)piece * 2 + 1) * all : dv;
