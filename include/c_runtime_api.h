@@ -489,8 +489,8 @@ int DLGpuHeadRotaryBackward(const DLHeadGradientPart *parts, int n_parts, const 
  * These are spans[i] = (first, last): first <= j < last, spans [batch, queries, 2] or [queries, 2]; without spans all.  With `causal` of
  * them those with j <= i + keys - queries.  A query that sees none has the output 0 and the statistic -inf.  What a query does not see counts for nothing, whatever
  * it holds.
- * (The second term has the rounding of its size, 1e-3 at 1e4, and counts from the end of the keys, also where spans
- * leave the end out.)
+ * (The second term counts from the end of the keys, also where spans leave the end out.  Shares have the rounding of distances from the nearest key that
+ * a query sees; a statistic has that of its size, and with it the backward pass, which reads it: 1e-3 at 1e4.)
  * statistics [batch, heads, queries] are what the backward pass reads; one of output and statistics may be NULL.
  * Results must not overlap what they are computed from.  A call that takes scratch is refused on a stream that is being captured
  * into a graph: TINYFLOW_SPLIT=0 in the environment keeps the products on the fp32 instruction, where only queries too few

@@ -39,6 +39,8 @@ struct Call {
   }
   __device__ inline int64_t key_at(int b, int g, int j) const { return (((int64_t)b * tk + j) * key_heads + g) * dim; }
   __device__ inline int64_t stat_at(int b, int g, int r) const { return ((int64_t)b * heads + g * group + r % group) * tq + r / group; }
+  // The key that query i stands at.
+  __device__ inline int own(int i) const { return i + tk - tq; }
   // The keys that query i sees: [lo, hi), lo >= hi for none.
   __device__ inline void seen(int b, int i, int &lo, int &hi) const {
     lo = 0;
@@ -53,7 +55,24 @@ struct Call {
         if (last < (float)tk) hi = last > 0.f ? (int)ceilf(last) : 0;
       }
     }
-    if (causal) hi = min(hi, i + tk - tq + 1);
+    if (causal) hi = min(hi, own(i) + 1);
+  }
+  // Distances are counted from the nearest key that a query sees, so that they are as small as what they tell apart: the kernels' s lacks slope times the distance
+  // of that key, from which all others are farther by as much.  It comes back with the statistic.  (With the distances themselves shares had the rounding of
+  // the farthest: 1e-3 over 131 072 keys of which 1 000 are used.)
+  __device__ inline int nearest(int i, int lo, int hi) const { return lo < hi ? min(max(own(i), lo), hi - 1) : own(i); }
+  // log2 of a row's sum to its statistic, and back to what the backward kernels take from a score
+  __device__ inline float statistic(int b, int g, int r, float log2_sum) const {
+    const float x = log2_sum * kLn2;
+    if (!slopes) return x;
+    int lo, hi;
+    seen(b, r / group, lo, hi);
+    return fmaf(-slopes[g * group + r % group], (float)abs(own(r / group) - nearest(r / group, lo, hi)), x);
+  }
+  __device__ inline float taken(int g, int r, int lo, int hi, float statistic) const {
+    if (!slopes) return statistic * kLog2e;
+    const int away = abs(own(r / group) - nearest(r / group, lo, hi));
+    return (float)(((double)statistic + (double)slopes[g * group + r % group] * (double)away) * 1.4426950408889634);
   }
 };
 
@@ -177,12 +196,12 @@ __device__ inline float row_end(const Call &c, const Pieces &to, float *out, flo
     row = to.sums + at * c.dim;
     return 1.f;
   }
-  if (stat && writes_mark) stat[c.stat_at(b, g, r)] = total == 0.f ? kNone : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  if (stat && writes_mark) stat[c.stat_at(b, g, r)] = total == 0.f ? kNone : c.statistic(b, g, r, top + __builtin_amdgcn_logf(total));
   row = out ? out + c.query_at(b, g, r) : nullptr;
   return total == 0.f ? 0.f : 1.f / total;
 }
 
-// What the backward kernels read of a row: its statistic times log2 e, delta, and the keys that it sees.
+// What the backward kernels read of a row: its statistic in their terms (Call::taken), delta, and the keys that it sees.
 struct Row {
   float stat, delta;
   int lo, hi;

@@ -171,9 +171,10 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
   const int lane = threadIdx.x % 64, half = lane / 32;
   const int r = tile * kRows + threadIdx.x / 64 * 32 + lane % 32;
   const bool live = r < c.rows;
-  const int i = (live ? r : c.rows - 1) / c.group, ahead = i + c.tk - c.tq;
+  const int i = (live ? r : c.rows - 1) / c.group;
   int lo, hi;
   c.seen(b, i, lo, hi);
+  const int near = c.nearest(i, lo, hi);
   const float slope = c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
   Hull mine;
   mine.of(lo, hi, live);
@@ -204,7 +205,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
 #pragma unroll
     for (int v = 0; v < 16; ++v) {
       const int j = j0 + key_of(v, half);
-      p[v] = score(s[v]) - slope * fabsf((float)(ahead - j));
+      p[v] = score(s[v]) - slope * fabsf((float)(near - j));
       if (!mine.covers(j0, j0 + kKeys)) p[v] = j >= lo && j < hi ? p[v] : kNone;
       most = fmaxf(most, p[v]);
     }
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(kThreads, DP * NC <= 128 ? 2 : 1) void few_kernel(c
   const int bg = (int)blockIdx.x % (c.batch * c.key_heads), piece = (int)blockIdx.x / (c.batch * c.key_heads);
   const int b = bg / c.key_heads, g = bg % c.key_heads;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, quarter = lane / 16, col = lane % 16;
-  int lo[NC], hi[NC], ahead[NC], all_lo = INT32_MAX, all_hi = 0, inner_lo = 0, inner_hi = INT32_MAX;
+  int lo[NC], hi[NC], near[NC], all_lo = INT32_MAX, all_hi = 0, inner_lo = 0, inner_hi = INT32_MAX;
   float slope[NC];
   f32x4 q[NC][GD];
 #pragma unroll
@@ -265,8 +266,8 @@ __global__ __launch_bounds__(kThreads, DP * NC <= 128 ? 2 : 1) void few_kernel(c
     const bool live = r < c.rows;
     const int i = (live ? r : 0) / c.group;
     c.seen(b, i, lo[n], hi[n]);
+    near[n] = c.nearest(i, lo[n], hi[n]);
     if (!live) hi[n] = 0;
-    ahead[n] = i + c.tk - c.tq;
     slope[n] = c.slopes && live ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
     const float *row = c.q + c.query_at(b, g, live ? r : 0);
 #pragma unroll
@@ -363,7 +364,7 @@ __global__ __launch_bounds__(kThreads, DP * NC <= 128 ? 2 : 1) void few_kernel(c
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const int j = j0 + 4 * quarter + v;
-        p[n][v] = score(s[v]) - slope[n] * fabsf((float)(ahead[n] - j));
+        p[n][v] = score(s[v]) - slope[n] * fabsf((float)(near[n] - j));
         if (!whole) p[n][v] = j >= lo[n] && j < hi[n] && j < end ? p[n][v] : kNone;
         most = fmaxf(most, p[n][v]);
       }
@@ -559,7 +560,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void join_kernel(const Call c
       for (int w = 1; w < W; ++w) sum[e] += parts[w][e][lane];
   }
   const int r = (int)(row % c.rows), g = (int)(row / c.rows % c.key_heads), b = (int)(row / c.rows / c.key_heads);
-  if (stat && lane == 0) stat[c.stat_at(b, g, r)] = total == 0.f ? kNone : (top + __builtin_amdgcn_logf(total)) * kLn2;
+  if (stat && lane == 0) stat[c.stat_at(b, g, r)] = total == 0.f ? kNone : c.statistic(b, g, r, top + __builtin_amdgcn_logf(total));
   if (!out) return;
   const float scale = total == 0.f ? 0.f : 1.f / total;
   float *to = out + c.query_at(b, g, r);
@@ -584,7 +585,7 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(const Call c, const f
   if (lane > 0) return;
   Row row;
   c.seen(b, r / c.group, row.lo, row.hi);
-  row.stat = stat[c.stat_at(b, g, r)] * kLog2e;
+  row.stat = c.taken(g, r, row.lo, row.hi, stat[c.stat_at(b, g, r)]);
   row.delta = delta;
   if (row.lo >= row.hi || row.stat == kNone) row.lo = row.hi = 0;
   rows[at] = row;
@@ -603,7 +604,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
   const int r = tile * kRows + threadIdx.x / 64 * 32 + lane % 32;
   const bool live = r < c.rows;
   const Row row = rows[(int64_t)bg * c.rows + (live ? r : 0)];
-  const int ahead = (live ? r : 0) / c.group + c.tk - c.tq;
+  const int near = c.nearest((live ? r : 0) / c.group, row.lo, row.hi);
   const float slope = c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
   const int64_t at = c.query_at(b, g, live ? r : 0);
   Hull mine;
@@ -637,7 +638,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
     for (int v = 0; v < 16; ++v) {
       const int j = j0 + key_of(v, half);
       float p;
-      gradient(score, s[v], dp[v], slope * fabsf((float)(ahead - j)), row.stat, row.delta, j >= row.lo && j < row.hi, p, ds[v]);
+      gradient(score, s[v], dp[v], slope * fabsf((float)(near - j)), row.stat, row.delta, j >= row.lo && j < row.hi, p, ds[v]);
     }
     sum.add(kt, ds);
     if (clean && found) sum.add_back(found, [&](int n) { return c.k + c.key_at(b, g, j0 + n); }, c.dim, ds);
@@ -653,6 +654,7 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float
   __shared__ __align__(16) Tile<DP> qt, dt;
   __shared__ Row info[32];
   __shared__ float slopes[32];
+  __shared__ int nears[32];
   __shared__ int meet[3];  // least and greatest key that a row of the step sees, whether any sees less than all of the tile
   __shared__ uint32_t found_q, found_d;
   const int bg = (int)blockIdx.x % (c.batch * c.key_heads), rest = (int)blockIdx.x / (c.batch * c.key_heads);
@@ -684,6 +686,7 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float
       if (is) row = of[r];
       if (threadIdx.x < 32) {
         info[threadIdx.x] = row;
+        nears[threadIdx.x] = c.nearest(r / c.group, row.lo, row.hi);
         slopes[threadIdx.x] = c.slopes && is ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
       }
       const bool sees = is && row.lo < tile_hi && row.hi > tile_lo;
@@ -711,7 +714,7 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float
     for (int e = 0; e < 16; ++e) {
       const int n = key_of(e, half);
       const Row row = info[n];
-      const float bias = slopes[n] * fabsf((float)((r0 + n) / c.group + c.tk - c.tq - j));
+      const float bias = slopes[n] * fabsf((float)(nears[n] - j));
       gradient(score, s[e], dp[e], bias, row.stat, row.delta, live && j >= row.lo && j < row.hi, p[e], ds[e]);
     }
     if (DV) {

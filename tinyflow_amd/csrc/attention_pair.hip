@@ -63,7 +63,7 @@ __host__ __device__ constexpr int64_t block_size(int dp) { return dp * 128; }
 // By value: a bit cast of an element of a vector takes the vector's first one, whichever it is.
 __device__ inline uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
 
-enum Info { kStat = 0, kDelta, kLo, kHi, kSlope, kAhead };
+enum Info { kStat = 0, kDelta, kLo, kHi, kSlope, kNear };
 
 struct Job {
   const float *src;
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
     }
     delta = lanes::sum_over<8>(delta);
     if (tid % 8 == 0) {
-      if (used) info.stat = p.stat[c.stat_at(b, g, n)] * kLog2e;
+      if (used) info.stat = c.taken(g, n, info.lo, info.hi, p.stat[c.stat_at(b, g, n)]);
       if (!used || info.stat == kNone) info = Row{0.f, 0.f, 0, 0};
       else info.delta = delta;
       if (n < c.rows) p.rows[(int64_t)head * c.rows + n] = info;
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
         to[32 * kLo] = __builtin_bit_cast(float, mine.lo);
         to[32 * kHi] = __builtin_bit_cast(float, mine.hi);
         to[32 * kSlope] = c.slopes && r < c.rows ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
-        to[32 * kAhead] = (float)(r / c.group + c.tk - c.tq);
+        to[32 * kNear] = (float)c.nearest(r / c.group, mine.lo, mine.hi);
       }
       if (tid == 0) p.hulls[of_block] = seen;
     }
@@ -498,9 +498,10 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
   const int group = __builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
   const int r = tile * kRows + wave * 32 + lane % 32;
   const bool live = r < c.rows;
-  const int i = (live ? r : c.rows - 1) / c.group, ahead = i + c.tk - c.tq;
+  const int i = (live ? r : c.rows - 1) / c.group;
   int lo, hi;
   c.seen(b, i, lo, hi);
+  const int near = c.nearest(i, lo, hi);
   Hull mine;
   mine.of(lo, hi, live);
   const Hull all = mine.all(room);  // the second group's waves have the first's rows
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
       if (!PLAIN) {
         p[v] *= factor;
         if (score.capped) p[v] = score.top * tanh_of(p[v]);
-        p[v] -= slope * fabsf((float)(ahead - (j0 + key_of(v, half))));
+        p[v] -= slope * fabsf((float)(near - (j0 + key_of(v, half))));
       }
     }
     if (!whole)
@@ -667,7 +668,7 @@ __global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_k
   const int r = tile * kRows + wave * 32 + lane % 32;
   const bool live = r < c.rows;
   const Row row = rows[(int64_t)bg * c.rows + (live ? r : 0)];
-  const int ahead = (live ? r : 0) / c.group + c.tk - c.tq;
+  const int near = c.nearest((live ? r : 0) / c.group, row.lo, row.hi);
   Hull mine;
   mine.of(row.lo, row.hi, live);
   const Hull all = mine.all(room);
@@ -719,7 +720,7 @@ __global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_k
         spread<decltype(place)::value, FIRST + 2, FIRST - 2, 16>([&](auto v_c) {
           constexpr int v = decltype(v_c)::value;
           const int j = j0 + key_of(v, half);
-          p[v] = weight<PLAIN>(score, s[0][v], factor, PLAIN ? 0.f : slope * fabsf((float)(ahead - j)), -stat, cap[v]);
+          p[v] = weight<PLAIN>(score, s[0][v], factor, PLAIN ? 0.f : slope * fabsf((float)(near - j)), -stat, cap[v]);
           if (!WHOLE) p[v] = ((j >= row.lo) & (j < row.hi)) ? p[v] : 0.f;
         });
       });
@@ -871,7 +872,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
           constexpr int x = decltype(x_c)::value, q = x / 4, e = x % 4;
           if constexpr (LATE && e == 0) shift[0] = (float)held - four(kStat, q);
           float bias = 0.f;
-          if (!PLAIN && c.slopes) bias = of[32 * kSlope + 8 * q + e] * fabsf(of[32 * kAhead + 8 * q + e] - (float)j);
+          if (!PLAIN && c.slopes) bias = of[32 * kSlope + 8 * q + e] * fabsf(of[32 * kNear + 8 * q + e] - (float)j);
           p[x] = weight<PLAIN>(score, s[0][x], factor, bias, shift[LATE ? 0 : q][e], cap[x]);
           if (!WHOLE) {
             const int lo = (int)bits_of(of[32 * kLo + 8 * q + e]), hi = (int)bits_of(of[32 * kHi + 8 * q + e]);
