@@ -484,13 +484,14 @@ int DLGpuHeadRotaryBackward(const DLHeadGradientPart *parts, int n_parts, const 
 
 /* Attention of `heads` query heads over `key_heads` key and value heads, a divisor: query head h reads key head h / (heads / key_heads).
  * query [batch * queries, heads * D] and key, value [batch * keys, key_heads * D] as head arrays, D up to 256, up to 2^24 queries and keys:
- *   s_ij = cap tanh(scale q_i k_j / cap) - slopes[h] |i + keys - queries - j|, with cap 0 s = scale q k, without slopes no second term
+ *   s_ij = cap tanh(scale q_i k_j / cap) - slopes[h] |a_i - j|, with cap 0 s = scale q k, without slopes no second term
  *   output_i = sum_j exp(s_ij - statistics_i) v_j, statistics_i = log sum_j exp(s_ij), over the keys j that query i sees.
  * These are spans[i] = (first, last): first <= j < last, spans [batch, queries, 2] or [queries, 2]; without spans all.  With `causal` of
- * them those with j <= i + keys - queries.  A query that sees none has the output 0 and the statistic -inf.  What a query does not see counts for nothing, whatever
+ * them those with j <= a_i.  A query stands at key a_i = i + keys - queries, or with spans of three at the third, a whole number of up to 2^24 (over a cache whose
+ * end is not used, say, which the first counts from).  A query that sees none has the output 0 and the statistic -inf.  What a query does not see counts for nothing, whatever
  * it holds.
- * (The second term counts from the end of the keys, also where spans leave the end out.  Shares have the rounding of distances from the nearest key that
- * a query sees; a statistic has that of its size, and with it the backward pass, which reads it: 1e-3 at 1e4.)
+ * (Shares have the rounding of distances from the nearest key that a query sees.  A statistic has that of its size, and with it the backward pass, which
+ * reads it: 1e-3 at 1e4, where a query stands far from all that it sees.)
  * statistics [batch, heads, queries] are what the backward pass reads; one of output and statistics may be NULL.
  * Results must not overlap what they are computed from.  A call that takes scratch is refused on a stream that is being captured
  * into a graph: TINYFLOW_SPLIT=0 in the environment keeps the products on the fp32 instruction, where only queries too few

@@ -231,3 +231,18 @@ def test_attention_backward_refuses():
 def test_the_structures_are_those_of_the_header():
     assert ctypes.sizeof(gpu_op.HeadPart) == 40 and gpu_op.HeadPart.heads.offset == 24
     assert ctypes.sizeof(gpu_op.HeadGradientPart) == 48 and gpu_op.HeadGradientPart.heads.offset == 40
+
+
+def test_spans_with_positions():
+    np.testing.assert_array_equal(gpu_op.attention_spans(2, 9, causal=True, used=[4, 9], positions=True),
+                                  [[[0, 3, 2], [0, 4, 3]], [[0, 8, 7], [0, 9, 8]]])
+    np.testing.assert_array_equal(gpu_op.attention_spans(2, 3, positions=True), [[0, 3, 1], [0, 3, 2]])
+    spans = gpu_op.attention_spans(3, documents=[[5, 5, 5], [1, 2, 2]], positions=True)
+    np.testing.assert_array_equal(spans, [[[0, 3, 0], [0, 3, 1], [0, 3, 2]], [[0, 1, 0], [1, 3, 1], [1, 3, 2]]])
+    assert spans.dtype == np.float32
+
+
+def test_attention_refuses_spans_of_other_widths():
+    q, k, v, o, s = _Fake((6, 32)), _Fake((8, 16)), _Fake((8, 16)), _Fake((6, 32)), _Fake((2, 4, 3))
+    for shape in ((3, 4), (3, 1), (6,), (9,), (2, 2, 3), (3, 3, 3), (2, 3, 4)):
+        _refused(gpu_op.attention_forward, q, k, v, _Fake(shape), None, o, s, 2, 4, 2, 0.5, 0.0, False)

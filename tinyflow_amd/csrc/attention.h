@@ -1,6 +1,6 @@
 // What the attention kernels share: the view of a call's arrays, which keys a query sees, and how a score comes out of a product.
 //
-//   s_ij = cap tanh(scale q_i k_j / cap) - slope |i + Tk - Tq - j|, seen keys only;   without a cap s = scale q k
+//   s_ij = cap tanh(scale q_i k_j / cap) - slope |a_i - j|, seen keys only, a_i = i + Tk - Tq or as given;   without a cap s = scale q k
 //   o_i = sum_j p_ij v_j, p_ij = exp(s_ij - stat_i), stat_i = log sum_j exp(s_ij);    nothing seen: o = 0, stat = -inf
 //   backward: ds_ij = p_ij (do_i v_j - delta_i) cap'_ij scale, delta_i = do_i o_i
 //             dq_i = sum_j ds_ij k_j, dk_j = sum_i ds_ij q_i, dv_j = sum_i p_ij do_i
@@ -26,9 +26,10 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 
 struct Call {
   const float *q, *k, *v;
-  const float *spans;      // [queries, 2], of each batch entry where span_stride is not 0
+  const float *spans;      // [queries, span_width], of each batch entry where span_stride is not 0
   const float *slopes;     // of each query head
   int64_t span_stride;
+  int span_width;          // 3: with the key that a query stands at
   int batch, tq, tk, heads, key_heads, group, dim;
   int rows;                // tq * group: of a key head
   float scale, cap;        // cap 0: none
@@ -39,15 +40,22 @@ struct Call {
   }
   __device__ inline int64_t key_at(int b, int g, int j) const { return (((int64_t)b * tk + j) * key_heads + g) * dim; }
   __device__ inline int64_t stat_at(int b, int g, int r) const { return ((int64_t)b * heads + g * group + r % group) * tq + r / group; }
-  // The key that query i stands at.
-  __device__ inline int own(int i) const { return i + tk - tq; }
-  // The keys that query i sees: [lo, hi), lo >= hi for none.
-  __device__ inline void seen(int b, int i, int &lo, int &hi) const {
+  // The key that query i stands at: the keys' last ones are the queries' own, or what its span says.  (A NaN counts as far in front.)
+  __device__ inline int own(int i, const float *span) const {
+    const float given = span[span_width - 1];  // read in any case: behind a branch it would wait for all other loads
+    return span_width < 3 ? i + tk - tq : (int)fminf(fmaxf(given, -0x1p24f), 0x1p24f);
+  }
+  __device__ inline const float *span_of(int b, int i) const { return spans + b * span_stride + span_width * (int64_t)i; }
+  __device__ inline int own(int b, int i) const { return spans ? own(i, span_of(b, i)) : i + tk - tq; }
+  // The keys that query i sees: [lo, hi), lo >= hi for none; and where it stands.
+  __device__ inline void seen(int b, int i, int &lo, int &hi, int &at) const {
     lo = 0;
     hi = tk;
+    at = i + tk - tq;
     if (spans) {
-      const float *span = spans + b * span_stride + 2 * (int64_t)i;
+      const float *span = span_of(b, i);
       const float first = span[0], last = span[1];
+      at = own(i, span);
       // key j is seen where first <= j < last; a NaN sees none
       if (!(first < last)) hi = 0;
       else {
@@ -55,23 +63,27 @@ struct Call {
         if (last < (float)tk) hi = last > 0.f ? (int)ceilf(last) : 0;
       }
     }
-    if (causal) hi = min(hi, own(i) + 1);
+    if (causal) hi = min(hi, at + 1);
+  }
+  __device__ inline void seen(int b, int i, int &lo, int &hi) const {
+    int at;
+    seen(b, i, lo, hi, at);
   }
   // Distances are counted from the nearest key that a query sees, so that they are as small as what they tell apart: the kernels' s lacks slope times the distance
   // of that key, from which all others are farther by as much.  It comes back with the statistic.  (With the distances themselves shares had the rounding of
   // the farthest: 1e-3 over 131 072 keys of which 1 000 are used.)
-  __device__ inline int nearest(int i, int lo, int hi) const { return lo < hi ? min(max(own(i), lo), hi - 1) : own(i); }
+  __device__ static inline int nearest(int at, int lo, int hi) { return lo < hi ? min(max(at, lo), hi - 1) : at; }
   // log2 of a row's sum to its statistic, and back to what the backward kernels take from a score
   __device__ inline float statistic(int b, int g, int r, float log2_sum) const {
     const float x = log2_sum * kLn2;
     if (!slopes) return x;
-    int lo, hi;
-    seen(b, r / group, lo, hi);
-    return fmaf(-slopes[g * group + r % group], (float)abs(own(r / group) - nearest(r / group, lo, hi)), x);
+    int lo, hi, at;
+    seen(b, r / group, lo, hi, at);
+    return fmaf(-slopes[g * group + r % group], (float)abs(at - nearest(at, lo, hi)), x);
   }
-  __device__ inline float taken(int g, int r, int lo, int hi, float statistic) const {
+  __device__ inline float taken(int b, int g, int r, int lo, int hi, float statistic) const {
     if (!slopes) return statistic * kLog2e;
-    const int away = abs(own(r / group) - nearest(r / group, lo, hi));
+    const int at = own(b, r / group), away = abs(at - nearest(at, lo, hi));
     return (float)(((double)statistic + (double)slopes[g * group + r % group] * (double)away) * 1.4426950408889634);
   }
 };

@@ -172,9 +172,9 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
   const int r = tile * kRows + threadIdx.x / 64 * 32 + lane % 32;
   const bool live = r < c.rows;
   const int i = (live ? r : c.rows - 1) / c.group;
-  int lo, hi;
-  c.seen(b, i, lo, hi);
-  const int near = c.nearest(i, lo, hi);
+  int lo, hi, at;
+  c.seen(b, i, lo, hi, at);
+  const int near = c.nearest(at, lo, hi);
   const float slope = c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
   Hull mine;
   mine.of(lo, hi, live);
@@ -265,8 +265,9 @@ __global__ __launch_bounds__(kThreads, DP * NC <= 128 ? 2 : 1) void few_kernel(c
     const int r = 16 * n + col;
     const bool live = r < c.rows;
     const int i = (live ? r : 0) / c.group;
-    c.seen(b, i, lo[n], hi[n]);
-    near[n] = c.nearest(i, lo[n], hi[n]);
+    int at;
+    c.seen(b, i, lo[n], hi[n], at);
+    near[n] = c.nearest(at, lo[n], hi[n]);
     if (!live) hi[n] = 0;
     slope[n] = c.slopes && live ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
     const float *row = c.q + c.query_at(b, g, live ? r : 0);
@@ -585,7 +586,7 @@ __global__ __launch_bounds__(kThreads) void prepare_kernel(const Call c, const f
   if (lane > 0) return;
   Row row;
   c.seen(b, r / c.group, row.lo, row.hi);
-  row.stat = c.taken(g, r, row.lo, row.hi, stat[c.stat_at(b, g, r)]);
+  row.stat = c.taken(b, g, r, row.lo, row.hi, stat[c.stat_at(b, g, r)]);
   row.delta = delta;
   if (row.lo >= row.hi || row.stat == kNone) row.lo = row.hi = 0;
   rows[at] = row;
@@ -604,7 +605,7 @@ __global__ __launch_bounds__(kThreads) void dq_kernel(const Call c, const float 
   const int r = tile * kRows + threadIdx.x / 64 * 32 + lane % 32;
   const bool live = r < c.rows;
   const Row row = rows[(int64_t)bg * c.rows + (live ? r : 0)];
-  const int near = c.nearest((live ? r : 0) / c.group, row.lo, row.hi);
+  const int near = c.nearest(c.own(b, (live ? r : 0) / c.group), row.lo, row.hi);
   const float slope = c.slopes ? c.slopes[g * c.group + (live ? r : 0) % c.group] * kLog2e : 0.f;
   const int64_t at = c.query_at(b, g, live ? r : 0);
   Hull mine;
@@ -686,7 +687,7 @@ __global__ __launch_bounds__(kThreads) void dkv_kernel(const Call c, const float
       if (is) row = of[r];
       if (threadIdx.x < 32) {
         info[threadIdx.x] = row;
-        nears[threadIdx.x] = c.nearest(r / c.group, row.lo, row.hi);
+        nears[threadIdx.x] = is ? c.nearest(c.own(b, r / c.group), row.lo, row.hi) : 0;
         slopes[threadIdx.x] = c.slopes && is ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
       }
       const bool sees = is && row.lo < tile_hi && row.hi > tile_lo;
@@ -796,11 +797,12 @@ int describe(const char *what, Call &c, const DLArray *query, const DLArray *key
   if (!(scale > 0.f) || !finite(scale)) return refuse("scale must be positive");
   if (!(cap >= 0.f) || !finite(cap)) return refuse("cap must be positive, or 0 for none");
   if (spans) {
-    if (!on_gpu(spans) || spans->ndim < 2 || spans->shape[spans->ndim - 1] != 2) return refuse("spans must be [batch, queries, 2] or [queries, 2] and live on the GPU");
-    const int64_t n = numel(spans);
-    if (n != 2 * tq && n != 2 * tq * batch) return refuse("spans must hold a pair for each query");
+    const int64_t n = numel(spans), width = spans->ndim < 2 ? 0 : spans->shape[spans->ndim - 1];
+    if (!on_gpu(spans) || (width != 2 && width != 3)) return refuse("spans must be [batch, queries, 2 or 3] or [queries, 2 or 3] and live on the GPU");
+    if (n != width * tq && n != width * tq * batch) return refuse("spans must hold two or three numbers for each query");
     c.spans = (const float *)spans->data;
-    c.span_stride = n == 2 * tq * batch ? 2 * tq : 0;
+    c.span_width = (int)width;
+    c.span_stride = n == width * tq * batch ? width * tq : 0;
   }
   if (slopes) {
     if (!on_gpu(slopes) || numel(slopes) != heads) return refuse("slopes must hold a value for each head and live on the GPU");

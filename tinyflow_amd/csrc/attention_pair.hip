@@ -178,7 +178,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
     }
     delta = lanes::sum_over<8>(delta);
     if (tid % 8 == 0) {
-      if (used) info.stat = c.taken(g, n, info.lo, info.hi, p.stat[c.stat_at(b, g, n)]);
+      if (used) info.stat = c.taken(b, g, n, info.lo, info.hi, p.stat[c.stat_at(b, g, n)]);
       if (!used || info.stat == kNone) info = Row{0.f, 0.f, 0, 0};
       else info.delta = delta;
       if (n < c.rows) p.rows[(int64_t)head * c.rows + n] = info;
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
         to[32 * kLo] = __builtin_bit_cast(float, mine.lo);
         to[32 * kHi] = __builtin_bit_cast(float, mine.hi);
         to[32 * kSlope] = c.slopes && r < c.rows ? c.slopes[g * c.group + r % c.group] * kLog2e : 0.f;
-        to[32 * kNear] = (float)c.nearest(r / c.group, mine.lo, mine.hi);
+        to[32 * kNear] = r < c.rows ? (float)c.nearest(c.own(b, r / c.group), mine.lo, mine.hi) : 0.f;
       }
       if (tid == 0) p.hulls[of_block] = seen;
     }
@@ -499,9 +499,9 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
   const int r = tile * kRows + wave * 32 + lane % 32;
   const bool live = r < c.rows;
   const int i = (live ? r : c.rows - 1) / c.group;
-  int lo, hi;
-  c.seen(b, i, lo, hi);
-  const int near = c.nearest(i, lo, hi);
+  int lo, hi, at;
+  c.seen(b, i, lo, hi, at);
+  const int near = c.nearest(at, lo, hi);
   Hull mine;
   mine.of(lo, hi, live);
   const Hull all = mine.all(room);  // the second group's waves have the first's rows
@@ -668,7 +668,7 @@ __global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_k
   const int r = tile * kRows + wave * 32 + lane % 32;
   const bool live = r < c.rows;
   const Row row = rows[(int64_t)bg * c.rows + (live ? r : 0)];
-  const int near = c.nearest((live ? r : 0) / c.group, row.lo, row.hi);
+  const int near = c.nearest(c.own(b, (live ? r : 0) / c.group), row.lo, row.hi);
   Hull mine;
   mine.of(row.lo, row.hi, live);
   const Hull all = mine.all(room);

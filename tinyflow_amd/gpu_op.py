@@ -564,12 +564,14 @@ def rotary_frequencies(columns, base=10000.0, factor=1.0, context=None, slow=1.0
     return (f * (kept + (1.0 - kept) / factor)).astype(np.float32)
 
 
-def attention_spans(queries, keys=None, causal=False, documents=None, prefix=None, window=None, used=None):
+def attention_spans(queries, keys=None, causal=False, documents=None, prefix=None, window=None, used=None, positions=False):
     """The first key that each query sees and the one behind the last, [queries, 2] or [batch, queries, 2], for
     ``attention_forward`` (a numpy array).  Query i stands at key i + keys - queries, or with ``used`` [batch], the keys of a
     cache that are filled, at i + used - queries.  ``causal``: none behind the query.  ``documents`` [batch, keys]: numbers that are
     the same all over a document and nowhere else next to it; only keys of the query's own.  ``prefix`` [batch]: that many first
-    keys (of its document) are seen by every query, whatever ``causal`` says.  ``window``: so many keys up to the query's own."""
+    keys (of its document) are seen by every query, whatever ``causal`` says.  ``window``: so many keys up to the query's own.
+    ``positions``: with the key that each query stands at as a third number, which the slopes' distances are counted from: with ``used``
+    they are otherwise counted from the end of the cache."""
     keys = queries if keys is None else keys
     end = np.asarray(keys if used is None else used, np.int64).reshape(-1, 1)
     at = np.arange(queries)[None, :] + end - queries
@@ -596,7 +598,8 @@ def attention_spans(queries, keys=None, causal=False, documents=None, prefix=Non
     if window is not None:
         first = np.maximum(first, at + 1 - window)
     first, last = np.broadcast_arrays(first, last)
-    spans = np.stack([first, np.maximum(first, last)], 2).astype(np.float32)
+    spans = [first, np.maximum(first, last)] + ([np.broadcast_to(at, first.shape)] if positions else [])
+    spans = np.stack(spans, 2).astype(np.float32)
     return spans[0] if len(spans) == 1 else spans
 
 
