@@ -246,3 +246,19 @@ def test_attention_refuses_spans_of_other_widths():
     q, k, v, o, s = _Fake((6, 32)), _Fake((8, 16)), _Fake((8, 16)), _Fake((6, 32)), _Fake((2, 4, 3))
     for shape in ((3, 4), (3, 1), (6,), (9,), (2, 2, 3), (3, 3, 3), (2, 3, 4)):
         _refused(gpu_op.attention_forward, q, k, v, _Fake(shape), None, o, s, 2, 4, 2, 0.5, 0.0, False)
+
+
+def test_attention_refuses_numbers_at_the_ends_of_the_range():
+    """A cap that is meant as none, one that leaves nothing, and scales whose product or quotient is no number with digits."""
+    q, k, v, o, s = _Fake((6, 32)), _Fake((8, 16)), _Fake((8, 16)), _Fake((6, 32)), _Fake((2, 4, 3))
+    grads = _Fake((6, 32)), _Fake((6, 32)), _Fake((8, 16)), _Fake((8, 16))
+    largest = float(np.finfo(np.float32).max)
+    for scale, cap in ((0.5, largest), (0.5, 1e-39), (1e-20, 1e20), (1e20, 1e-20), (largest, 0.0)):
+        _refused(gpu_op.attention_forward, q, k, v, None, None, o, s, 2, 4, 2, scale, cap, False)
+        _refused(gpu_op.attention_backward, q, k, v, None, None, o, s, *grads, 2, 4, 2, scale, cap, False)
+
+
+def test_frequencies_refuse_parts_without_extent():
+    for slow, fast in ((1.0, 1.0), (32.0, 1.0), (float("nan"), 32.0)):
+        with pytest.raises(ValueError):
+            gpu_op.rotary_frequencies(8, factor=4, context=2048, slow=slow, fast=fast)

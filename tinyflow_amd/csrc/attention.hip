@@ -796,6 +796,9 @@ int describe(const char *what, Call &c, const DLArray *query, const DLArray *key
   if (tq * (heads / key_heads) > INT32_MAX / 2) return refuse("too many queries of a key head");
   if (!(scale > 0.f) || !finite(scale)) return refuse("scale must be positive");
   if (!(cap >= 0.f) || !finite(cap)) return refuse("cap must be positive, or 0 for none");
+  // what the kernels make of them (Score): an infinity would turn scores of 0 into NaNs, a number without its digits all of them into others
+  if (!finite(cap * kLog2e) || !finite(scale * kLog2e) || (cap > 0.f && !(scale / cap >= 0x1p-126f && finite(scale / cap))))
+    return refuse("scale, cap and their quotient must be well inside the range of fp32");
   if (spans) {
     const int64_t n = numel(spans), width = spans->ndim < 2 ? 0 : spans->shape[spans->ndim - 1];
     if (!on_gpu(spans) || (width != 2 && width != 3)) return refuse("spans must be [batch, queries, 2 or 3] or [queries, 2 or 3] and live on the GPU");
