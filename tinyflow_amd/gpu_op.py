@@ -557,6 +557,8 @@ def rotary_frequencies(columns, base=10000.0, factor=1.0, context=None, slow=1.0
     over it, none that turns ``fast`` times or more, and those between by parts."""
     if columns < 2 or columns % 2:
         raise ValueError("rotary_frequencies: %r columns" % (columns,))
+    if context is not None and not fast > slow:
+        raise ValueError("rotary_frequencies: slow %r and fast %r" % (slow, fast))
     f = base ** (-2.0 * np.arange(columns // 2) / columns)
     kept = 0.0
     if context is not None:
