@@ -233,3 +233,19 @@ def test_large_values_of_which_little_is_taken(rt, monkeypatch, split, power, fi
         assert _off(got, value) <= 2.0 ** -12.4, what
         if what in ("dk", "dv"):
             assert _off(got[:, block], value[:, block]) <= 2.0 ** -12.4, what
+
+
+def test_a_scale_that_only_a_cap_bears(rt):
+    """Scores past every digit under a cap: each is the cap, or its opposite."""
+    from tinyflow_amd import gpu_op, ndarray
+    rng = np.random.RandomState(42)
+    q, k = (np.sign(rng.normal(0, 1, (1, 256, 1, 64))).astype(np.float32) for _ in range(2))
+    q[..., 0] *= 1.5   # no product is 0
+    v = rng.normal(0, 1, (1, 256, 1, 64)).astype(np.float32)
+    a = [ndarray.array(x, ctx=rt.ctx) for x in (q, k, v)]
+    out = ndarray.array(np.full(q.shape, 7.25, np.float32), ctx=rt.ctx)
+    assert gpu_op.attention_forward(*a, None, None, out, None, 1, 1, 1, 1e37, 1e30, False, rt.stream) == 0
+    # exp2 of a difference of 2e30 is 0, of none 1
+    above = (q[0, :, 0].astype(np.float64) @ k[0, :, 0].T.astype(np.float64)) > 0
+    want = above @ v[0, :, 0].astype(np.float64) / above.sum(1, keepdims=True)
+    assert np.abs(out.asnumpy()[0, :, 0] - want).max() <= 300 * 2.0 ** -24 * 4   # sums of up to 256 values of up to 4

@@ -1028,7 +1028,7 @@ void pack(const Call &c, Pack &p, int2 *seen, hipStream_t s) {
 // Exponents::least_sum: elements of a block are less than 2^15 times 2^-exponent
 int least_sum(const Call &c) {
   int exponent;
-  (void)frexpf(c.scale * (float)c.dim, &exponent);   // 2^exponent is more
+  (void)frexp((double)c.scale * c.dim, &exponent);   // 2^exponent is more
   return exponent + 30 - 18;
 }
 
