@@ -249,3 +249,24 @@ def test_a_scale_that_only_a_cap_bears(rt):
     above = (q[0, :, 0].astype(np.float64) @ k[0, :, 0].T.astype(np.float64)) > 0
     want = above @ v[0, :, 0].astype(np.float64) / above.sum(1, keepdims=True)
     assert np.abs(out.asnumpy()[0, :, 0] - want).max() <= 300 * 2.0 ** -24 * 4   # sums of up to 256 values of up to 4
+
+
+@pytest.mark.parametrize("distance", [False, True])
+def test_errors_are_those_of_fp32(rt, monkeypatch, distance):
+    """Gradients of documents, whose shares grow by powers of ten on the way through the rows.  A pair's elements are off by 2^-24.8 in the mean, two of them and
+    the product left out by 2^-23.5, an fp32 product and its sum by as much; the rest both engines have: the errors' ratio is at most that of one
+    such error and of two, the square root of two, and is given a tenth for chance."""
+    from tinyflow_amd import gpu_op
+    q, k, v, do = _data(2, 1001, 1001, 4, 2, 72, 43)
+    documents = np.repeat(np.arange(4), [100, 201, 300, 400])[None].repeat(2, 0)
+    spans = gpu_op.attention_spans(1001, documents=documents, causal=True)
+    slopes = 2.0 ** (-2.0 * np.arange(1, 5)) if distance else None
+    want = ref.Attention(q, k, v, spans, slopes, 72 ** -0.5)
+    off = {}
+    for split in ("0", "1"):
+        monkeypatch.setenv("TINYFLOW_SPLIT", split)
+        out, stat, grads = _run(rt, q, k, v, do, spans=spans, slopes=slopes)
+        values = [want.out] + [value for value, _ in want.backward(want.out, want.stat, do)]
+        off[split] = [_off(got, value) for got, value in zip([out] + grads, values)]
+    for what, ours, fp32 in zip(("out", "dq", "dk", "dv"), off["1"], off["0"]):
+        assert ours <= 1.55 * fp32, "%s is %.2g off, %.2g on the fp32 instruction" % (what, ours, fp32)

@@ -10,8 +10,8 @@
 // sum is multiplied; a lane holds one row's or key's, so that is one factor a lane.
 //
 // Bound: the part's power and, with one or two waves a SIMD, the vector work between the products.  4 096 causal tokens, 16 heads on 4 of 128, 69 GFLOP
-// forward: pack 19 us, forward 195 to 208 (344 TFLOP/s; the fp32 instruction 1 094); backward: pack 53, dq 291 to 321 (343, three products), dkv 408 to 458
-// (320, four).  A product of the library on the fp16 instruction reaches a third of 1 178 to 1 347.
+// forward: pack 20 us, forward 187 to 206 (334 to 367 TFLOP/s; the fp32 instruction 1 094); backward: pack 55, dq 288 to 327 (315 to 358, three products), dkv 413 to 474
+// (290 to 333, four).  A product of the library on the fp16 instruction reaches a third of 1 178 to 1 347.
 //
 // A block has kBad for its exponent if it holds an infinity or a NaN, or gradients with a row whose statistic or delta is not finite, if its values pass
 // 2^55 or stay below 2^-96, or if a row or a column of it is smaller than 2^-16 of its largest value and would lose its digits (of queries and keys in the forward
@@ -625,13 +625,16 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
 
 // ------------------------------------------------------------------------------ backward
 
-// The unit of the sum of a lane's row or key, of gradients times what has exponent `other`: the step's largest gradient, held times 2^held, has to stay below
-// 2^15 in it.  Where one has to be lowered it becomes less than 2^6, and so do those of more than 2^10, so that it seldom has to.
-__device__ __forceinline__ int gradient_unit(float most, int held, int other, int unit, bool &lowers) {
-  const int field = (int)(bits_of(fmaxf(most, other_half(most))) >> 23), limit = field == 0 || field == 255 ? INT32_MAX : 141 - field + held + other;
+// The unit of the sum of a lane's row or key, of gradients times what has exponent `other`: the step's largest gradient has to stay below 2^15 in it (the
+// smallest ones lower, so that the factor is a number).  Where one has to be lowered it becomes less than 2^6, and so do those of more than 2^10, so that
+// it seldom has to.
+__device__ __forceinline__ int gradient_unit(float most, int other, int unit, bool &lowers) {
+  const int field = (int)(bits_of(fmaxf(most, other_half(most))) >> 23), limit = field == 0 || field == 255 ? INT32_MAX : 141 - max(field, 15) + other;
   lowers = __any(unit > limit);
   return lowers && unit > limit - 5 ? min(unit, limit - 9) : unit;
 }
+// The factor that brings such a gradient to it; a sum of nothing but zeros so far has none.
+__device__ __forceinline__ float to_unit(int unit, int other) { return __builtin_ldexpf(1.f, unit == kNoUnit ? 0 : min(unit - other, 126)); }
 
 // p times 2^x, for shift = x - the row's statistic, and the derivative of the cap, from a product.
 template <bool PLAIN>
@@ -736,17 +739,17 @@ __global__ __launch_bounds__(kThreads, (kTwoWaves<DP, PLAIN>) ? 2 : 1) void dq_k
 #pragma unroll
     for (int v = 0; v < 16; ++v) most = fmaxf(most, fabsf(ds[v]));
     bool lowers;
-    const int new_unit = gradient_unit(most, 0, ek, unit, lowers);
+    const int new_unit = gradient_unit(most, ek, unit, lowers);
     if (lowers) {
       multiply(sum, __builtin_ldexpf(1.f, max(new_unit - unit, -200)));
       keep<!TWO>(sum);
       unit = new_unit;
     }
-    const int shift = unit == kNoUnit ? 0 : unit - ek;  // nothing but zeros so far
+    const float scale = to_unit(unit, ek);
     Weights w;
     auto set = [&](auto n_c) {
       constexpr int n = decltype(n_c)::value;
-      w.set<n>(__builtin_ldexpf(ds[2 * n], shift), __builtin_ldexpf(ds[2 * n + 1], shift));
+      w.set<n>(ds[2 * n] * scale, ds[2 * n + 1] * scale);
     };
     static_for<4>(set);
     add_product<DP, AHEAD>(sum, lds[slot] + 2 * BLOCK, w,
@@ -851,9 +854,10 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
     }
     const char *const at = lds[slot];
     const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(sign, -(ed + ev));
-    // p is held times 2^this, as the sum of dv needs it, or 2^60 where that leaves fp32 no room
-    auto held_by = [&](int u) { return min(max(u - ed, -47), kMostHeld); };
-    int held = held_by(unit_v);
+    // p enters the sum of dv times this; 2^60 at most, until the key's first share says what that is.  (As part of its exponent it would cost nothing, but
+    // the exponents of the shares that count would be rounded at its size: dk and dv of documents with distances 7.7e-7 off, and so 2.9e-7 to 3.7e-7.)
+    auto held_by = [&](int u) { return min(max(u - ed, -126), kMostHeld); };
+    const float scale = __builtin_ldexpf(1.f, held_by(unit_v));
     const float *const of = reinterpret_cast<const float *>(at + 4 * BLOCK) + 4 * half;
     auto four = [&](int array, int q) { return *reinterpret_cast<const f32x4 *>(of + 32 * array + 8 * q); };
     float p[16], cap[16], ds[16], most = 0.f;
@@ -864,13 +868,13 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
       // all at once, or, where the registers are full, as they are needed
       constexpr bool LATE = !PLAIN && DP == 64;
       f32x4 shift[LATE ? 1 : 4];
-      if constexpr (!LATE) static_for<4>([&](auto q) { shift[decltype(q)::value] = (float)held - four(kStat, decltype(q)::value); });
+      if constexpr (!LATE) static_for<4>([&](auto q) { shift[decltype(q)::value] = -four(kStat, decltype(q)::value); });
       products<DP, 2, AHEAD>(at, {&k, &v}, s, [&](auto place) {
         constexpr int FIRST = 3 * DP / 16;
         spread<decltype(place)::value, 0, FIRST, decltype(coming)::kCount>([&](auto f) { coming.template one<decltype(f)::value>(); });
         spread<decltype(place)::value, FIRST + 2, FIRST - 4, 16>([&](auto x_c) {
           constexpr int x = decltype(x_c)::value, q = x / 4, e = x % 4;
-          if constexpr (LATE && e == 0) shift[0] = (float)held - four(kStat, q);
+          if constexpr (LATE && e == 0) shift[0] = -four(kStat, q);
           float bias = 0.f;
           if (!PLAIN && c.slopes) bias = of[32 * kSlope + 8 * q + e] * fabsf(of[32 * kNear + 8 * q + e] - (float)j);
           p[x] = weight<PLAIN>(score, s[0][x], factor, bias, shift[LATE ? 0 : q][e], cap[x]);
@@ -883,7 +887,7 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
         // two values behind
         spread<decltype(place)::value, FIRST + 4, FIRST - 4, 8>([&](auto n_c) {
           constexpr int n = decltype(n_c)::value;
-          w.set<n>(p[2 * n], p[2 * n + 1]);
+          w.set<n>(p[2 * n] * scale, p[2 * n + 1] * scale);
         });
       });
     };
@@ -894,29 +898,27 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
     // others.
     most = fmaxf(most, other_half(most));
     asm("" : "+v"(unit_v));  // what follows from it is computed again, not kept all along
-    held = held_by(unit_v);
-    const float passes = unit_v - ed > kMostHeld && unit_v != kNoUnit ? 0.f : 65000.f;
+    const int held = held_by(unit_v);
+    const float passes = unit_v - ed > kMostHeld && unit_v != kNoUnit ? 0.f : __builtin_ldexpf(65000.f, -held);
     int next_unit = unit_v == kNoUnit && most > 0.f ? held + ed : unit_v;
     if (__any(most > passes)) {
-      const bool lowers = most > fminf(passes, 1024.f);
-      const int to = lowers ? min(unit_v - ed, held + 132 - (int)(bits_of(most) >> 23)) : held;
+      const bool lowers = most > passes * 0x1p-6f;
+      const int to = lowers ? min(unit_v - ed, 132 - (int)(bits_of(most) >> 23)) : held;
       static_for<8>([&](auto n_c) {
         constexpr int n = decltype(n_c)::value;
-        p[2 * n] = __builtin_ldexpf(p[2 * n], to - held);
-        p[2 * n + 1] = __builtin_ldexpf(p[2 * n + 1], to - held);
-        w.set<n>(p[2 * n], p[2 * n + 1]);
+        w.set<n>(__builtin_ldexpf(p[2 * n], to), __builtin_ldexpf(p[2 * n + 1], to));
       });
       if (lowers) next_unit = to + ed;
       multiply(dvs, __builtin_ldexpf(1.f, max(next_unit - unit_v, -200)));
       keep<(DP > 64)>(dvs);
-      held = to;
     }
     unit_v = next_unit;
     // While dv is summed: ds, the unit that dk's sum takes for it, and ds as that product's operand.
     f32x4 delta[4];
     static_for<4>([&](auto q) { delta[decltype(q)::value] = four(kDelta, decltype(q)::value); });
     constexpr int PLACES = 3 * DP / 16, HALF = PLACES / 2;
-    int new_unit = unit, shift = 0;
+    int new_unit = unit;
+    float to_sum = 1.f;
     float largest = 0.f;
     bool lowers = false;
     Weights wd;
@@ -929,12 +931,12 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
         if constexpr (x % 2) largest = fmaxf(fmaxf(largest, fabsf(ds[x - 1])), fabsf(ds[x]));
       });
       if constexpr (at_place == HALF - 1) {
-        new_unit = gradient_unit(largest, held, eq, unit, lowers);
-        shift = new_unit == kNoUnit ? 0 : new_unit - eq - held;  // nothing but zeros so far
+        new_unit = gradient_unit(largest, eq, unit, lowers);
+        to_sum = to_unit(new_unit, eq);
       }
       spread<at_place, HALF, PLACES - HALF, 8>([&](auto n_c) {
         constexpr int n = decltype(n_c)::value;
-        wd.set<n>(__builtin_ldexpf(ds[2 * n], shift), __builtin_ldexpf(ds[2 * n + 1], shift));
+        wd.set<n>(ds[2 * n] * to_sum, ds[2 * n + 1] * to_sum);
       });
     });
     if (lowers) {
