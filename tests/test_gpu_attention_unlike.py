@@ -270,3 +270,19 @@ def test_errors_are_those_of_fp32(rt, monkeypatch, distance):
         off[split] = [_off(got, value) for got, value in zip([out] + grads, values)]
     for what, ours, fp32 in zip(("out", "dq", "dk", "dv"), off["1"], off["0"]):
         assert ours <= 1.55 * fp32, "%s is %.2g off, %.2g on the fp32 instruction" % (what, ours, fp32)
+
+
+@pytest.mark.parametrize("split", ["0", "1"])
+@pytest.mark.parametrize("power", [80, 95, 105])
+def test_shares_near_the_smallest_numbers(rt, monkeypatch, split, power):
+    """Keys that every query gives 2^-power: dv is as small, and has its digits."""
+    monkeypatch.setenv("TINYFLOW_SPLIT", split)
+    q, k, v, do = _data(1, 200, 300, 2, 1, 64, 44)
+    low = np.arange(300) % 11 == 3
+    q[..., 0], k[..., 0] = 4, 0
+    k[:, low, :, 0] = -power * np.log(2) * 8 / 4
+    do *= np.float32(100)
+    out, stat, (_, _, dv) = _run(rt, q, k, v, do)
+    value = ref.Attention(q, k, v, None, None, 0.125).backward(out, stat, do)[2][0]
+    # scores of up to 73 and 10: 2^-24 40 83 off, and so are shares: 2^-12.3
+    assert _off(dv[:, low], value[:, low]) <= 2.0 ** -12

@@ -6,7 +6,7 @@
 // left off is 2^-23 of an element, or 2^-40 of its block's largest value where that is more, and l l', up to 2^-22 of a product.
 // Scales are a block's, so a product's scale is known for a whole tile and costs nothing: it is part of the factor of a score, of the
 // exponent of p, of ds.  The sum over blocks has a scale of its own for each row (out, dq) or key (dk, dv): that of the largest p v, ds k, ds q or p do that it
-// has had, so that what is left off p or ds is 2^-30 of that at most, whatever lies beside the row or was next to nothing in it.  When a larger one comes the
+// has had, so that what is left off p or ds is 2^-34 of that at most, whatever lies beside the row or was next to nothing in it.  When a larger one comes the
 // sum is multiplied; a lane holds one row's or key's, so that is one factor a lane.
 //
 // Bound: the part's power and, with one or two waves a SIMD, the vector work between the products.  4 096 causal tokens, 16 heads on 4 of 128, 69 GFLOP
@@ -53,7 +53,7 @@ constexpr int kSmallest = 110;   // the largest exponent: of zeros, and of queri
 constexpr int kLargest = -40;
 constexpr int kSpansReadByAll = 2048;
 constexpr int kNoUnit = INT32_MAX / 2;  // of a sum of nothing
-constexpr int kMostHeld = 60;
+constexpr int kFirstHeld = 60;
 
 // Bytes of a block of 32 rows: DP columns of h and l.
 __host__ __device__ constexpr int64_t block_size(int dp) { return dp * 128; }
@@ -626,12 +626,12 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
 // ------------------------------------------------------------------------------ backward
 
 // The unit of the sum of a lane's row or key, of gradients times what has exponent `other`: the step's largest gradient has to stay below 2^15 in it (the
-// smallest ones lower, so that the factor is a number).  Where one has to be lowered it becomes less than 2^6, and so do those of more than 2^10, so that
-// it seldom has to.
+// smallest ones lower, so that the factor is a number).  Where one has to be lowered it becomes less than 2^10, and so do those of more than 2^13, so that
+// it seldom has to.  (A floor of 2^-34 of the largest.  To 2^6 the backward pass of 4 096 tokens of 16 heads of 128 takes 738 us, to 2^12 765, and so 749.)
 __device__ __forceinline__ int gradient_unit(float most, int other, int unit, bool &lowers) {
   const int field = (int)(bits_of(fmaxf(most, other_half(most))) >> 23), limit = field == 0 || field == 255 ? INT32_MAX : 141 - max(field, 15) + other;
   lowers = __any(unit > limit);
-  return lowers && unit > limit - 5 ? min(unit, limit - 9) : unit;
+  return lowers && unit > limit - 2 ? min(unit, limit - 5) : unit;
 }
 // The factor that brings such a gradient to it; a sum of nothing but zeros so far has none.
 __device__ __forceinline__ float to_unit(int unit, int other) { return __builtin_ldexpf(1.f, unit == kNoUnit ? 0 : min(unit - other, 126)); }
@@ -854,9 +854,9 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
     }
     const char *const at = lds[slot];
     const float factor = unscaled(score.factor, eq, ek), d_factor = __builtin_ldexpf(sign, -(ed + ev));
-    // p enters the sum of dv times this; 2^60 at most, until the key's first share says what that is.  (As part of its exponent it would cost nothing, but
+    // p enters the sum of dv times this, 2^60 until the key's first share says what it is to be.  (As part of its exponent it would cost nothing, but
     // the exponents of the shares that count would be rounded at its size: dk and dv of documents with distances 7.7e-7 off, and so 2.9e-7 to 3.7e-7.)
-    auto held_by = [&](int u) { return min(max(u - ed, -126), kMostHeld); };
+    auto held_by = [&](int u) { return u == kNoUnit ? kFirstHeld : min(max(u - ed, -126), 126); };
     const float scale = __builtin_ldexpf(1.f, held_by(unit_v));
     const float *const of = reinterpret_cast<const float *>(at + 4 * BLOCK) + 4 * half;
     auto four = [&](int array, int q) { return *reinterpret_cast<const f32x4 *>(of + 32 * array + 8 * q); };
@@ -893,22 +893,23 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
     };
     if (seen.covers(j0, j0 + 32)) tile(std::true_type{});
     else tile(std::false_type{});
-    // A key's first share sets its unit.  Shares that pass what fp16 holds, or that are not held as the sum needs them, lower it so that they become less than 2^6, and
-    // of the wave's other keys that of those of more than 2^10, so that this is seldom.  A unit follows the largest p do that its key has had, whatever the rows give to
-    // others.
+    // A key's first share sets its unit.  Shares that pass what fp16 holds, or that are not held as the sum needs them, lower it so that they become less than 2^10, and
+    // of the wave's other keys that of those of more than 2^13, so that this is seldom; a first share too small for its digits raises it as far.  A unit follows the largest
+    // p do that its key has had, whatever the rows give to others.
     most = fmaxf(most, other_half(most));
     asm("" : "+v"(unit_v));  // what follows from it is computed again, not kept all along
     const int held = held_by(unit_v);
-    const float passes = unit_v - ed > kMostHeld && unit_v != kNoUnit ? 0.f : __builtin_ldexpf(65000.f, -held);
-    int next_unit = unit_v == kNoUnit && most > 0.f ? held + ed : unit_v;
-    if (__any(most > passes)) {
-      const bool lowers = most > passes * 0x1p-6f;
-      const int to = lowers ? min(unit_v - ed, 132 - (int)(bits_of(most) >> 23)) : held;
+    const float passes = unit_v - ed > 126 && unit_v != kNoUnit ? 0.f : __builtin_ldexpf(65000.f, -held);
+    const bool first = unit_v == kNoUnit && most > 0.f, small = first && most < __builtin_ldexpf(0.25f, -kFirstHeld);
+    int next_unit = first ? held + ed : unit_v;
+    if (__any(most > passes || small)) {
+      const bool moves = most > passes * 0x1p-3f || small;
+      const int to = moves ? min(min(unit_v - ed, 126), 136 - (int)(bits_of(most) >> 23)) : held;
       static_for<8>([&](auto n_c) {
         constexpr int n = decltype(n_c)::value;
         w.set<n>(__builtin_ldexpf(p[2 * n], to), __builtin_ldexpf(p[2 * n + 1], to));
       });
-      if (lowers) next_unit = to + ed;
+      if (moves) next_unit = to + ed;
       multiply(dvs, __builtin_ldexpf(1.f, max(next_unit - unit_v, -200)));
       keep<(DP > 64)>(dvs);
     }
