@@ -237,7 +237,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Call c, float *out
 // and sums column 64 d + 4 (row of D) + e into sum[d][e]: both operands are 16-byte loads from where they lie in memory, 16 lanes side by side.
 // What bounds it is HBM as long as a wave's next step is on its way all the time that one is worked on: with the next keys fetched behind the
 // scores and the next values behind their product, and loads behind branches, of which all are waited for, 100 003 keys of 2 heads of 128 took 49 us,
-// and so 35-39 (5.2-5.9 TB/s).
+// and so 39-41 (5.0-5.2 TB/s).
 constexpr int kFewKeys = 16;  // of a wave's step
 
 // op over the four lanes with the same lane % 16

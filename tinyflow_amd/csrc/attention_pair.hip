@@ -6,7 +6,7 @@
 // left off is 2^-23 of an element, or 2^-40 of its block's largest value where that is more, and l l', up to 2^-22 of a product.
 // Scales are a block's, so a product's scale is known for a whole tile and costs nothing: it is part of the factor of a score, of the
 // exponent of p, of ds.  The sum over blocks has a scale of its own for each row (out, dq) or key (dk, dv): that of the largest p v, ds k, ds q or p do that it
-// has had, so that what is left off p or ds is 2^-34 of that at most, whatever lies beside the row or was next to nothing in it.  When a larger one comes the
+// has had, so that what is left off p or ds is 2^-32 of that at most, whatever lies beside the row or was next to nothing in it.  When a larger one comes the
 // sum is multiplied; a lane holds one row's or key's, so that is one factor a lane.
 //
 // Bound: the part's power and, with one or two waves a SIMD, the vector work between the products.  4 096 causal tokens, 16 heads on 4 of 128, 69 GFLOP
@@ -115,7 +115,8 @@ __global__ __launch_bounds__(1024) void seen_kernel(const Call c, int2 *seen) {
 template <int DP>
 __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack p) {
   __shared__ __align__(16) float tile[32][DP + 4];
-  __shared__ uint32_t most[32], columns[4][8];
+  __shared__ uint32_t most[32];
+  __shared__ int finds[4];
   __shared__ int hull[2];
   int which = 0;
   for (int i = 1; i < p.n_jobs; ++i) which = (int)blockIdx.x >= p.jobs[i].first ? i : which;
@@ -208,37 +209,27 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
       if (tid == 0) p.hulls[of_block] = seen;
     }
   }
-  // Columns that are smaller than 2^-16 of the block's largest in all rows, and not all zeros: a bit for each of the lane's columns with an element
-  // that is not smaller, and one with any.  (Of a single row they are no column yet: its elements are what they are beside its largest.)
-  static_assert(DP <= 128, "16 columns a lane");
-  const uint32_t not_small = (uint32_t)max(field - 16, 0) << 23;
-  const uint64_t rows = __ballot(tid % 64 < 32 && most[tid % 32] != 0);  // with anything but zeros
-  const bool judged = job.digits && (rows & (rows - 1)) != 0;
-  if (judged) {
-    uint32_t marks = 0;
-#pragma unroll
-    for (int e = 0; e < DP / 32; ++e)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t size = bits_of(x[e][i]) & 0x7fffffffu;
-        marks |= (size >= not_small ? 1u << (4 * e + i) : 0u) | (size ? 0x10000u << (4 * e + i) : 0u);
-      }
-    marks = lanes::reduce<64, 8>(marks, [](uint32_t a, uint32_t b) { return a | b; });
-    if (tid % 64 < 8) columns[tid / 64][tid % 8] = marks;
-  }
+  // Elements smaller than 2^-16 of the largest, zeros among them, of the wave's eight rows.  A column of nothing else has one in each row that is not all zeros;
+  // as many beside what is zero by itself, rows and columns that are none, are a reason to look for it.
+  const float not_small = __builtin_bit_cast(float, (uint32_t)max(field - 16, 0) << 23);
+  int smalls = 0;
 #pragma unroll
   for (int e = 0; e < DP / 32; ++e) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[e][i] = __builtin_ldexpf(x[e][i], exponent);
+    for (int i = 0; i < 4; ++i) {
+      if (job.digits) smalls += __popcll(__ballot(fabsf(x[e][i]) < not_small));
+      x[e][i] = __builtin_ldexpf(x[e][i], exponent);
+    }
     *reinterpret_cast<f32x4 *>(&tile[row][32 * e + tid % 8 * 4]) = x[e];
   }
+  const int live_rows = __popcll(__ballot(top != 0)) / 8;
+  if (tid % 64 == 0) finds[tid / 64] = live_rows > 0 && smalls - 8 * DP + live_rows * c.dim >= live_rows;
   __syncthreads();
-  if (judged) {
-    const uint32_t marks = columns[0][tid % 8] | columns[1][tid % 8] | columns[2][tid % 8] | columns[3][tid % 8];
-    if (__any((marks >> 16 & ~marks) != 0)) exponent = kBad;
+  int *const exponent_at = job.exponents + (int64_t)head * blocks + block;
+  if (exponent == kBad) {
+    if (tid == 0) *exponent_at = kBad;
+    return;
   }
-  if (tid == 0) job.exponents[(int64_t)head * blocks + block] = exponent;
-  if (exponent == kBad) return;
   const int64_t to = ((int64_t)head * blocks + block) * block_size(DP);
   if (job.plain)
 #pragma unroll
@@ -272,6 +263,17 @@ __global__ __launch_bounds__(kThreads) void pack_kernel(const Call c, const Pack
       *reinterpret_cast<f16x8 *>(out) = h;
       *reinterpret_cast<f16x8 *>(out + kFragment) = l;
     }
+  // Columns that are that small in all rows, and not all zeros, cannot be split.  Of a single row they are no column yet: its elements are what they are beside
+  // its largest.
+  if (finds[0] | finds[1] | finds[2] | finds[3]) {
+    const uint64_t rows = __ballot(tid % 64 < 32 && most[tid % 32] != 0);
+    float top_of = 0.f;
+    if (tid < DP)
+#pragma unroll 4
+      for (int r = 0; r < 32; ++r) top_of = fmaxf(top_of, fabsf(tile[r][tid]));
+    if (__syncthreads_or(top_of > 0.f && top_of < __builtin_ldexpf(not_small, exponent)) && (rows & (rows - 1)) != 0) exponent = kBad;
+  }
+  if (tid == 0) *exponent_at = exponent;
 }
 
 // ------------------------------------------------------------------------------ what the products share
@@ -626,12 +628,12 @@ __global__ __launch_bounds__(2 * kThreads, DP <= 64 ? 4 : 2) void forward_kernel
 // ------------------------------------------------------------------------------ backward
 
 // The unit of the sum of a lane's row or key, of gradients times what has exponent `other`: the step's largest gradient has to stay below 2^15 in it (the
-// smallest ones lower, so that the factor is a number).  Where one has to be lowered it becomes less than 2^10, and so do those of more than 2^13, so that
-// it seldom has to.  (A floor of 2^-34 of the largest.  To 2^6 the backward pass of 4 096 tokens of 16 heads of 128 takes 738 us, to 2^12 765, and so 749.)
+// smallest ones lower, so that the factor is a number).  Where one has to be lowered it becomes less than 2^8, and so do those of more than 2^11, so that
+// it seldom has to.  (A floor of 2^-32 of the largest.  To 2^6 the backward pass of 4 096 tokens of 16 heads of 128 takes 738 us, to 2^10 749, and so 741.)
 __device__ __forceinline__ int gradient_unit(float most, int other, int unit, bool &lowers) {
   const int field = (int)(bits_of(fmaxf(most, other_half(most))) >> 23), limit = field == 0 || field == 255 ? INT32_MAX : 141 - max(field, 15) + other;
   lowers = __any(unit > limit);
-  return lowers && unit > limit - 2 ? min(unit, limit - 5) : unit;
+  return lowers && unit > limit - 4 ? min(unit, limit - 7) : unit;
 }
 // The factor that brings such a gradient to it; a sum of nothing but zeros so far has none.
 __device__ __forceinline__ float to_unit(int unit, int other) { return __builtin_ldexpf(1.f, unit == kNoUnit ? 0 : min(unit - other, 126)); }
@@ -893,8 +895,8 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
     };
     if (seen.covers(j0, j0 + 32)) tile(std::true_type{});
     else tile(std::false_type{});
-    // A key's first share sets its unit.  Shares that pass what fp16 holds, or that are not held as the sum needs them, lower it so that they become less than 2^10, and
-    // of the wave's other keys that of those of more than 2^13, so that this is seldom; a first share too small for its digits raises it as far.  A unit follows the largest
+    // A key's first share sets its unit.  Shares that pass what fp16 holds, or that are not held as the sum needs them, lower it so that they become less than 2^8, and
+    // of the wave's other keys that of those of more than 2^11, so that this is seldom; a first share too small for its digits raises it as far.  A unit follows the largest
     // p do that its key has had, whatever the rows give to others.
     most = fmaxf(most, other_half(most));
     asm("" : "+v"(unit_v));  // what follows from it is computed again, not kept all along
@@ -903,8 +905,8 @@ __global__ __launch_bounds__(kThreads, DP <= 64 ? 2 : 1) void dkv_kernel(const C
     const bool first = unit_v == kNoUnit && most > 0.f, small = first && most < __builtin_ldexpf(0.25f, -kFirstHeld);
     int next_unit = first ? held + ed : unit_v;
     if (__any(most > passes || small)) {
-      const bool moves = most > passes * 0x1p-3f || small;
-      const int to = moves ? min(min(unit_v - ed, 126), 136 - (int)(bits_of(most) >> 23)) : held;
+      const bool moves = most > passes * 0x1p-5f || small;
+      const int to = moves ? min(min(unit_v - ed, 126), 134 - (int)(bits_of(most) >> 23)) : held;
       static_for<8>([&](auto n_c) {
         constexpr int n = decltype(n_c)::value;
         w.set<n>(__builtin_ldexpf(p[2 * n], to), __builtin_ldexpf(p[2 * n + 1], to));
