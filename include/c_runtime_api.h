@@ -493,9 +493,11 @@ int DLGpuHeadRotaryBackward(const DLHeadGradientPart *parts, int n_parts, const 
  * (Shares have the rounding of distances from the nearest key that a query sees.  A statistic has that of its size, and with it the backward pass, which
  * reads it: 1e-3 at 1e4, where a query stands far from all that it sees.)
  * statistics [batch, heads, queries] are what the backward pass reads; one of output and statistics may be NULL.
- * Results must not overlap what they are computed from.  A call that takes scratch is refused on a stream that is being captured
- * into a graph: TINYFLOW_SPLIT=0 in the environment keeps the products on the fp32 instruction, where only queries too few
- * to give every CU work take some, over many keys. */
+ * Results must not overlap what they are computed from.  Calls of many rows, of heads up to 128, are computed on pairs of fp16 numbers: an element is off by 2^-23 of
+ * itself, a product by 2^-22.  Tiles of operands that these do not hold (not finite, rows or columns of 32 that differ by 2^16, scores that could pass 2^18) are computed
+ * on the fp32 instruction, which takes several times as long; TINYFLOW_SPLIT=0 in the environment keeps all of them there.
+ * A call that takes scratch is refused on a stream that is being captured into a graph: on pairs all do, on the fp32 instruction those of queries too few
+ * to give every CU work, over many keys. */
 int DLGpuAttentionForward(const DLArrayHandle query, const DLArrayHandle key, const DLArrayHandle value, const DLArrayHandle spans,
                           const DLArrayHandle slopes, DLArrayHandle output, DLArrayHandle statistics, int batch, int heads,
                           int key_heads, float scale, float cap, int causal, int *memorytoSaving, void **stream);

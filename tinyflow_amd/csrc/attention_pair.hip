@@ -10,8 +10,8 @@
 // sum is multiplied; a lane holds one row's or key's, so that is one factor a lane.
 //
 // Bound: the part's power and, with one or two waves a SIMD, the vector work between the products.  4 096 causal tokens, 16 heads on 4 of 128, 69 GFLOP
-// forward: pack 20 us, forward 187 to 206 (334 to 367 TFLOP/s; the fp32 instruction 1 094); backward: pack 55, dq 288 to 327 (315 to 358, three products), dkv 413 to 474
-// (290 to 333, four).  A product of the library on the fp16 instruction reaches a third of 1 178 to 1 347.
+// forward: pack 19 us, forward 178 to 206 (334 to 386 TFLOP/s; the fp32 instruction 1 094); backward: pack 54, dq 277 to 327 (315 to 372, three products), dkv 396 to 470
+// (292 to 347, four).  A product of the library on the fp16 instruction reaches a third of 1 178 to 1 347.
 //
 // A block has kBad for its exponent if it holds an infinity or a NaN, or gradients with a row whose statistic or delta is not finite, if its values pass
 // 2^55 or stay below 2^-96, or if a row or a column of it is smaller than 2^-16 of its largest value and would lose its digits (of queries and keys in the forward
